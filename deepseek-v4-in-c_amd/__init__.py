@@ -26,6 +26,7 @@ STUB_PATH = os.path.join(HERE, "lib", "libdsv4_gpu_stub.so")
 # enum values of include/dsv4_gpu.h and the reference's dsv4.h:92
 WF32, WBF16, WFP8, WFP4 = 0, 1, 2, 3
 KV_F32, KV_BF16, KV_FP8 = 0, 1, 2
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 MAX_BATCH = 64
 
 _f32p = ctypes.POINTER(ctypes.c_float)
@@ -84,6 +85,19 @@ class CkptStats(ctypes.Structure):
                 ("bytes", ctypes.c_longlong), ("seconds", ctypes.c_double)]
 
 
+class Rope(ctypes.Structure):
+    """dsv4_gpu_rope (include/dsv4_gpu.h); device pointers."""
+    _fields_ = [("cos", _vp), ("sin", _vp)] + [(n, _ci) for n in ("max_pos", "dim", "offset",
+                                                                  "layout")]
+
+
+class LogitRules(ctypes.Structure):
+    """dsv4_gpu_logit_rules (include/dsv4_gpu.h); device pointers."""
+    _fields_ = [("hist", _vp), ("n_hist", _ci), ("draft", _vp), ("mask", _vp),
+                ("repetition", _cf), ("frequency", _cf), ("presence", _cf), ("bias", _vp),
+                ("allow", _vp), ("allow_stride", _ci)]
+
+
 def build():
     """Compile lib/libdsv4_gpu.so (hipcc, gfx950) and the CPU stub."""
     subprocess.run(["make", "-s", "-C", HERE, "all"], check=True)
@@ -94,6 +108,10 @@ _QP = ctypes.POINTER(DSV4QMat)
 _EP = ctypes.POINTER(DSV4ExpertW)
 _ACP = ctypes.POINTER(AttnCfg)
 _AWP = ctypes.POINTER(AttnW)
+_RP = ctypes.POINTER(Rope)
+_LRP = ctypes.POINTER(LogitRules)
+_sz = ctypes.c_size_t
+_ll = ctypes.c_longlong
 
 _SIGS = {
     "dsv4_gpu_available": (_ci, []),
@@ -158,6 +176,16 @@ _SIGS = {
     "dsv4_gpu_attn_reset": (_ci, [_ci]),
     "dsv4_gpu_attn_step": (_ci, [_vp, _vp, _ci, _ci]),
     "dsv4_gpu_attn_step_d": (_ci, [_vp, _vp, _ci, _ci, _vp]),
+    "dsv4_gpu_rope_n_d": (_ci, [_vp, _ll, _vp, _ll, _ci, _vp, _ci, _ci, _ci, _RP, _ci, _vp]),
+    "dsv4_gpu_kv_append_d": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _ci, _ll, _ci, _ci, _vp, _ci,
+                                   _RP, _vp, _vp]),
+    "dsv4_gpu_kv_read_d": (_ci, [_vp, _ci, _ll, _vp, _vp, _ci, _ci, _ci, _vp, _ci, _ci, _ci,
+                                 _vp]),
+    "dsv4_gpu_tree_attn_scratch_bytes": (_sz, [_ci] * 8),
+    "dsv4_gpu_tree_attn_d": (_ci, [_vp, _vp, _ci, _ci, _ci, _ci, _ci, _vp, _vp, _ci, _ci, _ci,
+                                   _vp, _ci, _ci, _ci, _vp, _ci, _vp, _cf, _vp, _sz, _vp]),
+    "dsv4_gpu_logits_scratch_bytes": (_sz, [_ci, _ci]),
+    "dsv4_gpu_logits_adjust_d": (_ci, [_vp, _vp, _vp, _ci, _ci, _ll, _LRP, _vp, _sz, _vp]),
 }
 
 SYMBOLS = tuple(_SIGS)

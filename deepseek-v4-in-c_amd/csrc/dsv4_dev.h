@@ -184,3 +184,26 @@ __device__ __forceinline__ f32x4 ldf4(const float *p)
 {
     return *reinterpret_cast<const f32x4 *>(p);
 }
+
+/* ------------------------------------------------------------- argmax */
+
+/* The composite whose maximum is the greedy pick (dsv4_head.hip): the order
+ * of the values, ties to the lower index. */
+__device__ __forceinline__ unsigned long long am_key(float v, int i)
+{
+    if (v != v) return 0ull;                          /* NaN: never the maximum */
+    uint32_t u = __float_as_uint(v);
+    if ((u & 0x7FFFFFFFu) == 0u) u = 0u;              /* -0.0 == +0.0 */
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((unsigned long long)u << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)i);
+}
+
+__device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const unsigned long long t = __shfl_xor(v, o, 64);
+        v = t > v ? t : v;
+    }
+    return v;
+}

@@ -191,3 +191,41 @@ int dsv4_gpu_fp8_gemv_n_d(float *d_y, const float *d_x, const uint8_t *d_w,
                           void *stream)
 { (void)d_y; (void)d_x; (void)d_w; (void)d_s; (void)scale_fmt; (void)rows; (void)cols;
   (void)nt; (void)stream; return -1; }
+
+int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long long x_stride,
+                      int fmt, const int *d_pos, int nt, int heads, int head_dim,
+                      const dsv4_gpu_rope *rope, int inverse, void *stream)
+{ (void)d_out; (void)out_stride; (void)d_x; (void)x_stride; (void)fmt; (void)d_pos; (void)nt;
+  (void)heads; (void)head_dim; (void)rope; (void)inverse; (void)stream; return -1; }
+int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
+                         const void *d_x, int x_fmt, long long x_stride, int n, int row_dim,
+                         const int *d_rows, int row0, const dsv4_gpu_rope *rope,
+                         const int *d_pos, void *stream)
+{ (void)d_kv; (void)d_kv_scales; (void)kv_fmt; (void)kv_stride; (void)kv_rows; (void)d_x;
+  (void)x_fmt; (void)x_stride; (void)n; (void)row_dim; (void)d_rows; (void)row0; (void)rope;
+  (void)d_pos; (void)stream; return -1; }
+int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const void *d_kv,
+                       const float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
+                       const int *d_rows, int row0, int n, int row_dim, void *stream)
+{ (void)d_out; (void)out_fmt; (void)out_stride; (void)d_kv; (void)d_kv_scales; (void)kv_fmt;
+  (void)kv_stride; (void)kv_rows; (void)d_rows; (void)row0; (void)n; (void)row_dim;
+  (void)stream; return -1; }
+size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt,
+                                        int n_ctx, int window)
+{ (void)fmt; (void)nt; (void)h; (void)d_qk; (void)d_v; (void)kv_fmt; (void)n_ctx; (void)window;
+  return 0; }
+int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt, int h, int d_qk, int d_v,
+                         const void *d_kv, const float *d_kv_scales, int kv_fmt, int kv_stride,
+                         int kv_rows, const int *d_pages, int n_pages, int page_rows, int n_ctx,
+                         const uint64_t *d_mask, int window, const float *d_sink, float scale,
+                         void *d_scratch, size_t scratch_bytes, void *stream)
+{ (void)d_o; (void)d_q; (void)fmt; (void)nt; (void)h; (void)d_qk; (void)d_v; (void)d_kv;
+  (void)d_kv_scales; (void)kv_fmt; (void)kv_stride; (void)kv_rows; (void)d_pages; (void)n_pages;
+  (void)page_rows; (void)n_ctx; (void)d_mask; (void)window; (void)d_sink; (void)scale;
+  (void)d_scratch; (void)scratch_bytes; (void)stream; return -1; }
+size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab) { (void)nt; (void)vocab; return 0; }
+int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, int nt, int vocab,
+                             long long stride, const dsv4_gpu_logit_rules *rules,
+                             void *d_scratch, size_t scratch_bytes, void *stream)
+{ (void)d_out; (void)d_pick; (void)d_logits; (void)nt; (void)vocab; (void)stride; (void)rules;
+  (void)d_scratch; (void)scratch_bytes; (void)stream; return -1; }

@@ -341,3 +341,6 @@ int dsv4_qproj_launch(const float *qr, int cols, const float *nw, float eps, int
 int dsv4_comp_close_launch(float *out, float *kv_state, float *score_state, int ratio,
                            int hd, const float *w, float eps, int rd, const float *cs,
                            const float *sn, int pos, int half, hipStream_t st);
+
+/* What is wrong with a rotation of heads of head_dim elements, or nullptr. */
+const char *dsv4_rope_bad(const dsv4_gpu_rope *r, int head_dim);

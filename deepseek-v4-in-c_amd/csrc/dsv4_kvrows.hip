@@ -1,0 +1,423 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/* dsv4_kvrows.hip - rows of the latent cache written from f32 or bf16 rows
+ * on the device, and read back, on gfx950.
+ *
+ * APPEND. A row goes to its cache format by one wave: rotated if asked (the
+ * arithmetic of dsv4_rope.hip), then stored as f32, as bf16 (to nearest even)
+ * or as e4m3(x / s). s is the least power of two with max |x| <= 448 s over
+ * the finite elements, so x / s is exact and each element is rounded once;
+ * it comes from the maximum's bits alone: 448 is 1.75 * 2^8, so s has the
+ * maximum's exponent less 8, one more where the significand is over 1.75.
+ * A row read back as code * s has a maximum of 224 s (then it gets s / 2 and
+ * every code doubles, which e4m3 holds exactly) or more (then it gets s
+ * again), so writing it again keeps its values.
+ * Bound: x read once (twice past 768 elements), the codes written once. One
+ * row per wave keeps the maximum in registers: no LDS, no second launch.
+ * Where two tokens name one row the later is written: each workgroup looks
+ * its rows up among the later entries of the list, which costs the list's
+ * bytes once per four rows, from the L2.
+ *
+ * READ. A thread makes 16 bytes of output at a time, so that stores, the
+ * larger stream from an FP8 cache, are whole lines; four such pieces per
+ * thread keep the loads of four rows in flight.
+ */
+#include "dsv4_dev.h"
+#include "dsv4_internal.h"
+
+namespace {
+
+#include "dsv4_rows_io.h"
+
+constexpr int KR_THREADS = 256;
+constexpr int KR_ROWS = KR_THREADS / 64;          /* rows per workgroup      */
+constexpr int KR_DIM = 16384;                     /* the longest row         */
+
+struct AppendJob {
+    void *kv;
+    float *scales;
+    int kv_stride, kv_rows;
+    const void *x;
+    long long xs;
+    int n, dim;
+    const int *rows;
+    int row0;
+    const int *pos;                               /* nullptr: not rotated    */
+    dsv4_gpu_rope rp;
+};
+
+/* Elements c .. c + V - 1 of a row, rotated by the table row r (nullptr
+ * tables: a position outside them). */
+template <class T, int V>
+__device__ __forceinline__ void row_values(const AppendJob &a, const T *x, int c,
+                                           const float *cs, const float *sn, float *v)
+{
+    io_load<T, V>(x + c, v);
+    const int rc = c - a.rp.offset;
+    if (!a.pos || rc < 0 || rc >= a.rp.dim) return;
+    const int half = a.rp.dim / 2;
+    if (!cs) {
+#pragma unroll
+        for (int k = 0; k < V; k++) v[k] = __uint_as_float(0x7FC00000u);
+        return;
+    }
+    if (a.rp.layout == DSV4_GPU_ROPE_PAIRS) {
+        if constexpr (V == 1) {
+            float o;
+            io_load<T, 1>(x + (a.rp.offset + (rc ^ 1)), &o);
+            const float cc = cs[rc >> 1], ss = sn[rc >> 1];
+            v[0] = (rc & 1) ? o * ss + v[0] * cc : v[0] * cc - o * ss;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; k += 2) {
+                const float cc = cs[(rc + k) >> 1], ss = sn[(rc + k) >> 1];
+                const float x0 = v[k], x1 = v[k + 1];
+                v[k] = x0 * cc - x1 * ss;
+                v[k + 1] = x0 * ss + x1 * cc;
+            }
+        }
+        return;
+    }
+    const bool second = rc >= half;
+    const int p = second ? rc - half : rc;
+    float o[V];
+    io_load<T, V>(x + (second ? c - half : c + half), o);
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+        const float cc = cs[p + k], ss = sn[p + k];
+        v[k] = second ? o[k] * ss + v[k] * cc : v[k] * cc - o[k] * ss;
+    }
+}
+
+__device__ __forceinline__ bool finite_f(float v)
+{
+    return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u;
+}
+
+/* The row's scale and its inverse, both powers of two, from its largest
+ * finite magnitude. */
+__device__ __forceinline__ void row_scale(float top, float *s, float *inv)
+{
+    const uint32_t b = __float_as_uint(top);
+    int e = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    if (e < 1) e = 1;
+    if (b == 0u) e = 127;
+    *s = __uint_as_float((uint32_t)e << 23);
+    *inv = __uint_as_float((uint32_t)(254 - e) << 23);
+}
+
+/* Four e4m3 codes of four values at or below 448 in magnitude; what is not
+ * finite becomes NaN. */
+__device__ __forceinline__ uint32_t codes4(const float *v)
+{
+    float t[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) t[k] = finite_f(v[k]) ? v[k] : __uint_as_float(0x7FC00000u);
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], r, true);
+    return (uint32_t)r;
+}
+
+template <int KVF, int V>
+__device__ __forceinline__ void row_store(const AppendJob &a, size_t at, const float *v,
+                                          float inv)
+{
+    if constexpr (KVF == DSV4_GPU_KV_F32) {
+        io_store<float, V>((float *)a.kv + at, v);
+    } else if constexpr (KVF == DSV4_GPU_KV_BF16) {
+        io_store<uint16_t, V>((uint16_t *)a.kv + at, v);
+    } else {
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < V; k++) t[k] = v[k] * inv;
+        const uint32_t c = codes4(t);
+        if constexpr (V == 4) *(uint32_t *)((uint8_t *)a.kv + at) = c;
+        else ((uint8_t *)a.kv)[at] = (uint8_t)c;
+    }
+}
+
+/* NC pieces of V per lane kept in registers between the maximum and the
+ * store (the row is no longer than 64 V NC); NC 0: read again. */
+template <class T, int KVF, int V, int NC>
+__global__ void __launch_bounds__(KR_THREADS) k_append(AppendJob a)
+{
+    __shared__ int late[KR_ROWS];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int t0 = blockIdx.x * KR_ROWS, t = t0 + w;
+    const bool live = t < a.n;
+    const int row = !live ? -1 : a.rows ? a.rows[t] : a.row0 + t;
+    const T *x = (const T *)a.x + (live ? t : 0) * a.xs;
+    const float *cs = nullptr, *sn = nullptr;
+    if (a.pos && live) {
+        const int p = a.pos[t];
+        if (p >= 0 && p < a.rp.max_pos) {
+            cs = a.rp.cos + (size_t)p * (a.rp.dim / 2);
+            sn = a.rp.sin + (size_t)p * (a.rp.dim / 2);
+        }
+    }
+    constexpr int KEEP = NC > 0 ? NC : 1;
+    float v[KEEP][V];
+    if constexpr (NC > 0) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const int c = (i * 64 + lane) * V;
+            if (live && c < a.dim) {
+                row_values<T, V>(a, x, c, cs, sn, v[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k++) v[i][k] = 0.0f;
+            }
+        }
+    }
+    if (a.rows) {
+        if (threadIdx.x < KR_ROWS) late[threadIdx.x] = 0;
+        __syncthreads();
+        int mine[KR_ROWS];
+#pragma unroll
+        for (int k = 0; k < KR_ROWS; k++) mine[k] = a.rows[min(t0 + k, a.n - 1)];
+        for (int j = t0 + 1 + (int)threadIdx.x; j < a.n; j += KR_THREADS) {
+            const int r = a.rows[j];
+#pragma unroll
+            for (int k = 0; k < KR_ROWS; k++)
+                if (r == mine[k] && j > t0 + k) late[k] = 1;
+        }
+        __syncthreads();
+        if (late[w]) return;
+    }
+    if (!live || row < 0 || row >= a.kv_rows) return;
+    const size_t at = (size_t)row * a.kv_stride;
+    float inv = 1.0f;
+    if constexpr (KVF == DSV4_GPU_KV_FP8) {
+        float top = 0.0f;
+        if constexpr (NC > 0) {
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    if (finite_f(v[i][k])) top = fmaxf(top, fabsf(v[i][k]));
+        } else {
+            for (int c = lane * V; c < a.dim; c += 64 * V) {
+                row_values<T, V>(a, x, c, cs, sn, v[0]);
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    if (finite_f(v[0][k])) top = fmaxf(top, fabsf(v[0][k]));
+            }
+        }
+        top = wave_max(top);
+        float s;
+        row_scale(top, &s, &inv);
+        if (lane == 0) a.scales[row] = s;
+    }
+    if constexpr (NC > 0) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const int c = (i * 64 + lane) * V;
+            if (c < a.dim) row_store<KVF, V>(a, at + c, v[i], inv);
+        }
+    } else {
+        for (int c = lane * V; c < a.dim; c += 64 * V) {
+            row_values<T, V>(a, x, c, cs, sn, v[0]);
+            row_store<KVF, V>(a, at + c, v[0], inv);
+        }
+    }
+}
+
+struct ReadJob {
+    void *out;
+    long long os;
+    const void *kv;
+    const float *scales;
+    int kv_stride, kv_rows;
+    const int *rows;
+    int row0, items;
+    IoDiv units;
+};
+
+constexpr int RD_IL = 4;                          /* pieces per thread       */
+
+template <class T, int KVF, int V>
+__global__ void __launch_bounds__(KR_THREADS) k_read(ReadJob a)
+{
+    const uint32_t i0 = blockIdx.x * (KR_THREADS * RD_IL) + threadIdx.x;
+    float v[RD_IL][V];
+    T *o[RD_IL];
+#pragma unroll
+    for (int u = 0; u < RD_IL; u++) {
+        const uint32_t i = i0 + u * KR_THREADS;
+        o[u] = nullptr;
+#pragma unroll
+        for (int k = 0; k < V; k++) v[u][k] = 0.0f;
+        if (i >= (uint32_t)a.items) continue;
+        const uint32_t t = a.units.div(i);
+        const int c = (int)(i - t * a.units.d) * V;
+        o[u] = (T *)a.out + (long long)t * a.os + c;
+        const int row = a.rows ? a.rows[t] : a.row0 + (int)t;
+        if (row < 0 || row >= a.kv_rows) continue;
+        const size_t at = (size_t)row * a.kv_stride + c;
+        if constexpr (KVF == DSV4_GPU_KV_F32) {
+            io_load<float, V>((const float *)a.kv + at, v[u]);
+        } else if constexpr (KVF == DSV4_GPU_KV_BF16) {
+            io_load<uint16_t, V>((const uint16_t *)a.kv + at, v[u]);
+        } else {
+            const uint8_t *p = (const uint8_t *)a.kv + at;
+            const float s = a.scales[row];
+            if constexpr (V == 1) {
+                v[u][0] = dec_e4m3(p[0]) * s;
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k += 4) {
+                    dec_e4m3x4(((const uint32_t *)p)[k / 4], v[u] + k);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[u][k + e] *= s;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < RD_IL; u++)
+        if (o[u]) io_store<T, V>(o[u], v[u]);
+}
+
+/* -1 with a message unless the cache's own description holds. */
+int cache_ok(const char *what, const void *kv, const float *scales, int fmt, int stride, int rows,
+             int dim)
+{
+    if (fmt != DSV4_GPU_KV_F32 && fmt != DSV4_GPU_KV_BF16 && fmt != DSV4_GPU_KV_FP8) {
+        DSV4_ERR("%s: unknown cache format %d", what, fmt);
+        return -1;
+    }
+    if (dim <= 0 || stride < dim || rows <= 0) {
+        DSV4_ERR("%s: bad cache shape (rows %d of %d, stride %d)", what, rows, dim, stride);
+        return -1;
+    }
+    if (!kv || (fmt == DSV4_GPU_KV_FP8 && !scales)) {
+        DSV4_ERR("%s: no cache, or an FP8 cache without row scales", what);
+        return -1;
+    }
+    return 0;
+}
+
+int kv_size(int fmt) { return fmt == DSV4_GPU_KV_F32 ? 4 : fmt == DSV4_GPU_KV_BF16 ? 2 : 1; }
+
+template <class T, int KVF>
+void append_launch(const AppendJob &a, int V, hipStream_t st)
+{
+    const dim3 g((a.n + KR_ROWS - 1) / KR_ROWS), b(KR_THREADS);
+    if (V == 1)
+        hipLaunchKernelGGL((k_append<T, KVF, 1, 0>), g, b, 0, st, a);
+    else if (a.dim <= 64 * 4 * 3)
+        hipLaunchKernelGGL((k_append<T, KVF, 4, 3>), g, b, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_append<T, KVF, 4, 0>), g, b, 0, st, a);
+}
+
+template <class T>
+void append_fmt(const AppendJob &a, int fmt, int V, hipStream_t st)
+{
+    if (fmt == DSV4_GPU_KV_F32) append_launch<T, DSV4_GPU_KV_F32>(a, V, st);
+    else if (fmt == DSV4_GPU_KV_BF16) append_launch<T, DSV4_GPU_KV_BF16>(a, V, st);
+    else append_launch<T, DSV4_GPU_KV_FP8>(a, V, st);
+}
+
+template <class T, int V>
+void read_fmt(const ReadJob &a, int fmt, hipStream_t st)
+{
+    const int per = KR_THREADS * RD_IL;
+    const dim3 g((a.items + per - 1) / per), b(KR_THREADS);
+    if (fmt == DSV4_GPU_KV_F32)
+        hipLaunchKernelGGL((k_read<T, DSV4_GPU_KV_F32, V>), g, b, 0, st, a);
+    else if (fmt == DSV4_GPU_KV_BF16)
+        hipLaunchKernelGGL((k_read<T, DSV4_GPU_KV_BF16, V>), g, b, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_read<T, DSV4_GPU_KV_FP8, V>), g, b, 0, st, a);
+}
+
+} // namespace
+
+extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stride,
+                                    int kv_rows, const void *d_x, int x_fmt, long long x_stride,
+                                    int n, int row_dim, const int *d_rows, int row0,
+                                    const dsv4_gpu_rope *rope, const int *d_pos, void *stream)
+{
+    if (cache_ok("kv_append", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
+        return -1;
+    if (n < 0 || row_dim > KR_DIM || x_stride < row_dim ||
+        (x_fmt != DSV4_WF32 && x_fmt != DSV4_WBF16) || (n && !d_x)) {
+        DSV4_ERR("kv_append: bad arguments (n %d, row_dim %d, x_fmt %d, x_stride %lld)", n,
+                 row_dim, x_fmt, x_stride);
+        return -1;
+    }
+    if (!d_rows && (row0 < 0 || (long long)row0 + n > kv_rows)) {
+        DSV4_ERR("kv_append: rows %d .. %lld of a cache of %d", row0, (long long)row0 + n - 1,
+                 kv_rows);
+        return -1;
+    }
+    if (rope) {
+        const char *bad = dsv4_rope_bad(rope, row_dim);
+        if (!bad && n && !d_pos) bad = "no positions";
+        if (bad) {
+            DSV4_ERR("kv_append: rope: %s", bad);
+            return -1;
+        }
+    }
+    if (n == 0) return 0;
+    AppendJob a{d_kv, d_kv_scales, kv_stride, kv_rows, d_x, x_stride, n, row_dim, d_rows, row0,
+                rope ? d_pos : nullptr, rope ? *rope : dsv4_gpu_rope{}};
+    /* pieces of four elements where the shapes and addresses are whole ones */
+    const int xs = x_fmt == DSV4_WBF16 ? 2 : 4;
+    int V = 4;
+    if (row_dim % 4 || x_stride % 4 || kv_stride % 4 || (uintptr_t)d_x % (4 * xs) ||
+        (uintptr_t)d_kv % (4 * kv_size(kv_fmt)))
+        V = 1;
+    if (rope && (rope->offset % 4 || rope->dim % 4 ||
+                 (rope->layout == DSV4_GPU_ROPE_HALVES && rope->dim % 8)))
+        V = 1;
+    if (xs == 4) append_fmt<float>(a, kv_fmt, V, (hipStream_t)stream);
+    else append_fmt<uint16_t>(a, kv_fmt, V, (hipStream_t)stream);
+    HIP_OK(hipGetLastError(), "kv_append launch");
+    return 0;
+}
+
+extern "C" int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride,
+                                  const void *d_kv, const float *d_kv_scales, int kv_fmt,
+                                  int kv_stride, int kv_rows, const int *d_rows, int row0, int n,
+                                  int row_dim, void *stream)
+{
+    if (cache_ok("kv_read", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
+        return -1;
+    if (n < 0 || row_dim > KR_DIM || out_stride < row_dim || (out_fmt != DSV4_WF32 && out_fmt != DSV4_WBF16) ||
+        (n && !d_out)) {
+        DSV4_ERR("kv_read: bad arguments (n %d, row_dim %d, out_fmt %d, out_stride %lld)", n,
+                 row_dim, out_fmt, out_stride);
+        return -1;
+    }
+    if (!d_rows && (row0 < 0 || (long long)row0 + n > kv_rows)) {
+        DSV4_ERR("kv_read: rows %d .. %lld of a cache of %d", row0, (long long)row0 + n - 1,
+                 kv_rows);
+        return -1;
+    }
+    if (d_rows) row0 = 0;
+    const int es = out_fmt == DSV4_WBF16 ? 2 : 4, ks = kv_size(kv_fmt);
+    int V = 16 / es;
+    if (row_dim % V || out_stride % V || kv_stride % V || ((uintptr_t)d_out & 15) ||
+        (uintptr_t)d_kv % (V * ks < 16 ? V * ks : 16))
+        V = 1;
+    const int units = row_dim / V;
+    const int most = (1 << 30) / units;           /* rows of a launch         */
+    for (int t0 = 0; t0 < n; t0 += most) {
+        const int m = n - t0 < most ? n - t0 : most;
+        ReadJob a{(char *)d_out + (size_t)t0 * out_stride * es, out_stride, d_kv, d_kv_scales,
+                  kv_stride, kv_rows, d_rows ? d_rows + t0 : nullptr, row0 + t0, m * units,
+                  IoDiv((uint32_t)units)};
+        hipStream_t st = (hipStream_t)stream;
+        if (es == 4) {
+            if (V > 1) read_fmt<float, 4>(a, kv_fmt, st);
+            else read_fmt<float, 1>(a, kv_fmt, st);
+        } else {
+            if (V > 1) read_fmt<uint16_t, 8>(a, kv_fmt, st);
+            else read_fmt<uint16_t, 1>(a, kv_fmt, st);
+        }
+        HIP_OK(hipGetLastError(), "kv_read launch");
+    }
+    return 0;
+}

@@ -513,6 +513,139 @@ int dsv4_gpu_attn_step(float *out, const float *x, int layer, int pos);
 /* The same on device buffers (16-byte aligned), stream-ordered. */
 int dsv4_gpu_attn_step_d(float *d_out, const float *d_x, int layer, int pos, void *stream);
 
+/* ------------------------------------------------- drafted tokens ---------
+ * The device half of a step that checks several tokens of one sequence at
+ * once (drafted ones, or a short piece of a prompt) against a latent cache:
+ * beside the batched projections (dsv4_gpu_*_gemv_n_d), rotary positions for
+ * all tokens, their rows quantised into the cache, attention of a tree of
+ * them over it, and the request's rules on the logits of every row. The
+ * reference runs all of it token by token on the CPU.
+ *
+ * All are stream-ordered, allocate nothing, keep nothing between calls and
+ * use no library buffer: calls on different streams may overlap, and a call
+ * can be captured into a graph, as long as those that overlap are given
+ * workspaces of their own. They run on the current device, where every
+ * pointer must lie. Lengths and strides are in elements; nt or n of 0 does
+ * nothing and returns 0. Results do not depend on what else runs: no sum is
+ * taken in an order that varies. No counterpart in the reference's header. */
+
+/* How the two elements of a rotated pair lie: neighbours (2i, 2i + 1), the
+ * reference's layout (dsv4_rope.c:105-119), or i and i + dim/2. */
+enum { DSV4_GPU_ROPE_PAIRS = 0, DSV4_GPU_ROPE_HALVES = 1 };
+
+/* A rotation: elements [offset, offset + dim) of a head (dim even), by the
+ * device tables cos and sin [max_pos][dim/2], which the host builds as it does
+ * for the attention block (scaled for long contexts or not). */
+typedef struct {
+    const float *cos, *sin;
+    int max_pos, dim, offset, layout;
+} dsv4_gpu_rope;
+
+/* Rotate nt tokens' heads: token t's head i is x[t * x_stride + i * head_dim
+ * ...], turned by position d_pos[t] (inverse: back), (a, b) -> (a cos - b
+ * sin, a sin + b cos), in f32 with each product and sum rounded, rounded once
+ * to the type of x and out (fmt DSV4_WF32 or DSV4_WBF16). Elements outside
+ * the rotated part are copied. d_out may be d_x (with the same stride: the
+ * other elements then are not touched), but not overlap it otherwise. A
+ * position outside [0, max_pos) makes the token's rotated elements NaN. 0 /
+ * -1. */
+int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long long x_stride,
+                      int fmt, const int *d_pos, int nt, int heads, int head_dim,
+                      const dsv4_gpu_rope *rope, int inverse, void *stream);
+
+/* Write n rows of row_dim values (f32 or bf16, row t at d_x + t * x_stride)
+ * into a cache in a DSV4_GPU_KV_* format, rotated first by rope and d_pos if
+ * rope is not NULL (as one head). Row t goes to cache row d_rows[t], or row0 +
+ * t where d_rows is NULL; a row outside [0, kv_rows) is not written, and of
+ * several t that name one row the last is written. The cache's other rows,
+ * and a row's elements past row_dim, are left as they were. BF16 rounds to
+ * nearest even. FP8 stores e4m3(x / s), to nearest even, with s (d_kv_scales)
+ * the least power of two, 2^-126 at least, that brings the row's largest
+ * finite magnitude to 448 or less (1 for a row of zeros); infinities and NaN
+ * are stored as NaN. Rows written, read back and written again keep their
+ * values. kv_stride >= row_dim, which is at most 16384. d_x must not overlap
+ * the cache. 0 / -1. */
+int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
+                         const void *d_x, int x_fmt, long long x_stride, int n, int row_dim,
+                         const int *d_rows, int row0, const dsv4_gpu_rope *rope,
+                         const int *d_pos, void *stream);
+
+/* Read n cache rows back as f32 or bf16 (out_fmt): d_out + t * out_stride =
+ * row d_rows[t] (row0 + t where d_rows is NULL), an FP8 element as code *
+ * scale in f32, rounded to nearest even for bf16. A row outside [0, kv_rows)
+ * gives zeros and is never read. row_dim is at most 16384. 0 / -1. */
+int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const void *d_kv,
+                       const float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
+                       const int *d_rows, int row0, int n, int row_dim, void *stream);
+
+/* Attention of nt <= DSV4_MAX_BATCH tokens of one sequence over its cache,
+ * every head reading the one latent row: o[t][i] = softmax over the rows that
+ * token t sees of q[t][i] . row[:d_qk] * scale, applied to row[:d_v] (q
+ * [nt][h][d_qk], o [nt][h][d_v], both fmt DSV4_WF32 or DSV4_WBF16; d_v <= d_qk,
+ * d_qk <= 576, d_v <= 512). sink[i] enters the denominator only, or is absent
+ * when NULL.
+ *
+ * The sequence's positions 0 .. n_ctx - 1 are its context, n_ctx .. n_ctx +
+ * nt - 1 hold the tokens themselves (dsv4_gpu_kv_append_d). Position p is
+ * cache row p, or with d_pages row d_pages[p / page_rows] * page_rows + p %
+ * page_rows. Rows outside [0, kv_rows), and pages past n_pages, are treated
+ * as masked and never read.
+ *
+ * Token t sees token j where bit j of d_mask[t] is set (NULL: every j <= t),
+ * and its place in the sequence is n_ctx plus the other tokens it sees; with
+ * window > 0 it sees only rows less than window places back (0: all). A
+ * token that sees no row gets zeros. What a row holds does not reach tokens
+ * that do not see it, NaN and infinities included; one that sees a row with
+ * such an element gets NaN among its outputs.
+ *
+ * Scores, softmax and sums are in f32. With f32 q every product is exact
+ * (bf16 terms of q and of the weights; an F32 cache's elements in three terms
+ * as well), within 1e-5 relative; with bf16 q the weights are rounded to bf16
+ * before they meet the rows.
+ *
+ * d_scratch: dsv4_gpu_tree_attn_scratch_bytes of device memory for the call's
+ * shape, 16-byte aligned; the bytes do not fall as n_ctx grows, so a program
+ * can ask once for its longest context. Its contents are not kept. 0 / -1. */
+size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt,
+                                        int n_ctx, int window);
+int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt, int h, int d_qk, int d_v,
+                         const void *d_kv, const float *d_kv_scales, int kv_fmt, int kv_stride,
+                         int kv_rows, const int *d_pages, int n_pages, int page_rows, int n_ctx,
+                         const uint64_t *d_mask, int window, const float *d_sink, float scale,
+                         void *d_scratch, size_t scratch_bytes, void *stream);
+
+/* What a request asks of its logits (device pointers). A token's count in row
+ * t is how often it stands in hist[n_hist] and among the drafted tokens
+ * draft[j] whose bit j is set in mask[t] (mask NULL: every j <= t; draft
+ * NULL: none); ids outside the vocabulary count nowhere. Where the count is
+ * over 0, a logit v becomes v / repetition if v > 0, else v * repetition,
+ * and then loses count * frequency + presence. bias[vocab] (or NULL) is
+ * added. allow (or NULL): a bit per token, token v's in word v / 32 at v % 32,
+ * row t's words at t * allow_stride (0: one set for all rows); a token
+ * without its bit becomes -infinity. No rule: repetition 1, the rest 0. */
+typedef struct {
+    const int *hist;
+    int n_hist;
+    const int *draft;
+    const uint64_t *mask;
+    float repetition, frequency, presence;
+    const float *bias;
+    const uint32_t *allow;
+    int allow_stride;
+} dsv4_gpu_logit_rules;
+
+/* Apply the rules to nt <= DSV4_MAX_BATCH rows of f32 logits (row t at t *
+ * stride of both d_logits and d_out, stride >= vocab) and pick each row's
+ * token: dsv4_gpu_argmax_d's scan over the tokens that are allowed, -1 where
+ * none is. Each step is rounded in f32 in the order above. d_out may be
+ * d_logits, or NULL where only picks are wanted; d_pick may be NULL.
+ * d_scratch: dsv4_gpu_logits_scratch_bytes of device memory, 16-byte aligned,
+ * not kept. repetition must be over 0. 0 / -1. */
+size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab);
+int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, int nt, int vocab,
+                             long long stride, const dsv4_gpu_logit_rules *rules,
+                             void *d_scratch, size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
