@@ -1,13 +1,17 @@
 /* SPDX-License-Identifier: Apache-2.0 */
 /* dsv4_tree.hip - attention of a tree of drafted tokens over the latent cache
- * on gfx950.
+ * on gfx950: the plan, the join and the entry point (the kernel: dsv4_tree.h).
  *
- * o = sum_r e^(s_r - m) row_r[:d_v] / (sum_r e^(s_r - m) + e^(sink - m)) over
- * the rows r a token sees, s_r = scale q . row_r[:d_qk], in one pass over the
- * rows with the running maximum m and sum. One workgroup per (token, head).
+ * For a row of q (token, head) and the cache rows r that the token sees,
+ *   s_r = scale q . row_r[:d_qk],  o = sum e^(s_r - m) row_r[:d_v] / (sum e^(s_r
+ *   - m) + e^(sink - m)),
+ * in one pass over the cache with the running maximum m and sum. The rows of q
+ * of all tokens and heads read the same cache, so they are cut into blocks of
+ * 64 or 128 that share each tile of the cache; where the blocks do not fill
+ * the card the cache is cut into splits, whose sums k_tree_join adds with
+ * weights e^(m_split - m).
  */
-#include "dsv4_dev.h"
-#include "dsv4_internal.h"
+#include "dsv4_tree.h"
 
 #include <math.h>
 
@@ -15,129 +19,60 @@ namespace {
 
 #include "dsv4_rows_io.h"
 
-constexpr int TR_THREADS = 256;
-constexpr int TR_TILE = 64;
-constexpr int TR_DQK = 576, TR_DV = 512;
+constexpr int TJ_COLS = 64;                       /* columns of a workgroup  */
+constexpr int TJ_GROUPS = TR_THREADS / (TJ_COLS / 4);
 
-struct TreeJob {
-    void *o;
-    const void *q;
-    int nt, h, dqk, dv;
-    const void *kv;
-    const float *ks;
-    int stride, rows;
-    const int *pages;
-    int n_pages, page, ctx;
-    const uint64_t *mask;
-    int window;
-    const float *sink;
-    float scale;
-};
-
-__device__ __forceinline__ unsigned long long seen_drafts(const TreeJob &a, int t)
-{
-    if (a.mask) return a.mask[t];
-    return t >= 63 ? ~0ull : (2ull << t) - 1;
-}
-
-/* The drafts that token t sees beside itself: its depth. */
-__device__ __forceinline__ int depth_of(unsigned long long see, int t, int nt)
-{
-    if (nt < 64) see &= (1ull << nt) - 1;
-    return __popcll(see & ~(1ull << t));
-}
-
-/* Cache row of position p, or -1. */
-__device__ __forceinline__ long long cache_row(const TreeJob &a, int p)
-{
-    long long r = p;
-    if (a.pages) {
-        const int k = p / a.page;
-        if (k >= a.n_pages) return -1;
-        const int pg = a.pages[k];
-        if (pg < 0) return -1;
-        r = (long long)pg * a.page + (p - k * a.page);
-    }
-    return r < a.rows ? r : -1;
-}
-
-__device__ __forceinline__ float cache_at(const TreeJob &a, int fmt, long long row, int c)
-{
-    const size_t at = (size_t)row * a.stride + c;
-    if (fmt == DSV4_GPU_KV_F32) return ((const float *)a.kv)[at];
-    if (fmt == DSV4_GPU_KV_BF16)
-        return __uint_as_float((uint32_t)((const uint16_t *)a.kv)[at] << 16);
-    return dec_e4m3(((const uint8_t *)a.kv)[at]) * a.ks[row];
-}
-
+/* o of one row of q and 64 columns: thread (group of splits, 4 columns), the
+ * groups' sums added in order through LDS. */
 template <class T>
-__global__ void __launch_bounds__(TR_THREADS) k_tree(TreeJob a, int fmt)
+__global__ void __launch_bounds__(TR_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
 {
-    __shared__ float qs[TR_DQK], sc[TR_TILE];
-    __shared__ long long row[TR_TILE];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int t = blockIdx.x / a.h, hd = blockIdx.x - t * a.h;
-    for (int c = tid; c < a.dqk; c += TR_THREADS)
-        io_load<T, 1>((const T *)a.q + (size_t)blockIdx.x * a.dqk + c, qs + c);
-    const unsigned long long see = seen_drafts(a, t);
-    const int here = a.ctx + depth_of(see, t, a.nt);
-    const int lo = a.window ? max(0, here - a.window + 1) : 0;
-    float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-    const int n = a.ctx + a.nt;
-    for (int p0 = lo / TR_TILE * TR_TILE; p0 < n; p0 += TR_TILE) {
-        __syncthreads();
-        if (tid < TR_TILE) {
-            const int p = p0 + tid;
-            bool ok = p >= lo && p < n;
-            if (ok && p >= a.ctx) {
-                const int j = p - a.ctx;
-                ok = (see >> j) & 1;
-                if (ok && a.window)
-                    ok = here - (a.ctx + depth_of(seen_drafts(a, j), j, a.nt)) < a.window;
-            }
-            row[tid] = ok ? cache_row(a, p) : -1;
-        }
-        __syncthreads();
-        for (int k = w; k < TR_TILE; k += 4) {
-            const long long r = row[k];
-            float s = 0.0f;
-            if (r >= 0)
-                for (int c = lane; c < a.dqk; c += 64) s = fmaf(qs[c], cache_at(a, fmt, r, c), s);
-            s = wave_sum(s);
-            if (lane == 0) sc[k] = r >= 0 ? s * a.scale : -INFINITY;
-        }
-        __syncthreads();
-        float top = m;
-        for (int k = 0; k < TR_TILE; k++) top = fmaxf(top, sc[k]);
-        const float f = top == -INFINITY ? 0.0f : expf(m - top);
-        l *= f;
-        acc[0] *= f;
-        acc[1] *= f;
-        m = top;
-        /* the tile's own sums first: a chain as long as the context would lose
-         * bits where its terms are alike */
-        float tl = 0.0f, ta[2] = {0.0f, 0.0f};
-        for (int k = 0; k < TR_TILE; k++) {
-            if (row[k] < 0) continue;
-            const float e = m == -INFINITY && sc[k] == m ? 0.0f : expf(sc[k] - m);
-            tl += e;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int c = tid + i * TR_THREADS;
-                if (c < a.dv) ta[i] = fmaf(e, cache_at(a, fmt, row[k], c), ta[i]);
-            }
-        }
-        l += tl;
-        acc[0] += ta[0];
-        acc[1] += ta[1];
+    __shared__ float wt[1024];
+    __shared__ float red[TR_THREADS / 64];
+    __shared__ f32x4 sum[TJ_GROUPS][TJ_COLS / 4];
+    const int tid = threadIdx.x, r = blockIdx.x, R = a.nt * a.h;
+    float m = -INFINITY;
+    for (int s = tid; s < a.ns; s += TR_THREADS) m = fmaxf(m, a.pm[(size_t)s * R + r]);
+    m = wave_max(m);
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    m = red[0];
+    for (int k = 1; k < TR_THREADS / 64; k++) m = fmaxf(m, red[k]);
+    __syncthreads();
+    float l = 0.0f;
+    for (int s = tid; s < a.ns; s += TR_THREADS) {
+        const float ms = a.pm[(size_t)s * R + r], ls = a.pl[(size_t)s * R + r];
+        /* a split that saw nothing adds 0, whatever its maximum; NaN sums stay */
+        const float e = ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
+        wt[s] = e;
+        l += e * ls;
     }
-    if (l != 0.0f && a.sink) l += expf(a.sink[hd] - m);
+    l = wave_sum(l);
+    if ((tid & 63) == 0) red[tid >> 6] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int k = 0; k < TR_THREADS / 64; k++) l += red[k];
+    const int c4 = tid & (TJ_COLS / 4 - 1), gr = tid / (TJ_COLS / 4);
+    const int c = blockIdx.y * TJ_COLS + 4 * c4;
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (c < a.dvp)
+        for (int s = gr; s < a.ns; s += TJ_GROUPS)
+            v += wt[s] * ldf4(a.part + ((size_t)s * R + r) * a.dvp + c);
+    sum[gr][c4] = v;
+    __syncthreads();
+    if (gr != 0 || c >= a.dv) return;
+    for (int k = 1; k < TJ_GROUPS; k++) v += sum[k][c4];
+    if (a.sink && l != 0.0f)
+        l += __builtin_amdgcn_exp2f(a.sink[r % a.h] * 1.44269504088896340736f - m);
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    T *d = o + (size_t)r * a.dv + c;
+    if (a.ovec) {
+        io_store<T, 4>(d, y);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int c = tid + i * TR_THREADS;
-        const float v = acc[i] * inv;
-        if (c < a.dv) io_store<T, 1>((T *)a.o + (size_t)blockIdx.x * a.dv + c, &v);
+        for (int e = 0; e < 4; e++)
+            if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
     }
 }
 
@@ -155,13 +90,64 @@ const char *tree_bad(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int 
     return nullptr;
 }
 
+struct TreePlan {
+    int kc, tile0, tile1, nb, cap, ns, dvp;
+    size_t bytes;
+};
+
+/* The splits of a call: up to `cap`, two tiles each at least and 512 workgroups
+ * in all; of those the number whose last round of workgroups over the card's
+ * 256 CUs ends first, a workgroup taking its tiles and some eight tiles' time
+ * around them. */
+TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_ctx, int window)
+{
+    TreePlan p;
+    p.kc = dsv4_tree_chunks(d_qk, d_v);
+    const int lo = window && n_ctx >= window ? n_ctx - window + 1 : 0;
+    p.tile0 = lo / TR_TILE;
+    p.tile1 = (n_ctx + nt + TR_TILE - 1) / TR_TILE;
+    const int tiles = p.tile1 - p.tile0, br = dsv4_tree_block_rows(fmt, kv_fmt, p.kc);
+    p.nb = (nt * h + br - 1) / br;
+    p.dvp = (d_v + 15) / 16 * 16;
+    /* the workspace goes by the cap alone, and by the most tiles that a
+     * context of this length can have */
+    const int most = window ? (window + nt) / TR_TILE + 2 : tiles;
+    const int up = tiles < most ? tiles : most;
+    p.cap = up / 2 < 512 / p.nb ? up / 2 : 512 / p.nb;
+    if (p.cap < 1) p.cap = 1;
+    p.ns = 1;
+    long long best = -1;
+    for (int s = 1; s <= p.cap; s++) {
+        const long long rounds = ((long long)p.nb * s + 255) / 256;
+        const long long cost = rounds * ((tiles + s - 1) / s + 8);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p.ns = s;
+        }
+    }
+    p.bytes = p.cap > 1 ? (size_t)p.cap * nt * h * (p.dvp + 2) * sizeof(float) : 0;
+    return p;
+}
+
 } // namespace
+
+int dsv4_tree_chunks(int d_qk, int d_v)
+{
+    if (d_qk <= 128) return 4;
+    if (d_qk <= 256) return 8;
+    return d_qk <= 512 ? 16 : 18;
+}
+
+int dsv4_tree_block_rows(int fmt, int kv_fmt, int kc)
+{
+    return TR_WAVES * 16 * tree_qblocks(fmt, kv_fmt, kc);
+}
 
 extern "C" size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v,
                                                    int kv_fmt, int n_ctx, int window)
 {
-    if (tree_bad(fmt, nt, h, d_qk, d_v, kv_fmt, n_ctx, window)) return 0;
-    return 0;
+    if (nt == 0 || tree_bad(fmt, nt, h, d_qk, d_v, kv_fmt, n_ctx, window)) return 0;
+    return tree_plan(fmt, nt, h, d_qk, d_v, kv_fmt, n_ctx, window).bytes;
 }
 
 extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt, int h, int d_qk,
@@ -186,13 +172,60 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
         DSV4_ERR("tree_attn: a missing buffer");
         return -1;
     }
-    TreeJob a{d_o, d_q, nt, h, d_qk, d_v, d_kv, d_kv_scales, kv_stride, kv_rows, d_pages,
-              n_pages, page_rows, n_ctx, d_mask, window, d_sink, scale};
+    const TreePlan p = tree_plan(fmt, nt, h, d_qk, d_v, kv_fmt, n_ctx, window);
+    if (p.bytes && (!d_scratch || ((uintptr_t)d_scratch & 15) || scratch_bytes < p.bytes)) {
+        DSV4_ERR("tree_attn: %zu bytes of workspace at %p; the call needs %zu, 16-byte aligned",
+                 scratch_bytes, d_scratch, p.bytes);
+        return -1;
+    }
+    const IoDiv pd((uint32_t)(d_pages ? page_rows : 1));
+    const int es = fmt == DSV4_WBF16 ? 2 : 4;
+    /* pieces of eight cache elements: 8, 16 or 32 bytes, loaded 8 or 16 at a time */
+    const int ks = kv_fmt == DSV4_GPU_KV_F32 ? 4 : kv_fmt == DSV4_GPU_KV_BF16 ? 2 : 1;
+    const int al = ks == 1 ? 8 : 16;
+    Dsv4TreeJob a{};
+    a.o = d_o;
+    a.q = d_q;
+    a.nt = nt;
+    a.h = h;
+    a.dqk = d_qk;
+    a.dv = d_v;
+    a.kv = d_kv;
+    a.ks = d_kv_scales;
+    a.stride = kv_stride;
+    a.rows = kv_rows;
+    a.pages = d_pages;
+    a.n_pages = n_pages;
+    a.page = page_rows;
+    a.page_m = pd.m;
+    a.page_s = pd.s;
+    a.ctx = n_ctx;
+    a.mask = d_mask;
+    a.window = window;
+    a.sink = d_sink;
+    a.scale = scale;
+    a.tile0 = p.tile0;
+    a.tile1 = p.tile1;
+    a.ns = p.ns;
+    a.nb = p.nb;
+    a.dvp = p.dvp;
+    a.part = (float *)d_scratch;
+    a.pm = a.part + (size_t)p.ns * nt * h * p.dvp;
+    a.pl = a.pm + (size_t)p.ns * nt * h;
+    a.vec = d_qk % 8 == 0 && (long long)kv_stride * ks % al == 0 && (uintptr_t)d_kv % al == 0;
+    a.qvec = d_qk % 8 == 0 && ((uintptr_t)d_q & 15) == 0;
+    a.ovec = d_v % 4 == 0 && (uintptr_t)d_o % (4 * es) == 0;
     hipStream_t st = (hipStream_t)stream;
+    const int rc = kv_fmt == DSV4_GPU_KV_F32    ? dsv4_tree_f32_launch(a, fmt, p.kc, st)
+                 : kv_fmt == DSV4_GPU_KV_BF16 ? dsv4_tree_bf16_launch(a, fmt, p.kc, st)
+                                              : dsv4_tree_fp8_launch(a, fmt, p.kc, st);
+    if (rc != 0 || p.ns == 1) return rc;
+    const dim3 grid(nt * h, (d_v + TJ_COLS - 1) / TJ_COLS);
     if (fmt == DSV4_WF32)
-        hipLaunchKernelGGL(k_tree<float>, dim3(nt * h), dim3(TR_THREADS), 0, st, a, kv_fmt);
+        hipLaunchKernelGGL(k_tree_join<float>, grid, dim3(TR_THREADS), 0, st, a, (float *)d_o);
     else
-        hipLaunchKernelGGL(k_tree<uint16_t>, dim3(nt * h), dim3(TR_THREADS), 0, st, a, kv_fmt);
-    HIP_OK(hipGetLastError(), "tree attn launch");
+        hipLaunchKernelGGL(k_tree_join<uint16_t>, grid, dim3(TR_THREADS), 0, st, a,
+                           (uint16_t *)d_o);
+    HIP_OK(hipGetLastError(), "tree attn join launch");
     return 0;
 }

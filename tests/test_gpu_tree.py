@@ -241,3 +241,17 @@ def test_the_same_bits_again_and_the_workspace(gpu, dsv4):
         space = torch.zeros(need - 1, device="cuda:0", dtype=torch.uint8)
         assert dc.tree(dsv4, dq, False, cache, ks, 1, rows, dqk, dv, ctx, scale=0.04,
                        space=space)[0] == -1
+
+
+@pytest.mark.parametrize("fmt,bf", [(0, False), (1, False), (2, True)])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_scales_of_zero_and_below(gpu, dsv4, fmt, bf, scale):
+    """A scale of 0 averages the visible rows; a negative one turns the order."""
+    nt, h, dqk, dv, ctx = 5, 4, 64, 64, 70
+    rng, dq, q, v, cache, ks, rows, _ = problem(9, nt, h, dqk, ctx, fmt, bf)
+    w = dc.words(rng, nt)
+    rc, o = dc.tree(dsv4, dq, bf, cache, ks, fmt, rows, dqk, dv, ctx,
+                    dc.dev(np.array(w, np.uint64)), 20, scale=scale)
+    assert rc == 0
+    want, size = dc.attention(q, v, dc.visible(w, nt, ctx, 20), None, scale, dv)
+    check(dc.host(o), want, size, bf)
