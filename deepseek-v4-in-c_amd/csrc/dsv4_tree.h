@@ -7,8 +7,6 @@
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
 
-constexpr int TR_THREADS = 256;
-constexpr int TR_WAVES = TR_THREADS / 64;
 constexpr int TR_TILE = 32;                       /* cache rows of a step    */
 constexpr int TR_DQK = 576, TR_DV = 512;
 
@@ -47,12 +45,11 @@ constexpr int TR_TERMS = 3;
 constexpr int tree_terms(int fmt) { return fmt == DSV4_WF32 ? TR_TERMS : 1; }
 constexpr int tree_planes(int kv_fmt) { return kv_fmt == DSV4_GPU_KV_F32 ? TR_TERMS : 1; }
 constexpr int tree_vtiles(int kc) { return kc >= 16 ? 32 : 2 * kc; }
-/* Blocks of 16 rows of q per wave. A wave reads every row of a tile from LDS
- * for each of its blocks' products: with one term of q two blocks share the
- * read, with three the terms do. */
-constexpr int tree_qblocks(int fmt, int kv_fmt, int kc)
+/* Waves of a workgroup, 16 rows of q each: eight, two per SIMD, where a wave's
+ * part of q and its sums fit half the registers. */
+constexpr int tree_waves(int fmt, int kv_fmt, int kc)
 {
-    return tree_terms(fmt) * tree_planes(kv_fmt) == 1 && kc <= 4 ? 2 : 1;
+    return kc >= 16 && tree_terms(fmt) * tree_planes(kv_fmt) > 1 ? 4 : 8;
 }
 
 #ifdef DSV4_TREE_KERNEL
@@ -95,21 +92,45 @@ __device__ __forceinline__ f32x4 tr_mfma(tr_bf8 a, tr_bf8 b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-/* LDS of a workgroup: NBUF tiles of [planes][TR_TILE][pitch] bytes, then per
- * buffer the rows' scales and two words of row bits. */
+/* LDS of a workgroup: NBUF tiles of [planes][slabs of 64 columns][TR_TILE][128
+ * bytes], then per buffer the rows' places in the cache, their scales and
+ * whether they may not be used. Piece p (16 bytes) of a slab's row r is at p ^
+ * f(r), f 0, 2, 4, 6, 1, 3, 5, 7 for r % 8: the reads of the scores (one piece
+ * of 16 rows) and of the values (two pieces of four rows) then spread over all
+ * banks. */
 template <int KVF, int KC>
 struct TreeLds {
     static constexpr int KT = tree_planes(KVF);
-    static constexpr int PITCH = KC * 64 + 16;        /* + 16: spreads the banks */
-    static constexpr int PLANE = TR_TILE * PITCH;
-    static constexpr int NBUF = KT == 1 ? 2 : 1;
+    static constexpr int SLABS = KC / 2;
+    static constexpr int SLAB = TR_TILE * 128;
+    static constexpr int PLANE = SLABS * SLAB;
+    static constexpr int NBUF = KT > 1 ? 1 : KVF == DSV4_GPU_KV_BF16 ? 3 : 2;
     static constexpr int META = NBUF * KT * PLANE;
-    static constexpr int MSIZE = TR_TILE * 4 + 16;
+    static constexpr int MSIZE = 3 * TR_TILE * 4;
     static constexpr int BYTES = META + NBUF * MSIZE;
 };
 
-/* Workgroup (split, block of q's rows): wave w holds 16 QB rows of q as the
- * B operands of S^T = K Q^T (a row of q per column), in bf16 terms.
+__device__ __forceinline__ int tr_swz(int r) { return (r & 3) << 1 | (r >> 2 & 1); }
+
+typedef __attribute__((address_space(3))) void tr_lds_void;
+
+template <int N>
+__device__ __forceinline__ void tr_vm_wait()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+/* Every wave's LDS reads and writes so far are done; loads stay in flight. */
+__device__ __forceinline__ void tr_sync()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+template <class T>
+constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
+
+/* Workgroup (split, block of q's rows): wave w holds 16 rows of q as the B
+ * operands of S^T = K Q^T (a row of q per column), in bf16 terms.
  *
  * Per tile of 32 cache rows: S^T for two tiles of 16 keys; a lane then has
  * eight scores of its own column's row of q, which become that column's
@@ -121,25 +142,30 @@ struct TreeLds {
  * maximum follows only when it grows by 2^8, as the weights may be that much
  * over 1 without loss.
  *
- * The next tile's rows are loaded into registers while this one is used. A
- * tile with drafts, a window's edge or rows outside the cache is masked by a
- * word of 32 bits per row of q; in such a tile a cache row that holds NaN or
- * infinity is stored as zeros, which a weight of 0 leaves at 0, and gives NaN
- * scores to the rows of q that see it. */
+ * Tiles of a bf16 cache go to LDS by global_load_lds_dwordx4, two tiles ahead
+ * and through no register; the other formats' next tile is loaded into
+ * registers while this one is used. Operands are read from LDS a group ahead
+ * of the matrix core.
+ *
+ * A tile with drafts, a window's edge or rows outside the cache is masked by a
+ * word of 32 bits per row of q; its cache rows that hold NaN or infinity, or
+ * are not there, become zeros in LDS first, which a weight of 0 leaves at 0,
+ * and the former give NaN scores to the rows of q that see them. */
 template <class T, int KVF, int KC>
-__global__ void __launch_bounds__(TR_THREADS, KC >= 16 ? 1 : 2)
+__global__ void __launch_bounds__(64 * tree_waves(tr_fmt<T>(), KVF, KC),
+                                  tree_waves(tr_fmt<T>(), KVF, KC) / 4)
 k_tree(Dsv4TreeJob a)
 {
     using L = TreeLds<KVF, KC>;
-    constexpr int FMT = sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32;
-    constexpr int NT = tree_terms(FMT), KT = L::KT, NV = tree_vtiles(KC);
-    constexpr int QB = tree_qblocks(FMT, KVF, KC);
-    constexpr int NP = KC / 2;                         /* pieces of 8 per thread */
+    constexpr int NT = tree_terms(tr_fmt<T>()), KT = L::KT, NV = tree_vtiles(KC);
     constexpr int PT = NT > KT ? NT : KT;              /* term pairs i + j < PT  */
-    constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : KVF == DSV4_GPU_KV_BF16 ? 4 : 2;
+    constexpr int W = tree_waves(tr_fmt<T>(), KVF, KC), WS = W / 4;
+    constexpr int NP = (L::SLABS + WS - 1) / WS;       /* pieces of 8 per thread */
+    constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : 2;
+    constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int l16 = lane & 15, g = lane >> 4;
 
     /* Workgroup i runs on XCD i mod 8: each XCD takes a run of (split, block)
@@ -156,32 +182,29 @@ k_tree(Dsv4TreeJob a)
     const int i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
     const int R = a.nt * a.h;
 
-    /* this lane's rows of q: their tokens' drafts and first positions */
-    int rq[QB], lo[QB];
-    unsigned long long see[QB];
-    tr_bf8 q[QB][NT][KC];
-#pragma unroll
-    for (int b = 0; b < QB; b++) {
-        rq[b] = ((blk * TR_WAVES + w) * QB + b) * 16 + l16;
-        const int r = min(rq[b], R - 1), t = r / a.h;
+    /* this lane's row of q: its token's drafts and first position */
+    const int rq = (blk * W + w) * 16 + l16;
+    int lo;
+    unsigned long long see;
+    {
+        const int t = min(rq, R - 1) / a.h;
         const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
-        const unsigned long long own = a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1);
-        const int depth = __popcll(own & all & ~(1ull << t));
-        see[b] = own & all;
-        lo[b] = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
+        see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
+        const int depth = __popcll(see & ~(1ull << t));
+        lo = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
         if (a.window && a.window < a.nt)
             for (int j = 0; j < a.nt; j++) {
                 const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
-                if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see[b] &= ~(1ull << j);
+                if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
             }
     }
     /* elements past the row are zeroed by a mask in a register: the many lane
      * masks of comparisons would crowd out the scalar registers */
+    tr_bf8 q[NT][KC];
+    {
+        const T *qr = (const T *)a.q + (size_t)min(rq, R - 1) * a.dqk;
 #pragma unroll
-    for (int kc = 0; kc < KC; kc++)
-#pragma unroll
-        for (int b = 0; b < QB; b++) {
-            const T *qr = (const T *)a.q + (size_t)min(rq[b], R - 1) * a.dqk;
+        for (int kc = 0; kc < KC; kc++) {
             const int c = 32 * kc + 8 * g;
             float v[8];
             if (a.qvec) {
@@ -196,351 +219,407 @@ k_tree(Dsv4TreeJob a)
             tr_bf8 tm[NT];
             tr_terms<NT>(v, tm);
 #pragma unroll
-            for (int n = 0; n < NT; n++) q[b][n][kc] = tm[n];
-            __builtin_amdgcn_sched_barrier(0);     /* few of q's loads at a time */
+            for (int n = 0; n < NT; n++) q[n][kc] = tm[n];
+            __builtin_amdgcn_sched_barrier(0);         /* few of q's loads at a time */
         }
-    f32x4 o[QB][NV];
-    float m[QB], l[QB];
-#pragma unroll
-    for (int b = 0; b < QB; b++) {
-        m[b] = -INFINITY;
-        l[b] = 0.0f;
-#pragma unroll
-        for (int v = 0; v < NV; v++) o[b][v] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    f32x4 o[NV];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    /* ---- staging: thread tid has row tid / 8 of a tile and its pieces tid % 8
-     *      + 8 i ---- */
-    const int sr = tid >> 3, sp = tid & 7;
+    /* ---- staging: a thread has place sp of row sr of slabs ws, ws + WS, ... of a
+     *      tile: piece sp ^ f(sr) of 64 columns. Pieces past the cache row
+     *      repeat its last one: q is zero there. ---- */
+    const int sr = 8 * (w & 3) + (lane >> 3), ws = w >> 2;
+    const int pc = 8 * ((lane & 7) ^ tr_swz(sr));      /* the piece's first column */
+    const int home = sr * 128 + 16 * (lane & 7);
+    const bool speaks = (lane & 7) == 0 && ws == 0;
     const int end = a.ctx + a.nt;
-    /* the cache row of tile i's row, -1 where there is none */
+    /* the cache row of tile i's row sr, -1 where there is none */
     auto find = [&](int i) -> int {
         const int p = i * TR_TILE + sr;
         if (p >= end || i >= i1) return -1;
         if (!a.pages) return p < a.rows ? p : -1;
         const int k = (int)((__umulhi(a.page_m, (uint32_t)p) + (uint32_t)p) >> a.page_s);
         if (k >= a.n_pages) return -1;
-        const long long r = (long long)a.pages[k] * a.page + (p - k * a.page);
-        return r >= 0 && r < a.rows ? (int)r : -1;
-    };
-    /* Pieces past the row repeat its last one: q is zero there. */
-    uint32_t raw[NP][RAW];
-    float rks = 1.0f;
-    auto fetch = [&](int row) {
-        const size_t at = (size_t)max(row, 0) * a.stride;
-        if (KVF == DSV4_GPU_KV_FP8) rks = a.ks[max(row, 0)];
-        if (!a.vec) return;
-        constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : KVF == DSV4_GPU_KV_BF16 ? 2 : 1;
-        const unsigned char *p = (const unsigned char *)a.kv + at * ES;
-#pragma unroll
-        for (int i = 0; i < NP; i++) {
-            const int c = min(8 * (sp + 8 * i), a.dqk - 8);
-            if constexpr (ES == 1) {
-                const uint2 v = *(const uint2 *)(p + c);
-                raw[i][0] = v.x;
-                raw[i][1] = v.y;
-            } else {
-#pragma unroll
-                for (int k = 0; k < RAW; k += 4) {
-                    const u32x4 v = ld16(p + c * ES + 4 * k);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) raw[i][k + e] = v[e];
-                }
-            }
-        }
-    };
-    /* the same for one piece of a row that is not in whole pieces */
-    auto fetch1 = [&](int row, int i, uint32_t *r) {
-        const size_t at = (size_t)max(row, 0) * a.stride;
-#pragma unroll
-        for (int k = 0; k < RAW; k++) r[k] = 0u;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const size_t c = at + min(8 * (sp + 8 * i) + e, a.dqk - 1);
-            if constexpr (KVF == DSV4_GPU_KV_F32) r[e] = ((const uint32_t *)a.kv)[c];
-            else if constexpr (KVF == DSV4_GPU_KV_BF16)
-                r[e / 2] |= (uint32_t)((const uint16_t *)a.kv)[c] << (16 * (e & 1));
-            else r[e / 4] |= (uint32_t)((const uint8_t *)a.kv)[c] << (8 * (e & 3));
-        }
-    };
-    auto wild = [&](const uint32_t *r) {
-        bool bad = false;
-#pragma unroll
-        for (int k = 0; k < RAW; k++) {
-            if constexpr (KVF == DSV4_GPU_KV_F32) {
-                bad |= (r[k] & 0x7F800000u) == 0x7F800000u;
-            } else if constexpr (KVF == DSV4_GPU_KV_BF16) {
-                bad |= (r[k] & 0x7F80u) == 0x7F80u || (r[k] & 0x7F800000u) == 0x7F800000u;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) bad |= (r[k] >> e & 0x7Fu) == 0x7Fu;
-            }
-        }
-        return bad;
-    };
-    auto put = [&](unsigned char *d, const uint32_t *r, bool zero) {
-        if constexpr (KVF == DSV4_GPU_KV_F32) {
-            float v[8];
-            tr_bf8 tm[KT];
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = zero ? 0.0f : __uint_as_float(r[e]);
-            tr_terms<KT>(v, tm);
-#pragma unroll
-            for (int n = 0; n < KT; n++) *(tr_bf8 *)(d + n * L::PLANE) = tm[n];
-        } else {
-            u32x4 v;
-            if constexpr (KVF == DSV4_GPU_KV_BF16) {
-                v = u32x4{r[0], r[1], r[2], r[3]};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    v[2 * e] = __builtin_bit_cast(uint32_t,
-                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[e], 1.0f, false));
-                    v[2 * e + 1] = __builtin_bit_cast(uint32_t,
-                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[e], 1.0f, true));
-                }
-            }
-            *(u32x4 *)d = zero ? u32x4{0u, 0u, 0u, 0u} : v;
-        }
+        const long long c = (long long)a.pages[k] * a.page + (p - k * a.page);
+        return c >= 0 && c < a.rows ? (int)c : -1;
     };
     /* some row of q may not see some row of tile i */
     auto partial = [&](int i) {
         return (i + 1) * TR_TILE > a.ctx ||
                (a.window && i * TR_TILE < a.ctx + a.nt - a.window);
     };
-    auto store = [&](int i, int row, int buf) {
-        unsigned char *t = lds + (size_t)buf * KT * L::PLANE + sr * L::PITCH;
-        bool bad = false;
-        if (partial(i)) {
-            if (a.vec) {
+    auto meta = [&](int buf) { return lds + L::META + buf * L::MSIZE; };
+    auto plane = [&](int buf) { return lds + buf * KT * L::PLANE; };
+    /* one piece of a row that does not lie in whole pieces */
+    auto piece1 = [&](int row, int slab, uint32_t *r) {
+        const size_t at = (size_t)max(row, 0) * a.stride;
 #pragma unroll
-                for (int k = 0; k < NP; k++) bad |= wild(raw[k]);
-            } else {
-#pragma unroll 1
-                for (int k = 0; k < NP; k++) {
-                    uint32_t r[RAW];
-                    fetch1(row, k, r);
-                    bad |= wild(r);
-                }
-            }
-            if (KVF == DSV4_GPU_KV_FP8)
-                bad |= (__float_as_uint(rks) & 0x7F800000u) == 0x7F800000u;
+        for (int e = 0; e < 8; e++) {
+            const size_t c = at + min(64 * slab + pc + e, a.dqk - 1);
+            if constexpr (KVF == DSV4_GPU_KV_F32) r[e] = ((const uint32_t *)a.kv)[c];
+            else if constexpr (DMA)
+                r[e / 2] = (e & 1 ? r[e / 2] : 0u) | (uint32_t)((const uint16_t *)a.kv)[c]
+                                                         << (16 * (e & 1));
+            else r[e / 4] = (e & 3 ? r[e / 4] : 0u) | (uint32_t)((const uint8_t *)a.kv)[c]
+                                                          << (8 * (e & 3));
         }
-        /* the eight threads of a row, rows 8 w .. 8 w + 7 of the tile */
-        const unsigned long long vb = __ballot(bad), vr = __ballot(row >= 0);
-        bad = (vb >> (lane & 56) & 0xFFull) != 0;
-        unsigned char *meta = lds + L::META + buf * L::MSIZE;
-        if (lane == 0) {
-            uint32_t ok = 0, no = 0;
+    };
+    auto put = [&](unsigned char *d, const uint32_t *r) {
+        if constexpr (KVF == DSV4_GPU_KV_F32) {
+            float v[8];
+            tr_bf8 tm[KT];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                ok |= (uint32_t)(vr >> (8 * k) & 1) << k;
-                no |= (uint32_t)((vb >> (8 * k) & 0xFFull) != 0) << k;
-            }
-            meta[TR_TILE * 4 + w] = (unsigned char)ok;
-            meta[TR_TILE * 4 + 4 + w] = (unsigned char)(no & ok);
-        }
-        if (KVF == DSV4_GPU_KV_FP8 && sp == 0) ((float *)meta)[sr] = bad || row < 0 ? 0.0f : rks;
-        const bool zero = bad || row < 0;
-        if (a.vec) {
+            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(r[e]);
+            tr_terms<KT>(v, tm);
 #pragma unroll
-            for (int k = 0; k < NP; k++) put(t + 16 * (sp + 8 * k), raw[k], zero);
+            for (int n = 0; n < KT; n++) *(tr_bf8 *)(d + n * L::PLANE) = tm[n];
+        } else if constexpr (DMA) {
+            *(u32x4 *)d = u32x4{r[0], r[1], r[2], r[3]};
         } else {
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                v[2 * e] = __builtin_bit_cast(uint32_t,
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[e], 1.0f, false));
+                v[2 * e + 1] = __builtin_bit_cast(uint32_t,
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[e], 1.0f, true));
+            }
+            *(u32x4 *)d = v;
+        }
+    };
+    /* rows not in whole pieces go to LDS at once, without a tile's time between */
+    auto crawl = [&](int row, int buf) {
 #pragma unroll 1
-            for (int k = 0; k < NP; k++) {
-                uint32_t r[RAW];
-                fetch1(row, k, r);
-                put(t + 16 * (sp + 8 * k), r, zero);
+        for (int s = ws; s < L::SLABS; s += WS) {
+            uint32_t r[8];
+            piece1(row, s, r);
+            put(plane(buf) + s * L::SLAB + home, r);
+        }
+    };
+    auto name = [&](int row, int buf, float ks) {
+        if (!speaks) return;
+        ((int *)meta(buf))[sr] = row;
+        if (KVF == DSV4_GPU_KV_FP8) ((float *)meta(buf))[TR_TILE + sr] = row >= 0 ? ks : 0.0f;
+    };
+    /* the bf16 cache: into LDS directly */
+    auto dma = [&](int row, int buf) {
+        name(row, buf, 1.0f);
+        if (!a.vec) {
+            crawl(row, buf);
+            return;
+        }
+        const uint16_t *p = (const uint16_t *)a.kv + (size_t)max(row, 0) * a.stride;
+        unsigned char *d = plane(buf) + 1024 * (w & 3);
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int s = ws + WS * k;
+            if (L::SLABS % WS == 0 || s < L::SLABS)
+                __builtin_amdgcn_global_load_lds(
+                    (const void *)(p + min(64 * s + pc, a.dqk - 8)),
+                    (tr_lds_void *)(d + s * L::SLAB), 16, 0, 0);
+        }
+    };
+    /* this wave's loads but those of the newest tile are done */
+    auto dma_wait = [&](bool newest) {
+        if (!newest) tr_vm_wait<0>();
+        else if (L::SLABS % WS == 0 || ws == 0) tr_vm_wait<NP>();
+        else tr_vm_wait<NP - 1>();
+    };
+    /* the other formats: through registers */
+    uint32_t raw[NP][RAW];
+    float rks = 1.0f;
+    auto fetch = [&](int row) {
+        if (KVF == DSV4_GPU_KV_FP8) rks = a.ks[max(row, 0)];
+        if (!a.vec) return;
+        constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : 1;
+        const unsigned char *p = (const unsigned char *)a.kv + (size_t)max(row, 0) * a.stride * ES;
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int c = min(64 * (ws + WS * k) + pc, a.dqk - 8);
+            if constexpr (ES == 1) {
+                const uint2 v = *(const uint2 *)(p + c);
+                raw[k][0] = v.x;
+                raw[k][1] = v.y;
+            } else {
+#pragma unroll
+                for (int h = 0; h < 8; h += 4) {
+                    const u32x4 v = ld16(p + 4 * (c + h));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) raw[k][h + e] = v[e];
+                }
             }
         }
     };
+    auto store = [&](int row, int buf) {
+        name(row, buf, rks);
+        if (!a.vec) {
+            crawl(row, buf);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int s = ws + WS * k;
+            if (L::SLABS % WS == 0 || s < L::SLABS) put(plane(buf) + s * L::SLAB + home, raw[k]);
+        }
+    };
+    /* a masked tile's rows that are not there or hold what is not finite (in the
+     * first plane, which has f32's infinities and NaN too) to zeros; the
+     * eight threads of a row are lanes 8 k .. 8 k + 7, of one wave or of two */
+    auto mend = [&](int buf) {
+        int *mi = (int *)meta(buf);
+        bool bad = false;
+        /* (every thread looks at all slabs, so that both waves agree) */
+#pragma unroll 1
+        for (int s = 0; s < L::SLABS; s++) {
+            const u32x4 v = *(const u32x4 *)(plane(buf) + s * L::SLAB + home);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                bad |= (v[e] & 0x7F80u) == 0x7F80u || (v[e] & 0x7F800000u) == 0x7F800000u;
+        }
+        const int row = mi[sr];
+        if (KVF == DSV4_GPU_KV_FP8)
+            bad |= (((const uint32_t *)mi)[TR_TILE + sr] & 0x7F800000u) == 0x7F800000u;
+        bad = (__ballot(bad) >> (lane & 56) & 0xFFull) != 0;
+        tr_sync();                                     /* all have looked        */
+        if (speaks) {
+            mi[2 * TR_TILE + sr] = bad && row >= 0;
+            if (KVF == DSV4_GPU_KV_FP8 && bad) ((float *)mi)[TR_TILE + sr] = 0.0f;
+        }
+        if (bad || row < 0)
+            for (int s = ws; s < L::SLABS; s += WS)
+                for (int n = 0; n < KT; n++)
+                    *(u32x4 *)(plane(buf) + n * L::PLANE + s * L::SLAB + home) =
+                        u32x4{0u, 0u, 0u, 0u};
+        tr_sync();
+    };
 
     const float c2 = a.scale * 1.44269504088896340736f;       /* to powers of two */
+    /* a lane's places in a slab: row l16's piece g for the scores (the other
+     * half of a slab at ^ 64), row 4 g + l16 / 4's four columns 4 (l16 % 4) for
+     * the values (the slab's other column tiles at ^ 32, 64 and 96) */
+    const int ka = l16 * 128 + 16 * (g ^ tr_swz(l16));
+    const int va = (4 * g + (l16 >> 2)) * 128 + 8 * (l16 & 1) +
+                   16 * ((l16 >> 1 & 1) ^ tr_swz(4 * g + (l16 >> 2)));
     auto use = [&](int i, int buf) {
-        const unsigned char *t = lds + (size_t)buf * KT * L::PLANE;
-        const unsigned char *meta = lds + L::META + buf * L::MSIZE;
-        /* one sum per order of the terms: the small ones do not round at the
-         * size of the large */
-        f32x4 s[QB][2], so[QB][2][PT];
+        const unsigned char *t = plane(buf);
+        const int *mi = (const int *)meta(buf);
+        const uint32_t ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
+        const bool masked = partial(i) || ok != 0xFFFFFFFFu;
+        if (masked) mend(buf);
+
+        /* ---- S^T: one sum per order of the terms, so that the small ones do
+         *      not round at the size of the large ---- */
+        f32x4 so[2][PT], s[2];
 #pragma unroll
-        for (int b = 0; b < QB; b++)
+        for (int n = 0; n < PT; n++) so[0][n] = so[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int KG = KT > 1 || W == 8 ? 1 : 2;
+        tr_bf8 row[2][KG][KT][2];
+        auto rows_of = [&](int kg, tr_bf8 (&r)[KG][KT][2]) {
 #pragma unroll
-            for (int n = 0; n < PT; n++) so[b][0][n] = so[b][1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < KG; u++)
 #pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
+                for (int p = 0; p < KT; p++)
 #pragma unroll
-            for (int p = 0; p < KT; p++)
+                    for (int k = 0; k < 2; k++) {
+                        const int kc = kg * KG + u;
+                        r[u][p][k] = *(const tr_bf8 *)(t + p * L::PLANE + (kc >> 1) * L::SLAB +
+                                                       k * 2048 + (ka ^ (kc & 1) * 64));
+                    }
+        };
+        rows_of(0, row[0]);
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const tr_bf8 row = *(const tr_bf8 *)(t + p * L::PLANE +
-                                                         (16 * k + l16) * L::PITCH + 64 * kc +
-                                                         16 * g);
+        for (int kg = 0; kg < KC / KG; kg++) {
+            if (kg + 1 < KC / KG) rows_of(kg + 1, row[(kg + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < KG; u++)
+#pragma unroll
+                for (int p = 0; p < KT; p++)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
                         if (n + p < PT)
 #pragma unroll
-                            for (int b = 0; b < QB; b++)
-                                so[b][k][n + p] = tr_mfma(row, q[b][n][kc], so[b][k][n + p]);
-                }
+                            for (int k = 0; k < 2; k++)
+                                so[k][n + p] = tr_mfma(row[kg & 1][u][p][k], q[n][kg * KG + u],
+                                                       so[k][n + p]);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int b = 0; b < QB; b++)
+        for (int k = 0; k < 2; k++) {
+            s[k] = so[k][PT - 1];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                s[b][k] = so[b][k][PT - 1];
-#pragma unroll
-                for (int n = PT - 2; n >= 0; n--) s[b][k] += so[b][k][n];
-            }
-        const uint32_t ok = *(const uint32_t *)(meta + TR_TILE * 4);
-        const bool masked = partial(i) || ok != 0xFFFFFFFFu;
+            for (int n = PT - 2; n >= 0; n--) s[k] += so[k][n];
+        }
+
+        /* ---- the weights ---- */
         f32x4 ks[2];
         if (KVF == DSV4_GPU_KV_FP8) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                ks[k] = *(const f32x4 *)(meta + 4 * (16 * k + 4 * g));
-#pragma unroll
-                for (int b = 0; b < QB; b++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[b][k][j] *= ks[k][j];
+                ks[k] = *(const f32x4 *)(mi + TR_TILE + 16 * k + 4 * g);
+                s[k] *= ks[k];
             }
         }
-        uint32_t vis[QB];
-#pragma unroll
-        for (int b = 0; b < QB; b++) vis[b] = ~0u;
+        uint32_t vis = ~0u;
         if (masked) {
-            const uint32_t no = *(const uint32_t *)(meta + TR_TILE * 4 + 4);
+            const uint32_t no = (uint32_t)__ballot(mi[2 * TR_TILE + (lane & 31)] != 0);
             const int p0 = i * TR_TILE;
-#pragma unroll
-            for (int b = 0; b < QB; b++) {
-                /* positions [lo, ctx) of the context, then the drafts' bits */
-                vis[b] = 0u;
-                const int f = max(lo[b] - p0, 0), e = min(a.ctx - p0, TR_TILE);
-                if (f < e) vis[b] = (e >= 32 ? ~0u : (1u << e) - 1u) & ~((1u << f) - 1u);
-                const int d = p0 - a.ctx;
-                if (d > -TR_TILE && d < 64)
-                    vis[b] |= d >= 0 ? (uint32_t)(see[b] >> d) : (uint32_t)(see[b] << -d);
-                vis[b] &= ok;
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (no >> (16 * k + 4 * g + j) & 1u)
-                            s[b][k][j] = __uint_as_float(0x7FC00000u);
-            }
-        }
-        tr_bf8 pw[QB][PT];
-#pragma unroll
-        for (int b = 0; b < QB; b++) {
-            float top = -INFINITY;
+            /* positions [lo, ctx) of the context, then the drafts' bits */
+            vis = 0u;
+            const int f = max(lo - p0, 0), e = min(a.ctx - p0, TR_TILE);
+            if (f < e) vis = (e >= 32 ? ~0u : (1u << e) - 1u) & ~((1u << f) - 1u);
+            const int d = p0 - a.ctx;
+            if (d > -TR_TILE && d < 64) vis |= d >= 0 ? (uint32_t)(see >> d) : (uint32_t)(see << -d);
+            vis &= ok;
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float x = s[b][k][j] * c2;
-                    if (masked) x = vis[b] >> (16 * k + 4 * g + j) & 1u ? x : -INFINITY;
-                    top = fmaxf(top, x);
-                }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const bool grow = top > m[b] + 8.0f;
-            if (__any(grow)) {
-                const float f = grow ? __builtin_amdgcn_exp2f(m[b] - top) : 1.0f;
-                m[b] = grow ? top : m[b];
-                l[b] *= f;
-#pragma unroll
-                for (int v = 0; v < NV; v++) o[b][v] *= f;
-            }
-            const float mm = m[b] == -INFINITY ? 0.0f : m[b];
-            float e[8], sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float x = __builtin_amdgcn_exp2f(fmaf(s[b][k][j], c2, -mm));
-                    if (masked) x = vis[b] >> (16 * k + 4 * g + j) & 1u ? x : 0.0f;
-                    sum += x;
-                    e[4 * k + j] = KVF == DSV4_GPU_KV_FP8 ? x * ks[k][j] : x;
-                }
-            l[b] += sum;
-            tr_terms<NT>(e, pw[b]);
+                for (int j = 0; j < 4; j++)
+                    if (no >> (16 * k + 4 * g + j) & 1u) s[k][j] = __uint_as_float(0x7FC00000u);
+            vis >>= 4 * g;
         }
+        float top = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int p = 0; p < KT; p++) {
-                const unsigned char *at = t + p * L::PLANE + (4 * g + (l16 >> 2)) * L::PITCH +
-                                          2 * (16 * v + 4 * (l16 & 3));
-                const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
-                const tr_s4 y =
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 16 * L::PITCH));
-                const tr_bf8 col = __builtin_bit_cast(
-                    tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int j = 0; j < 4; j++) {
+                float x = s[k][j] * c2;
+                if (masked) x = vis >> (16 * k + j) & 1u ? x : -INFINITY;
+                top = fmaxf(top, x);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const bool grow = top > m + 8.0f;
+        if (__any(grow)) {
+            const float f = grow ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = grow ? top : m;
+            l *= f;
+#pragma unroll
+            for (int v = 0; v < NV; v++) o[v] *= f;
+        }
+        const float mm = m == -INFINITY ? 0.0f : m;
+        float e[8], sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x = __builtin_amdgcn_exp2f(fmaf(s[k][j], c2, -mm));
+                if (masked) x = vis >> (16 * k + j) & 1u ? x : 0.0f;
+                sum += x;
+                e[4 * k + j] = KVF == DSV4_GPU_KV_FP8 ? x * ks[k][j] : x;
+            }
+        l += sum;
+        tr_bf8 pw[NT];
+        tr_terms<NT>(e, pw);
+
+        /* ---- O^T ---- */
+        constexpr int VG = KT > 1 ? 1 : W == 8 ? 2 : 4;
+        tr_bf8 col[2][VG][KT];
+        auto cols_of = [&](int vg, tr_bf8 (&c)[VG][KT]) {
+#pragma unroll
+            for (int u = 0; u < VG; u++)
+#pragma unroll
+                for (int p = 0; p < KT; p++) {
+                    const int v = vg * VG + u;
+                    const unsigned char *at =
+                        t + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
+                    const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
+                    const tr_s4 y =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
+                    c[u][p] = __builtin_bit_cast(
+                        tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+        };
+        cols_of(0, col[0]);
+#pragma unroll
+        for (int vg = 0; vg < NV / VG; vg++) {
+            if (vg + 1 < NV / VG) cols_of(vg + 1, col[(vg + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < KT; p++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
                     if (n + p < PT)
 #pragma unroll
-                        for (int b = 0; b < QB; b++) o[b][v] = tr_mfma(col, pw[b][n], o[b][v]);
-            }
+                        for (int u = 0; u < VG; u++)
+                            o[vg * VG + u] = tr_mfma(col[vg & 1][u][p], pw[n], o[vg * VG + u]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     if (i0 < i1) {
-        int row = find(i0), next = find(i0 + 1);
-        fetch(row);
-        store(i0, row, 0);
-        __syncthreads();
-        for (int i = i0; i < i1; i++) {
-            const int buf = L::NBUF == 2 ? (i - i0) & 1 : 0;
-            const bool more = i + 1 < i1;
-            row = next;
-            if (more) {
-                fetch(row);
-                next = find(i + 2);
+        if constexpr (DMA) {
+            int r2 = find(i0 + 2);
+            dma(find(i0), 0);
+            if (i0 + 1 < i1) dma(find(i0 + 1), 1);
+            int buf = 0;
+            for (int i = i0; i < i1; i++) {
+                dma_wait(i + 1 < i1);
+                tr_sync();               /* tile i is in LDS, tile i - 1's buffer free */
+                if (i + 2 < i1) {
+                    const int row = r2;
+                    r2 = find(i + 3);
+                    dma(row, buf == 0 ? 2 : buf - 1);
+                }
+                use(i, buf);
+                buf = buf == 2 ? 0 : buf + 1;
             }
-            use(i, buf);
-            if (more) {
-                if (L::NBUF == 1) __syncthreads();
-                store(i + 1, row, L::NBUF == 2 ? buf ^ 1 : 0);
-                __syncthreads();
+        } else {
+            int row = find(i0), next = find(i0 + 1);
+            fetch(row);
+            store(row, 0);
+            for (int i = i0; i < i1; i++) {
+                const int buf = L::NBUF == 2 ? (i - i0) & 1 : 0;
+                const bool more = i + 1 < i1;
+                row = next;
+                tr_sync();
+                if (more) {
+                    fetch(row);
+                    next = find(i + 2);
+                }
+                use(i, buf);
+                if (more) {
+                    if (L::NBUF == 1) tr_sync();
+                    store(row, L::NBUF == 2 ? buf ^ 1 : 0);
+                }
             }
         }
     }
 
     /* ---- the split's sums, or the result ---- */
-#pragma unroll
-    for (int b = 0; b < QB; b++) {
-        l[b] += __shfl_xor(l[b], 16, 64);
-        l[b] += __shfl_xor(l[b], 32, 64);
-        if (rq[b] >= R) continue;
-        if (a.ns > 1) {
-            const size_t at = (size_t)split * R + rq[b];
-            if (g == 0) {
-                a.pm[at] = m[b];
-                a.pl[at] = l[b];
-            }
-            float *d = a.part + at * a.dvp + 4 * g;
-#pragma unroll
-            for (int v = 0; v < NV; v++)
-                if (16 * v < a.dvp) *(f32x4 *)(d + 16 * v) = o[b][v];
-            continue;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (rq >= R) return;
+    if (a.ns > 1) {
+        const size_t at = (size_t)split * R + rq;
+        if (g == 0) {
+            a.pm[at] = m;
+            a.pl[at] = l;
         }
-        float den = l[b];
-        if (a.sink && den != 0.0f)
-            den += __builtin_amdgcn_exp2f(a.sink[rq[b] % a.h] * 1.44269504088896340736f - m[b]);
-        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
-        T *d = (T *)a.o + (size_t)rq[b] * a.dv + 4 * g;
+        float *d = a.part + at * a.dvp + 4 * g;
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            const f32x4 x = o[b][v] * inv;
-            const float y[4] = {x.x, x.y, x.z, x.w};
-            const int c = 16 * v + 4 * g;
-            if (a.ovec) {
-                if (c < a.dv) io_store<T, 4>(d + 16 * v, y);
-            } else {
+        for (int v = 0; v < NV; v++)
+            if (16 * v < a.dvp) *(f32x4 *)(d + 16 * v) = o[v];
+        return;
+    }
+    if (a.sink && l != 0.0f)
+        l += __builtin_amdgcn_exp2f(a.sink[rq % a.h] * 1.44269504088896340736f - m);
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    T *d = (T *)a.o + (size_t)rq * a.dv + 4 * g;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (c + e < a.dv) io_store<T, 1>(d + 16 * v + e, y + e);
-            }
+    for (int v = 0; v < NV; v++) {
+        const f32x4 x = o[v] * inv;
+        const float y[4] = {x.x, x.y, x.z, x.w};
+        const int c = 16 * v + 4 * g;
+        if (a.ovec) {
+            if (c < a.dv) io_store<T, 4>(d + 16 * v, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c + e < a.dv) io_store<T, 1>(d + 16 * v + e, y + e);
         }
     }
 }
@@ -559,8 +638,8 @@ int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
             if (dev >= 0 && dev < 64) asked[dev] = true;
         }
     }
-    hipLaunchKernelGGL((k_tree<T, KVF, KC>), dim3((unsigned)(a.ns * a.nb)), dim3(TR_THREADS),
-                       L::BYTES, st, a);
+    hipLaunchKernelGGL((k_tree<T, KVF, KC>), dim3((unsigned)(a.ns * a.nb)),
+                       dim3(64 * tree_waves(tr_fmt<T>(), KVF, KC)), L::BYTES, st, a);
     HIP_OK(hipGetLastError(), "tree attn launch");
     return 0;
 }

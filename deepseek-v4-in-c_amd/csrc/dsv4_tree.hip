@@ -19,28 +19,29 @@ namespace {
 
 #include "dsv4_rows_io.h"
 
+constexpr int TJ_THREADS = 256;
 constexpr int TJ_COLS = 64;                       /* columns of a workgroup  */
-constexpr int TJ_GROUPS = TR_THREADS / (TJ_COLS / 4);
+constexpr int TJ_GROUPS = TJ_THREADS / (TJ_COLS / 4);
 
 /* o of one row of q and 64 columns: thread (group of splits, 4 columns), the
  * groups' sums added in order through LDS. */
 template <class T>
-__global__ void __launch_bounds__(TR_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
+__global__ void __launch_bounds__(TJ_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
 {
     __shared__ float wt[1024];
-    __shared__ float red[TR_THREADS / 64];
+    __shared__ float red[TJ_THREADS / 64];
     __shared__ f32x4 sum[TJ_GROUPS][TJ_COLS / 4];
     const int tid = threadIdx.x, r = blockIdx.x, R = a.nt * a.h;
     float m = -INFINITY;
-    for (int s = tid; s < a.ns; s += TR_THREADS) m = fmaxf(m, a.pm[(size_t)s * R + r]);
+    for (int s = tid; s < a.ns; s += TJ_THREADS) m = fmaxf(m, a.pm[(size_t)s * R + r]);
     m = wave_max(m);
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
     m = red[0];
-    for (int k = 1; k < TR_THREADS / 64; k++) m = fmaxf(m, red[k]);
+    for (int k = 1; k < TJ_THREADS / 64; k++) m = fmaxf(m, red[k]);
     __syncthreads();
     float l = 0.0f;
-    for (int s = tid; s < a.ns; s += TR_THREADS) {
+    for (int s = tid; s < a.ns; s += TJ_THREADS) {
         const float ms = a.pm[(size_t)s * R + r], ls = a.pl[(size_t)s * R + r];
         /* a split that saw nothing adds 0, whatever its maximum; NaN sums stay */
         const float e = ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(TR_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
     if ((tid & 63) == 0) red[tid >> 6] = l;
     __syncthreads();
     l = 0.0f;
-    for (int k = 0; k < TR_THREADS / 64; k++) l += red[k];
+    for (int k = 0; k < TJ_THREADS / 64; k++) l += red[k];
     const int c4 = tid & (TJ_COLS / 4 - 1), gr = tid / (TJ_COLS / 4);
     const int c = blockIdx.y * TJ_COLS + 4 * c4;
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -140,7 +141,7 @@ int dsv4_tree_chunks(int d_qk, int d_v)
 
 int dsv4_tree_block_rows(int fmt, int kv_fmt, int kc)
 {
-    return TR_WAVES * 16 * tree_qblocks(fmt, kv_fmt, kc);
+    return 16 * tree_waves(fmt, kv_fmt, kc);
 }
 
 extern "C" size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v,
@@ -222,9 +223,9 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
     if (rc != 0 || p.ns == 1) return rc;
     const dim3 grid(nt * h, (d_v + TJ_COLS - 1) / TJ_COLS);
     if (fmt == DSV4_WF32)
-        hipLaunchKernelGGL(k_tree_join<float>, grid, dim3(TR_THREADS), 0, st, a, (float *)d_o);
+        hipLaunchKernelGGL(k_tree_join<float>, grid, dim3(TJ_THREADS), 0, st, a, (float *)d_o);
     else
-        hipLaunchKernelGGL(k_tree_join<uint16_t>, grid, dim3(TR_THREADS), 0, st, a,
+        hipLaunchKernelGGL(k_tree_join<uint16_t>, grid, dim3(TJ_THREADS), 0, st, a,
                            (uint16_t *)d_o);
     HIP_OK(hipGetLastError(), "tree attn join launch");
     return 0;
