@@ -94,7 +94,8 @@ __device__ __forceinline__ f32x4 tr_mfma(tr_bf8 a, tr_bf8 b, f32x4 c)
 
 /* LDS of a workgroup: NBUF tiles of [planes][slabs of 64 columns][TR_TILE][128
  * bytes], then per buffer the rows' places in the cache, their scales and
- * whether they may not be used. Piece p (16 bytes) of a slab's row r is at p ^
+ * whether they may not be used, then what q's rows see (kept out of the
+ * registers, as only masked tiles ask). Piece p (16 bytes) of a slab's row r is at p ^
  * f(r), f 0, 2, 4, 6, 1, 3, 5, 7 for r % 8: the reads of the scores (one piece
  * of 16 rows) and of the values (two pieces of four rows) then spread over all
  * banks. */
@@ -107,12 +108,11 @@ struct TreeLds {
     static constexpr int NBUF = KT > 1 ? 1 : KVF == DSV4_GPU_KV_BF16 ? 3 : 2;
     static constexpr int META = NBUF * KT * PLANE;
     static constexpr int MSIZE = 3 * TR_TILE * 4;
-    static constexpr int BYTES = META + NBUF * MSIZE;
+    static constexpr int ROWS = META + NBUF * MSIZE;   /* q's rows: see, lo      */
+    static constexpr int BYTES = ROWS + 8 * 16 * 16;
 };
 
 __device__ __forceinline__ int tr_swz(int r) { return (r & 3) << 1 | (r >> 2 & 1); }
-
-typedef __attribute__((address_space(3))) void tr_lds_void;
 
 template <int N>
 __device__ __forceinline__ void tr_vm_wait()
@@ -120,10 +120,29 @@ __device__ __forceinline__ void tr_vm_wait()
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+/* 16 bytes per lane from p to dst + 16 lane in LDS (dst the same in every lane).
+ * As the builtin the compiler would wait for it before each later transposed
+ * read of LDS; this way nothing waits but tr_vm_wait. It writes no register,
+ * and its addresses are read as it issues. */
+__device__ __forceinline__ void tr_to_lds(const void *p, const unsigned char *dst)
+{
+    const uint32_t d = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char *)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 ::"s"(d), "v"(p) : "memory", "m0");
+}
+
 /* Every wave's LDS reads and writes so far are done; loads stay in flight. */
 __device__ __forceinline__ void tr_sync()
 {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+/* v, so that what is computed from it in a loop is not kept across the loop. */
+__device__ __forceinline__ int tr_fresh(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 template <class T>
@@ -182,45 +201,73 @@ k_tree(Dsv4TreeJob a)
     const int i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
     const int R = a.nt * a.h;
 
-    /* this lane's row of q: its token's drafts and first position */
+    /* this lane's row of q: the drafts its token sees and its first position */
     const int rq = (blk * W + w) * 16 + l16;
-    int lo;
-    unsigned long long see;
-    {
+    if (g == 0) {
         const int t = min(rq, R - 1) / a.h;
         const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
-        see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
+        unsigned long long see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
         const int depth = __popcll(see & ~(1ull << t));
-        lo = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
         if (a.window && a.window < a.nt)
             for (int j = 0; j < a.nt; j++) {
                 const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
                 if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
             }
+        unsigned char *d = lds + L::ROWS + 16 * (16 * w + l16);
+        *(unsigned long long *)d = see;
+        *(int *)(d + 8) = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
     }
-    /* elements past the row are zeroed by a mask in a register: the many lane
-     * masks of comparisons would crowd out the scalar registers */
+    /* q, a few chunks' loads at a time; elements past the row are zeroed by a
+     * mask in a register, as the many lane masks of comparisons would crowd out
+     * the scalar registers */
     tr_bf8 q[NT][KC];
     {
         const T *qr = (const T *)a.q + (size_t)min(rq, R - 1) * a.dqk;
+        constexpr int G = KC % 6 == 0 ? 6 : 4;
+        if (a.qvec) {
 #pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            const int c = 32 * kc + 8 * g;
-            float v[8];
-            if (a.qvec) {
-                io_load<T, 8>(qr + min(c, a.dqk - 8), v);
-            } else {
+            for (int k0 = 0; k0 < KC; k0 += G) {
+                u32x4 v[G][sizeof(T) / 2];
 #pragma unroll
-                for (int e = 0; e < 8; e++) io_load<T, 1>(qr + min(c + e, a.dqk - 1), v + e);
+                for (int u = 0; u < G; u++)
+#pragma unroll
+                    for (int h = 0; h < (int)sizeof(T) / 2; h++)
+                        v[u][h] = ld16((const unsigned char *)(qr + min(32 * (k0 + u) + 8 * g,
+                                                                         a.dqk - 8)) + 16 * h);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < G; u++) {
+                    const uint32_t in = (uint32_t)((32 * (k0 + u) + 8 * g - a.dqk) >> 31);
+                    if constexpr (sizeof(T) == 2) {
+                        q[0][k0 + u] = __builtin_bit_cast(tr_bf8, v[u][0] & in);
+                    } else {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[u][e / 4][e % 4] & in);
+                        tr_bf8 tm[NT];
+                        tr_terms<NT>(f, tm);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) q[n][k0 + u] = tm[n];
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                v[e] = __int_as_float(__float_as_int(v[e]) & ((c + e - a.dqk) >> 31));
-            tr_bf8 tm[NT];
-            tr_terms<NT>(v, tm);
+            for (int kc = 0; kc < KC; kc++) {
+                const int c = 32 * kc + 8 * g;
+                float f[8];
 #pragma unroll
-            for (int n = 0; n < NT; n++) q[n][kc] = tm[n];
-            __builtin_amdgcn_sched_barrier(0);         /* few of q's loads at a time */
+                for (int e = 0; e < 8; e++) {
+                    io_load<T, 1>(qr + min(c + e, a.dqk - 1), f + e);
+                    f[e] = __int_as_float(__float_as_int(f[e]) & ((c + e - a.dqk) >> 31));
+                }
+                tr_bf8 tm[NT];
+                tr_terms<NT>(f, tm);
+#pragma unroll
+                for (int n = 0; n < NT; n++) q[n][kc] = tm[n];
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
     f32x4 o[NV];
@@ -313,13 +360,12 @@ k_tree(Dsv4TreeJob a)
         }
         const uint16_t *p = (const uint16_t *)a.kv + (size_t)max(row, 0) * a.stride;
         unsigned char *d = plane(buf) + 1024 * (w & 3);
+        const int c = tr_fresh(pc);
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int s = ws + WS * k;
             if (L::SLABS % WS == 0 || s < L::SLABS)
-                __builtin_amdgcn_global_load_lds(
-                    (const void *)(p + min(64 * s + pc, a.dqk - 8)),
-                    (tr_lds_void *)(d + s * L::SLAB), 16, 0, 0);
+                tr_to_lds(p + min(64 * s + c, a.dqk - 8), d + s * L::SLAB);
         }
     };
     /* this wave's loads but those of the newest tile are done */
@@ -400,11 +446,12 @@ k_tree(Dsv4TreeJob a)
     /* a lane's places in a slab: row l16's piece g for the scores (the other
      * half of a slab at ^ 64), row 4 g + l16 / 4's four columns 4 (l16 % 4) for
      * the values (the slab's other column tiles at ^ 32, 64 and 96) */
-    const int ka = l16 * 128 + 16 * (g ^ tr_swz(l16));
-    const int va = (4 * g + (l16 >> 2)) * 128 + 8 * (l16 & 1) +
-                   16 * ((l16 >> 1 & 1) ^ tr_swz(4 * g + (l16 >> 2)));
+    const int ka0 = l16 * 128 + 16 * (g ^ tr_swz(l16));
+    const int va0 = (4 * g + (l16 >> 2)) * 128 + 8 * (l16 & 1) +
+                    16 * ((l16 >> 1 & 1) ^ tr_swz(4 * g + (l16 >> 2)));
     auto use = [&](int i, int buf) {
         const unsigned char *t = plane(buf);
+        const int ka = tr_fresh(ka0), va = tr_fresh(va0);
         const int *mi = (const int *)meta(buf);
         const uint32_t ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
         const bool masked = partial(i) || ok != 0xFFFFFFFFu;
@@ -466,7 +513,9 @@ k_tree(Dsv4TreeJob a)
         uint32_t vis = ~0u;
         if (masked) {
             const uint32_t no = (uint32_t)__ballot(mi[2 * TR_TILE + (lane & 31)] != 0);
-            const int p0 = i * TR_TILE;
+            const unsigned char *rs = lds + L::ROWS + 16 * (16 * w + l16);
+            const unsigned long long see = *(const unsigned long long *)rs;
+            const int lo = *(const int *)(rs + 8), p0 = i * TR_TILE;
             /* positions [lo, ctx) of the context, then the drafts' bits */
             vis = 0u;
             const int f = max(lo - p0, 0), e = min(a.ctx - p0, TR_TILE);
