@@ -95,10 +95,12 @@ __device__ __forceinline__ f32x4 tr_mfma(tr_bf8 a, tr_bf8 b, f32x4 c)
 /* LDS of a workgroup: NBUF tiles of [planes][slabs of 64 columns][TR_TILE][128
  * bytes], then per buffer the rows' places in the cache, their scales and
  * whether they may not be used, then what q's rows see (kept out of the
- * registers, as only masked tiles ask). Piece p (16 bytes) of a slab's row r is at p ^
- * f(r), f 0, 2, 4, 6, 1, 3, 5, 7 for r % 8: the reads of the scores (one piece
- * of 16 rows) and of the values (two pieces of four rows) then spread over all
- * banks. */
+ * registers, as only masked tiles ask). Piece p (16 bytes) of a slab's row r is at
+ * p ^ (r & 7). Then the reads of the scores (eight rows' same piece at a time)
+ * and of the values (two pieces of rows 0 .. 7, even and odd ones in different
+ * halves of the 64 banks) take each bank once: SQ_LDS_BANK_CONFLICT counts
+ * none, and 4 cycles for each read of the values with f 0, 2, 4, 6, 1, 3, 5, 7.
+ */
 template <int KVF, int KC>
 struct TreeLds {
     static constexpr int KT = tree_planes(KVF);
@@ -112,7 +114,7 @@ struct TreeLds {
     static constexpr int BYTES = ROWS + 8 * 16 * 16;
 };
 
-__device__ __forceinline__ int tr_swz(int r) { return (r & 3) << 1 | (r >> 2 & 1); }
+__device__ __forceinline__ int tr_swz(int r) { return r & 7; }
 
 template <int N>
 __device__ __forceinline__ void tr_vm_wait()
@@ -122,14 +124,15 @@ __device__ __forceinline__ void tr_vm_wait()
 
 /* 16 bytes per lane from p to dst + 16 lane in LDS (dst the same in every lane).
  * As the builtin the compiler would wait for it before each later transposed
- * read of LDS; this way nothing waits but tr_vm_wait. It writes no register,
- * and its addresses are read as it issues. */
+ * read of LDS; this way nothing waits but tr_vm_wait. It writes no
+ * register but M0, which the compiler sets anew before each use of its own, and
+ * its addresses are read as it issues. */
 __device__ __forceinline__ void tr_to_lds(const void *p, const unsigned char *dst)
 {
     const uint32_t d = (uint32_t)__builtin_amdgcn_readfirstlane(
         (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char *)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 ::"s"(d), "v"(p) : "memory", "m0");
+                 ::"s"(d), "v"(p) : "memory");
 }
 
 /* Every wave's LDS reads and writes so far are done; loads stay in flight. */
