@@ -45,11 +45,14 @@ constexpr int TR_TERMS = 3;
 constexpr int tree_terms(int fmt) { return fmt == DSV4_WF32 ? TR_TERMS : 1; }
 constexpr int tree_planes(int kv_fmt) { return kv_fmt == DSV4_GPU_KV_F32 ? TR_TERMS : 1; }
 constexpr int tree_vtiles(int kc) { return kc >= 16 ? 32 : 2 * kc; }
-/* Waves of a workgroup, 16 rows of q each: eight, two per SIMD, where a wave's
- * part of q and its sums fit half the registers. */
-constexpr int tree_waves(int fmt, int kv_fmt, int kc)
+/* A workgroup is eight waves, two per SIMD. A wave holds 16 rows of q and their
+ * sums, or, where with all terms that is more than half the registers, two
+ * waves share 16 rows: each takes half of the d_qk columns of the scores, adds
+ * the other's half through LDS, and sums half of the d_v columns. */
+constexpr int TR_WAVES = 8;
+constexpr int tree_split(int fmt, int kv_fmt, int kc)
 {
-    return kc >= 16 && tree_terms(fmt) * tree_planes(kv_fmt) > 1 ? 4 : 8;
+    return kc >= 16 && tree_terms(fmt) * tree_planes(kv_fmt) > 1 ? 2 : 1;
 }
 
 #ifdef DSV4_TREE_KERNEL
@@ -111,7 +114,8 @@ struct TreeLds {
     static constexpr int META = NBUF * KT * PLANE;
     static constexpr int MSIZE = 3 * TR_TILE * 4;
     static constexpr int ROWS = META + NBUF * MSIZE;   /* q's rows: see, lo      */
-    static constexpr int BYTES = ROWS + 8 * 16 * 16;
+    static constexpr int HALF = ROWS + 16 * 16 * TR_WAVES;     /* halves of scores */
+    static constexpr int BYTES = HALF + 2048 * TR_WAVES;
 };
 
 __device__ __forceinline__ int tr_swz(int r) { return r & 7; }
@@ -174,14 +178,15 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * are not there, become zeros in LDS first, which a weight of 0 leaves at 0,
  * and the former give NaN scores to the rows of q that see them. */
 template <class T, int KVF, int KC>
-__global__ void __launch_bounds__(64 * tree_waves(tr_fmt<T>(), KVF, KC),
-                                  tree_waves(tr_fmt<T>(), KVF, KC) / 4)
+__global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4)
 k_tree(Dsv4TreeJob a)
 {
     using L = TreeLds<KVF, KC>;
     constexpr int NT = tree_terms(tr_fmt<T>()), KT = L::KT, NV = tree_vtiles(KC);
     constexpr int PT = NT > KT ? NT : KT;              /* term pairs i + j < PT  */
-    constexpr int W = tree_waves(tr_fmt<T>(), KVF, KC), WS = W / 4;
+    constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);
+    constexpr int W = TR_WAVES, WS = W / 4;
+    constexpr int KC1 = KC / SPLIT, NV1 = NV / SPLIT;  /* this wave's part       */
     constexpr int NP = (L::SLABS + WS - 1) / WS;       /* pieces of 8 per thread */
     constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : 2;
     constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
@@ -205,7 +210,9 @@ k_tree(Dsv4TreeJob a)
     const int R = a.nt * a.h;
 
     /* this lane's row of q: the drafts its token sees and its first position */
-    const int rq = (blk * W + w) * 16 + l16;
+    const int qb = SPLIT == 2 ? w & 3 : w, half = SPLIT == 2 ? w >> 2 : 0;
+    const int rq = (blk * (W / SPLIT) + qb) * 16 + l16;
+    const bool live = (blk * (W / SPLIT) + qb) * 16 < R;
     if (g == 0) {
         const int t = min(rq, R - 1) / a.h;
         const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
@@ -220,64 +227,6 @@ k_tree(Dsv4TreeJob a)
         *(unsigned long long *)d = see;
         *(int *)(d + 8) = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
     }
-    /* q, a few chunks' loads at a time; elements past the row are zeroed by a
-     * mask in a register, as the many lane masks of comparisons would crowd out
-     * the scalar registers */
-    tr_bf8 q[NT][KC];
-    {
-        const T *qr = (const T *)a.q + (size_t)min(rq, R - 1) * a.dqk;
-        constexpr int G = KC % 6 == 0 ? 6 : 4;
-        if (a.qvec) {
-#pragma unroll
-            for (int k0 = 0; k0 < KC; k0 += G) {
-                u32x4 v[G][sizeof(T) / 2];
-#pragma unroll
-                for (int u = 0; u < G; u++)
-#pragma unroll
-                    for (int h = 0; h < (int)sizeof(T) / 2; h++)
-                        v[u][h] = ld16((const unsigned char *)(qr + min(32 * (k0 + u) + 8 * g,
-                                                                         a.dqk - 8)) + 16 * h);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < G; u++) {
-                    const uint32_t in = (uint32_t)((32 * (k0 + u) + 8 * g - a.dqk) >> 31);
-                    if constexpr (sizeof(T) == 2) {
-                        q[0][k0 + u] = __builtin_bit_cast(tr_bf8, v[u][0] & in);
-                    } else {
-                        float f[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[u][e / 4][e % 4] & in);
-                        tr_bf8 tm[NT];
-                        tr_terms<NT>(f, tm);
-#pragma unroll
-                        for (int n = 0; n < NT; n++) q[n][k0 + u] = tm[n];
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-#pragma unroll
-            for (int kc = 0; kc < KC; kc++) {
-                const int c = 32 * kc + 8 * g;
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    io_load<T, 1>(qr + min(c + e, a.dqk - 1), f + e);
-                    f[e] = __int_as_float(__float_as_int(f[e]) & ((c + e - a.dqk) >> 31));
-                }
-                tr_bf8 tm[NT];
-                tr_terms<NT>(f, tm);
-#pragma unroll
-                for (int n = 0; n < NT; n++) q[n][kc] = tm[n];
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-    }
-    f32x4 o[NV];
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int v = 0; v < NV; v++) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     /* ---- staging: a thread has place sp of row sr of slabs ws, ws + WS, ... of a
      *      tile: piece sp ^ f(sr) of 64 columns. Pieces past the cache row
      *      repeat its last one: q is zero there. ---- */
@@ -445,6 +394,79 @@ k_tree(Dsv4TreeJob a)
         tr_sync();
     };
 
+    /* the first tiles' loads go out before q's */
+    int r0 = -1, r1 = -1, r2 = -1;
+    if (i0 < i1) {
+        r0 = find(i0);
+        r1 = find(i0 + 1);
+        if constexpr (DMA) {
+            r2 = find(i0 + 2);
+            dma(r0, 0);
+            if (i0 + 1 < i1) dma(r1, 1);
+        } else {
+            fetch(r0);
+        }
+    }
+
+    /* q, a few chunks' loads at a time; elements past the row are zeroed by a
+     * mask in a register, as the many lane masks of comparisons would crowd out
+     * the scalar registers */
+    tr_bf8 q[NT][KC1];
+    {
+        const T *qr = (const T *)a.q + (size_t)min(rq, R - 1) * a.dqk;
+        constexpr int G = KC1 % 3 == 0 ? 3 : KC1 < 4 ? KC1 : 4;
+        const int c0 = 32 * KC1 * half + 8 * g;
+        if (a.qvec) {
+#pragma unroll
+            for (int k0 = 0; k0 < KC1; k0 += G) {
+                u32x4 v[G][sizeof(T) / 2];
+#pragma unroll
+                for (int u = 0; u < G; u++)
+#pragma unroll
+                    for (int h = 0; h < (int)sizeof(T) / 2; h++)
+                        v[u][h] = ld16((const unsigned char *)(qr + min(c0 + 32 * (k0 + u),
+                                                                         a.dqk - 8)) + 16 * h);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < G; u++) {
+                    const uint32_t in = (uint32_t)((c0 + 32 * (k0 + u) - a.dqk) >> 31);
+                    if constexpr (sizeof(T) == 2) {
+                        q[0][k0 + u] = __builtin_bit_cast(tr_bf8, v[u][0] & in);
+                    } else {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[u][e / 4][e % 4] & in);
+                        tr_bf8 tm[NT];
+                        tr_terms<NT>(f, tm);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) q[n][k0 + u] = tm[n];
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int kc = 0; kc < KC1; kc++) {
+                const int c = c0 + 32 * kc;
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    io_load<T, 1>(qr + min(c + e, a.dqk - 1), f + e);
+                    f[e] = __int_as_float(__float_as_int(f[e]) & ((c + e - a.dqk) >> 31));
+                }
+                tr_bf8 tm[NT];
+                tr_terms<NT>(f, tm);
+#pragma unroll
+                for (int n = 0; n < NT; n++) q[n][kc] = tm[n];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    f32x4 o[NV1];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV1; v++) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+
     const float c2 = a.scale * 1.44269504088896340736f;       /* to powers of two */
     /* a lane's places in a slab: row l16's piece g for the scores (the other
      * half of a slab at ^ 64), row 4 g + l16 / 4's four columns 4 (l16 % 4) for
@@ -459,14 +481,23 @@ k_tree(Dsv4TreeJob a)
         const uint32_t ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
         const bool masked = partial(i) || ok != 0xFFFFFFFFu;
         if (masked) mend(buf);
+        if (!live) {                                   /* no rows of q: only the syncs */
+            if (SPLIT == 2) tr_sync();
+            return;
+        }
 
         /* ---- S^T: one sum per order of the terms, so that the small ones do
          *      not round at the size of the large ---- */
         f32x4 so[2][PT], s[2];
 #pragma unroll
         for (int n = 0; n < PT; n++) so[0][n] = so[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int KG = KT > 1 || W == 8 ? 1 : 2;
+        constexpr int KG = 1;
         tr_bf8 row[2][KG][KT][2];
+        /* chunk kc of this wave's: the second half's first is chunk KC1 of the
+         * row, in the upper half of a slab where KC1 is odd */
+        const unsigned char *tk = t + half * (KC1 >> 1) * L::SLAB;
+        const int kb = ka ^ (KC1 & 1 & half) * 64;
+        const int up = (KC1 & 1 & half) * L::SLAB;
         auto rows_of = [&](int kg, tr_bf8 (&r)[KG][KT][2]) {
 #pragma unroll
             for (int u = 0; u < KG; u++)
@@ -475,14 +506,15 @@ k_tree(Dsv4TreeJob a)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
                         const int kc = kg * KG + u;
-                        r[u][p][k] = *(const tr_bf8 *)(t + p * L::PLANE + (kc >> 1) * L::SLAB +
-                                                       k * 2048 + (ka ^ (kc & 1) * 64));
+                        r[u][p][k] = *(const tr_bf8 *)(tk + p * L::PLANE + (kc >> 1) * L::SLAB +
+                                                       (kc & 1 ? up : 0) + k * 2048 +
+                                                       (kb ^ (kc & 1) * 64));
                     }
         };
         rows_of(0, row[0]);
 #pragma unroll
-        for (int kg = 0; kg < KC / KG; kg++) {
-            if (kg + 1 < KC / KG) rows_of(kg + 1, row[(kg + 1) & 1]);
+        for (int kg = 0; kg < KC1 / KG; kg++) {
+            if (kg + 1 < KC1 / KG) rows_of(kg + 1, row[(kg + 1) & 1]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < KG; u++)
@@ -502,6 +534,14 @@ k_tree(Dsv4TreeJob a)
             s[k] = so[k][PT - 1];
 #pragma unroll
             for (int n = PT - 2; n >= 0; n--) s[k] += so[k][n];
+        }
+        if constexpr (SPLIT == 2) {
+            unsigned char *x = lds + L::HALF + 16 * lane;
+#pragma unroll
+            for (int k = 0; k < 2; k++) *(f32x4 *)(x + 1024 * (2 * w + k)) = s[k];
+            tr_sync();
+#pragma unroll
+            for (int k = 0; k < 2; k++) s[k] += *(const f32x4 *)(x + 1024 * (2 * (w ^ 4) + k));
         }
 
         /* ---- the weights ---- */
@@ -550,7 +590,7 @@ k_tree(Dsv4TreeJob a)
             m = grow ? top : m;
             l *= f;
 #pragma unroll
-            for (int v = 0; v < NV; v++) o[v] *= f;
+            for (int v = 0; v < NV1; v++) o[v] *= f;
         }
         const float mm = m == -INFINITY ? 0.0f : m;
         float e[8], sum = 0.0f;
@@ -568,7 +608,8 @@ k_tree(Dsv4TreeJob a)
         tr_terms<NT>(e, pw);
 
         /* ---- O^T ---- */
-        constexpr int VG = KT > 1 ? 1 : W == 8 ? 2 : 4;
+        constexpr int VG = KT > 1 ? 1 : 2;
+        const unsigned char *tv = t + half * (NV1 / 4) * L::SLAB;
         tr_bf8 col[2][VG][KT];
         auto cols_of = [&](int vg, tr_bf8 (&c)[VG][KT]) {
 #pragma unroll
@@ -577,7 +618,7 @@ k_tree(Dsv4TreeJob a)
                 for (int p = 0; p < KT; p++) {
                     const int v = vg * VG + u;
                     const unsigned char *at =
-                        t + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
+                        tv + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
                     const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
                     const tr_s4 y =
                         __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
@@ -587,8 +628,8 @@ k_tree(Dsv4TreeJob a)
         };
         cols_of(0, col[0]);
 #pragma unroll
-        for (int vg = 0; vg < NV / VG; vg++) {
-            if (vg + 1 < NV / VG) cols_of(vg + 1, col[(vg + 1) & 1]);
+        for (int vg = 0; vg < NV1 / VG; vg++) {
+            if (vg + 1 < NV1 / VG) cols_of(vg + 1, col[(vg + 1) & 1]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int p = 0; p < KT; p++)
@@ -602,41 +643,34 @@ k_tree(Dsv4TreeJob a)
         }
     };
 
-    if (i0 < i1) {
-        if constexpr (DMA) {
-            int r2 = find(i0 + 2);
-            dma(find(i0), 0);
-            if (i0 + 1 < i1) dma(find(i0 + 1), 1);
-            int buf = 0;
-            for (int i = i0; i < i1; i++) {
-                dma_wait(i + 1 < i1);
-                tr_sync();               /* tile i is in LDS, tile i - 1's buffer free */
-                if (i + 2 < i1) {
-                    const int row = r2;
-                    r2 = find(i + 3);
-                    dma(row, buf == 0 ? 2 : buf - 1);
-                }
-                use(i, buf);
-                buf = buf == 2 ? 0 : buf + 1;
+    if constexpr (DMA) {
+        int buf = 0;
+        for (int i = i0; i < i1; i++) {
+            dma_wait(i + 1 < i1);
+            tr_sync();                   /* tile i is in LDS, tile i - 1's buffer free */
+            if (i + 2 < i1) {
+                const int row = r2;
+                r2 = find(i + 3);
+                dma(row, buf == 0 ? 2 : buf - 1);
             }
-        } else {
-            int row = find(i0), next = find(i0 + 1);
-            fetch(row);
-            store(row, 0);
-            for (int i = i0; i < i1; i++) {
-                const int buf = L::NBUF == 2 ? (i - i0) & 1 : 0;
-                const bool more = i + 1 < i1;
-                row = next;
-                tr_sync();
-                if (more) {
-                    fetch(row);
-                    next = find(i + 2);
-                }
-                use(i, buf);
-                if (more) {
-                    if (L::NBUF == 1) tr_sync();
-                    store(row, L::NBUF == 2 ? buf ^ 1 : 0);
-                }
+            use(i, buf);
+            buf = buf == 2 ? 0 : buf + 1;
+        }
+    } else if (i0 < i1) {
+        store(r0, 0);
+        for (int i = i0; i < i1; i++) {
+            const int buf = L::NBUF == 2 ? (i - i0) & 1 : 0;
+            const bool more = i + 1 < i1;
+            const int row = r1;
+            tr_sync();
+            if (more) {
+                fetch(row);
+                r1 = find(i + 2);
+            }
+            use(i, buf);
+            if (more) {
+                if (L::NBUF == 1) tr_sync();
+                store(row, L::NBUF == 2 ? buf ^ 1 : 0);
             }
         }
     }
@@ -647,25 +681,25 @@ k_tree(Dsv4TreeJob a)
     if (rq >= R) return;
     if (a.ns > 1) {
         const size_t at = (size_t)split * R + rq;
-        if (g == 0) {
+        if (g == 0 && half == 0) {
             a.pm[at] = m;
             a.pl[at] = l;
         }
-        float *d = a.part + at * a.dvp + 4 * g;
+        float *d = a.part + at * a.dvp + 16 * NV1 * half + 4 * g;
 #pragma unroll
-        for (int v = 0; v < NV; v++)
-            if (16 * v < a.dvp) *(f32x4 *)(d + 16 * v) = o[v];
+        for (int v = 0; v < NV1; v++)
+            if (16 * (NV1 * half + v) < a.dvp) *(f32x4 *)(d + 16 * v) = o[v];
         return;
     }
     if (a.sink && l != 0.0f)
         l += __builtin_amdgcn_exp2f(a.sink[rq % a.h] * 1.44269504088896340736f - m);
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    T *d = (T *)a.o + (size_t)rq * a.dv + 4 * g;
+    T *d = (T *)a.o + (size_t)rq * a.dv + 16 * NV1 * half + 4 * g;
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
+    for (int v = 0; v < NV1; v++) {
         const f32x4 x = o[v] * inv;
         const float y[4] = {x.x, x.y, x.z, x.w};
-        const int c = 16 * v + 4 * g;
+        const int c = 16 * (NV1 * half + v) + 4 * g;
         if (a.ovec) {
             if (c < a.dv) io_store<T, 4>(d + 16 * v, y);
         } else {
@@ -691,7 +725,7 @@ int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
         }
     }
     hipLaunchKernelGGL((k_tree<T, KVF, KC>), dim3((unsigned)(a.ns * a.nb)),
-                       dim3(64 * tree_waves(tr_fmt<T>(), KVF, KC)), L::BYTES, st, a);
+                       dim3(64 * TR_WAVES), L::BYTES, st, a);
     HIP_OK(hipGetLastError(), "tree attn launch");
     return 0;
 }

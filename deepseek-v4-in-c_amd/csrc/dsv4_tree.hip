@@ -141,7 +141,7 @@ int dsv4_tree_chunks(int d_qk, int d_v)
 
 int dsv4_tree_block_rows(int fmt, int kv_fmt, int kc)
 {
-    return 16 * tree_waves(fmt, kv_fmt, kc);
+    return 16 * TR_WAVES / tree_split(fmt, kv_fmt, kc);
 }
 
 extern "C" size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v,
