@@ -145,6 +145,16 @@ __device__ __forceinline__ void tr_sync()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+/* The largest of the four lanes l16, l16 + 16, + 32 and + 48, in each of them
+ * (exchanges within the vector unit: no trip through LDS). */
+__device__ __forceinline__ float tr_max4(float v)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 /* v, so that what is computed from it in a loop is not kept across the loop. */
 __device__ __forceinline__ int tr_fresh(int v)
 {
@@ -478,8 +488,13 @@ k_tree(Dsv4TreeJob a)
         const unsigned char *t = plane(buf);
         const int ka = tr_fresh(ka0), va = tr_fresh(va0);
         const int *mi = (const int *)meta(buf);
-        const uint32_t ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
-        const bool masked = partial(i) || ok != 0xFFFFFFFFu;
+        /* unpaged, rows are missing past the cache's end alone */
+        uint32_t ok = 0xFFFFFFFFu;
+        bool masked = partial(i) || (i + 1) * TR_TILE > a.rows;
+        if (masked || a.pages) {
+            ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
+            masked |= ok != 0xFFFFFFFFu;
+        }
         if (masked) mend(buf);
         if (!live) {                                   /* no rows of q: only the syncs */
             if (SPLIT == 2) tr_sync();
@@ -544,6 +559,28 @@ k_tree(Dsv4TreeJob a)
             for (int k = 0; k < 2; k++) s[k] += *(const f32x4 *)(x + 1024 * (2 * (w ^ 4) + k));
         }
 
+        /* the first columns of V, while the weights are computed */
+        constexpr int VG = KT > 1 ? 1 : 2;
+        const unsigned char *tv = t + half * (NV1 / 4) * L::SLAB;
+        tr_bf8 col[2][VG][KT];
+        auto cols_of = [&](int vg, tr_bf8 (&c)[VG][KT]) {
+#pragma unroll
+            for (int u = 0; u < VG; u++)
+#pragma unroll
+                for (int p = 0; p < KT; p++) {
+                    const int v = vg * VG + u;
+                    const unsigned char *at =
+                        tv + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
+                    const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
+                    const tr_s4 y =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
+                    c[u][p] = __builtin_bit_cast(
+                        tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+        };
+        cols_of(0, col[0]);
+        __builtin_amdgcn_sched_barrier(0);
+
         /* ---- the weights ---- */
         f32x4 ks[2];
         if (KVF == DSV4_GPU_KV_FP8) {
@@ -582,8 +619,7 @@ k_tree(Dsv4TreeJob a)
                 if (masked) x = vis >> (16 * k + j) & 1u ? x : -INFINITY;
                 top = fmaxf(top, x);
             }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = tr_max4(top);
         const bool grow = top > m + 8.0f;
         if (__any(grow)) {
             const float f = grow ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
@@ -608,25 +644,6 @@ k_tree(Dsv4TreeJob a)
         tr_terms<NT>(e, pw);
 
         /* ---- O^T ---- */
-        constexpr int VG = KT > 1 ? 1 : 2;
-        const unsigned char *tv = t + half * (NV1 / 4) * L::SLAB;
-        tr_bf8 col[2][VG][KT];
-        auto cols_of = [&](int vg, tr_bf8 (&c)[VG][KT]) {
-#pragma unroll
-            for (int u = 0; u < VG; u++)
-#pragma unroll
-                for (int p = 0; p < KT; p++) {
-                    const int v = vg * VG + u;
-                    const unsigned char *at =
-                        tv + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
-                    const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
-                    const tr_s4 y =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
-                    c[u][p] = __builtin_bit_cast(
-                        tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-        };
-        cols_of(0, col[0]);
 #pragma unroll
         for (int vg = 0; vg < NV1 / VG; vg++) {
             if (vg + 1 < NV1 / VG) cols_of(vg + 1, col[(vg + 1) & 1]);
