@@ -96,15 +96,14 @@ __device__ __forceinline__ f32x4 tr_mfma(tr_bf8 a, tr_bf8 b, f32x4 c)
 }
 
 /* LDS of a workgroup: NBUF tiles of [planes][slabs of 64 columns][TR_TILE][128
- * bytes], then per buffer the rows' places in the cache, their scales and
- * whether they may not be used, then what q's rows see (kept out of the
- * registers, as only masked tiles ask). Piece p (16 bytes) of a slab's row r is at
- * p ^ (r & 7). Then the reads of the scores (eight rows' same piece at a time)
- * and of the values (two pieces of rows 0 .. 7, even and odd ones in different
- * halves of the 64 banks) take each bank once: SQ_LDS_BANK_CONFLICT counts
- * none, and 4 cycles for each read of the values with f 0, 2, 4, 6, 1, 3, 5, 7.
- */
-template <int KVF, int KC>
+ * bytes], then per buffer the rows' scales and whether they may not be used,
+ * then what q's rows see (kept out of the registers, as only masked tiles ask)
+ * and the halves of scores. Piece p (16 bytes) of a slab's row r is at p ^ (r &
+ * 7). Then the reads of the scores (eight rows' same piece at a time) and of
+ * the values (two pieces of rows 0 .. 7, even and odd ones in different halves
+ * of the 64 banks) take each bank once: SQ_LDS_BANK_CONFLICT counts none, and 4
+ * cycles for each read of the values with p ^ (0, 2, 4, 6, 1, 3, 5, 7). */
+template <int KVF, int KC, int SPLIT>
 struct TreeLds {
     static constexpr int KT = tree_planes(KVF);
     static constexpr int SLABS = KC / 2;
@@ -112,10 +111,10 @@ struct TreeLds {
     static constexpr int PLANE = SLABS * SLAB;
     static constexpr int NBUF = KT > 1 ? 1 : KVF == DSV4_GPU_KV_BF16 ? 3 : 2;
     static constexpr int META = NBUF * KT * PLANE;
-    static constexpr int MSIZE = 3 * TR_TILE * 4;
+    static constexpr int MSIZE = 2 * TR_TILE * 4;
     static constexpr int ROWS = META + NBUF * MSIZE;   /* q's rows: see, lo      */
-    static constexpr int HALF = ROWS + 16 * 16 * TR_WAVES;     /* halves of scores */
-    static constexpr int BYTES = HALF + 2048 * TR_WAVES;
+    static constexpr int HALF = ROWS + 16 * 16 * TR_WAVES;
+    static constexpr int BYTES = HALF + (SPLIT == 2 ? 2048 * TR_WAVES : 0);
 };
 
 __device__ __forceinline__ int tr_swz(int r) { return r & 7; }
@@ -126,17 +125,15 @@ __device__ __forceinline__ void tr_vm_wait()
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-/* 16 bytes per lane from p to dst + 16 lane in LDS (dst the same in every lane).
- * As the builtin the compiler would wait for it before each later transposed
- * read of LDS; this way nothing waits but tr_vm_wait. It writes no
+/* 16 bytes per lane from p to LDS byte dst + 16 lane (dst the same in every
+ * lane). As the builtin the compiler would wait for it before each later
+ * transposed read of LDS; this way nothing waits but tr_vm_wait. It writes no
  * register but M0, which the compiler sets anew before each use of its own, and
  * its addresses are read as it issues. */
-__device__ __forceinline__ void tr_to_lds(const void *p, const unsigned char *dst)
+__device__ __forceinline__ void tr_to_lds(const void *p, uint32_t dst)
 {
-    const uint32_t d = (uint32_t)__builtin_amdgcn_readfirstlane(
-        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char *)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 ::"s"(d), "v"(p) : "memory");
+                 ::"s"(dst), "v"(p) : "memory");
 }
 
 /* Every wave's LDS reads and writes so far are done; loads stay in flight. */
@@ -165,8 +162,9 @@ __device__ __forceinline__ int tr_fresh(int v)
 template <class T>
 constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
 
-/* Workgroup (split, block of q's rows): wave w holds 16 rows of q as the B
- * operands of S^T = K Q^T (a row of q per column), in bf16 terms.
+/* Workgroup (split, block of q's rows): a wave holds 16 rows of q (or half of
+ * their columns) as the B operands of S^T = K Q^T, a row of q per column, in
+ * bf16 terms.
  *
  * Per tile of 32 cache rows: S^T for two tiles of 16 keys; a lane then has
  * eight scores of its own column's row of q, which become that column's
@@ -180,8 +178,9 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  *
  * Tiles of a bf16 cache go to LDS by global_load_lds_dwordx4, two tiles ahead
  * and through no register; the other formats' next tile is loaded into
- * registers while this one is used. Operands are read from LDS a group ahead
- * of the matrix core.
+ * registers while this one is used. Operands are read from LDS a few products
+ * ahead of the matrix core. What a thread can make from its lane's number again
+ * is made again (place(), tr_fresh): the registers are full of q and the sums.
  *
  * A tile with drafts, a window's edge or rows outside the cache is masked by a
  * word of 32 bits per row of q; its cache rows that hold NaN or infinity, or
@@ -191,40 +190,42 @@ template <class T, int KVF, int KC>
 __global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4)
 k_tree(Dsv4TreeJob a)
 {
-    using L = TreeLds<KVF, KC>;
+    constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);
+    using L = TreeLds<KVF, KC, SPLIT>;
     constexpr int NT = tree_terms(tr_fmt<T>()), KT = L::KT, NV = tree_vtiles(KC);
     constexpr int PT = NT > KT ? NT : KT;              /* term pairs i + j < PT  */
-    constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);
     constexpr int W = TR_WAVES, WS = W / 4;
     constexpr int KC1 = KC / SPLIT, NV1 = NV / SPLIT;  /* this wave's part       */
     constexpr int NP = (L::SLABS + WS - 1) / WS;       /* pieces of 8 per thread */
     constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : 2;
+    constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : KVF == DSV4_GPU_KV_BF16 ? 2 : 1;
     constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int lane = threadIdx.x & 63;
+    const int lane0 = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int l16 = lane & 15, g = lane >> 4;
+    const int ws = w >> 2;
+    const int qb = SPLIT == 2 ? w & 3 : w, half = SPLIT == 2 ? ws : 0;
 
     /* Workgroup i runs on XCD i mod 8: each XCD takes a run of (split, block)
      * in split order, so blocks that read the same rows share its L2. */
-    int split, blk;
+    int i0, i1, blk, split;
     {
         const int all = gridDim.x, id = blockIdx.x, k = id & 7;
         const int at = k * (all >> 3) + min(k, all & 7) + (id >> 3);
-        split = at / a.nb;
+        split = __builtin_amdgcn_readfirstlane(at / a.nb);
         blk = at - split * a.nb;
+        const int tiles = a.tile1 - a.tile0;
+        i0 = a.tile0 + (int)((long long)tiles * split / a.ns);
+        i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
     }
-    const int tiles = a.tile1 - a.tile0;
-    const int i0 = a.tile0 + (int)((long long)tiles * split / a.ns);
-    const int i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
-    const int R = a.nt * a.h;
+    const int R = a.nt * a.h, end = a.ctx + a.nt;
+    const int row0 = (blk * (W / SPLIT) + qb) * 16;    /* this wave's rows of q  */
+    const bool live = row0 < R;
 
-    /* this lane's row of q: the drafts its token sees and its first position */
-    const int qb = SPLIT == 2 ? w & 3 : w, half = SPLIT == 2 ? w >> 2 : 0;
-    const int rq = (blk * (W / SPLIT) + qb) * 16 + l16;
-    const bool live = (blk * (W / SPLIT) + qb) * 16 < R;
-    if (g == 0) {
-        const int t = min(rq, R - 1) / a.h;
+    /* ---- the drafts that the token of each row of q sees, and the first
+     *      position ---- */
+    if (lane0 < 16) {
+        const int t = min(row0 + lane0, R - 1) / a.h;
         const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
         unsigned long long see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
         const int depth = __popcll(see & ~(1ull << t));
@@ -233,38 +234,52 @@ k_tree(Dsv4TreeJob a)
                 const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
                 if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
             }
-        unsigned char *d = lds + L::ROWS + 16 * (16 * w + l16);
+        unsigned char *d = lds + L::ROWS + 16 * (16 * w + lane0);
         *(unsigned long long *)d = see;
         *(int *)(d + 8) = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
     }
-    /* ---- staging: a thread has place sp of row sr of slabs ws, ws + WS, ... of a
-     *      tile: piece sp ^ f(sr) of 64 columns. Pieces past the cache row
-     *      repeat its last one: q is zero there. ---- */
-    const int sr = 8 * (w & 3) + (lane >> 3), ws = w >> 2;
-    const int pc = 8 * ((lane & 7) ^ tr_swz(sr));      /* the piece's first column */
-    const int home = sr * 128 + 16 * (lane & 7);
-    const bool speaks = (lane & 7) == 0 && ws == 0;
-    const int end = a.ctx + a.nt;
-    /* the cache row of tile i's row sr, -1 where there is none */
-    auto find = [&](int i) -> int {
-        const int p = i * TR_TILE + sr;
-        if (p >= end || i >= i1) return -1;
-        if (!a.pages) return p < a.rows ? p : -1;
+
+    /* ---- staging: a thread has place (lane % 8) of row sr of slabs ws, ws + WS,
+     *      ... of a tile, which is piece (lane % 8) ^ (sr & 7) of 64 columns.
+     *      Pieces past the cache row repeat its last one: q is zero there. ---- */
+    struct Place {
+        int sr, pc, home;                              /* pc: the piece's first column */
+    };
+    auto place = [&]() {
+        const int ln = tr_fresh(lane0), sr = 8 * (w & 3) + (ln >> 3);
+        return Place{sr, 8 * ((ln & 7) ^ tr_swz(sr)), sr * 128 + 16 * (ln & 7)};
+    };
+    auto slot = [&](int i) { return (int)((uint32_t)(i - i0) % (uint32_t)L::NBUF); };
+    auto plane = [&](int buf) { return lds + buf * KT * L::PLANE; };
+    auto meta = [&](int buf) { return lds + L::META + buf * L::MSIZE; };
+    const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds);
+    /* the cache row of row r of tile i, -1 where there is none */
+    auto find = [&](int i, int r) -> int {
+        const int p = i * TR_TILE + r;
+        if (!a.pages) return p < min(end, a.rows) ? p : -1;
+        if (p >= end) return -1;
         const int k = (int)((__umulhi(a.page_m, (uint32_t)p) + (uint32_t)p) >> a.page_s);
         if (k >= a.n_pages) return -1;
         const long long c = (long long)a.pages[k] * a.page + (p - k * a.page);
         return c >= 0 && c < a.rows ? (int)c : -1;
     };
-    /* some row of q may not see some row of tile i */
-    auto partial = [&](int i) {
-        return (i + 1) * TR_TILE > a.ctx ||
-               (a.window && i * TR_TILE < a.ctx + a.nt - a.window);
+    /* a page's entry is asked for a tile before it is needed: lane l has row l % 32
+     * of the tile to be loaded next, and `there` says which of its rows exist */
+    int ahead = -1;
+    auto ask = [&](int i) {
+        if (a.pages && i < i1) ahead = find(i, tr_fresh(lane0) & 31);
     };
-    auto meta = [&](int buf) { return lds + L::META + buf * L::MSIZE; };
-    auto plane = [&](int buf) { return lds + buf * KT * L::PLANE; };
+    auto there = [&](int i) -> uint32_t {
+        if (a.pages) return (uint32_t)__ballot(ahead >= 0);
+        const int n = min(end, a.rows) - i * TR_TILE;
+        return n >= TR_TILE ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
+    };
+    auto my_row = [&](int i, const Place &h) {
+        return max(0, a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
+    };
     /* one piece of a row that does not lie in whole pieces */
-    auto piece1 = [&](int row, int slab, uint32_t *r) {
-        const size_t at = (size_t)max(row, 0) * a.stride;
+    auto piece1 = [&](size_t at, int slab, int pc, uint32_t *r) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const size_t c = at + min(64 * slab + pc + e, a.dqk - 1);
@@ -300,37 +315,30 @@ k_tree(Dsv4TreeJob a)
         }
     };
     /* rows not in whole pieces go to LDS at once, without a tile's time between */
-    auto crawl = [&](int row, int buf) {
+    auto crawl = [&](int row, int buf, const Place &h) {
 #pragma unroll 1
         for (int s = ws; s < L::SLABS; s += WS) {
             uint32_t r[8];
-            piece1(row, s, r);
-            put(plane(buf) + s * L::SLAB + home, r);
+            piece1((size_t)row * a.stride, s, h.pc, r);
+            put(plane(buf) + s * L::SLAB + h.home, r);
         }
     };
-    auto name = [&](int row, int buf, float ks) {
-        if (!speaks) return;
-        ((int *)meta(buf))[sr] = row;
-        if (KVF == DSV4_GPU_KV_FP8) ((float *)meta(buf))[TR_TILE + sr] = row >= 0 ? ks : 0.0f;
-    };
-    /* the bf16 cache: into LDS directly */
-    auto dma = [&](int row, int buf) {
-        name(row, buf, 1.0f);
+    /* the bf16 cache: tile i into LDS directly */
+    auto dma = [&](int i, int buf) {
+        const Place h = place();
+        const int row = my_row(i, h);
         if (!a.vec) {
-            crawl(row, buf);
+            crawl(row, buf, h);
             return;
         }
-        const uint16_t *p = (const uint16_t *)a.kv + (size_t)max(row, 0) * a.stride;
-        unsigned char *d = plane(buf) + 1024 * (w & 3);
-        const int c = tr_fresh(pc);
+        const uint16_t *p = (const uint16_t *)a.kv + (size_t)row * a.stride;
+        const uint32_t d = lds0 + buf * L::PLANE + 1024 * (w & 3) + ws * L::SLAB;
 #pragma unroll
-        for (int k = 0; k < NP; k++) {
-            const int s = ws + WS * k;
-            if (L::SLABS % WS == 0 || s < L::SLABS)
-                tr_to_lds(p + min(64 * s + c, a.dqk - 8), d + s * L::SLAB);
-        }
+        for (int k = 0; k < NP; k++)
+            if (L::SLABS % WS == 0 || ws + WS * k < L::SLABS)
+                tr_to_lds(p + min(64 * (ws + WS * k) + h.pc, a.dqk - 8), d + WS * k * L::SLAB);
     };
-    /* this wave's loads but those of the newest tile are done */
+    /* this wave's loads but those of the newest tile are done, or all */
     auto dma_wait = [&](bool newest) {
         if (!newest) tr_vm_wait<0>();
         else if (L::SLABS % WS == 0 || ws == 0) tr_vm_wait<NP>();
@@ -339,91 +347,103 @@ k_tree(Dsv4TreeJob a)
     /* the other formats: through registers */
     uint32_t raw[NP][RAW];
     float rks = 1.0f;
-    auto fetch = [&](int row) {
-        if (KVF == DSV4_GPU_KV_FP8) rks = a.ks[max(row, 0)];
-        if (!a.vec) return;
-        constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : 1;
-        const unsigned char *p = (const unsigned char *)a.kv + (size_t)max(row, 0) * a.stride * ES;
+    int held = 0;                                      /* the row, not in whole pieces */
+    auto fetch = [&](int i) {
+        const Place h = place();
+        const int row = my_row(i, h);
+        if (KVF == DSV4_GPU_KV_FP8) rks = a.ks[row];
+        if (!a.vec) {
+            held = row;
+            return;
+        }
+        const unsigned char *p = (const unsigned char *)a.kv + (size_t)row * a.stride * ES;
 #pragma unroll
         for (int k = 0; k < NP; k++) {
-            const int c = min(64 * (ws + WS * k) + pc, a.dqk - 8);
+            const int c = min(64 * (ws + WS * k) + h.pc, a.dqk - 8);
             if constexpr (ES == 1) {
                 const uint2 v = *(const uint2 *)(p + c);
                 raw[k][0] = v.x;
                 raw[k][1] = v.y;
             } else {
 #pragma unroll
-                for (int h = 0; h < 8; h += 4) {
-                    const u32x4 v = ld16(p + 4 * (c + h));
+                for (int u = 0; u < RAW; u += 4) {
+                    const u32x4 v = ld16(p + 4 * (c + u));
 #pragma unroll
-                    for (int e = 0; e < 4; e++) raw[k][h + e] = v[e];
+                    for (int e = 0; e < 4; e++) raw[k][(u + e) % RAW] = v[e];
                 }
             }
         }
     };
-    auto store = [&](int row, int buf) {
-        name(row, buf, rks);
+    auto store = [&](int buf) {
+        const Place h = place();
+        if (KVF == DSV4_GPU_KV_FP8 && ws == 0 && (h.home & 112) == 0) ((float *)meta(buf))[h.sr] = rks;
         if (!a.vec) {
-            crawl(row, buf);
+            crawl(held, buf, h);
             return;
         }
 #pragma unroll
-        for (int k = 0; k < NP; k++) {
-            const int s = ws + WS * k;
-            if (L::SLABS % WS == 0 || s < L::SLABS) put(plane(buf) + s * L::SLAB + home, raw[k]);
-        }
+        for (int k = 0; k < NP; k++)
+            if (L::SLABS % WS == 0 || ws + WS * k < L::SLABS)
+                put(plane(buf) + (ws + WS * k) * L::SLAB + h.home, raw[k]);
     };
-    /* a masked tile's rows that are not there or hold what is not finite (in the
-     * first plane, which has f32's infinities and NaN too) to zeros; the
-     * eight threads of a row are lanes 8 k .. 8 k + 7, of one wave or of two */
-    auto mend = [&](int buf) {
+    /* a masked tile's rows that are not there (ok) or hold what is not finite (in
+     * the first plane, which has f32's infinities and NaN too) to zeros; the
+     * eight threads of a row are lanes 8 k .. 8 k + 7 of two waves, and all look
+     * at the whole row */
+    auto mend = [&](int buf, uint32_t ok) {
         int *mi = (int *)meta(buf);
+        const Place h = place();
         bool bad = false;
-        /* (every thread looks at all slabs, so that both waves agree) */
 #pragma unroll 1
         for (int s = 0; s < L::SLABS; s++) {
-            const u32x4 v = *(const u32x4 *)(plane(buf) + s * L::SLAB + home);
+            const u32x4 v = *(const u32x4 *)(plane(buf) + s * L::SLAB + h.home);
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 bad |= (v[e] & 0x7F80u) == 0x7F80u || (v[e] & 0x7F800000u) == 0x7F800000u;
         }
-        const int row = mi[sr];
+        const bool gone = !(ok >> h.sr & 1u);
         if (KVF == DSV4_GPU_KV_FP8)
-            bad |= (((const uint32_t *)mi)[TR_TILE + sr] & 0x7F800000u) == 0x7F800000u;
-        bad = (__ballot(bad) >> (lane & 56) & 0xFFull) != 0;
+            bad |= (((const uint32_t *)mi)[h.sr] & 0x7F800000u) == 0x7F800000u;
+        bad = (__ballot(bad) >> (lane0 & 56) & 0xFFull) != 0;
         tr_sync();                                     /* all have looked        */
-        if (speaks) {
-            mi[2 * TR_TILE + sr] = bad && row >= 0;
-            if (KVF == DSV4_GPU_KV_FP8 && bad) ((float *)mi)[TR_TILE + sr] = 0.0f;
+        if (ws == 0 && (h.home & 112) == 0) {
+            mi[TR_TILE + h.sr] = bad && !gone;
+            if (KVF == DSV4_GPU_KV_FP8 && (bad || gone)) ((float *)mi)[h.sr] = 0.0f;
         }
-        if (bad || row < 0)
+        if (bad || gone)
             for (int s = ws; s < L::SLABS; s += WS)
                 for (int n = 0; n < KT; n++)
-                    *(u32x4 *)(plane(buf) + n * L::PLANE + s * L::SLAB + home) =
+                    *(u32x4 *)(plane(buf) + n * L::PLANE + s * L::SLAB + h.home) =
                         u32x4{0u, 0u, 0u, 0u};
         tr_sync();
     };
 
     /* the first tiles' loads go out before q's */
-    int r0 = -1, r1 = -1, r2 = -1;
+    uint32_t ok = 0u, ok1 = 0u, ok2 = 0u;              /* of tiles i, i + 1, i + 2 */
     if (i0 < i1) {
-        r0 = find(i0);
-        r1 = find(i0 + 1);
+        ask(i0);
+        ok = there(i0);
         if constexpr (DMA) {
-            r2 = find(i0 + 2);
-            dma(r0, 0);
-            if (i0 + 1 < i1) dma(r1, 1);
+            dma(i0, 0);
+            ask(i0 + 1);
+            if (i0 + 1 < i1) {
+                ok1 = there(i0 + 1);
+                dma(i0 + 1, 1);
+            }
+            ask(i0 + 2);
         } else {
-            fetch(r0);
+            fetch(i0);
+            ask(i0 + 1);
         }
     }
 
-    /* q, a few chunks' loads at a time; elements past the row are zeroed by a
-     * mask in a register, as the many lane masks of comparisons would crowd out
-     * the scalar registers */
+    /* ---- q, a few chunks' loads at a time; elements past the row are zeroed by
+     *      a mask in a register, as the many lane masks of comparisons would
+     *      crowd out the scalar registers ---- */
     tr_bf8 q[NT][KC1];
     {
-        const T *qr = (const T *)a.q + (size_t)min(rq, R - 1) * a.dqk;
+        const int l16 = lane0 & 15, g = lane0 >> 4;
+        const T *qr = (const T *)a.q + (size_t)min(row0 + l16, R - 1) * a.dqk;
         constexpr int G = KC1 % 3 == 0 ? 3 : KC1 < 4 ? KC1 : 4;
         const int c0 = 32 * KC1 * half + 8 * g;
         if (a.qvec) {
@@ -476,72 +496,51 @@ k_tree(Dsv4TreeJob a)
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV1; v++) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    /* to powers of two; a scale of 0 becomes one that still turns the infinity of
+     * a masked score into a weight of 0 */
+    const float c2 = (a.scale != 0.0f ? a.scale : 1e-38f) * 1.44269504088896340736f;
+    const float blank = c2 > 0.0f ? -INFINITY : INFINITY;
 
-    const float c2 = a.scale * 1.44269504088896340736f;       /* to powers of two */
-    /* a lane's places in a slab: row l16's piece g for the scores (the other
-     * half of a slab at ^ 64), row 4 g + l16 / 4's four columns 4 (l16 % 4) for
-     * the values (the slab's other column tiles at ^ 32, 64 and 96) */
-    const int ka0 = l16 * 128 + 16 * (g ^ tr_swz(l16));
-    const int va0 = (4 * g + (l16 >> 2)) * 128 + 8 * (l16 & 1) +
-                    16 * ((l16 >> 1 & 1) ^ tr_swz(4 * g + (l16 >> 2)));
-    auto use = [&](int i, int buf) {
+    f32x4 s[2];                                        /* the scores of a tile   */
+    auto score = [&](int buf) {
         const unsigned char *t = plane(buf);
-        const int ka = tr_fresh(ka0), va = tr_fresh(va0);
-        const int *mi = (const int *)meta(buf);
-        /* unpaged, rows are missing past the cache's end alone */
-        uint32_t ok = 0xFFFFFFFFu;
-        bool masked = partial(i) || (i + 1) * TR_TILE > a.rows;
-        if (masked || a.pages) {
-            ok = (uint32_t)__ballot(mi[lane & 31] >= 0);
-            masked |= ok != 0xFFFFFFFFu;
-        }
-        if (masked) mend(buf);
-        if (!live) {                                   /* no rows of q: only the syncs */
-            if (SPLIT == 2) tr_sync();
-            return;
-        }
-
-        /* ---- S^T: one sum per order of the terms, so that the small ones do
-         *      not round at the size of the large ---- */
-        f32x4 so[2][PT], s[2];
+        /* row l16's piece g of a slab, and its other half's at ^ 64 */
+        const int ln = tr_fresh(lane0), l16 = ln & 15, g = ln >> 4;
+        const int ka = l16 * 128 + 16 * (g ^ tr_swz(l16));
+        /* one sum per order of the terms, so that the small ones do not round at
+         * the size of the large */
+        f32x4 so[2][PT];
 #pragma unroll
         for (int n = 0; n < PT; n++) so[0][n] = so[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int KG = 1;
-        tr_bf8 row[2][KG][KT][2];
         /* chunk kc of this wave's: the second half's first is chunk KC1 of the
          * row, in the upper half of a slab where KC1 is odd */
         const unsigned char *tk = t + half * (KC1 >> 1) * L::SLAB;
         const int kb = ka ^ (KC1 & 1 & half) * 64;
         const int up = (KC1 & 1 & half) * L::SLAB;
-        auto rows_of = [&](int kg, tr_bf8 (&r)[KG][KT][2]) {
+        /* reads of 16 keys' piece of a chunk, KD of them ahead of the products */
+        constexpr int KU = 2 * KC1, KD = KT > 1 ? 2 : KU < 6 ? KU : 6;
+        tr_bf8 row[KD][KT];
+        auto rows_of = [&](int u) {
+            const int kc = u >> 1;
 #pragma unroll
-            for (int u = 0; u < KG; u++)
-#pragma unroll
-                for (int p = 0; p < KT; p++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int kc = kg * KG + u;
-                        r[u][p][k] = *(const tr_bf8 *)(tk + p * L::PLANE + (kc >> 1) * L::SLAB +
-                                                       (kc & 1 ? up : 0) + k * 2048 +
-                                                       (kb ^ (kc & 1) * 64));
-                    }
+            for (int p = 0; p < KT; p++)
+                row[u % KD][p] = *(const tr_bf8 *)(tk + p * L::PLANE + (kc >> 1) * L::SLAB +
+                                                   (kc & 1 ? up : 0) + (u & 1) * 2048 +
+                                                   (kb ^ (kc & 1) * 64));
         };
-        rows_of(0, row[0]);
 #pragma unroll
-        for (int kg = 0; kg < KC1 / KG; kg++) {
-            if (kg + 1 < KC1 / KG) rows_of(kg + 1, row[(kg + 1) & 1]);
+        for (int u = 0; u < KD; u++) rows_of(u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+#pragma unroll
+            for (int p = 0; p < KT; p++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    if (n + p < PT)
+                        so[u & 1][n + p] = tr_mfma(row[u % KD][p], q[n][u >> 1], so[u & 1][n + p]);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int u = 0; u < KG; u++)
-#pragma unroll
-                for (int p = 0; p < KT; p++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        if (n + p < PT)
-#pragma unroll
-                            for (int k = 0; k < 2; k++)
-                                so[k][n + p] = tr_mfma(row[kg & 1][u][p][k], q[n][kg * KG + u],
-                                                       so[k][n + p]);
+            if (u + KD < KU) rows_of(u + KD);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -551,34 +550,42 @@ k_tree(Dsv4TreeJob a)
             for (int n = PT - 2; n >= 0; n--) s[k] += so[k][n];
         }
         if constexpr (SPLIT == 2) {
-            unsigned char *x = lds + L::HALF + 16 * lane;
+            unsigned char *x = lds + L::HALF + 16 * ln;
 #pragma unroll
             for (int k = 0; k < 2; k++) *(f32x4 *)(x + 1024 * (2 * w + k)) = s[k];
-            tr_sync();
+        }
+    };
+    auto value = [&](int i, int buf, bool masked) {
+        const unsigned char *t = plane(buf);
+        const int ln = tr_fresh(lane0), l16 = ln & 15, g = ln >> 4;
+        /* row 4 g + l16 / 4's columns 4 (l16 % 4) of a slab, and its other tiles of
+         * 16 columns at ^ 32, 64 and 96 */
+        const int vr = 4 * g + (l16 >> 2);
+        const int va = vr * 128 + 8 * (l16 & 1) + 16 * ((l16 >> 1 & 1) ^ tr_swz(vr));
+        const int *mi = (const int *)meta(buf);
+        if constexpr (SPLIT == 2) {
+            const unsigned char *x = lds + L::HALF + 16 * ln;
 #pragma unroll
             for (int k = 0; k < 2; k++) s[k] += *(const f32x4 *)(x + 1024 * (2 * (w ^ 4) + k));
         }
-
         /* the first columns of V, while the weights are computed */
-        constexpr int VG = KT > 1 ? 1 : 2;
+        constexpr int VD = KT > 1 ? 2 : NV1 < 5 ? NV1 : 5;
         const unsigned char *tv = t + half * (NV1 / 4) * L::SLAB;
-        tr_bf8 col[2][VG][KT];
-        auto cols_of = [&](int vg, tr_bf8 (&c)[VG][KT]) {
+        tr_bf8 col[VD][KT];
+        auto cols_of = [&](int v) {
 #pragma unroll
-            for (int u = 0; u < VG; u++)
-#pragma unroll
-                for (int p = 0; p < KT; p++) {
-                    const int v = vg * VG + u;
-                    const unsigned char *at =
-                        tv + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
-                    const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
-                    const tr_s4 y =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
-                    c[u][p] = __builtin_bit_cast(
-                        tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
+            for (int p = 0; p < KT; p++) {
+                const unsigned char *at =
+                    tv + p * L::PLANE + (v >> 2) * L::SLAB + (va ^ (v & 3) * 32);
+                const tr_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)at);
+                const tr_s4 y =
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_s4 *)(at + 2048));
+                col[v % VD][p] = __builtin_bit_cast(
+                    tr_bf8, (tr_s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
         };
-        cols_of(0, col[0]);
+#pragma unroll
+        for (int v = 0; v < VD; v++) cols_of(v);
         __builtin_amdgcn_sched_barrier(0);
 
         /* ---- the weights ---- */
@@ -586,18 +593,17 @@ k_tree(Dsv4TreeJob a)
         if (KVF == DSV4_GPU_KV_FP8) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                ks[k] = *(const f32x4 *)(mi + TR_TILE + 16 * k + 4 * g);
+                ks[k] = *(const f32x4 *)(mi + 16 * k + 4 * g);
                 s[k] *= ks[k];
             }
         }
-        uint32_t vis = ~0u;
         if (masked) {
-            const uint32_t no = (uint32_t)__ballot(mi[2 * TR_TILE + (lane & 31)] != 0);
+            const uint32_t no = (uint32_t)__ballot(mi[TR_TILE + (ln & 31)] != 0);
             const unsigned char *rs = lds + L::ROWS + 16 * (16 * w + l16);
             const unsigned long long see = *(const unsigned long long *)rs;
             const int lo = *(const int *)(rs + 8), p0 = i * TR_TILE;
             /* positions [lo, ctx) of the context, then the drafts' bits */
-            vis = 0u;
+            uint32_t vis = 0u;
             const int f = max(lo - p0, 0), e = min(a.ctx - p0, TR_TILE);
             if (f < e) vis = (e >= 32 ? ~0u : (1u << e) - 1u) & ~((1u << f) - 1u);
             const int d = p0 - a.ctx;
@@ -606,18 +612,18 @@ k_tree(Dsv4TreeJob a)
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (no >> (16 * k + 4 * g + j) & 1u) s[k][j] = __uint_as_float(0x7FC00000u);
-            vis >>= 4 * g;
+                for (int j = 0; j < 4; j++) {
+                    const int key = 16 * k + 4 * g + j;
+                    const float x = no >> key & 1u ? __uint_as_float(0x7FC00000u) : s[k][j];
+                    s[k][j] = vis >> key & 1u ? x : blank;
+                }
         }
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 2; k++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                float x = s[k][j] * c2;
-                if (masked) x = vis >> (16 * k + j) & 1u ? x : -INFINITY;
-                top = fmaxf(top, x);
+                top = fmaxf(top, s[k][j] * c2);
             }
         top = tr_max4(top);
         const bool grow = top > m + 8.0f;
@@ -634,8 +640,7 @@ k_tree(Dsv4TreeJob a)
         for (int k = 0; k < 2; k++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                float x = __builtin_amdgcn_exp2f(fmaf(s[k][j], c2, -mm));
-                if (masked) x = vis >> (16 * k + j) & 1u ? x : 0.0f;
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[k][j], c2, -mm));
                 sum += x;
                 e[4 * k + j] = KVF == DSV4_GPU_KV_FP8 ? x * ks[k][j] : x;
             }
@@ -645,54 +650,70 @@ k_tree(Dsv4TreeJob a)
 
         /* ---- O^T ---- */
 #pragma unroll
-        for (int vg = 0; vg < NV1 / VG; vg++) {
-            if (vg + 1 < NV1 / VG) cols_of(vg + 1, col[(vg + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int v = 0; v < NV1; v++) {
 #pragma unroll
             for (int p = 0; p < KT; p++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
-                    if (n + p < PT)
-#pragma unroll
-                        for (int u = 0; u < VG; u++)
-                            o[vg * VG + u] = tr_mfma(col[vg & 1][u][p], pw[n], o[vg * VG + u]);
+                    if (n + p < PT) o[v] = tr_mfma(col[v % VD][p], pw[n], o[v]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (v + VD < NV1) cols_of(v + VD);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    if constexpr (DMA) {
-        int buf = 0;
-        for (int i = i0; i < i1; i++) {
+
+    /* every token sees every position of tiles [ic0, ic1) */
+    const int ic0 = a.window ? (max(0, a.ctx + a.nt - a.window) + TR_TILE - 1) / TR_TILE : 0;
+    const int ic1 = a.ctx / TR_TILE;
+    if (!DMA && L::NBUF > 1 && i0 < i1) {
+        store(0);
+        if (i0 + 1 < i1) {
+            ok1 = there(i0 + 1);
+            fetch(i0 + 1);
+            ask(i0 + 2);
+        }
+    }
+    for (int i = i0; i < i1; i++) {
+        const int buf = slot(i);
+        /* tile i to where it can be used, and a later tile's loads out */
+        if constexpr (DMA) {
             dma_wait(i + 1 < i1);
-            tr_sync();                   /* tile i is in LDS, tile i - 1's buffer free */
+            tr_sync();                                 /* and tile i - 1's buffer free */
             if (i + 2 < i1) {
-                const int row = r2;
-                r2 = find(i + 3);
-                dma(row, buf == 0 ? 2 : buf - 1);
+                ok2 = there(i + 2);
+                dma(i + 2, buf == 0 ? 2 : buf - 1);
+                ask(i + 3);
             }
-            use(i, buf);
-            buf = buf == 2 ? 0 : buf + 1;
-        }
-    } else if (i0 < i1) {
-        store(r0, 0);
-        for (int i = i0; i < i1; i++) {
-            const int buf = L::NBUF == 2 ? (i - i0) & 1 : 0;
-            const bool more = i + 1 < i1;
-            const int row = r1;
+        } else if constexpr (L::NBUF > 1) {
             tr_sync();
-            if (more) {
-                fetch(row);
-                r1 = find(i + 2);
+            if (i + 1 < i1) store(buf ^ 1);
+            if (i + 2 < i1) {
+                ok2 = there(i + 2);
+                fetch(i + 2);
+                ask(i + 3);
             }
-            use(i, buf);
-            if (more) {
-                if (L::NBUF == 1) tr_sync();
-                store(row, L::NBUF == 2 ? buf ^ 1 : 0);
+        } else {
+            store(0);
+            if (i + 1 < i1) {
+                ok1 = there(i + 1);
+                fetch(i + 1);
+                ask(i + 2);
             }
+            tr_sync();
         }
+        const bool masked = i < ic0 || i >= ic1 || ok != ~0u;
+        if (masked) mend(buf, ok);
+        if (live) score(buf);
+        if (SPLIT == 2) tr_sync();
+        if (live) value(i, buf, masked);
+        if (L::NBUF == 1) tr_sync();
+        ok = ok1;
+        ok1 = ok2;
     }
 
     /* ---- the split's sums, or the result ---- */
+    const int ln = tr_fresh(lane0), g = ln >> 4, rq = row0 + (ln & 15);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (rq >= R) return;
@@ -730,7 +751,7 @@ k_tree(Dsv4TreeJob a)
 template <class T, int KVF, int KC>
 int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
 {
-    using L = TreeLds<KVF, KC>;
+    using L = TreeLds<KVF, KC, tree_split(tr_fmt<T>(), KVF, KC)>;
     if (L::BYTES > 64 * 1024) {
         /* once per device, as the attribute is the device's */
         static bool asked[64];
