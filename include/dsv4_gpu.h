@@ -596,7 +596,7 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  * window > 0 it sees only rows less than window places back (0: all). A
  * token that sees no row gets zeros. What a row holds does not reach tokens
  * that do not see it, NaN and infinities included; one that sees a row with
- * such an element gets NaN among its outputs.
+ * such an element may get NaN in any of its outputs.
  *
  * Scores, softmax and sums are in f32. With f32 q every product is exact
  * (bf16 terms of q and of the weights; an F32 cache's elements in three terms
@@ -640,7 +640,8 @@ typedef struct {
  * none is. Each step is rounded in f32 in the order above. d_out may be
  * d_logits, or NULL where only picks are wanted; d_pick may be NULL.
  * d_scratch: dsv4_gpu_logits_scratch_bytes of device memory, 16-byte aligned,
- * not kept. repetition must be over 0. 0 / -1. */
+ * not kept (without picks it may be NULL; long histories are then slower).
+ * repetition must be over 0. 0 / -1. */
 size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab);
 int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, int nt, int vocab,
                              long long stride, const dsv4_gpu_logit_rules *rules,

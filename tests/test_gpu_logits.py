@@ -154,3 +154,26 @@ def test_without_rules_the_pick_is_the_heads(gpu, dsv4):
         row = dc.dev(x[t])
         assert gpu.dsv4_gpu_argmax_d(tok.data_ptr(), row.data_ptr(), 20001, dc.stream()) == 0
         assert tok.item() == picks[t]
+
+
+@pytest.mark.parametrize("nt,vocab", [(1, 5), (1, 40001), (5, 8192), (64, 3001)])
+@pytest.mark.parametrize("hist", [24576, 24577, 100003])
+def test_long_histories(gpu, dsv4, nt, vocab, hist):
+    """Histories that a launch of their own counts, and the same without a
+    workspace, where only rows are asked for."""
+    import torch
+    rng = np.random.default_rng(nt * vocab + hist)
+    x = (rng.standard_normal((nt, vocab)) * 3).astype(np.float32)
+    ids = rng.integers(-3, vocab + 3, hist).astype(np.int32)
+    drafts = rng.integers(-1, vocab + 1, nt).astype(np.int32)
+    words = dc.words(rng, nt)
+    want = dc.logit_rules(x, ids, drafts, words, 1.3, 0.25, 0.5, None, None)
+    check(run(dsv4, x, ids, drafts, words, 1.3, 0.25, 0.5), want)
+    keep = [dc.dev(a) for a in (x, ids, drafts, np.array(words, np.uint64))]
+    out = torch.empty(nt, vocab, device="cuda:0")
+    r = dsv4.LogitRules(hist=dc.ptr(keep[1]), n_hist=hist, draft=dc.ptr(keep[2]),
+                        mask=dc.ptr(keep[3]), repetition=1.3, frequency=0.25, presence=0.5,
+                        bias=None, allow=None, allow_stride=0)
+    assert gpu.dsv4_gpu_logits_adjust_d(out.data_ptr(), None, dc.ptr(keep[0]), nt, vocab, vocab,
+                                        ctypes.byref(r), None, 0, dc.stream()) == 0
+    assert common.bits_equal(dc.host(out), want[0])
