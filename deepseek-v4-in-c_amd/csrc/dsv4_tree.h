@@ -27,7 +27,7 @@ struct Dsv4TreeJob {
     float scale;
     /* set by the plan: tiles [tile0, tile1) in ns splits of the rows of q's nb
      * blocks; part [ns][nt h][dvp] and its maxima and sums [ns][nt h] */
-    int tile0, tile1, ns, nb, dvp;
+    int tile0, tile1, ns, nb, br, dvp;
     float *part, *pm, *pl;
     int vec, qvec, ovec;                          /* whole pieces            */
 };
@@ -200,11 +200,13 @@ k_tree(Dsv4TreeJob a)
     constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : 2;
     constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : KVF == DSV4_GPU_KV_BF16 ? 2 : 1;
     constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
+    /* where the next tile and all of q are in registers, few are left */
+    constexpr bool SHALLOW = NT == 1 && KVF == DSV4_GPU_KV_FP8 && KC >= 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane0 = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int ws = w >> 2;
-    const int qb = SPLIT == 2 ? w & 3 : w, half = SPLIT == 2 ? ws : 0;
+    const int qb = w / SPLIT, half = w % SPLIT;
 
     /* Workgroup i runs on XCD i mod 8: each XCD takes a run of (split, block)
      * in split order, so blocks that read the same rows share its L2. */
@@ -219,25 +221,8 @@ k_tree(Dsv4TreeJob a)
         i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
     }
     const int R = a.nt * a.h, end = a.ctx + a.nt;
-    const int row0 = (blk * (W / SPLIT) + qb) * 16;    /* this wave's rows of q  */
-    const bool live = row0 < R;
-
-    /* ---- the drafts that the token of each row of q sees, and the first
-     *      position ---- */
-    if (lane0 < 16) {
-        const int t = min(row0 + lane0, R - 1) / a.h;
-        const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
-        unsigned long long see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
-        const int depth = __popcll(see & ~(1ull << t));
-        if (a.window && a.window < a.nt)
-            for (int j = 0; j < a.nt; j++) {
-                const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
-                if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
-            }
-        unsigned char *d = lds + L::ROWS + 16 * (16 * w + lane0);
-        *(unsigned long long *)d = see;
-        *(int *)(d + 8) = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
-    }
+    const int row0 = blk * a.br + qb * 16;             /* this wave's rows of q  */
+    const bool live = 16 * qb < a.br && row0 < R;
 
     /* ---- staging: a thread has place (lane % 8) of row sr of slabs ws, ws + WS,
      *      ... of a tile, which is piece (lane % 8) ^ (sr & 7) of 64 columns.
@@ -437,14 +422,16 @@ k_tree(Dsv4TreeJob a)
         }
     }
 
-    /* ---- q, a few chunks' loads at a time; elements past the row are zeroed by
+    /* ---- q, its loads all on their way at once, or a few chunks' where the first
+     *      tile's f32 rows are in registers; elements past the row are zeroed by
      *      a mask in a register, as the many lane masks of comparisons would
      *      crowd out the scalar registers ---- */
     tr_bf8 q[NT][KC1];
-    {
+    if (live) {
         const int l16 = lane0 & 15, g = lane0 >> 4;
         const T *qr = (const T *)a.q + (size_t)min(row0 + l16, R - 1) * a.dqk;
-        constexpr int G = KC1 % 3 == 0 ? 3 : KC1 < 4 ? KC1 : 4;
+        constexpr int G = KVF != DSV4_GPU_KV_F32 ? KC1 : KC1 % 3 == 0 ? KC1 / 3 : 4;
+        static_assert(KC1 % G == 0, "whole groups");
         const int c0 = 32 * KC1 * half + 8 * g;
         if (a.qvec) {
 #pragma unroll
@@ -492,6 +479,23 @@ k_tree(Dsv4TreeJob a)
             }
         }
     }
+    /* ---- the drafts that the token of each row of q sees, and the first
+     *      position ---- */
+    if (lane0 < 16) {
+        const int t = min(row0 + lane0, R - 1) / a.h;
+        const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
+        unsigned long long see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
+        const int depth = __popcll(see & ~(1ull << t));
+        if (a.window && a.window < a.nt)
+            for (int j = 0; j < a.nt; j++) {
+                const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
+                if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
+            }
+        unsigned char *d = lds + L::ROWS + 16 * (16 * w + lane0);
+        *(unsigned long long *)d = see;
+        *(int *)(d + 8) = a.window ? max(0, a.ctx + depth - a.window + 1) : 0;
+    }
+
     f32x4 o[NV1];
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -518,7 +522,7 @@ k_tree(Dsv4TreeJob a)
         const int kb = ka ^ (KC1 & 1 & half) * 64;
         const int up = (KC1 & 1 & half) * L::SLAB;
         /* reads of 16 keys' piece of a chunk, KD of them ahead of the products */
-        constexpr int KU = 2 * KC1, KD = KT > 1 ? 2 : KU < 6 ? KU : 6;
+        constexpr int KU = 2 * KC1, KD = KT > 1 || SHALLOW ? 2 : KU < 6 ? KU : 6;
         tr_bf8 row[KD][KT];
         auto rows_of = [&](int u) {
             const int kc = u >> 1;
@@ -566,10 +570,10 @@ k_tree(Dsv4TreeJob a)
         if constexpr (SPLIT == 2) {
             const unsigned char *x = lds + L::HALF + 16 * ln;
 #pragma unroll
-            for (int k = 0; k < 2; k++) s[k] += *(const f32x4 *)(x + 1024 * (2 * (w ^ 4) + k));
+            for (int k = 0; k < 2; k++) s[k] += *(const f32x4 *)(x + 1024 * (2 * (w ^ 1) + k));
         }
         /* the first columns of V, while the weights are computed */
-        constexpr int VD = KT > 1 ? 2 : NV1 < 5 ? NV1 : 5;
+        constexpr int VD = KT > 1 || SHALLOW ? 2 : NV1 < 5 ? NV1 : 5;
         const unsigned char *tv = t + half * (NV1 / 4) * L::SLAB;
         tr_bf8 col[VD][KT];
         auto cols_of = [&](int v) {
@@ -716,7 +720,7 @@ k_tree(Dsv4TreeJob a)
     const int ln = tr_fresh(lane0), g = ln >> 4, rq = row0 + (ln & 15);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if (rq >= R) return;
+    if (!live || rq >= R) return;
     if (a.ns > 1) {
         const size_t at = (size_t)split * R + rq;
         if (g == 0 && half == 0) {

@@ -92,14 +92,21 @@ const char *tree_bad(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int 
 }
 
 struct TreePlan {
-    int kc, tile0, tile1, nb, cap, ns, dvp;
+    int kc, tile0, tile1, nb, br, cap, ns, dvp;
     size_t bytes;
 };
 
-/* The splits of a call: up to `cap`, two tiles each at least and 512 workgroups
- * in all; of those the number whose last round of workgroups over the card's
- * 256 CUs ends first, a workgroup taking its tiles and some eight tiles' time
- * around them. */
+/* Rows of q of a workgroup and splits of the cache, by what a workgroup takes, in
+ * halves of the time of a tile on a lone wave (0.55 us for bf16 q over 576
+ * columns, 0.8 for f32 q): 2 a tile for up to four waves with rows of q and 3 for
+ * eight; 8 for the start and 2 for each such wave's q and sums; 5 for the join's
+ * launch and 1 for each 4 MB of its sums. A workgroup has a CU to itself, so
+ * beyond 256 they come in rounds. Few rows are thus spread over workgroups of 16
+ * of them and read the cache through L2 as often, until the splits fill the
+ * card; then wider ones win. Measured, one token's 64 heads of f32 q over a bf16
+ * cache, at the best split for 16, 32 and 64 rows a workgroup: 16.0, 17.8 and 23.4 us
+ * at 1500 rows of cache, 21.4, 23.2, 28.7 at 8192, 41.9, 34.3, 39.0 at 32768, 122,
+ * 77, 74 at 131072. */
 TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_ctx, int window)
 {
     TreePlan p;
@@ -108,22 +115,30 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
     p.tile0 = lo / TR_TILE;
     p.tile1 = (n_ctx + nt + TR_TILE - 1) / TR_TILE;
     const int tiles = p.tile1 - p.tile0, br = dsv4_tree_block_rows(fmt, kv_fmt, p.kc);
-    p.nb = (nt * h + br - 1) / br;
+    const int wide = (nt * h + br - 1) / br;
     p.dvp = (d_v + 15) / 16 * 16;
     /* the workspace goes by the cap alone, and by the most tiles that a
      * context of this length can have */
     const int most = window ? (window + nt) / TR_TILE + 2 : tiles;
     const int up = tiles < most ? tiles : most;
-    p.cap = up / 2 < 512 / p.nb ? up / 2 : 512 / p.nb;
+    p.cap = up / 2 < 512 / wide ? up / 2 : 512 / wide;
     if (p.cap < 1) p.cap = 1;
-    p.ns = 1;
     long long best = -1;
-    for (int s = 1; s <= p.cap; s++) {
-        const long long rounds = ((long long)p.nb * s + 255) / 256;
-        const long long cost = rounds * ((tiles + s - 1) / s + 8);
-        if (best < 0 || cost < best) {
+    for (int r = 16; r <= br; r *= 2) {
+        const int nb = (nt * h + r - 1) / r, waves = r / 16 * tree_split(fmt, kv_fmt, p.kc);
+        for (int k = 0; k < 4; k++) {
+            long long ns = 256ll * ((nb + 255) / 256 + k) / nb;
+            if (ns > p.cap) ns = p.cap;
+            const long long each = (tiles + ns - 1) / ns;
+            ns = (tiles + each - 1) / each;
+            const long long rounds = (nb * ns + 255) / 256;
+            const long long cost = rounds * (each * (waves > 4 ? 3 : 2) + 8 + 2 * waves) +
+                                   (ns > 1 ? 5 + ((ns * nt * h * p.dvp) >> 20) : 0);
+            if (best >= 0 && cost >= best) continue;
             best = cost;
-            p.ns = s;
+            p.br = r;
+            p.nb = nb;
+            p.ns = (int)ns;
         }
     }
     p.bytes = p.cap > 1 ? (size_t)p.cap * nt * h * (p.dvp + 2) * sizeof(float) : 0;
@@ -209,6 +224,7 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
     a.tile1 = p.tile1;
     a.ns = p.ns;
     a.nb = p.nb;
+    a.br = p.br;
     a.dvp = p.dvp;
     a.part = (float *)d_scratch;
     a.pm = a.part + (size_t)p.ns * nt * h * p.dvp;
