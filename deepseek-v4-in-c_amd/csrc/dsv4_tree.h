@@ -678,25 +678,28 @@ k_tree(Dsv4TreeJob a)
             ask(i0 + 2);
         }
     }
+    /* a later tile's loads out, and for formats that pass registers the next one
+     * to LDS. Of the two waves of a SIMD one does so before its scores and one
+     * after them, while the other's products run. */
+    auto next = [&](int i, int buf) {
+        if constexpr (DMA) {
+            if (i + 2 >= i1) return;
+            dma(i + 2, buf == 0 ? 2 : buf - 1);
+            ask(i + 3);
+        } else {
+            if (i + 1 < i1) store(buf ^ 1);
+            if (i + 2 >= i1) return;
+            fetch(i + 2);
+            ask(i + 3);
+        }
+    };
     for (int i = i0; i < i1; i++) {
         const int buf = slot(i);
-        /* tile i to where it can be used, and a later tile's loads out */
-        if constexpr (DMA) {
-            dma_wait(i + 1 < i1);
-            tr_sync();                                 /* and tile i - 1's buffer free */
-            if (i + 2 < i1) {
-                ok2 = there(i + 2);
-                dma(i + 2, buf == 0 ? 2 : buf - 1);
-                ask(i + 3);
-            }
-        } else if constexpr (L::NBUF > 1) {
-            tr_sync();
-            if (i + 1 < i1) store(buf ^ 1);
-            if (i + 2 < i1) {
-                ok2 = there(i + 2);
-                fetch(i + 2);
-                ask(i + 3);
-            }
+        if constexpr (L::NBUF > 1) {
+            if (DMA) dma_wait(i + 1 < i1);
+            tr_sync();                                 /* tile i there, i - 1 used */
+            if (i + 2 < i1) ok2 = there(i + 2);
+            if (ws == 0) next(i, buf);
         } else {
             store(0);
             if (i + 1 < i1) {
@@ -709,6 +712,7 @@ k_tree(Dsv4TreeJob a)
         const bool masked = i < ic0 || i >= ic1 || ok != ~0u;
         if (masked) mend(buf, ok);
         if (live) score(buf);
+        if (L::NBUF > 1 && ws == 1) next(i, buf);
         if (SPLIT == 2) tr_sync();
         if (live) value(i, buf, masked);
         if (L::NBUF == 1) tr_sync();
