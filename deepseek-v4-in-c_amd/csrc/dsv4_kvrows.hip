@@ -13,9 +13,13 @@
  * again), so writing it again keeps its values.
  * Bound: x read once (twice past 768 elements), the codes written once. One
  * row per wave keeps the maximum in registers: no LDS, no second launch.
- * Where two tokens name one row the later is written: each workgroup looks
- * its rows up among the later entries of the list, which costs the list's
- * bytes once per four rows, from the L2.
+ * Where two tokens name one row the later is written. A workgroup compares the
+ * later entries of a short list with its four tokens' rows; with a long one it
+ * hashes its tokens' rows into LDS and looks the entries up there, so that one
+ * costs an LDS read however many tokens the workgroup has, and it takes more
+ * of them, 256 at most, as the list grows: of rows of 512 f32 to FP8, 2000 take
+ * 4.4 us compared and 4.8 looked up, 6000 9.1 and 8.2, 60000 270 and 46 (29 where
+ * they follow row0); of rows of 32, 118000 take 824 and 70.
  *
  * READ. A thread makes 16 bytes of output at a time, so that stores, the
  * larger stream from an FP8 cache, are whole lines; four such pieces per
@@ -31,6 +35,7 @@ namespace {
 constexpr int KR_THREADS = 256;
 constexpr int KR_ROWS = KR_THREADS / 64;          /* rows per workgroup      */
 constexpr int KR_DIM = 16384;                     /* the longest row         */
+constexpr int KR_MOST = 1 << 30;                  /* most rows of a call     */
 
 struct AppendJob {
     void *kv;
@@ -43,7 +48,64 @@ struct AppendJob {
     int row0;
     const int *pos;                               /* nullptr: not rotated    */
     dsv4_gpu_rope rp;
+    int tok;                                      /* tokens of a workgroup   */
 };
+
+constexpr int AP_WAVES = 16;                      /* of a workgroup with a list */
+constexpr int AP_TOK = 256;                       /* its most tokens         */
+constexpr int AP_BITS = 12;                       /* slots, 16 a token at least */
+constexpr int AP_SHORT = 4096;                    /* lists that are compared */
+enum { AP_NONE, AP_COMPARE, AP_HASH };            /* what a list takes       */
+
+__device__ __forceinline__ uint32_t row_slot(int row)
+{
+    return ((uint32_t)row * 2654435761u) >> (32 - AP_BITS);
+}
+
+/* late[k] for tokens t0 + k of a workgroup, k < tok: a later token of the list
+ * names the same row. The table holds the last of the workgroup's tokens for
+ * each row. */
+__device__ __forceinline__ void find_late(const int *list, int n, int kv_rows, int t0, int tok,
+                                          int *row, int *late, int *tbl)
+{
+    const int tid = threadIdx.x, nth = blockDim.x;
+    for (int i = tid; i < 1 << AP_BITS; i += nth) tbl[i] = -1;
+    for (int k = tid; k < tok; k += nth) {
+        row[k] = t0 + k < n ? list[t0 + k] : -1;
+        late[k] = 0;
+    }
+    __syncthreads();
+    for (int k = tid; k < tok; k += nth) {
+        const int r = row[k];
+        if (r < 0 || r >= kv_rows) continue;
+        /* a slot's row does not change once it is taken, and at most 256 of the
+         * 4096 are, so this ends */
+        for (uint32_t s = row_slot(r);; s = (s + 1) & ((1 << AP_BITS) - 1)) {
+            const int was = atomicCAS(&tbl[s], -1, k);
+            if (was == -1) break;
+            if (row[was] != r) continue;
+            late[min(k, atomicMax(&tbl[s], k))] = 1;
+            break;
+        }
+    }
+    __syncthreads();
+    constexpr int G = 4;                          /* loads in flight         */
+    for (int j = t0 + tok + tid; j < n; j += G * nth) {
+        int r[G];
+#pragma unroll
+        for (int u = 0; u < G; u++) r[u] = list[min(j + u * nth, n - 1)];
+#pragma unroll
+        for (int u = 0; u < G; u++) {             /* the last entry again: no harm */
+            uint32_t s = row_slot(r[u]);
+            for (int k; (k = tbl[s]) >= 0; s = (s + 1) & ((1 << AP_BITS) - 1))
+                if (row[k] == r[u]) {
+                    late[k] = 1;
+                    break;
+                }
+        }
+    }
+    __syncthreads();
+}
 
 /* Elements c .. c + V - 1 of a row, rotated by the table row r (nullptr
  * tables: a position outside them). */
@@ -137,39 +199,95 @@ __device__ __forceinline__ void row_store(const AppendJob &a, size_t at, const f
 
 /* NC pieces of V per lane kept in registers between the maximum and the
  * store (the row is no longer than 64 V NC); NC 0: read again. */
-template <class T, int KVF, int V, int NC>
-__global__ void __launch_bounds__(KR_THREADS) k_append(AppendJob a)
+template <class T, int KVF, int V, int NC, int LIST>
+__global__ void __launch_bounds__(LIST == AP_HASH ? 64 * AP_WAVES : KR_THREADS)
+k_append(AppendJob a)
 {
-    __shared__ int late[KR_ROWS];
+    constexpr int WV = LIST == AP_HASH ? AP_WAVES : KR_ROWS;
+    __shared__ int late[LIST == AP_HASH ? AP_TOK : KR_ROWS];
+    __shared__ int lrow[LIST == AP_HASH ? AP_TOK : 1];
+    __shared__ int tbl[LIST == AP_HASH ? 1 << AP_BITS : 1];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int t0 = blockIdx.x * KR_ROWS, t = t0 + w;
-    const bool live = t < a.n;
-    const int row = !live ? -1 : a.rows ? a.rows[t] : a.row0 + t;
-    const T *x = (const T *)a.x + (live ? t : 0) * a.xs;
-    const float *cs = nullptr, *sn = nullptr;
-    if (a.pos && live) {
-        const int p = a.pos[t];
-        if (p >= 0 && p < a.rp.max_pos) {
-            cs = a.rp.cos + (size_t)p * (a.rp.dim / 2);
-            sn = a.rp.sin + (size_t)p * (a.rp.dim / 2);
-        }
-    }
+    const int t0 = blockIdx.x * (LIST == AP_HASH ? a.tok : KR_ROWS);
     constexpr int KEEP = NC > 0 ? NC : 1;
     float v[KEEP][V];
-    if constexpr (NC > 0) {
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-            const int c = (i * 64 + lane) * V;
-            if (live && c < a.dim) {
-                row_values<T, V>(a, x, c, cs, sn, v[i]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; k++) v[i][k] = 0.0f;
+    const float *cs, *sn;
+    auto load = [&](int t) {
+        cs = sn = nullptr;
+        if (a.pos) {
+            const int p = a.pos[t];
+            if (p >= 0 && p < a.rp.max_pos) {
+                cs = a.rp.cos + (size_t)p * (a.rp.dim / 2);
+                sn = a.rp.sin + (size_t)p * (a.rp.dim / 2);
             }
         }
+        if constexpr (NC > 0) {
+            const T *x = (const T *)a.x + t * a.xs;
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int c = (i * 64 + lane) * V;
+                if (c < a.dim) {
+                    row_values<T, V>(a, x, c, cs, sn, v[i]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; k++) v[i][k] = 0.0f;
+                }
+            }
+        }
+    };
+    auto store = [&](int t, int row) {
+        const T *x = (const T *)a.x + t * a.xs;
+        const size_t at = (size_t)row * a.kv_stride;
+        float inv = 1.0f;
+        if constexpr (KVF == DSV4_GPU_KV_FP8) {
+            float top = 0.0f;
+            if constexpr (NC > 0) {
+#pragma unroll
+                for (int i = 0; i < NC; i++)
+#pragma unroll
+                    for (int k = 0; k < V; k++)
+                        if (finite_f(v[i][k])) top = fmaxf(top, fabsf(v[i][k]));
+            } else {
+                for (int c = lane * V; c < a.dim; c += 64 * V) {
+                    row_values<T, V>(a, x, c, cs, sn, v[0]);
+#pragma unroll
+                    for (int k = 0; k < V; k++)
+                        if (finite_f(v[0][k])) top = fmaxf(top, fabsf(v[0][k]));
+                }
+            }
+            top = wave_max(top);
+            float s;
+            row_scale(top, &s, &inv);
+            if (lane == 0) a.scales[row] = s;
+        }
+        if constexpr (NC > 0) {
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int c = (i * 64 + lane) * V;
+                if (c < a.dim) row_store<KVF, V>(a, at + c, v[i], inv);
+            }
+        } else {
+            for (int c = lane * V; c < a.dim; c += 64 * V) {
+                row_values<T, V>(a, x, c, cs, sn, v[0]);
+                row_store<KVF, V>(a, at + c, v[0], inv);
+            }
+        }
+    };
+    /* the first row's loads are out while the list is looked through */
+    const int t = t0 + w;
+    if (t < a.n) load(t);
+    if constexpr (LIST == AP_HASH) {
+        find_late(a.rows, a.n, a.kv_rows, t0, a.tok, lrow, late, tbl);
+        for (int k = w; k < a.tok && t0 + k < a.n; k += WV) {
+            const int row = lrow[k];
+            if (row < 0 || row >= a.kv_rows || late[k]) continue;
+            if (k != w) load(t0 + k);
+            store(t0 + k, row);
+        }
+        return;
     }
-    if (a.rows) {
+    if constexpr (LIST == AP_COMPARE) {
         if (threadIdx.x < KR_ROWS) late[threadIdx.x] = 0;
         __syncthreads();
         int mine[KR_ROWS];
@@ -184,42 +302,9 @@ __global__ void __launch_bounds__(KR_THREADS) k_append(AppendJob a)
         __syncthreads();
         if (late[w]) return;
     }
-    if (!live || row < 0 || row >= a.kv_rows) return;
-    const size_t at = (size_t)row * a.kv_stride;
-    float inv = 1.0f;
-    if constexpr (KVF == DSV4_GPU_KV_FP8) {
-        float top = 0.0f;
-        if constexpr (NC > 0) {
-#pragma unroll
-            for (int i = 0; i < NC; i++)
-#pragma unroll
-                for (int k = 0; k < V; k++)
-                    if (finite_f(v[i][k])) top = fmaxf(top, fabsf(v[i][k]));
-        } else {
-            for (int c = lane * V; c < a.dim; c += 64 * V) {
-                row_values<T, V>(a, x, c, cs, sn, v[0]);
-#pragma unroll
-                for (int k = 0; k < V; k++)
-                    if (finite_f(v[0][k])) top = fmaxf(top, fabsf(v[0][k]));
-            }
-        }
-        top = wave_max(top);
-        float s;
-        row_scale(top, &s, &inv);
-        if (lane == 0) a.scales[row] = s;
-    }
-    if constexpr (NC > 0) {
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-            const int c = (i * 64 + lane) * V;
-            if (c < a.dim) row_store<KVF, V>(a, at + c, v[i], inv);
-        }
-    } else {
-        for (int c = lane * V; c < a.dim; c += 64 * V) {
-            row_values<T, V>(a, x, c, cs, sn, v[0]);
-            row_store<KVF, V>(a, at + c, v[0], inv);
-        }
-    }
+    if (t >= a.n) return;
+    const int row = LIST == AP_NONE ? a.row0 + t : a.rows[t];
+    if (row >= 0 && row < a.kv_rows) store(t, row);
 }
 
 struct ReadJob {
@@ -299,24 +384,34 @@ int cache_ok(const char *what, const void *kv, const float *scales, int fmt, int
 
 int kv_size(int fmt) { return fmt == DSV4_GPU_KV_F32 ? 4 : fmt == DSV4_GPU_KV_BF16 ? 2 : 1; }
 
-template <class T, int KVF>
+template <class T, int KVF, int LIST>
 void append_launch(const AppendJob &a, int V, hipStream_t st)
 {
-    const dim3 g((a.n + KR_ROWS - 1) / KR_ROWS), b(KR_THREADS);
+    const int tok = LIST == AP_HASH ? a.tok : KR_ROWS;
+    const dim3 g((unsigned)(((long long)a.n + tok - 1) / tok));
+    const dim3 b(LIST == AP_HASH ? 64 * AP_WAVES : KR_THREADS);
     if (V == 1)
-        hipLaunchKernelGGL((k_append<T, KVF, 1, 0>), g, b, 0, st, a);
+        hipLaunchKernelGGL((k_append<T, KVF, 1, 0, LIST>), g, b, 0, st, a);
     else if (a.dim <= 64 * 4 * 3)
-        hipLaunchKernelGGL((k_append<T, KVF, 4, 3>), g, b, 0, st, a);
+        hipLaunchKernelGGL((k_append<T, KVF, 4, 3, LIST>), g, b, 0, st, a);
     else
-        hipLaunchKernelGGL((k_append<T, KVF, 4, 0>), g, b, 0, st, a);
+        hipLaunchKernelGGL((k_append<T, KVF, 4, 0, LIST>), g, b, 0, st, a);
+}
+
+template <class T, int KVF>
+void append_list(const AppendJob &a, int V, hipStream_t st)
+{
+    if (!a.rows) append_launch<T, KVF, AP_NONE>(a, V, st);
+    else if (a.n <= AP_SHORT) append_launch<T, KVF, AP_COMPARE>(a, V, st);
+    else append_launch<T, KVF, AP_HASH>(a, V, st);
 }
 
 template <class T>
 void append_fmt(const AppendJob &a, int fmt, int V, hipStream_t st)
 {
-    if (fmt == DSV4_GPU_KV_F32) append_launch<T, DSV4_GPU_KV_F32>(a, V, st);
-    else if (fmt == DSV4_GPU_KV_BF16) append_launch<T, DSV4_GPU_KV_BF16>(a, V, st);
-    else append_launch<T, DSV4_GPU_KV_FP8>(a, V, st);
+    if (fmt == DSV4_GPU_KV_F32) append_list<T, DSV4_GPU_KV_F32>(a, V, st);
+    else if (fmt == DSV4_GPU_KV_BF16) append_list<T, DSV4_GPU_KV_BF16>(a, V, st);
+    else append_list<T, DSV4_GPU_KV_FP8>(a, V, st);
 }
 
 template <class T, int V>
@@ -341,7 +436,7 @@ extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, 
 {
     if (cache_ok("kv_append", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
         return -1;
-    if (n < 0 || row_dim > KR_DIM || x_stride < row_dim ||
+    if (n < 0 || n > KR_MOST || row_dim > KR_DIM || x_stride < row_dim ||
         (x_fmt != DSV4_WF32 && x_fmt != DSV4_WBF16) || (n && !d_x)) {
         DSV4_ERR("kv_append: bad arguments (n %d, row_dim %d, x_fmt %d, x_stride %lld)", n,
                  row_dim, x_fmt, x_stride);
@@ -362,7 +457,10 @@ extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, 
     }
     if (n == 0) return 0;
     AppendJob a{d_kv, d_kv_scales, kv_stride, kv_rows, d_x, x_stride, n, row_dim, d_rows, row0,
-                rope ? d_pos : nullptr, rope ? *rope : dsv4_gpu_rope{}};
+                rope ? d_pos : nullptr, rope ? *rope : dsv4_gpu_rope{}, 0};
+    /* a long list's workgroups: 512 of them fill the card's waves */
+    const int per = n / (AP_WAVES * 512) + 1;
+    a.tok = AP_WAVES * (per < AP_TOK / AP_WAVES ? per : AP_TOK / AP_WAVES);
     /* pieces of four elements where the shapes and addresses are whole ones */
     const int xs = x_fmt == DSV4_WBF16 ? 2 : 4;
     int V = 4;
@@ -385,8 +483,8 @@ extern "C" int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride
 {
     if (cache_ok("kv_read", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
         return -1;
-    if (n < 0 || row_dim > KR_DIM || out_stride < row_dim || (out_fmt != DSV4_WF32 && out_fmt != DSV4_WBF16) ||
-        (n && !d_out)) {
+    if (n < 0 || n > KR_MOST || row_dim > KR_DIM || out_stride < row_dim ||
+        (out_fmt != DSV4_WF32 && out_fmt != DSV4_WBF16) || (n && !d_out)) {
         DSV4_ERR("kv_read: bad arguments (n %d, row_dim %d, out_fmt %d, out_stride %lld)", n,
                  row_dim, out_fmt, out_stride);
         return -1;

@@ -310,7 +310,7 @@ extern "C" int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *
                  stride);
         return -1;
     }
-    if (rules->n_hist < 0 || (rules->n_hist && !rules->hist) || !(rules->repetition > 0.0f) ||
+    if (rules->n_hist < 0 || rules->n_hist > 1 << 30 || (rules->n_hist && !rules->hist) || !(rules->repetition > 0.0f) ||
         (rules->allow && rules->allow_stride &&
          rules->allow_stride < (int)(((long long)vocab + 31) / 32))) {
         DSV4_ERR("logits_adjust: bad rules (n_hist %d, repetition %g, allow_stride %d)",

@@ -142,7 +142,7 @@ extern "C" int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *
                                  void *stream)
 {
     const long long width = (long long)heads * head_dim;
-    if (nt < 0 || heads <= 0 || head_dim <= 0 || x_stride < width || out_stride < width ||
+    if (nt < 0 || nt > 1 << 30 || heads <= 0 || head_dim <= 0 || x_stride < width || out_stride < width ||
         width > INT32_MAX / 2 || (fmt != DSV4_WF32 && fmt != DSV4_WBF16)) {
         DSV4_ERR("rope: bad arguments (nt %d, heads %d, head_dim %d, fmt %d, strides %lld, %lld)",
                  nt, heads, head_dim, fmt, x_stride, out_stride);

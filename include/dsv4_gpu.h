@@ -547,8 +547,8 @@ typedef struct {
  * to the type of x and out (fmt DSV4_WF32 or DSV4_WBF16). Elements outside
  * the rotated part are copied. d_out may be d_x (with the same stride: the
  * other elements then are not touched), but not overlap it otherwise. A
- * position outside [0, max_pos) makes the token's rotated elements NaN. 0 /
- * -1. */
+ * position outside [0, max_pos) makes the token's rotated elements NaN. nt is
+ * at most 2^30. 0 / -1. */
 int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long long x_stride,
                       int fmt, const int *d_pos, int nt, int heads, int head_dim,
                       const dsv4_gpu_rope *rope, int inverse, void *stream);
@@ -563,8 +563,8 @@ int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long l
  * the least power of two, 2^-126 at least, that brings the row's largest
  * finite magnitude to 448 or less (1 for a row of zeros); infinities and NaN
  * are stored as NaN. Rows written, read back and written again keep their
- * values. kv_stride >= row_dim, which is at most 16384. d_x must not overlap
- * the cache. 0 / -1. */
+ * values. kv_stride >= row_dim, which is at most 16384, and n at most 2^30.
+ * d_x must not overlap the cache. 0 / -1. */
 int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
                          const void *d_x, int x_fmt, long long x_stride, int n, int row_dim,
                          const int *d_rows, int row0, const dsv4_gpu_rope *rope,
@@ -573,7 +573,8 @@ int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stri
 /* Read n cache rows back as f32 or bf16 (out_fmt): d_out + t * out_stride =
  * row d_rows[t] (row0 + t where d_rows is NULL), an FP8 element as code *
  * scale in f32, rounded to nearest even for bf16. A row outside [0, kv_rows)
- * gives zeros and is never read. row_dim is at most 16384. 0 / -1. */
+ * gives zeros and is never read. row_dim is at most 16384, n at most 2^30.
+ * 0 / -1. */
 int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const void *d_kv,
                        const float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
                        const int *d_rows, int row0, int n, int row_dim, void *stream);
@@ -641,7 +642,7 @@ typedef struct {
  * d_logits, or NULL where only picks are wanted; d_pick may be NULL.
  * d_scratch: dsv4_gpu_logits_scratch_bytes of device memory, 16-byte aligned,
  * not kept (without picks it may be NULL; long histories are then slower).
- * repetition must be over 0. 0 / -1. */
+ * repetition must be over 0, n_hist at most 2^30. 0 / -1. */
 size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab);
 int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, int nt, int vocab,
                              long long stride, const dsv4_gpu_logit_rules *rules,

@@ -41,17 +41,17 @@ CALLS = {
         dict(rope=rope(max_pos=0)), dict(rope=rope(dim=31)), dict(rope=rope(dim=0)),
         dict(rope=rope(dim=-2)), dict(rope=rope(offset=-1)), dict(rope=rope(offset=33)),
         dict(rope=rope(dim=66)), dict(rope=rope(layout=2)), dict(rope=rope(offset=2 ** 31 - 1)),
-        dict(heads=1 << 16, hd=1 << 16, xs=BIG, os=BIG)], dict(nt=0)),
+        dict(heads=1 << 16, hd=1 << 16, xs=BIG, os=BIG), dict(nt=(1 << 30) + 1)], dict(nt=0)),
     "dsv4_gpu_kv_append_d": (APPEND, [
         dict(kv=None), dict(ks=None), dict(fmt=3), dict(fmt=-1), dict(stride=63), dict(rows=0),
         dict(x=None), dict(xf=2), dict(xs=63), dict(n=-1), dict(dim=0),
         dict(dim=16385, stride=16385, xs=16385), dict(at=None, row0=7), dict(at=None, row0=-1),
         dict(at=None, row0=2 ** 31 - 1), dict(pos=None), dict(rope=rope(dim=66)),
-        dict(rope=rope(layout=-1)), dict(rope=rope(cos=None))], dict(n=0)),
+        dict(rope=rope(layout=-1)), dict(rope=rope(cos=None)), dict(n=(1 << 30) + 1)], dict(n=0)),
     "dsv4_gpu_kv_read_d": (READ, [
         dict(kv=None), dict(ks=None), dict(fmt=3), dict(stride=63), dict(rows=0), dict(out=None),
         dict(of=2), dict(os=63), dict(n=-1), dict(dim=0), dict(dim=16385, stride=16385, os=16385),
-        dict(at=None, row0=7), dict(at=None, row0=-1)], dict(n=0)),
+        dict(at=None, row0=7), dict(at=None, row0=-1), dict(n=(1 << 30) + 1)], dict(n=0)),
     "dsv4_gpu_tree_attn_d": (TREE, [
         dict(o=None), dict(q=None), dict(kv=None), dict(ks=None), dict(fmt=2), dict(kf=3),
         dict(nt=-1), dict(nt=65), dict(h=0), dict(h=4097), dict(dqk=0, dv=0), dict(dv=0),
@@ -61,6 +61,7 @@ CALLS = {
     "dsv4_gpu_logits_adjust_d": (LOGITS, [
         dict(x=None), dict(nt=-1), dict(nt=65), dict(vocab=0), dict(vocab=(1 << 30) + 1,
         stride=BIG), dict(stride=99), dict(rules=None), dict(rules=rules(n_hist=-1)),
+        dict(rules=rules(n_hist=(1 << 30) + 1)),
         dict(rules=rules(hist=None)), dict(rules=rules(repetition=0.0)),
         dict(rules=rules(repetition=-1.0)), dict(rules=rules(repetition=float("nan"))),
         dict(rules=rules(allow=p, allow_stride=3)), dict(rules=rules(allow=p, allow_stride=-1)),

@@ -158,6 +158,28 @@ def test_rows_named_twice_and_rows_outside(gpu, dsv4, n):
     assert np.array_equal(dc.cache_values(cache, 2, ks), want)
 
 
+@pytest.mark.parametrize("n,d", [(4096, 8), (4097, 8), (9001, 7), (20000, 32), (70001, 4)])
+@pytest.mark.parametrize("rows", [1, 300, 1 << 20])
+def test_long_lists(gpu, dsv4, n, d, rows):
+    """Lists that are looked up in a table: one row for all, a few rows, and
+    rows far apart, named once or more."""
+    rng = np.random.default_rng(n + rows)
+    x = rng.integers(-8, 9, (n, d)).astype(np.float32)
+    at = rng.integers(-2, rows + 2, n).astype(np.int32)
+    if rows > n:
+        at[:n // 2] = np.arange(n // 2) * (rows // n)
+        at[n // 2:n // 2 + 100] = at[:100]
+    at[-1] = at[0]
+    cache, _ = dc.cache_of(np.full((rows, d), 99.0, np.float32), 0)
+    assert _append(dsv4, cache, None, 0, d, rows, dc.dev(x), False, d, n, d, dc.dev(at)) == 0
+    want = np.full((rows, d), 99.0, np.float32)
+    fine = (at >= 0) & (at < rows)
+    last = np.full(rows, -1)
+    np.maximum.at(last, at[fine], np.nonzero(fine)[0])
+    want[last >= 0] = x[last[last >= 0]]
+    assert np.array_equal(dc.cache_values(cache, 0, None), want)
+
+
 @pytest.mark.parametrize("fmt", [0, 1, 2])
 def test_rows_moved_keep_their_values(gpu, dsv4, fmt):
     """What a verified path does with its rows: read back, written elsewhere.
