@@ -23,6 +23,41 @@ constexpr int TJ_THREADS = 256;
 constexpr int TJ_COLS = 64;                       /* columns of a workgroup  */
 constexpr int TJ_GROUPS = TJ_THREADS / (TJ_COLS / 4);
 
+/* The sums' weight of split s in a row whose maximum is m, and what it adds to
+ * the row's sum. A split that saw nothing adds 0, whatever its maximum; NaN
+ * sums stay. */
+__device__ __forceinline__ float join_weight(const Dsv4TreeJob &a, int s, int r, float m, float *l)
+{
+    const size_t at = (size_t)s * (a.nt * a.h) + r;
+    const float ms = a.pm[at], ls = a.pl[at];
+    const float e = ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
+    *l += e * ls;
+    return e;
+}
+
+/* 1 / (a row's sum with its sink), 0 where the row saw nothing. */
+__device__ __forceinline__ float join_scale(const Dsv4TreeJob &a, int r, float m, float l)
+{
+    if (a.sink && l != 0.0f)
+        l += __builtin_amdgcn_exp2f(a.sink[r % a.h] * 1.44269504088896340736f - m);
+    return l != 0.0f ? 1.0f / l : 0.0f;
+}
+
+template <class T>
+__device__ __forceinline__ void join_store(const Dsv4TreeJob &a, T *o, int r, int c, f32x4 v)
+{
+    if (c >= a.dv) return;
+    const float y[4] = {v.x, v.y, v.z, v.w};
+    T *d = o + (size_t)r * a.dv + c;
+    if (a.ovec) {
+        io_store<T, 4>(d, y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
+    }
+}
+
 /* o of one row of q and 64 columns: thread (group of splits, 4 columns), the
  * groups' sums added in order through LDS. */
 template <class T>
@@ -41,13 +76,7 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
     for (int k = 1; k < TJ_THREADS / 64; k++) m = fmaxf(m, red[k]);
     __syncthreads();
     float l = 0.0f;
-    for (int s = tid; s < a.ns; s += TJ_THREADS) {
-        const float ms = a.pm[(size_t)s * R + r], ls = a.pl[(size_t)s * R + r];
-        /* a split that saw nothing adds 0, whatever its maximum; NaN sums stay */
-        const float e = ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
-        wt[s] = e;
-        l += e * ls;
-    }
+    for (int s = tid; s < a.ns; s += TJ_THREADS) wt[s] = join_weight(a, s, r, m, &l);
     l = wave_sum(l);
     if ((tid & 63) == 0) red[tid >> 6] = l;
     __syncthreads();
@@ -63,18 +92,46 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
     __syncthreads();
     if (gr != 0 || c >= a.dv) return;
     for (int k = 1; k < TJ_GROUPS; k++) v += sum[k][c4];
-    if (a.sink && l != 0.0f)
-        l += __builtin_amdgcn_exp2f(a.sink[r % a.h] * 1.44269504088896340736f - m);
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-    T *d = o + (size_t)r * a.dv + c;
-    if (a.ovec) {
-        io_store<T, 4>(d, y);
-    } else {
+    join_store(a, o, r, c, v * join_scale(a, r, m, l));
+}
+
+/* The same by one wave for a row, where the rows alone fill the card: lane s has
+ * split s's weight, and each lane up to eight columns. */
+template <class T>
+__global__ void __launch_bounds__(TJ_THREADS) k_tree_join_rows(Dsv4TreeJob a, T *o)
+{
+    const int lane = threadIdx.x & 63, R = a.nt * a.h;
+    const int r = blockIdx.x * (TJ_THREADS / 64) +
+                  __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (r >= R) return;
+    const float m = wave_max(lane < a.ns ? a.pm[(size_t)lane * R + r] : -INFINITY);
+    float l = 0.0f;
+    const float wt = lane < a.ns ? join_weight(a, lane, r, m, &l) : 0.0f;
+    const float inv = join_scale(a, r, m, wave_sum(l));
+    f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    const float *p = a.part + (size_t)r * a.dvp + 4 * lane;
+    for (int s = 0; s < a.ns; s++, p += (size_t)R * a.dvp) {
+        const float e = __shfl(wt, s, 64);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
+        for (int k = 0; k < 2; k++)
+            if (256 * k + 4 * lane < a.dvp) v[k] += e * ldf4(p + 256 * k);
     }
+#pragma unroll
+    for (int k = 0; k < 2; k++) join_store(a, o, r, 256 * k + 4 * lane, v[k] * inv);
+}
+
+/* A wave for a row from 2048 rows on, eight waves a CU; the plan then leaves 32
+ * splits at most. 8192 rows of 4 splits: 13.3 us, 64.8 by 64 columns a workgroup. */
+template <class T>
+void join_launch(const Dsv4TreeJob &a, hipStream_t st)
+{
+    const int R = a.nt * a.h;
+    if (R >= 2048)
+        hipLaunchKernelGGL(k_tree_join_rows<T>, dim3((R + TJ_THREADS / 64 - 1) / (TJ_THREADS / 64)),
+                           dim3(TJ_THREADS), 0, st, a, (T *)a.o);
+    else
+        hipLaunchKernelGGL(k_tree_join<T>, dim3(R, (a.dv + TJ_COLS - 1) / TJ_COLS),
+                           dim3(TJ_THREADS), 0, st, a, (T *)a.o);
 }
 
 /* What is wrong with a call's shape, or nullptr. */
@@ -105,8 +162,8 @@ struct TreePlan {
  * of them and read the cache through L2 as often, until the splits fill the
  * card; then wider ones win. Measured, one token's 64 heads of f32 q over a bf16
  * cache, at the best split for 16, 32 and 64 rows a workgroup: 16.0, 17.8 and 23.4 us
- * at 1500 rows of cache, 21.4, 23.2, 28.7 at 8192, 41.9, 34.3, 39.0 at 32768, 122,
- * 77, 74 at 131072. */
+ * at 1500 rows of cache (and 14.1 with a tile a split where these had two), 21.4,
+ * 23.2 and 28.7 at 8192, 41.9, 34.3 and 39.0 at 32768, 122, 77 and 74 at 131072. */
 TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_ctx, int window)
 {
     TreePlan p;
@@ -121,13 +178,13 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
      * context of this length can have */
     const int most = window ? (window + nt) / TR_TILE + 2 : tiles;
     const int up = tiles < most ? tiles : most;
-    p.cap = up / 2 < 512 / wide ? up / 2 : 512 / wide;
+    p.cap = up < 512 / wide ? up : 512 / wide;
     if (p.cap < 1) p.cap = 1;
     long long best = -1;
     for (int r = 16; r <= br; r *= 2) {
         const int nb = (nt * h + r - 1) / r, waves = r / 16 * tree_split(fmt, kv_fmt, p.kc);
-        for (int k = 0; k < 4; k++) {
-            long long ns = 256ll * ((nb + 255) / 256 + k) / nb;
+        for (int k = 0; k < 5; k++) {             /* one split, or k rounds and more */
+            long long ns = k ? 256ll * ((nb + 255) / 256 + k - 1) / nb : 1;
             if (ns > p.cap) ns = p.cap;
             const long long each = (tiles + ns - 1) / ns;
             ns = (tiles + each - 1) / each;
@@ -237,12 +294,8 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
                  : kv_fmt == DSV4_GPU_KV_BF16 ? dsv4_tree_bf16_launch(a, fmt, p.kc, st)
                                               : dsv4_tree_fp8_launch(a, fmt, p.kc, st);
     if (rc != 0 || p.ns == 1) return rc;
-    const dim3 grid(nt * h, (d_v + TJ_COLS - 1) / TJ_COLS);
-    if (fmt == DSV4_WF32)
-        hipLaunchKernelGGL(k_tree_join<float>, grid, dim3(TJ_THREADS), 0, st, a, (float *)d_o);
-    else
-        hipLaunchKernelGGL(k_tree_join<uint16_t>, grid, dim3(TJ_THREADS), 0, st, a,
-                           (uint16_t *)d_o);
+    if (fmt == DSV4_WF32) join_launch<float>(a, st);
+    else join_launch<uint16_t>(a, st);
     HIP_OK(hipGetLastError(), "tree attn join launch");
     return 0;
 }
