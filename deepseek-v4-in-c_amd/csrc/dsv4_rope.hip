@@ -8,11 +8,14 @@
  * attention block's are, so both rotate to the same bits.
  *
  * Bound: the element stream, read and written once; the tables are dim/2
- * pairs per token against heads * head_dim elements. A thread owns one
- * 16-byte piece (neighbours) or two pieces dim/2 apart (halves) of a head, so
- * a pair's elements meet in one thread and d_out may be d_x. Where a head
- * has elements outside the rotated part and d_out is not d_x, further threads
- * copy them.
+ * pairs per token against heads * head_dim elements and come from L2. A thread
+ * owns one 16-byte piece (neighbours) or two pieces dim/2 apart (halves) of a
+ * head, so a pair's elements meet in one thread and d_out may be d_x. Where a
+ * head has elements outside the rotated part and d_out is not d_x, further
+ * threads copy them. 4099 tokens of 64 heads of 128, bf16: 26.7 us (halves) and
+ * 27.9 us (pairs) from HBM, 5.0 TB/s, a large copy's rate. Four heads a thread,
+ * to read the tables' entries once for them, were slower nearly everywhere (31.1
+ * us here, 4.2 against 2.7 us for one token).
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -29,15 +32,14 @@ struct RopeJob {
     long long xs, os;
     const int *pos;
     const float *cos, *sin;
-    int items, heads, hd, max_pos, half, off, inverse;
+    int items, hd, max_pos, half, off, inverse;
     int nrot;                    /* a head's rotated units; copied ones follow */
-    IoDiv units, groups;
+    IoDiv units, heads;
 };
 
 /* V: elements per piece (16 bytes, or 1 where the shape or an address is not
- * aligned to them); HG: heads that one thread turns by the same table
- * entries. */
-template <class T, int V, bool HALVES, int HG>
+ * aligned to them). */
+template <class T, int V, bool HALVES>
 __global__ void __launch_bounds__(RO_THREADS) k_rope(RopeJob a)
 {
     constexpr int W = HALVES ? V : (V > 1 ? V / 2 : 1);      /* pairs per unit */
@@ -45,36 +47,26 @@ __global__ void __launch_bounds__(RO_THREADS) k_rope(RopeJob a)
     if (i >= (uint32_t)a.items) return;
     const uint32_t q = a.units.div(i);
     const int u = (int)(i - q * a.units.d);
-    const int t = (int)a.groups.div(q);
-    const int h0 = (int)(q - (uint32_t)t * a.groups.d) * HG;
-    const T *x = (const T *)a.x + t * a.xs + (long long)h0 * a.hd;
-    T *o = (T *)a.out + t * a.os + (long long)h0 * a.hd;
-    const int nh = min(HG, a.heads - h0);
+    const int t = (int)a.heads.div(q), h = (int)(q - (uint32_t)t * a.heads.d);
+    const T *x = (const T *)a.x + t * a.xs + (long long)h * a.hd;
+    T *o = (T *)a.out + t * a.os + (long long)h * a.hd;
     if (u >= a.nrot) {                                       /* copied as it is */
         int c = (u - a.nrot) * V;
         if (c >= a.off) c += 2 * a.half;
-        float v[HG][V];
-#pragma unroll
-        for (int h = 0; h < HG; h++)
-            if (h < nh) io_load<T, V>(x + h * a.hd + c, v[h]);
-#pragma unroll
-        for (int h = 0; h < HG; h++)
-            if (h < nh) io_store<T, V>(o + h * a.hd + c, v[h]);
+        float v[V];
+        io_load<T, V>(x + c, v);
+        io_store<T, V>(o + c, v);
         return;
     }
     const int p = a.pos[t];
     const int c0 = a.off + (HALVES ? u * W : 2 * u * W);
-    float v[HG][2 * W], cs[W], sn[W];
-#pragma unroll
-    for (int h = 0; h < HG; h++)
-        if (h < nh) {
-            if constexpr (HALVES) {
-                io_load<T, W>(x + h * a.hd + c0, v[h]);
-                io_load<T, W>(x + h * a.hd + c0 + a.half, v[h] + W);
-            } else {
-                io_load<T, 2 * W>(x + h * a.hd + c0, v[h]);
-            }
-        }
+    float v[2 * W], cs[W], sn[W];
+    if constexpr (HALVES) {
+        io_load<T, W>(x + c0, v);
+        io_load<T, W>(x + c0 + a.half, v + W);
+    } else {
+        io_load<T, 2 * W>(x + c0, v);
+    }
     if (p >= 0 && p < a.max_pos) {
         const size_t r = (size_t)p * a.half + u * W;
         io_load<float, W>(a.cos + r, cs);
@@ -84,42 +76,30 @@ __global__ void __launch_bounds__(RO_THREADS) k_rope(RopeJob a)
         for (int k = 0; k < W; k++) cs[k] = sn[k] = __uint_as_float(0x7FC00000u);
     }
 #pragma unroll
-    for (int k = 0; k < W; k++) if (a.inverse) sn[k] = -sn[k];
-#pragma unroll
-    for (int h = 0; h < HG; h++) {
-        if (h >= nh) break;
-#pragma unroll
-        for (int k = 0; k < W; k++) {
-            float &e0 = HALVES ? v[h][k] : v[h][2 * k];
-            float &e1 = HALVES ? v[h][W + k] : v[h][2 * k + 1];
-            const float x0 = e0, x1 = e1;
-            e0 = x0 * cs[k] - x1 * sn[k];
-            e1 = x0 * sn[k] + x1 * cs[k];
-        }
-        if constexpr (HALVES) {
-            io_store<T, W>(o + h * a.hd + c0, v[h]);
-            io_store<T, W>(o + h * a.hd + c0 + a.half, v[h] + W);
-        } else {
-            io_store<T, 2 * W>(o + h * a.hd + c0, v[h]);
-        }
+    for (int k = 0; k < W; k++) {
+        if (a.inverse) sn[k] = -sn[k];
+        float &e0 = HALVES ? v[k] : v[2 * k];
+        float &e1 = HALVES ? v[W + k] : v[2 * k + 1];
+        const float x0 = e0, x1 = e1;
+        e0 = x0 * cs[k] - x1 * sn[k];
+        e1 = x0 * sn[k] + x1 * cs[k];
+    }
+    if constexpr (HALVES) {
+        io_store<T, W>(o + c0, v);
+        io_store<T, W>(o + c0 + a.half, v + W);
+    } else {
+        io_store<T, 2 * W>(o + c0, v);
     }
 }
 
-template <class T, int V, bool HALVES>
-void rope_launch(const RopeJob &a, int hg, hipStream_t st)
+template <class T, int V>
+void rope_launch(const RopeJob &a, int layout, hipStream_t st)
 {
     const dim3 grid((a.items + RO_THREADS - 1) / RO_THREADS);
-    if (hg == 4)
-        hipLaunchKernelGGL((k_rope<T, V, HALVES, 4>), grid, dim3(RO_THREADS), 0, st, a);
+    if (layout == DSV4_GPU_ROPE_HALVES)
+        hipLaunchKernelGGL((k_rope<T, V, true>), grid, dim3(RO_THREADS), 0, st, a);
     else
-        hipLaunchKernelGGL((k_rope<T, V, HALVES, 1>), grid, dim3(RO_THREADS), 0, st, a);
-}
-
-template <class T, int V>
-void rope_layout(const RopeJob &a, int layout, int hg, hipStream_t st)
-{
-    if (layout == DSV4_GPU_ROPE_HALVES) rope_launch<T, V, true>(a, hg, st);
-    else rope_launch<T, V, false>(a, hg, st);
+        hipLaunchKernelGGL((k_rope<T, V, false>), grid, dim3(RO_THREADS), 0, st, a);
 }
 
 } // namespace
@@ -142,8 +122,9 @@ extern "C" int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *
                                  void *stream)
 {
     const long long width = (long long)heads * head_dim;
-    if (nt < 0 || nt > 1 << 30 || heads <= 0 || head_dim <= 0 || x_stride < width || out_stride < width ||
-        width > INT32_MAX / 2 || (fmt != DSV4_WF32 && fmt != DSV4_WBF16)) {
+    if (nt < 0 || nt > 1 << 30 || heads <= 0 || head_dim <= 0 || x_stride < width ||
+        out_stride < width || width > INT32_MAX / 2 ||
+        (fmt != DSV4_WF32 && fmt != DSV4_WBF16)) {
         DSV4_ERR("rope: bad arguments (nt %d, heads %d, head_dim %d, fmt %d, strides %lld, %lld)",
                  nt, heads, head_dim, fmt, x_stride, out_stride);
         return -1;
@@ -167,28 +148,23 @@ extern "C" int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *
         V = 1;
     const int nrot = halves ? half / V : V > 1 ? rope->dim / V : half;
     const int units = nrot + (here ? 0 : (head_dim - rope->dim) / V);
-    /* four heads per thread share the table's entries and keep four loads in
-     * flight; one head per thread where that leaves more than a workgroup per
-     * CU short of work */
-    const int hg = (long long)nt * units * ((heads + 3) / 4) >= 4 * 256 * RO_THREADS ? 4 : 1;
-    const int groups = (heads + hg - 1) / hg;
     /* a launch's items stay below 2^30 */
-    const long long per = (long long)units * groups;
+    const long long per = (long long)units * heads;
     const int most = (int)((1ll << 30) / per);
     for (int t0 = 0; t0 < nt; t0 += most) {
         const int n = nt - t0 < most ? nt - t0 : most;
         RopeJob a{(const char *)d_x + (size_t)t0 * x_stride * es,
                   (char *)d_out + (size_t)t0 * out_stride * es, x_stride, out_stride,
-                  d_pos + t0, rope->cos, rope->sin, (int)(n * per), heads, head_dim,
+                  d_pos + t0, rope->cos, rope->sin, (int)(n * per), head_dim,
                   rope->max_pos, half, rope->offset, inverse != 0, nrot,
-                  IoDiv((uint32_t)units), IoDiv((uint32_t)groups)};
+                  IoDiv((uint32_t)units), IoDiv((uint32_t)heads)};
         hipStream_t st = (hipStream_t)stream;
         if (es == 4) {
-            if (V > 1) rope_layout<float, 4>(a, rope->layout, hg, st);
-            else rope_layout<float, 1>(a, rope->layout, hg, st);
+            if (V > 1) rope_launch<float, 4>(a, rope->layout, st);
+            else rope_launch<float, 1>(a, rope->layout, st);
         } else {
-            if (V > 1) rope_layout<uint16_t, 8>(a, rope->layout, hg, st);
-            else rope_layout<uint16_t, 1>(a, rope->layout, hg, st);
+            if (V > 1) rope_launch<uint16_t, 8>(a, rope->layout, st);
+            else rope_launch<uint16_t, 1>(a, rope->layout, st);
         }
         HIP_OK(hipGetLastError(), "rope launch");
     }
