@@ -22,17 +22,13 @@ namespace {
 constexpr int TJ_THREADS = 256;
 constexpr int TJ_COLS = 64;                       /* columns of a workgroup  */
 constexpr int TJ_GROUPS = TJ_THREADS / (TJ_COLS / 4);
+constexpr int TJ_SPLITS = 512;                    /* most splits of a call   */
 
-/* The sums' weight of split s in a row whose maximum is m, and what it adds to
- * the row's sum. A split that saw nothing adds 0, whatever its maximum; NaN
- * sums stay. */
-__device__ __forceinline__ float join_weight(const Dsv4TreeJob &a, int s, int r, float m, float *l)
+/* The weight of a split's sums, its maximum ms and sum ls, in a row whose maximum
+ * is m. A split that saw nothing adds 0, whatever its maximum; NaN sums stay. */
+__device__ __forceinline__ float join_weight(float ms, float ls, float m)
 {
-    const size_t at = (size_t)s * (a.nt * a.h) + r;
-    const float ms = a.pm[at], ls = a.pl[at];
-    const float e = ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
-    *l += e * ls;
-    return e;
+    return ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
 }
 
 /* 1 / (a row's sum with its sink), 0 where the row saw nothing. */
@@ -59,38 +55,58 @@ __device__ __forceinline__ void join_store(const Dsv4TreeJob &a, T *o, int r, in
 }
 
 /* o of one row of q and 64 columns: thread (group of splits, 4 columns), the
- * groups' sums added in order through LDS. */
+ * groups' sums added in order through LDS. Each wave weighs all splits for
+ * itself, and the first 64 splits' sums are on their way meanwhile. */
 template <class T>
 __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
 {
-    __shared__ float wt[1024];
-    __shared__ float red[TJ_THREADS / 64];
+    constexpr int NK = TJ_SPLITS / 64, NI = 64 / TJ_GROUPS;
     __shared__ f32x4 sum[TJ_GROUPS][TJ_COLS / 4];
-    const int tid = threadIdx.x, r = blockIdx.x, R = a.nt * a.h;
-    float m = -INFINITY;
-    for (int s = tid; s < a.ns; s += TJ_THREADS) m = fmaxf(m, a.pm[(size_t)s * R + r]);
-    m = wave_max(m);
-    if ((tid & 63) == 0) red[tid >> 6] = m;
-    __syncthreads();
-    m = red[0];
-    for (int k = 1; k < TJ_THREADS / 64; k++) m = fmaxf(m, red[k]);
-    __syncthreads();
-    float l = 0.0f;
-    for (int s = tid; s < a.ns; s += TJ_THREADS) wt[s] = join_weight(a, s, r, m, &l);
-    l = wave_sum(l);
-    if ((tid & 63) == 0) red[tid >> 6] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int k = 0; k < TJ_THREADS / 64; k++) l += red[k];
+    const int tid = threadIdx.x, lane = tid & 63, r = blockIdx.x, R = a.nt * a.h;
     const int c4 = tid & (TJ_COLS / 4 - 1), gr = tid / (TJ_COLS / 4);
     const int c = blockIdx.y * TJ_COLS + 4 * c4;
+    auto part = [&](int s) {
+        return s < a.ns && c < a.dvp ? ldf4(a.part + ((size_t)s * R + r) * a.dvp + c)
+                                     : f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    float ms[NK], ls[NK], m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const int s = 64 * k + lane;
+        ms[k] = -INFINITY;
+        ls[k] = 0.0f;
+        if (64 * k < a.ns && s < a.ns) {
+            ms[k] = a.pm[(size_t)s * R + r];
+            ls[k] = a.pl[(size_t)s * R + r];
+        }
+    }
+    f32x4 x[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) x[i] = part(gr + TJ_GROUPS * i);
+#pragma unroll
+    for (int k = 0; k < NK; k++) m = fmaxf(m, ms[k]);
+    m = wave_max(m);
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        if (64 * k >= a.ns) break;
+        ms[k] = join_weight(ms[k], ls[k], m);
+        l += ms[k] * ls[k];
+    }
+    l = wave_sum(l);
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (c < a.dvp)
-        for (int s = gr; s < a.ns; s += TJ_GROUPS)
-            v += wt[s] * ldf4(a.part + ((size_t)s * R + r) * a.dvp + c);
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        if (64 * k >= a.ns) break;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int s = gr + TJ_GROUPS * i;
+            v += __shfl(ms[k], s, 64) * (k == 0 ? x[i] : part(64 * k + s));
+        }
+    }
     sum[gr][c4] = v;
     __syncthreads();
-    if (gr != 0 || c >= a.dv) return;
+    if (gr != 0) return;
     for (int k = 1; k < TJ_GROUPS; k++) v += sum[k][c4];
     join_store(a, o, r, c, v * join_scale(a, r, m, l));
 }
@@ -104,10 +120,10 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join_rows(Dsv4TreeJob a, T 
     const int r = blockIdx.x * (TJ_THREADS / 64) +
                   __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (r >= R) return;
-    const float m = wave_max(lane < a.ns ? a.pm[(size_t)lane * R + r] : -INFINITY);
-    float l = 0.0f;
-    const float wt = lane < a.ns ? join_weight(a, lane, r, m, &l) : 0.0f;
-    const float inv = join_scale(a, r, m, wave_sum(l));
+    const float ms = lane < a.ns ? a.pm[(size_t)lane * R + r] : -INFINITY;
+    const float ls = lane < a.ns ? a.pl[(size_t)lane * R + r] : 0.0f;
+    const float m = wave_max(ms), wt = join_weight(ms, ls, m);
+    const float inv = join_scale(a, r, m, wave_sum(wt * ls));
     f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     const float *p = a.part + (size_t)r * a.dvp + 4 * lane;
     for (int s = 0; s < a.ns; s++, p += (size_t)R * a.dvp) {
@@ -178,7 +194,7 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
      * context of this length can have */
     const int most = window ? (window + nt) / TR_TILE + 2 : tiles;
     const int up = tiles < most ? tiles : most;
-    p.cap = up < 512 / wide ? up : 512 / wide;
+    p.cap = up < TJ_SPLITS / wide ? up : TJ_SPLITS / wide;
     if (p.cap < 1) p.cap = 1;
     long long best = -1;
     for (int r = 16; r <= br; r *= 2) {
