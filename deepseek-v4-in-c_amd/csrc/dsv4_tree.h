@@ -185,7 +185,19 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * A tile with drafts, a window's edge or rows outside the cache is masked by a
  * word of 32 bits per row of q; its cache rows that hold NaN or infinity, or
  * are not there, become zeros in LDS first, which a weight of 0 leaves at 0,
- * and the former give NaN scores to the rows of q that see them. */
+ * and the former give NaN scores to the rows of q that see them.
+ *
+ * Bound: the matrix core where there are rows of q enough, and the start (q's
+ * loads and terms, one tile's trip from HBM, about 4 us) where there are not.
+ * 8192 rows of q in bf16 over 131072 cache rows in bf16 (d_qk 576, d_v 512): 2053
+ * to 2230 us with the clock of the card, 1.05 to 1.14 PFLOP/s, where a library
+ * product of 8192^3 reaches 1.20. Per tile and SIMD the products take 2176 cycles
+ * of some 4000; the rest is the softmax's vector instructions (1000 cycles for two
+ * waves) and the loads' issue, of which the other wave's products hide the most.
+ * 1024 rows of f32 q over 32768 of FP8: 186 us, 1.11 PFLOP/s of bf16 terms. Waves
+ * half a tile apart, deeper reads ahead, wave priorities and loads issued between
+ * products measured the same or slower; 32 rows of q a wave do not fit the
+ * registers. */
 template <class T, int KVF, int KC>
 __global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4)
 k_tree(Dsv4TreeJob a)
@@ -200,7 +212,9 @@ k_tree(Dsv4TreeJob a)
     constexpr int RAW = KVF == DSV4_GPU_KV_F32 ? 8 : 2;
     constexpr int ES = KVF == DSV4_GPU_KV_F32 ? 4 : KVF == DSV4_GPU_KV_BF16 ? 2 : 1;
     constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
-    /* where the next tile and all of q are in registers, few are left */
+    /* where the next tile and all of q are in registers, few are left: with operands
+     * six ahead spills took 1052 us where two ahead take 734 (8192 rows of bf16 q over
+     * 32768 of FP8) */
     constexpr bool SHALLOW = NT == 1 && KVF == DSV4_GPU_KV_FP8 && KC >= 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane0 = threadIdx.x & 63;

@@ -7,8 +7,8 @@
  *   - m) + e^(sink - m)),
  * in one pass over the cache with the running maximum m and sum. The rows of q
  * of all tokens and heads read the same cache, so they are cut into blocks of
- * 64 or 128 that share each tile of the cache; where the blocks do not fill
- * the card the cache is cut into splits, whose sums k_tree_join adds with
+ * 16 to 128 that share each tile of the cache; where the blocks do not fill
+ * the card the cache is cut into splits, whose sums a second launch adds with
  * weights e^(m_split - m).
  */
 #include "dsv4_tree.h"
