@@ -255,3 +255,44 @@ def test_scales_of_zero_and_below(gpu, dsv4, fmt, bf, scale):
     assert rc == 0
     want, size = dc.attention(q, v, dc.visible(w, nt, ctx, 20), None, scale, dv)
     check(dc.host(o), want, size, bf)
+
+
+# (nt, h, dqk, dv, ctx): workgroups of 16 rows of q and of all they can take, one split, a tile
+# a split, over 64 splits, and joins of many rows, odd widths among them
+PLANS = [(1, 16, 576, 512, 40), (1, 64, 576, 512, 1500), (2, 128, 576, 512, 6000),
+         (1, 16, 512, 512, 16500), (1, 5, 96, 64, 20011), (64, 40, 100, 75, 700),
+         (63, 33, 512, 509, 1100), (64, 128, 160, 128, 900), (64, 64, 576, 512, 2000)]
+
+
+@pytest.mark.parametrize("shape", PLANS)
+@pytest.mark.parametrize("fmt,bf", [(0, False), (1, False), (2, False), (1, True), (2, True)])
+def test_plans(gpu, dsv4, shape, fmt, bf):
+    nt, h, dqk, dv, ctx = shape
+    rng, dq, q, v, cache, ks, rows, pages = problem(nt * h + ctx, nt, h, dqk, ctx, fmt, bf, 1.0, 16)
+    w = dc.words(rng, nt)
+    sink = rng.standard_normal(h).astype(np.float32)
+    scale = 1.0 / np.sqrt(dqk)
+    rc, o = dc.tree(dsv4, dq, bf, cache, ks, fmt, rows, dqk, dv, ctx,
+                    dc.dev(np.array(w, np.uint64)), 0, pages, 16, sink=dc.dev(sink), scale=scale)
+    assert rc == 0
+    # rows of q of a few heads, the first and the last among them
+    few = sorted({0, h // 3, h - 1})
+    want, size = dc.attention(q[:, few], v, dc.visible(w, nt, ctx, 0), sink[few], scale, dv)
+    check(dc.host(o)[:, few], want, size, bf)
+
+
+@pytest.mark.parametrize("bf", [False, True])
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("ctx", [1, 31, 32, 33, 63, 64, 96, 127])
+def test_edges_of_tiles_and_windows(gpu, dsv4, fmt, bf, ctx):
+    """Contexts that end at, before and after a tile's end, with windows of the
+    same lengths: whole tiles inside the window, at its edge and none."""
+    nt, h, dqk, dv = 40, 2, 64, 64
+    rng, dq, q, v, cache, ks, rows, _ = problem(ctx, nt, h, dqk, ctx, fmt, bf)
+    w = dc.words(rng, nt)
+    dw = dc.dev(np.array(w, np.uint64))
+    for window in (0, 1, 31, 32, 33, 64, ctx, ctx + nt):
+        rc, o = dc.tree(dsv4, dq, bf, cache, ks, fmt, rows, dqk, dv, ctx, dw, window, scale=0.2)
+        assert rc == 0
+        want, size = dc.attention(q, v, dc.visible(w, nt, ctx, window), None, 0.2, dv)
+        check(dc.host(o), want, size, bf)
