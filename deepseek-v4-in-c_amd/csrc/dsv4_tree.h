@@ -29,7 +29,8 @@ struct Dsv4TreeJob {
      * blocks; part [ns][nt h][dvp] and its maxima and sums [ns][nt h] */
     int tile0, tile1, ns, nb, br, dvp;
     float *part, *pm, *pl;
-    int vec, qvec, ovec;                          /* whole pieces            */
+    int vec, qvec, ovec;                          /* the bf16 cache, q and o: whole
+                                                   * and aligned pieces of 8, 8, 4 */
 };
 
 /* The width class of a call (32-element chunks of d_qk that the kernel holds),
@@ -277,17 +278,23 @@ k_tree(Dsv4TreeJob a)
     auto my_row = [&](int i, const Place &h) {
         return max(0, a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
     };
-    /* one piece of a row that does not lie in whole pieces */
-    auto piece1 = [&](size_t at, int slab, int pc, uint32_t *r) {
+    /* the eight elements from column c of a row: where they are all there, in one
+     * or two loads that need no alignment (the target's own; the LDS-direct ones
+     * need it), else one by one */
+    auto piece = [&](size_t at, int c, uint32_t *r) {
+        const unsigned char *p = (const unsigned char *)a.kv + at * ES;
+        if (c + 8 <= a.dqk) {
+            __builtin_memcpy(r, p + c * ES, 8 * ES);
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const size_t c = at + min(64 * slab + pc + e, a.dqk - 1);
-            if constexpr (KVF == DSV4_GPU_KV_F32) r[e] = ((const uint32_t *)a.kv)[c];
-            else if constexpr (DMA)
-                r[e / 2] = (e & 1 ? r[e / 2] : 0u) | (uint32_t)((const uint16_t *)a.kv)[c]
+            const int k = min(c + e, a.dqk - 1);
+            if constexpr (ES == 4) r[e] = ((const uint32_t *)p)[k];
+            else if constexpr (ES == 2)
+                r[e / 2] = (e & 1 ? r[e / 2] : 0u) | (uint32_t)((const uint16_t *)p)[k]
                                                          << (16 * (e & 1));
-            else r[e / 4] = (e & 3 ? r[e / 4] : 0u) | (uint32_t)((const uint8_t *)a.kv)[c]
-                                                          << (8 * (e & 3));
+            else r[e / 4] = (e & 3 ? r[e / 4] : 0u) | (uint32_t)p[k] << (8 * (e & 3));
         }
     };
     auto put = [&](unsigned char *d, const uint32_t *r) {
@@ -313,21 +320,20 @@ k_tree(Dsv4TreeJob a)
             *(u32x4 *)d = v;
         }
     };
-    /* rows not in whole pieces go to LDS at once, without a tile's time between */
-    auto crawl = [&](int row, int buf, const Place &h) {
-#pragma unroll 1
-        for (int s = ws; s < L::SLABS; s += WS) {
-            uint32_t r[8];
-            piece1((size_t)row * a.stride, s, h.pc, r);
-            put(plane(buf) + s * L::SLAB + h.home, r);
-        }
-    };
     /* the bf16 cache: tile i into LDS directly */
     auto dma = [&](int i, int buf) {
         const Place h = place();
         const int row = my_row(i, h);
-        if (!a.vec) {
-            crawl(row, buf, h);
+        if (!a.vec) {                                  /* at once, two pieces at a time */
+#pragma unroll 1
+            for (int s = ws; s < L::SLABS; s += 2 * WS) {
+                const int s2 = min(s + WS, L::SLABS - 1);  /* or again, the same    */
+                uint32_t r[2][4];
+                piece((size_t)row * a.stride, 64 * s + h.pc, r[0]);
+                piece((size_t)row * a.stride, 64 * s2 + h.pc, r[1]);
+                put(plane(buf) + s * L::SLAB + h.home, r[0]);
+                put(plane(buf) + s2 * L::SLAB + h.home, r[1]);
+            }
             return;
         }
         const uint16_t *p = (const uint16_t *)a.kv + (size_t)row * a.stride;
@@ -343,47 +349,48 @@ k_tree(Dsv4TreeJob a)
         else if (L::SLABS % WS == 0 || ws == 0) tr_vm_wait<NP>();
         else tr_vm_wait<NP - 1>();
     };
-    /* the other formats: through registers */
+    /* the other formats: through registers. The piece that holds the row's last
+     * elements, if it is not whole, is loaded as the last eight and moved down
+     * when it is stored; a row of less than eight is loaded then. */
     uint32_t raw[NP][RAW];
     float rks = 1.0f;
-    int held = 0;                                      /* the row, not in whole pieces */
+    int held = 0;                                      /* the short row         */
     auto fetch = [&](int i) {
         const Place h = place();
         const int row = my_row(i, h);
         if (KVF == DSV4_GPU_KV_FP8) rks = a.ks[row];
-        if (!a.vec) {
+        if (KC == 4 && a.dqk < 8) {
             held = row;
             return;
         }
         const unsigned char *p = (const unsigned char *)a.kv + (size_t)row * a.stride * ES;
 #pragma unroll
-        for (int k = 0; k < NP; k++) {
-            const int c = min(64 * (ws + WS * k) + h.pc, a.dqk - 8);
-            if constexpr (ES == 1) {
-                const uint2 v = *(const uint2 *)(p + c);
-                raw[k][0] = v.x;
-                raw[k][1] = v.y;
-            } else {
+        for (int k = 0; k < NP; k++)
+            __builtin_memcpy(raw[k], p + min(64 * (ws + WS * k) + h.pc, a.dqk - 8) * ES, 8 * ES);
+    };
+    auto move_down = [&](uint32_t *r, bool mine) {
+#pragma unroll 1
+        for (int u = a.dqk & 7; u < 8; u++)
 #pragma unroll
-                for (int u = 0; u < RAW; u += 4) {
-                    const u32x4 v = ld16(p + 4 * (c + u));
-#pragma unroll
-                    for (int e = 0; e < 4; e++) raw[k][(u + e) % RAW] = v[e];
-                }
+            for (int e = 0; e < RAW; e++) {
+                const uint32_t up = r[e + 1 < RAW ? e + 1 : e];
+                const uint32_t v = ES == 4 ? up : e + 1 < RAW ? r[e] >> (8 * ES) | up << (32 - 8 * ES)
+                                 : (r[e] >> (8 * ES)) | (r[e] & ~0u << (32 - 8 * ES));
+                r[e] = mine ? v : r[e];
             }
-        }
     };
     auto store = [&](int buf) {
         const Place h = place();
         if (KVF == DSV4_GPU_KV_FP8 && ws == 0 && (h.home & 112) == 0) ((float *)meta(buf))[h.sr] = rks;
-        if (!a.vec) {
-            crawl(held, buf, h);
-            return;
-        }
+        if (KC == 4 && a.dqk < 8) piece((size_t)held * a.stride, h.pc, raw[0]);
 #pragma unroll
-        for (int k = 0; k < NP; k++)
-            if (L::SLABS % WS == 0 || ws + WS * k < L::SLABS)
-                put(plane(buf) + (ws + WS * k) * L::SLAB + h.home, raw[k]);
+        for (int k = 0; k < NP; k++) {
+            const int s = ws + WS * k;
+            if ((a.dqk & 7) && a.dqk > 8 && s == a.dqk >> 6)
+                move_down(raw[k], 64 * s + h.pc == (a.dqk & ~7));
+            if (L::SLABS % WS == 0 || s < L::SLABS)
+                put(plane(buf) + s * L::SLAB + h.home, raw[k]);
+        }
     };
     /* a masked tile's rows that are not there (ok) or hold what is not finite (in
      * the first plane, which has f32's infinities and NaN too) to zeros; the
@@ -480,10 +487,17 @@ k_tree(Dsv4TreeJob a)
             for (int kc = 0; kc < KC1; kc++) {
                 const int c = c0 + 32 * kc;
                 float f[8];
+                if (c + 8 <= a.dqk) {                  /* loads that need no alignment */
+                    T v[8];
+                    __builtin_memcpy(v, qr + c, sizeof(v));
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    io_load<T, 1>(qr + min(c + e, a.dqk - 1), f + e);
-                    f[e] = __int_as_float(__float_as_int(f[e]) & ((c + e - a.dqk) >> 31));
+                    for (int e = 0; e < 8; e++) io_load<T, 1>(v + e, f + e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        io_load<T, 1>(qr + min(c + e, a.dqk - 1), f + e);
+                        f[e] = __int_as_float(__float_as_int(f[e]) & ((c + e - a.dqk) >> 31));
+                    }
                 }
                 tr_bf8 tm[NT];
                 tr_terms<NT>(f, tm);

@@ -269,9 +269,6 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
     }
     const IoDiv pd((uint32_t)(d_pages ? page_rows : 1));
     const int es = fmt == DSV4_WBF16 ? 2 : 4;
-    /* pieces of eight cache elements: 8, 16 or 32 bytes, loaded 8 or 16 at a time */
-    const int ks = kv_fmt == DSV4_GPU_KV_F32 ? 4 : kv_fmt == DSV4_GPU_KV_BF16 ? 2 : 1;
-    const int al = ks == 1 ? 8 : 16;
     Dsv4TreeJob a{};
     a.o = d_o;
     a.q = d_q;
@@ -302,7 +299,7 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
     a.part = (float *)d_scratch;
     a.pm = a.part + (size_t)p.ns * nt * h * p.dvp;
     a.pl = a.pm + (size_t)p.ns * nt * h;
-    a.vec = d_qk % 8 == 0 && (long long)kv_stride * ks % al == 0 && (uintptr_t)d_kv % al == 0;
+    a.vec = d_qk % 8 == 0 && kv_stride % 8 == 0 && ((uintptr_t)d_kv & 15) == 0;
     a.qvec = d_qk % 8 == 0 && ((uintptr_t)d_q & 15) == 0;
     a.ovec = d_v % 4 == 0 && (uintptr_t)d_o % (4 * es) == 0;
     hipStream_t st = (hipStream_t)stream;
