@@ -296,3 +296,18 @@ def test_edges_of_tiles_and_windows(gpu, dsv4, fmt, bf, ctx):
         assert rc == 0
         want, size = dc.attention(q, v, dc.visible(w, nt, ctx, window), None, 0.2, dv)
         check(dc.host(o), want, size, bf)
+
+
+@pytest.mark.parametrize("fmt,bf", [(0, False), (1, False), (2, False), (0, True), (1, True),
+                                    (2, True)])
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 7, 8, 9, 15, 63, 65, 129, 257, 449, 513, 575])
+def test_rows_of_any_width(gpu, dsv4, fmt, bf, d):
+    """Rows of less than one piece of eight elements, and last pieces of any
+    length in every width class."""
+    nt, h, ctx = 4, 5, 45
+    rng, dq, q, v, cache, ks, rows, _ = problem(d, nt, h, d, ctx, fmt, bf)
+    dv = min(d, 512)
+    rc, o = dc.tree(dsv4, dq, bf, cache, ks, fmt, rows, d, dv, ctx, scale=0.3)
+    assert rc == 0
+    want, size = dc.attention(q, v, dc.visible(None, nt, ctx, 0), None, 0.3, dv)
+    check(dc.host(o), want, size, bf)
