@@ -193,12 +193,14 @@ __device__ __forceinline__ void row_store(const AppendJob &a, size_t at, const f
 #pragma unroll
         for (int k = 0; k < V; k++) t[k] = v[k] * inv;
         const uint32_t c = codes4(t);
-        if constexpr (V == 4) *(uint32_t *)((uint8_t *)a.kv + at) = c;
+        if constexpr (V == 4) __builtin_memcpy((uint8_t *)a.kv + at, &c, 4);
         else ((uint8_t *)a.kv)[at] = (uint8_t)c;
     }
 }
 
-/* NC pieces of V per lane kept in registers between the maximum and the
+/* Pieces of V from element c, the last moved back to end with the row: what it
+ * shares with the one before it is computed and written twice, the same. NC
+ * pieces per lane kept in registers between the maximum and the
  * store (the row is no longer than 64 V NC); NC 0: read again. */
 template <class T, int KVF, int V, int NC, int LIST>
 __global__ void __launch_bounds__(LIST == AP_HASH ? 64 * AP_WAVES : KR_THREADS)
@@ -229,7 +231,7 @@ k_append(AppendJob a)
             for (int i = 0; i < NC; i++) {
                 const int c = (i * 64 + lane) * V;
                 if (c < a.dim) {
-                    row_values<T, V>(a, x, c, cs, sn, v[i]);
+                    row_values<T, V>(a, x, min(c, a.dim - V), cs, sn, v[i]);
                 } else {
 #pragma unroll
                     for (int k = 0; k < V; k++) v[i][k] = 0.0f;
@@ -251,7 +253,7 @@ k_append(AppendJob a)
                         if (finite_f(v[i][k])) top = fmaxf(top, fabsf(v[i][k]));
             } else {
                 for (int c = lane * V; c < a.dim; c += 64 * V) {
-                    row_values<T, V>(a, x, c, cs, sn, v[0]);
+                    row_values<T, V>(a, x, min(c, a.dim - V), cs, sn, v[0]);
 #pragma unroll
                     for (int k = 0; k < V; k++)
                         if (finite_f(v[0][k])) top = fmaxf(top, fabsf(v[0][k]));
@@ -266,12 +268,12 @@ k_append(AppendJob a)
 #pragma unroll
             for (int i = 0; i < NC; i++) {
                 const int c = (i * 64 + lane) * V;
-                if (c < a.dim) row_store<KVF, V>(a, at + c, v[i], inv);
+                if (c < a.dim) row_store<KVF, V>(a, at + min(c, a.dim - V), v[i], inv);
             }
         } else {
             for (int c = lane * V; c < a.dim; c += 64 * V) {
-                row_values<T, V>(a, x, c, cs, sn, v[0]);
-                row_store<KVF, V>(a, at + c, v[0], inv);
+                row_values<T, V>(a, x, min(c, a.dim - V), cs, sn, v[0]);
+                row_store<KVF, V>(a, at + min(c, a.dim - V), v[0], inv);
             }
         }
     };
@@ -315,7 +317,7 @@ struct ReadJob {
     const float *scales;
     int kv_stride, kv_rows;
     const int *rows;
-    int row0, items;
+    int row0, dim, items;
     IoDiv units;
 };
 
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(KR_THREADS) k_read(ReadJob a)
         for (int k = 0; k < V; k++) v[u][k] = 0.0f;
         if (i >= (uint32_t)a.items) continue;
         const uint32_t t = a.units.div(i);
-        const int c = (int)(i - t * a.units.d) * V;
+        const int c = min((int)(i - t * a.units.d) * V, a.dim - V);
         o[u] = (T *)a.out + (long long)t * a.os + c;
         const int row = a.rows ? a.rows[t] : a.row0 + (int)t;
         if (row < 0 || row >= a.kv_rows) continue;
@@ -352,7 +354,9 @@ __global__ void __launch_bounds__(KR_THREADS) k_read(ReadJob a)
             } else {
 #pragma unroll
                 for (int k = 0; k < V; k += 4) {
-                    dec_e4m3x4(((const uint32_t *)p)[k / 4], v[u] + k);
+                    uint32_t w;
+                    __builtin_memcpy(&w, p + k, 4);
+                    dec_e4m3x4(w, v[u] + k);
 #pragma unroll
                     for (int e = 0; e < 4; e++) v[u][k + e] *= s;
                 }
@@ -382,8 +386,6 @@ int cache_ok(const char *what, const void *kv, const float *scales, int fmt, int
     }
     return 0;
 }
-
-int kv_size(int fmt) { return fmt == DSV4_GPU_KV_F32 ? 4 : fmt == DSV4_GPU_KV_BF16 ? 2 : 1; }
 
 template <class T, int KVF, int LIST>
 void append_launch(const AppendJob &a, int V, hipStream_t st)
@@ -462,16 +464,13 @@ extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, 
     /* a long list's workgroups: 512 of them fill the card's waves */
     const int per = n / (AP_WAVES * 512) + 1;
     a.tok = AP_WAVES * (per < AP_TOK / AP_WAVES ? per : AP_TOK / AP_WAVES);
-    /* pieces of four elements where the shapes and addresses are whole ones */
-    const int xs = x_fmt == DSV4_WBF16 ? 2 : 4;
-    int V = 4;
-    if (row_dim % 4 || x_stride % 4 || kv_stride % 4 || (uintptr_t)d_x % (4 * xs) ||
-        (uintptr_t)d_kv % (4 * kv_size(kv_fmt)))
-        V = 1;
-    if (rope && (rope->offset % 4 || rope->dim % 4 ||
+    /* pieces of four elements, the last one moved back to the row's end; one by
+     * one in rows of less, and where the rotation's pairs do not fall into pieces */
+    int V = row_dim < 4 ? 1 : 4;
+    if (rope && (row_dim % 4 || rope->offset % 4 || rope->dim % 4 ||
                  (rope->layout == DSV4_GPU_ROPE_HALVES && rope->dim % 8)))
         V = 1;
-    if (xs == 4) append_fmt<float>(a, kv_fmt, V, (hipStream_t)stream);
+    if (x_fmt == DSV4_WF32) append_fmt<float>(a, kv_fmt, V, (hipStream_t)stream);
     else append_fmt<uint16_t>(a, kv_fmt, V, (hipStream_t)stream);
     HIP_OK(hipGetLastError(), "kv_append launch");
     return 0;
@@ -496,17 +495,16 @@ extern "C" int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride
         return -1;
     }
     if (d_rows) row0 = 0;
-    const int es = out_fmt == DSV4_WBF16 ? 2 : 4, ks = kv_size(kv_fmt);
-    int V = 16 / es;
-    if (row_dim % V || out_stride % V || kv_stride % V || ((uintptr_t)d_out & 15) ||
-        (uintptr_t)d_kv % (V * ks < 16 ? V * ks : 16))
-        V = 1;
-    const int units = row_dim / V;
+    /* 16 bytes of output, the last piece moved back to the row's end; one by one
+     * in rows of less */
+    const int es = out_fmt == DSV4_WBF16 ? 2 : 4;
+    const int V = row_dim < 16 / es ? 1 : 16 / es;
+    const int units = (row_dim + V - 1) / V;
     const int most = (1 << 30) / units;           /* rows of a launch         */
     for (int t0 = 0; t0 < n; t0 += most) {
         const int m = n - t0 < most ? n - t0 : most;
         ReadJob a{(char *)d_out + (size_t)t0 * out_stride * es, out_stride, d_kv, d_kv_scales,
-                  kv_stride, kv_rows, d_rows ? d_rows + t0 : nullptr, row0 + t0, m * units,
+                  kv_stride, kv_rows, d_rows ? d_rows + t0 : nullptr, row0 + t0, row_dim, m * units,
                   IoDiv((uint32_t)units)};
         hipStream_t st = (hipStream_t)stream;
         if (es == 4) {

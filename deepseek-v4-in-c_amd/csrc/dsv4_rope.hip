@@ -37,8 +37,8 @@ struct RopeJob {
     IoDiv units, heads;
 };
 
-/* V: elements per piece (16 bytes, or 1 where the shape or an address is not
- * aligned to them). */
+/* V: elements per piece (16 bytes at any address, or 1 where a head or its
+ * rotated part is not whole pieces). */
 template <class T, int V, bool HALVES>
 __global__ void __launch_bounds__(RO_THREADS) k_rope(RopeJob a)
 {
@@ -142,10 +142,7 @@ extern "C" int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *
     const int half = rope->dim / 2, es = fmt == DSV4_WBF16 ? 2 : 4;
     const bool halves = rope->layout == DSV4_GPU_ROPE_HALVES;
     int V = 16 / es;
-    if (head_dim % V || rope->offset % V || (halves ? half : rope->dim) % V || x_stride % V ||
-        out_stride % V || (((uintptr_t)d_x | (uintptr_t)d_out) & 15) ||
-        (((uintptr_t)rope->cos | (uintptr_t)rope->sin) & 15))
-        V = 1;
+    if (head_dim % V || rope->offset % V || (halves ? half : rope->dim) % V) V = 1;
     const int nrot = halves ? half / V : V > 1 ? rope->dim / V : half;
     const int units = nrot + (here ? 0 : (head_dim - rope->dim) / V);
     /* a launch's items stay below 2^30 */

@@ -15,7 +15,8 @@ __device__ __forceinline__ uint32_t io_bf2(float a, float b)
 }
 
 /* N consecutive elements as floats; 16 bytes or 8 at a time where N elements
- * are that many (the caller's pointer is then aligned to them). */
+ * are that many, at any address of an element (the target's loads and stores of
+ * global memory need no more). */
 template <class T, int N>
 __device__ __forceinline__ void io_load(const T *p, float *v)
 {
@@ -23,13 +24,15 @@ __device__ __forceinline__ void io_load(const T *p, float *v)
     if constexpr (!BF && N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const f32x4 t = *reinterpret_cast<const f32x4 *>(p + i);
+            f32x4 t;
+            __builtin_memcpy(&t, p + i, 16);
             v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
         }
     } else if constexpr (BF && N % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
-            const u32x4 t = *reinterpret_cast<const u32x4 *>(p + i);
+            u32x4 t;
+            __builtin_memcpy(&t, p + i, 16);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 v[i + 2 * k] = __uint_as_float(t[k] << 16);
@@ -37,7 +40,8 @@ __device__ __forceinline__ void io_load(const T *p, float *v)
             }
         }
     } else if constexpr (BF && N == 4) {
-        const uint2 t = *reinterpret_cast<const uint2 *>(p);
+        uint2 t;
+        __builtin_memcpy(&t, p, 8);
         v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xFFFF0000u);
         v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xFFFF0000u);
     } else {
@@ -55,16 +59,20 @@ __device__ __forceinline__ void io_store(T *p, const float *v)
     constexpr bool BF = sizeof(T) == 2;
     if constexpr (!BF && N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<f32x4 *>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 t{v[i], v[i + 1], v[i + 2], v[i + 3]};
+            __builtin_memcpy(p + i, &t, 16);
+        }
     } else if constexpr (BF && N % 8 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i += 8)
-            *reinterpret_cast<u32x4 *>(p + i) =
-                u32x4{io_bf2(v[i], v[i + 1]), io_bf2(v[i + 2], v[i + 3]),
-                      io_bf2(v[i + 4], v[i + 5]), io_bf2(v[i + 6], v[i + 7])};
+        for (int i = 0; i < N; i += 8) {
+            const u32x4 t{io_bf2(v[i], v[i + 1]), io_bf2(v[i + 2], v[i + 3]),
+                          io_bf2(v[i + 4], v[i + 5]), io_bf2(v[i + 6], v[i + 7])};
+            __builtin_memcpy(p + i, &t, 16);
+        }
     } else if constexpr (BF && N == 4) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(io_bf2(v[0], v[1]), io_bf2(v[2], v[3]));
+        const uint2 t = make_uint2(io_bf2(v[0], v[1]), io_bf2(v[2], v[3]));
+        __builtin_memcpy(p, &t, 8);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {
