@@ -42,7 +42,6 @@ struct LogitJob {
     long long stride;
     int nt, vocab, rpg;
     dsv4_gpu_logit_rules r;
-    int vec, hvec;                                /* 16-byte pieces          */
     const int *count;                             /* [vocab], or NULL        */
     unsigned long long *best;                     /* [nt][slices]            */
     uint32_t *first;
@@ -59,26 +58,21 @@ __device__ __forceinline__ unsigned long long path_of(const LogitJob &a, int t)
 template <int THREADS>
 __device__ __forceinline__ void count_slice(const LogitJob &a, int v0, uint32_t lim, int *cnt)
 {
-    int i = 0;
-    if (a.hvec) {
-        const u32x4 *h4 = reinterpret_cast<const u32x4 *>(a.r.hist);
-        const int n4 = a.r.n_hist / 4;
-        constexpr int G = 4;                      /* loads in flight         */
-        for (int k = threadIdx.x; k < n4; k += G * THREADS) {
-            u32x4 v[G];
+    const int n4 = a.r.n_hist / 4;
+    constexpr int G = 4;                          /* loads in flight         */
+    for (int k = threadIdx.x; k < n4; k += G * THREADS) {
+        u32x4 v[G];
 #pragma unroll
-            for (int u = 0; u < G; u++) v[u] = h4[min(k + u * THREADS, n4 - 1)];
+        for (int u = 0; u < G; u++)
+            __builtin_memcpy(&v[u], a.r.hist + 4 * min(k + u * THREADS, n4 - 1), 16);
 #pragma unroll
-            for (int u = 0; u < G; u++)
-                if (k + u * THREADS < n4)
+        for (int u = 0; u < G; u++)
+            if (k + u * THREADS < n4)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (v[u][e] - (uint32_t)v0 < lim)
-                            atomicAdd(&cnt[v[u][e] - (uint32_t)v0], 1);
-        }
-        i = 4 * n4;
+                for (int e = 0; e < 4; e++)
+                    if (v[u][e] - (uint32_t)v0 < lim) atomicAdd(&cnt[v[u][e] - (uint32_t)v0], 1);
     }
-    for (i += threadIdx.x; i < a.r.n_hist; i += THREADS) {
+    for (int i = 4 * n4 + threadIdx.x; i < a.r.n_hist; i += THREADS) {
         const uint32_t k = (uint32_t)a.r.hist[i] - (uint32_t)v0;
         if (k < lim) atomicAdd(&cnt[k], 1);
     }
@@ -110,12 +104,15 @@ __global__ void __launch_bounds__(LG_THREADS) k_logits(LogitJob a)
     const int v0 = blockIdx.x * SW;
     const int t0 = blockIdx.y * a.rpg, t1 = min(t0 + a.rpg, a.nt);
     const bool counts = a.r.n_hist > 0 || a.r.draft;
-    const bool whole = a.vec && v0 + SW <= a.vocab;
+    const bool whole = v0 + SW <= a.vocab;
 
-    /* 4 tokens from v0 + c of a row; 0 past the vocabulary */
+    /* 4 tokens from v0 + c of a row, at any address; 0 past the vocabulary */
     auto load4 = [&](const float *x, int c) -> f32x4 {
-        if (whole) return ldf4(x + v0 + c);
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (whole) {
+            __builtin_memcpy(&v, x + v0 + c, 16);
+            return v;
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++)
             if (v0 + c + k < a.vocab) v[k] = x[v0 + c + k];
@@ -215,7 +212,7 @@ __global__ void __launch_bounds__(LG_THREADS) k_logits(LogitJob a)
 #pragma unroll
             for (int p = 0; p < NP; p++) {
                 if (whole) {
-                    *reinterpret_cast<f32x4 *>(y + p * LG_PIECE) = v[p];
+                    __builtin_memcpy(y + p * LG_PIECE, &v[p], 16);
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; k++)
@@ -338,9 +335,6 @@ extern "C" int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *
     int np;
     plan(nt, vocab, &np, &a.rpg);
     a.r = *rules;
-    a.vec = stride % 4 == 0 && (((uintptr_t)d_logits | (uintptr_t)d_out |
-                                 (uintptr_t)rules->bias) & 15) == 0;
-    a.hvec = rules->n_hist && ((uintptr_t)rules->hist & 15) == 0;
     const int sw = np * LG_PIECE, ns = (int)(((long long)vocab + sw - 1) / sw);
     const size_t n = (size_t)nt * ns;
     if (d_pick) {
