@@ -215,7 +215,8 @@ k_tree(Dsv4TreeJob a)
     constexpr bool DMA = KVF == DSV4_GPU_KV_BF16;
     /* where the next tile and all of q are in registers, few are left: with operands
      * six ahead spills took 1052 us where two ahead take 734 (8192 rows of bf16 q over
-     * 32768 of FP8) */
+     * 32768 of FP8); with the widest rows the scales are read twice as well (687 us,
+     * and 639 so; narrower rows lose 2 % by it) */
     constexpr bool SHALLOW = NT == 1 && KVF == DSV4_GPU_KV_FP8 && KC >= 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane0 = threadIdx.x & 63;
@@ -674,9 +675,18 @@ k_tree(Dsv4TreeJob a)
             for (int j = 0; j < 4; j++) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[k][j], c2, -mm));
                 sum += x;
-                e[4 * k + j] = KVF == DSV4_GPU_KV_FP8 ? x * ks[k][j] : x;
+                e[4 * k + j] = x;
             }
         l += sum;
+        if (KVF == DSV4_GPU_KV_FP8) {
+            const int again = 4 * (tr_fresh(lane0) >> 4);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                if (SHALLOW && KC > 16) ks[k] = *(const f32x4 *)(mi + 16 * k + again);
+#pragma unroll
+                for (int j = 0; j < 4; j++) e[4 * k + j] *= ks[k][j];
+            }
+        }
         tr_bf8 pw[NT];
         tr_terms<NT>(e, pw);
 
