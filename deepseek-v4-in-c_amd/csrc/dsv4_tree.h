@@ -218,6 +218,7 @@ k_tree(Dsv4TreeJob a)
      * 32768 of FP8); with the widest rows the scales are read twice as well (687 us,
      * and 639 so; narrower rows lose 2 % by it) */
     constexpr bool SHALLOW = NT == 1 && KVF == DSV4_GPU_KV_FP8 && KC >= 16;
+    constexpr bool AGAIN = SHALLOW && KC > 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane0 = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -679,10 +680,11 @@ k_tree(Dsv4TreeJob a)
             }
         l += sum;
         if (KVF == DSV4_GPU_KV_FP8) {
-            const int again = 4 * (tr_fresh(lane0) >> 4);
+            int at = 0;
+            if constexpr (AGAIN) at = 4 * (tr_fresh(lane0) >> 4);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                if (SHALLOW && KC > 16) ks[k] = *(const f32x4 *)(mi + 16 * k + again);
+                if constexpr (AGAIN) ks[k] = *(const f32x4 *)(mi + 16 * k + at);
 #pragma unroll
                 for (int j = 0; j < 4; j++) e[4 * k + j] *= ks[k][j];
             }
