@@ -601,8 +601,10 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  *
  * Scores, softmax and sums are in f32. With f32 q every product is exact
  * (bf16 terms of q and of the weights; an F32 cache's elements in three terms
- * as well), within 1e-5 relative; with bf16 q the weights are rounded to bf16
- * before they meet the rows.
+ * as well), within 1e-5 relative for f32 elements that are 0 or between 1e-30
+ * and 3e38 in magnitude (below, terms underflow; larger ones count as
+ * infinities); with bf16 q the weights are rounded to bf16 before they meet the
+ * rows.
  *
  * d_scratch: dsv4_gpu_tree_attn_scratch_bytes of device memory for the call's
  * shape, 16-byte aligned; the bytes do not fall as n_ctx grows, so a program
