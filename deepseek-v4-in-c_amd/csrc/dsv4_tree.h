@@ -706,7 +706,6 @@ k_tree(Dsv4TreeJob a)
         }
     };
 
-
     /* every token sees every position of tiles [ic0, ic1) */
     const int ic0 = a.window ? (max(0, a.ctx + a.nt - a.window) + TR_TILE - 1) / TR_TILE : 0;
     const int ic1 = a.ctx / TR_TILE;
