@@ -195,8 +195,8 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * product of 8192^3 reaches 1.20. Per tile and SIMD the products take 2176 cycles
  * of some 4000; the rest is the softmax's vector instructions (1000 cycles for two
  * waves) and the loads' issue, of which the other wave's products hide the most.
- * 1024 rows of f32 q over 32768 of FP8: 186 us, 1.11 PFLOP/s of bf16 terms. Waves
- * half a tile apart, deeper reads ahead, wave priorities and loads issued between
+ * 1024 rows of f32 q over 32768 of FP8: 186 to 193 us, 1.07 to 1.11 PFLOP/s of bf16
+ * terms. Waves half a tile apart, deeper reads ahead, wave priorities and loads issued between
  * products measured the same or slower; 32 rows of q a wave do not fit the
  * registers. */
 template <class T, int KVF, int KC>
