@@ -44,7 +44,13 @@ int dsv4_tree_fp8_launch(const Dsv4TreeJob &a, int fmt, int kc, hipStream_t st);
 /* bf16 terms that carry an f32 value exactly. */
 constexpr int TR_TERMS = 3;
 constexpr int tree_terms(int fmt) { return fmt == DSV4_WF32 ? TR_TERMS : 1; }
-constexpr int tree_planes(int kv_fmt) { return kv_fmt == DSV4_GPU_KV_F32 ? TR_TERMS : 1; }
+/* An F32 cache's elements in as many for f32 q, and in two, to 2^-18 of each, for
+ * bf16 q, whose weights are rounded to 2^-9 (2048 rows of q over 16384 of 512: 195
+ * us, 265 with three). */
+constexpr int tree_planes(int fmt, int kv_fmt)
+{
+    return kv_fmt != DSV4_GPU_KV_F32 ? 1 : fmt == DSV4_WF32 ? TR_TERMS : 2;
+}
 constexpr int tree_vtiles(int kc) { return kc >= 16 ? 32 : 2 * kc; }
 /* A workgroup is eight waves, two per SIMD. A wave holds 16 rows of q and their
  * sums, or, where with all terms that is more than half the registers, two
@@ -53,7 +59,7 @@ constexpr int tree_vtiles(int kc) { return kc >= 16 ? 32 : 2 * kc; }
 constexpr int TR_WAVES = 8;
 constexpr int tree_split(int fmt, int kv_fmt, int kc)
 {
-    return kc >= 16 && tree_terms(fmt) * tree_planes(kv_fmt) > 1 ? 2 : 1;
+    return kc >= 16 && tree_terms(fmt) * tree_planes(fmt, kv_fmt) > 1 ? 2 : 1;
 }
 
 #ifdef DSV4_TREE_KERNEL
@@ -104,18 +110,19 @@ __device__ __forceinline__ f32x4 tr_mfma(tr_bf8 a, tr_bf8 b, f32x4 c)
  * the values (two pieces of rows 0 .. 7, even and odd ones in different halves
  * of the 64 banks) take each bank once: SQ_LDS_BANK_CONFLICT counts none, and 4
  * cycles for each read of the values with p ^ (0, 2, 4, 6, 1, 3, 5, 7). */
-template <int KVF, int KC, int SPLIT>
+template <int KVF, int KC, int SPLIT, int PLANES>
 struct TreeLds {
-    static constexpr int KT = tree_planes(KVF);
+    static constexpr int KT = PLANES;
     static constexpr int SLABS = KC / 2;
     static constexpr int SLAB = TR_TILE * 128;
     static constexpr int PLANE = SLABS * SLAB;
-    static constexpr int NBUF = KT > 1 ? 1 : KVF == DSV4_GPU_KV_BF16 ? 3 : 2;
+    static constexpr int NBUF = KT * KC > 32 || KT > 2 ? 1 : KVF == DSV4_GPU_KV_BF16 ? 3 : 2;
     static constexpr int META = NBUF * KT * PLANE;
     static constexpr int MSIZE = 2 * TR_TILE * 4;
     static constexpr int ROWS = META + NBUF * MSIZE;   /* q's rows: see, lo      */
     static constexpr int HALF = ROWS + 16 * 16 * TR_WAVES;
     static constexpr int BYTES = HALF + (SPLIT == 2 ? 2048 * TR_WAVES : 0);
+    static_assert(BYTES <= 160 * 1024, "a CU's LDS");
 };
 
 __device__ __forceinline__ int tr_swz(int r) { return r & 7; }
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4)
 k_tree(Dsv4TreeJob a)
 {
     constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);
-    using L = TreeLds<KVF, KC, SPLIT>;
+    using L = TreeLds<KVF, KC, SPLIT, tree_planes(tr_fmt<T>(), KVF)>;
     constexpr int NT = tree_terms(tr_fmt<T>()), KT = L::KT, NV = tree_vtiles(KC);
     constexpr int PT = NT > KT ? NT : KT;              /* term pairs i + j < PT  */
     constexpr int W = TR_WAVES, WS = W / 4;
@@ -798,7 +805,7 @@ k_tree(Dsv4TreeJob a)
 template <class T, int KVF, int KC>
 int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
 {
-    using L = TreeLds<KVF, KC, tree_split(tr_fmt<T>(), KVF, KC)>;
+    using L = TreeLds<KVF, KC, tree_split(tr_fmt<T>(), KVF, KC), tree_planes(tr_fmt<T>(), KVF)>;
     if (L::BYTES > 64 * 1024) {
         /* once per device, as the attribute is the device's */
         static bool asked[64];

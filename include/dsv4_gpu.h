@@ -604,7 +604,7 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  * as well), within 1e-5 relative for f32 elements that are 0 or between 1e-30
  * and 3e38 in magnitude (below, terms underflow; larger ones count as
  * infinities); with bf16 q the weights are rounded to bf16 before they meet the
- * rows.
+ * rows, and an F32 cache's elements are taken to 2^-18 of each.
  *
  * d_scratch: dsv4_gpu_tree_attn_scratch_bytes of device memory for the call's
  * shape, 16-byte aligned; the bytes do not fall as n_ctx grows, so a program
