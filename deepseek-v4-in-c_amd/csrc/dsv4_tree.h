@@ -284,8 +284,13 @@ k_tree(Dsv4TreeJob a)
         const int n = min(end, a.rows) - i * TR_TILE;
         return n >= TR_TILE ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
     };
+    /* (__shfl's lane number is a register that the widest rows lack with DMA, and
+     * its reload would wait for all loads; the other formats measure better so) */
     auto my_row = [&](int i, const Place &h) {
-        return max(0, a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
+        if constexpr (DMA)
+            return max(0, a.pages ? __builtin_amdgcn_ds_bpermute(4 * h.sr, ahead) : find(i, h.sr));
+        else
+            return max(0, a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
     };
     /* the eight elements from column c of a row: where they are all there, in one
      * or two loads that need no alignment (the target's own; the LDS-direct ones
