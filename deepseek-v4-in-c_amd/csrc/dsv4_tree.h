@@ -62,6 +62,11 @@ constexpr int tree_split(int fmt, int kv_fmt, int kc)
     return kc >= 16 && tree_terms(fmt) * tree_planes(fmt, kv_fmt) > 1 ? 2 : 1;
 }
 
+/* Workgroups that a CU holds: two of the narrowest rows with bf16 q, whose waves
+ * need no more than 128 registers (f32 q spills in so few and is slower: 1920
+ * rows over 65536 of 128 bf16 188 us, and 207 so). */
+constexpr int tree_per_cu(int fmt, int kc) { return fmt == DSV4_WBF16 && kc == 4 ? 2 : 1; }
+
 #ifdef DSV4_TREE_KERNEL
 
 namespace {
@@ -207,7 +212,7 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * products measured the same or slower; 32 rows of q a wave do not fit the
  * registers. */
 template <class T, int KVF, int KC>
-__global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4)
+__global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4 * tree_per_cu(tr_fmt<T>(), KC))
 k_tree(Dsv4TreeJob a)
 {
     constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);

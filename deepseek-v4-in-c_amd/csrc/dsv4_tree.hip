@@ -173,13 +173,16 @@ struct TreePlan {
  * halves of the time of a tile on a lone wave (0.55 us for bf16 q over 576
  * columns, 0.8 for f32 q): 2 a tile for up to four waves with rows of q and 3 for
  * eight; 8 for the start and 2 for each such wave's q and sums; 5 for the join's
- * launch and 1 for each 4 MB of its sums. A workgroup has a CU to itself, so
- * beyond 256 they come in rounds. Few rows are thus spread over workgroups of 16
+ * launch and 1 for each 4 MB of its sums. A workgroup has a CU to itself but for
+ * the narrowest rows, so beyond 256 they come in rounds. Few rows are thus spread over workgroups of 16
  * of them and read the cache through L2 as often, until the splits fill the
  * card; then wider ones win. Measured, one token's 64 heads of f32 q over a bf16
  * cache, at the best split for 16, 32 and 64 rows a workgroup: 16.0, 17.8 and 23.4 us
  * at 1500 rows of cache (and 14.1 with a tile a split where these had two), 21.4,
- * 23.2 and 28.7 at 8192, 41.9, 34.3 and 39.0 at 32768, 122, 77 and 74 at 131072. */
+ * 23.2 and 28.7 at 8192, 41.9, 34.3 and 39.0 at 32768, 122, 77 and 74 at 131072.
+ * The narrowest rows with bf16 q share a CU by two workgroups, whose tiles then
+ * take 1.6 times as long each (1920 rows over 65536 of 128 FP8: 139 us in 256
+ * workgroups of 128 rows, 110 in 512). */
 TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_ctx, int window)
 {
     TreePlan p;
@@ -204,8 +207,11 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
             if (ns > p.cap) ns = p.cap;
             const long long each = (tiles + ns - 1) / ns;
             ns = (tiles + each - 1) / each;
-            const long long rounds = (nb * ns + 255) / 256;
-            const long long cost = rounds * (each * (waves > 4 ? 3 : 2) + 8 + 2 * waves) +
+            /* rounds in fifths: two that share the CUs take eight */
+            const long long full = (nb * ns + 255) / 256;
+            const long long fifths = tree_per_cu(fmt, p.kc) == 2 ? full / 2 * 8 + full % 2 * 5
+                                                                 : full * 5;
+            const long long cost = fifths * (each * (waves > 4 ? 3 : 2) + 8 + 2 * waves) / 5 +
                                    (ns > 1 ? 5 + ((ns * nt * h * p.dvp) >> 20) : 0);
             if (best >= 0 && cost >= best) continue;
             best = cost;
