@@ -193,10 +193,11 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
     const int tiles = p.tile1 - p.tile0, br = dsv4_tree_block_rows(fmt, kv_fmt, p.kc);
     const int wide = (nt * h + br - 1) / br;
     p.dvp = (d_v + 15) / 16 * 16;
-    /* the workspace goes by the cap alone, and by the most tiles that a
-     * context of this length can have */
-    const int most = window ? (window + nt) / TR_TILE + 2 : tiles;
-    const int up = tiles < most ? tiles : most;
+    /* the workspace goes by the cap alone, and the cap by the most tiles that any
+     * context up to this length can have: the tiles of this one go up and down by
+     * one as its window's start passes a tile's edge */
+    const int most = window ? (window + nt) / TR_TILE + 2 : p.tile1;
+    const int up = p.tile1 < most ? p.tile1 : most;
     p.cap = up < TJ_SPLITS / wide ? up : TJ_SPLITS / wide;
     if (p.cap < 1) p.cap = 1;
     long long best = -1;
@@ -205,6 +206,7 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
         for (int k = 0; k < 5; k++) {             /* one split, or k rounds and more */
             long long ns = k ? 256ll * ((nb + 255) / 256 + k - 1) / nb : 1;
             if (ns > p.cap) ns = p.cap;
+            if (ns > tiles) ns = tiles;
             const long long each = (tiles + ns - 1) / ns;
             ns = (tiles + each - 1) / each;
             /* rounds in fifths: two that share the CUs take eight */

@@ -1,0 +1,37 @@
+"""The workspaces of the operators on drafted tokens: what a program may ask for
+once and then use for every smaller call. CPU only: nothing is launched."""
+import hip_shim
+
+COMMON = r"""
+buf = np.zeros(1 << 12, np.uint8)
+p = (buf.ctypes.data + 255) // 256 * 256                     # nothing reads it
+assert L.dsv4_gpu_init() == 0
+size = L.dsv4_gpu_tree_attn_scratch_bytes
+
+
+def tree(shape, bytes):
+    fmt, nt, h, dqk, dv, kf, ctx, window = shape
+    shim.shim_reset(-1, 0)
+    return L.dsv4_gpu_tree_attn_d(p, p, fmt, nt, h, dqk, dv, p, p, kf, dqk, ctx + nt, None, 0, 0, ctx,
+                                  p, window, None, 1.0, p, bytes, None)
+"""
+
+
+def test_a_windows_workspace_serves_every_shorter_context(tmp_path):
+    """The bytes do not fall as the context grows, whatever the window, and a
+    call with those of the longest is taken at each shorter length."""
+    child = COMMON + r"""
+for fmt, nt, h, dqk, dv, kf in ((0, 1, 64, 576, 512, 2), (1, 13, 64, 128, 128, 1),
+                                (0, 64, 3, 512, 512, 0)):
+    for window in (1, 31, 32, 33, 100, 128, 5000):
+        ctxs = list(range(0, 6000)) + [65536 + k for k in range(-70, 70)]
+        last = 0
+        for ctx in ctxs:
+            n = size(fmt, nt, h, dqk, dv, kf, ctx, window)
+            assert n >= last, (fmt, nt, window, ctx, n, last)
+            last = n
+        for ctx in ctxs[::7] + ctxs[-140:]:
+            assert tree((fmt, nt, h, dqk, dv, kf, ctx, window), last) == 0, (fmt, nt, window, ctx)
+print("done")
+"""
+    assert hip_shim.run(tmp_path, child).endswith("done\n")
