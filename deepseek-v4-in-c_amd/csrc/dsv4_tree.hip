@@ -196,8 +196,8 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
     /* the workspace goes by the cap alone, and the cap by the most tiles that any
      * context up to this length can have: the tiles of this one go up and down by
      * one as its window's start passes a tile's edge */
-    const int most = window ? (window + nt) / TR_TILE + 2 : p.tile1;
-    const int up = p.tile1 < most ? p.tile1 : most;
+    const long long most = window ? ((long long)window + nt) / TR_TILE + 2 : p.tile1;
+    const int up = p.tile1 < most ? p.tile1 : (int)most;
     p.cap = up < TJ_SPLITS / wide ? up : TJ_SPLITS / wide;
     if (p.cap < 1) p.cap = 1;
     long long best = -1;

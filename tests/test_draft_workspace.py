@@ -35,3 +35,23 @@ for fmt, nt, h, dqk, dv, kf in ((0, 1, 64, 576, 512, 2), (1, 13, 64, 128, 128, 1
 print("done")
 """
     assert hip_shim.run(tmp_path, child).endswith("done\n")
+
+
+def test_a_window_longer_than_the_context_is_no_window(tmp_path):
+    """Up to the largest number there is: the same bytes, and where the cache is
+    split without a window (two launches) it is split with one."""
+    child = COMMON + r"""
+for fmt, nt, h, dqk, dv, kf in ((0, 1, 64, 576, 512, 1), (1, 13, 64, 128, 128, 2),
+                                (0, 64, 3, 512, 512, 0)):
+    for ctx in (0, 1, 33, 1000, 32768, 100000):
+        want = size(fmt, nt, h, dqk, dv, kf, ctx, 0)
+        assert tree((fmt, nt, h, dqk, dv, kf, ctx, 0), want) == 0
+        launches = shim.shim_launches()
+        assert launches == 2 or ctx < 32768
+        for window in (2 ** 31 - 1, 2 ** 31 - 1 - nt, 2 ** 31 - nt, 2 ** 30, ctx + 4096):
+            assert size(fmt, nt, h, dqk, dv, kf, ctx, window) == want, (ctx, window)
+            assert tree((fmt, nt, h, dqk, dv, kf, ctx, window), want) == 0
+            assert shim.shim_launches() == launches, (ctx, window)
+print("done")
+"""
+    assert hip_shim.run(tmp_path, child).endswith("done\n")
