@@ -193,9 +193,8 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
     const int tiles = p.tile1 - p.tile0, br = dsv4_tree_block_rows(fmt, kv_fmt, p.kc);
     const int wide = (nt * h + br - 1) / br;
     p.dvp = (d_v + 15) / 16 * 16;
-    /* the workspace goes by the cap alone, and the cap by the most tiles that any
-     * context up to this length can have: the tiles of this one go up and down by
-     * one as its window's start passes a tile's edge */
+    /* the most tiles that any context up to this length can have: the tiles of this
+     * one go up and down by one as its window's start passes a tile's edge */
     const long long most = window ? ((long long)window + nt) / TR_TILE + 2 : p.tile1;
     const int up = p.tile1 < most ? p.tile1 : (int)most;
     p.cap = up < TJ_SPLITS / wide ? up : TJ_SPLITS / wide;
@@ -222,7 +221,11 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
             p.ns = (int)ns;
         }
     }
-    p.bytes = p.cap > 1 ? (size_t)p.cap * nt * h * (p.dvp + 2) * sizeof(float) : 0;
+    /* the workspace: not what this plan writes, whose splits fall in steps as the
+     * rows of q grow, but the least that holds it and never falls with a size */
+    const long long all = (long long)(up < TJ_SPLITS ? up : TJ_SPLITS) * nt * h;
+    const long long most_rows = (long long)TJ_SPLITS * br;
+    p.bytes = up > 1 ? (size_t)(all < most_rows ? all : most_rows) * (p.dvp + 2) * sizeof(float) : 0;
     return p;
 }
 
@@ -270,7 +273,7 @@ extern "C" int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt,
         return -1;
     }
     const TreePlan p = tree_plan(fmt, nt, h, d_qk, d_v, kv_fmt, n_ctx, window);
-    if (p.bytes && (!d_scratch || ((uintptr_t)d_scratch & 15) || scratch_bytes < p.bytes)) {
+    if (p.ns > 1 && (!d_scratch || ((uintptr_t)d_scratch & 15) || scratch_bytes < p.bytes)) {
         DSV4_ERR("tree_attn: %zu bytes of workspace at %p; the call needs %zu, 16-byte aligned",
                  scratch_bytes, d_scratch, p.bytes);
         return -1;

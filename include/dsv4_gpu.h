@@ -607,8 +607,10 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  * rows, and an F32 cache's elements are taken to 2^-18 of each.
  *
  * d_scratch: dsv4_gpu_tree_attn_scratch_bytes of device memory for the call's
- * shape, 16-byte aligned; the bytes do not fall as n_ctx grows, so a program
- * can ask once for its longest context. Its contents are not kept. 0 / -1. */
+ * shape, 16-byte aligned; the bytes do not fall as n_ctx, nt or h grows, so a
+ * program can ask once for its longest context and its largest tree. A call that
+ * does not split its cache writes none and takes any. Its contents are not kept.
+ * 0 / -1. */
 size_t dsv4_gpu_tree_attn_scratch_bytes(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt,
                                         int n_ctx, int window);
 int dsv4_gpu_tree_attn_d(void *d_o, const void *d_q, int fmt, int nt, int h, int d_qk, int d_v,

@@ -55,3 +55,28 @@ for fmt, nt, h, dqk, dv, kf in ((0, 1, 64, 576, 512, 1), (1, 13, 64, 128, 128, 2
 print("done")
 """
     assert hip_shim.run(tmp_path, child).endswith("done\n")
+
+
+def test_a_trees_workspace_serves_smaller_trees(tmp_path):
+    """The attention's bytes do not fall as tokens or heads are added, and calls
+    of fewer are taken with those of the most; a call of one split takes any."""
+    child = COMMON + r"""
+for fmt, dqk, dv, kf in ((0, 576, 512, 1), (0, 512, 512, 0), (1, 576, 512, 1), (1, 128, 128, 2)):
+    for ctx, window in ((100000, 0), (3000, 0), (70000, 128), (40, 0)):
+        for hs in ((1, 5, 16, 40, 64, 65, 128, 1000, 4096), (64,)):
+            prev = {}
+            for h in hs:
+                last = 0
+                for nt in range(1, 65):
+                    n = size(fmt, nt, h, dqk, dv, kf, ctx, window)
+                    assert n >= last, (fmt, h, nt, ctx, window, n, last)
+                    assert n >= prev.get(nt, 0), (fmt, h, nt, ctx, window)
+                    last = prev[nt] = n
+                for nt in range(1, 65, 3 if len(hs) > 1 else 1):
+                    assert tree((fmt, nt, h, dqk, dv, kf, ctx, window), last) == 0, (h, nt, ctx)
+# one split: nothing is written to a workspace
+for shape in ((0, 64, 4096, 576, 512, 1, 100000, 0), (0, 1, 16, 64, 64, 1, 20, 0)):
+    assert tree(shape, 0) == 0 and shim.shim_launches() == 1, shape
+print("done")
+"""
+    assert hip_shim.run(tmp_path, child).endswith("done\n")
