@@ -289,9 +289,9 @@ void plan(int nt, int vocab, int *np, int *rpg)
 extern "C" size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab)
 {
     if (nt <= 0 || vocab <= 0 || nt > DSV4_MAX_BATCH) return 0;
-    int np, rpg;
-    plan(nt, vocab, &np, &rpg);
-    const size_t sw = np * LG_PIECE, n = (size_t)nt * ((vocab + sw - 1) / sw);
+    /* slices of one piece whatever the plan takes, so that the bytes of more rows
+     * are enough for fewer, whose slices may be shorter */
+    const size_t n = (size_t)nt * (((size_t)vocab + LG_PIECE - 1) / LG_PIECE);
     return (n * (sizeof(unsigned long long) + sizeof(uint32_t)) + 15) / 16 * 16 +
            ((size_t)vocab + 3) / 4 * 4 * sizeof(int);
 }

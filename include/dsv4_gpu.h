@@ -645,7 +645,8 @@ typedef struct {
  * none is. Each step is rounded in f32 in the order above. d_out may be
  * d_logits, or NULL where only picks are wanted; d_pick may be NULL.
  * d_scratch: dsv4_gpu_logits_scratch_bytes of device memory, 16-byte aligned,
- * not kept (without picks it may be NULL; long histories are then slower).
+ * not kept (without picks it may be NULL; long histories are then slower); the
+ * bytes do not fall as nt or vocab grows, so those of the most rows serve fewer.
  * repetition must be over 0, n_hist at most 2^30. 0 / -1. */
 size_t dsv4_gpu_logits_scratch_bytes(int nt, int vocab);
 int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, int nt, int vocab,

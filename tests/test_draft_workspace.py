@@ -80,3 +80,25 @@ for shape in ((0, 64, 4096, 576, 512, 1, 100000, 0), (0, 1, 16, 64, 64, 1, 20, 0
 print("done")
 """
     assert hip_shim.run(tmp_path, child).endswith("done\n")
+
+
+def test_the_logits_workspace_serves_fewer_rows(tmp_path):
+    """The bytes do not fall as rows or the vocabulary grow; calls of fewer rows
+    are taken with those of the most."""
+    child = COMMON + r"""
+size = L.dsv4_gpu_logits_scratch_bytes
+prev = [0] * 65
+for vocab in (1, 100, 1023, 1024, 1025, 2049, 32000, 129280, 200001):
+    last = 0
+    for nt in range(1, 65):
+        n = size(nt, vocab)
+        assert n >= last and n >= prev[nt], (nt, vocab, n, last, prev[nt])
+        last = prev[nt] = n
+    for nt in range(1, 65):
+        for hist in (0, 100, 100000):
+            r = D.LogitRules(hist=p, n_hist=hist, repetition=1.5)
+            assert L.dsv4_gpu_logits_adjust_d(p, p, p, nt, vocab, vocab, ctypes.byref(r), p, last,
+                                              None) == 0, (nt, vocab)
+print("done")
+"""
+    assert hip_shim.run(tmp_path, child).endswith("done\n")
