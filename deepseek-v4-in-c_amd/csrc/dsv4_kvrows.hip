@@ -56,6 +56,11 @@ constexpr int AP_WAVES = 16;                      /* of a workgroup with a list 
 constexpr int AP_TOK = 256;                       /* its most tokens         */
 constexpr int AP_BITS = 12;                       /* slots, 16 a token at least */
 constexpr int AP_SHORT = 4096;                    /* lists that are compared */
+/* Most tokens of a launch. Of a list's launches a later one writes over the rows of
+ * those before it, so each looks for later tokens among its own only and a list's
+ * cost grows with its length, not its square; without a list 64 threads a token
+ * stay below a launch's 2^32. */
+constexpr int AP_LIST = 1 << 17, AP_RUN = 1 << 25;
 enum { AP_NONE, AP_COMPARE, AP_HASH };            /* what a list takes       */
 
 __device__ __forceinline__ uint32_t row_slot(int row)
@@ -459,20 +464,27 @@ extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, 
         }
     }
     if (n == 0) return 0;
-    AppendJob a{d_kv, d_kv_scales, kv_stride, kv_rows, d_x, x_stride, n, row_dim, d_rows, row0,
-                rope ? d_pos : nullptr, rope ? *rope : dsv4_gpu_rope{}, 0};
-    /* a long list's workgroups: 512 of them fill the card's waves */
-    const int per = n / (AP_WAVES * 512) + 1;
-    a.tok = AP_WAVES * (per < AP_TOK / AP_WAVES ? per : AP_TOK / AP_WAVES);
     /* pieces of four elements, the last one moved back to the row's end; one by
      * one in rows of less, and where the rotation's pairs do not fall into pieces */
     int V = row_dim < 4 ? 1 : 4;
     if (rope && (row_dim % 4 || rope->offset % 4 || rope->dim % 4 ||
                  (rope->layout == DSV4_GPU_ROPE_HALVES && rope->dim % 8)))
         V = 1;
-    if (x_fmt == DSV4_WF32) append_fmt<float>(a, kv_fmt, V, (hipStream_t)stream);
-    else append_fmt<uint16_t>(a, kv_fmt, V, (hipStream_t)stream);
-    HIP_OK(hipGetLastError(), "kv_append launch");
+    const int es = x_fmt == DSV4_WBF16 ? 2 : 4;
+    const int most = d_rows ? AP_LIST : AP_RUN;
+    for (int t0 = 0; t0 < n; t0 += most) {
+        const int m = n - t0 < most ? n - t0 : most;
+        AppendJob a{d_kv, d_kv_scales, kv_stride, kv_rows,
+                    (const char *)d_x + (size_t)t0 * x_stride * es, x_stride, m, row_dim,
+                    d_rows ? d_rows + t0 : nullptr, row0 + (d_rows ? 0 : t0),
+                    rope ? d_pos + t0 : nullptr, rope ? *rope : dsv4_gpu_rope{}, 0};
+        /* a long list's workgroups: 512 of them fill the card's waves */
+        const int per = m / (AP_WAVES * 512) + 1;
+        a.tok = AP_WAVES * (per < AP_TOK / AP_WAVES ? per : AP_TOK / AP_WAVES);
+        if (x_fmt == DSV4_WF32) append_fmt<float>(a, kv_fmt, V, (hipStream_t)stream);
+        else append_fmt<uint16_t>(a, kv_fmt, V, (hipStream_t)stream);
+        HIP_OK(hipGetLastError(), "kv_append launch");
+    }
     return 0;
 }
 
