@@ -373,9 +373,10 @@ __global__ void __launch_bounds__(KR_THREADS) k_read(ReadJob a)
         if (o[u]) io_store<T, V>(o[u], v[u]);
 }
 
-/* -1 with a message unless the cache's own description holds. */
+/* -1 with a message unless the cache's own description holds, for a call of n
+ * rows. */
 int cache_ok(const char *what, const void *kv, const float *scales, int fmt, int stride, int rows,
-             int dim)
+             int dim, int n)
 {
     if (fmt != DSV4_GPU_KV_F32 && fmt != DSV4_GPU_KV_BF16 && fmt != DSV4_GPU_KV_FP8) {
         DSV4_ERR("%s: unknown cache format %d", what, fmt);
@@ -385,7 +386,7 @@ int cache_ok(const char *what, const void *kv, const float *scales, int fmt, int
         DSV4_ERR("%s: bad cache shape (rows %d of %d, stride %d)", what, rows, dim, stride);
         return -1;
     }
-    if (!kv || (fmt == DSV4_GPU_KV_FP8 && !scales)) {
+    if (n && (!kv || (fmt == DSV4_GPU_KV_FP8 && !scales))) {
         DSV4_ERR("%s: no cache, or an FP8 cache without row scales", what);
         return -1;
     }
@@ -442,7 +443,7 @@ extern "C" int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, 
                                     int n, int row_dim, const int *d_rows, int row0,
                                     const dsv4_gpu_rope *rope, const int *d_pos, void *stream)
 {
-    if (cache_ok("kv_append", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
+    if (cache_ok("kv_append", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim, n) != 0)
         return -1;
     if (n < 0 || n > KR_MOST || row_dim > KR_DIM || x_stride < row_dim ||
         (x_fmt != DSV4_WF32 && x_fmt != DSV4_WBF16) || (n && !d_x)) {
@@ -493,7 +494,7 @@ extern "C" int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride
                                   int kv_stride, int kv_rows, const int *d_rows, int row0, int n,
                                   int row_dim, void *stream)
 {
-    if (cache_ok("kv_read", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim) != 0)
+    if (cache_ok("kv_read", d_kv, d_kv_scales, kv_fmt, kv_stride, kv_rows, row_dim, n) != 0)
         return -1;
     if (n < 0 || n > KR_MOST || row_dim > KR_DIM || out_stride < row_dim ||
         (out_fmt != DSV4_WF32 && out_fmt != DSV4_WBF16) || (n && !d_out)) {

@@ -525,9 +525,11 @@ int dsv4_gpu_attn_step_d(float *d_out, const float *d_x, int layer, int pos, voi
  * use no library buffer: calls on different streams may overlap, and a call
  * can be captured into a graph, as long as those that overlap are given
  * workspaces of their own. They run on the current device, where every
- * pointer must lie. Lengths and strides are in elements; nt or n of 0 does
- * nothing and returns 0. Results do not depend on what else runs: no sum is
- * taken in an order that varies. No counterpart in the reference's header. */
+ * pointer must lie. Lengths and strides are in elements; a call whose nt or n
+ * is 0 needs no buffers, does nothing and returns 0, but its sizes, types,
+ * ranges, rotation and rules are checked as ever. Results do not depend on
+ * what else runs: no sum is taken in an order that varies. No counterpart in
+ * the reference's header. */
 
 /* How the two elements of a rotated pair lie: neighbours (2i, 2i + 1), the
  * reference's layout (dsv4_rope.c:105-119), or i and i + dim/2. */
@@ -555,9 +557,10 @@ int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long l
 
 /* Write n rows of row_dim values (f32 or bf16, row t at d_x + t * x_stride)
  * into a cache in a DSV4_GPU_KV_* format, rotated first by rope and d_pos if
- * rope is not NULL (as one head). Row t goes to cache row d_rows[t], or row0 +
- * t where d_rows is NULL; a row outside [0, kv_rows) is not written, and of
- * several t that name one row the last is written. The cache's other rows,
+ * rope is not NULL (as one head). Row t goes to cache row d_rows[t], where one
+ * outside [0, kv_rows) is not written and of several t that name one row the
+ * last is; or, with d_rows NULL, to row0 + t, and a call whose row0 .. row0 +
+ * n - 1 are not all in the cache is refused. The cache's other rows,
  * and a row's elements past row_dim, are left as they were. BF16 rounds to
  * nearest even. FP8 stores e4m3(x / s), to nearest even, with s (d_kv_scales)
  * the least power of two, 2^-126 at least, that brings the row's largest
@@ -572,8 +575,9 @@ int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stri
 
 /* Read n cache rows back as f32 or bf16 (out_fmt): d_out + t * out_stride =
  * row d_rows[t] (row0 + t where d_rows is NULL), an FP8 element as code *
- * scale in f32, rounded to nearest even for bf16. A row outside [0, kv_rows)
- * gives zeros and is never read. row_dim is at most 16384, n at most 2^30.
+ * scale in f32, rounded to nearest even for bf16. A d_rows[t] outside [0,
+ * kv_rows) gives zeros and is never read; a range behind row0 that is not all
+ * in the cache is refused. row_dim is at most 16384, n at most 2^30.
  * 0 / -1. */
 int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const void *d_kv,
                        const float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,

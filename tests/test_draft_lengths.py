@@ -63,3 +63,34 @@ def test_launches_of_the_most_rows(tmp_path, monkeypatch):
     assert keep in source
     monkeypatch.setattr(hip_shim, "SOURCE", source.replace(keep, "    (void)a;\n"))
     assert hip_shim.run(tmp_path, CHILD).endswith("done\n")
+
+
+EMPTY = r"""
+p = np.zeros(64, np.uint8).ctypes.data
+assert L.dsv4_gpu_init() == 0
+rope = D.Rope(cos=p, sin=p, max_pos=8, dim=2, offset=0, layout=0)
+rules = D.LogitRules(repetition=1.0)
+calls = {                                                    # (of 0, with a wrong size or rule)
+    "dsv4_gpu_rope_n_d": [(None, 8, None, 8, 0, None, 0, 1, hd, ctypes.byref(rope), 0, None)
+                          for hd in (8, 1)],
+    "dsv4_gpu_kv_append_d": [(None, None, 2, 8, 4, None, 0, 8, 0, 8, None, row0,
+                              ctypes.byref(rope), None, None) for row0 in (4, 5)],
+    "dsv4_gpu_kv_read_d": [(None, 0, 8, None, None, 2, 8, 4, None, row0, 0, 8, None)
+                           for row0 in (4, 5)],
+    "dsv4_gpu_tree_attn_d": [(None, None, 0, 0, 1, 8, dv, None, None, 2, 8, 4, None, 0, 0, 3, None,
+                              0, None, 1.0, None, 0, None) for dv in (8, 9)],
+    "dsv4_gpu_logits_adjust_d": [(None, None, None, 0, 8, 8, r, None, 0, None)
+                                 for r in (ctypes.byref(rules), None)],
+}
+for name, (good, bad) in calls.items():
+    shim.shim_reset(-1, 0)
+    assert getattr(L, name)(*good) == 0, name
+    assert getattr(L, name)(*bad) == -1, name
+    assert shim.shim_launches() == 0, name
+print("done")
+"""
+
+
+def test_a_length_of_zero_needs_no_buffers(tmp_path):
+    """Its sizes, types, ranges and rules are checked as ever."""
+    assert hip_shim.run(tmp_path, EMPTY).endswith("done\n")
