@@ -565,8 +565,8 @@ int dsv4_gpu_rope_n_d(void *d_out, long long out_stride, const void *d_x, long l
  * nearest even. FP8 stores e4m3(x / s), to nearest even, with s (d_kv_scales)
  * the least power of two, 2^-126 at least, that brings the row's largest
  * finite magnitude to 448 or less (1 for a row of zeros); infinities and NaN
- * are stored as NaN. Rows written, read back and written again keep their
- * values. kv_stride >= row_dim, which is at most 16384, and n at most 2^30.
+ * are stored as NaN. Rows written, read back as f32 and written again keep
+ * their values. kv_stride >= row_dim, which is at most 16384, and n at most 2^30.
  * d_x must not overlap the cache. 0 / -1. */
 int dsv4_gpu_kv_append_d(void *d_kv, float *d_kv_scales, int kv_fmt, int kv_stride, int kv_rows,
                          const void *d_x, int x_fmt, long long x_stride, int n, int row_dim,
