@@ -603,12 +603,16 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  * that do not see it, NaN and infinities included; one that sees a row with
  * such an element may get NaN in any of its outputs.
  *
- * Scores, softmax and sums are in f32. With f32 q every product is exact
- * (bf16 terms of q and of the weights; an F32 cache's elements in three terms
- * as well), within 1e-5 relative for f32 elements that are 0 or between 1e-30
- * and 3e38 in magnitude (below, terms underflow; larger ones count as
- * infinities); with bf16 q the weights are rounded to bf16 before they meet the
- * rows, and an F32 cache's elements are taken to 2^-18 of each.
+ * Scores, softmax and sums are in f32. With f32 q every product with a BF16 or
+ * FP8 row is exact (bf16 terms of q and of the weights), and one with an F32
+ * row, taken in three terms as well, to 2^-23 of it: o is within 1e-5 relative.
+ * With bf16 q the weights are rounded to bf16 before they meet the rows, and an
+ * F32 cache's elements are taken to 2^-18 of each. That holds for f32 elements
+ * that are 0 or at least 1e-30 in magnitude (below, terms underflow), where the
+ * largest element a token sees times the rows it sees is at most 1e36 (the sums
+ * are divided at the end, and a row's weight in them reaches 2^8) and q . row
+ * stays below 3e38; F32 elements over 3e38 count as infinities. d_o must not
+ * overlap what the call reads.
  *
  * d_scratch: dsv4_gpu_tree_attn_scratch_bytes of device memory for the call's
  * shape, 16-byte aligned; the bytes do not fall as n_ctx, nt or h grows, so a
