@@ -49,3 +49,33 @@ def test_the_largest_values(gpu, dsv4, fmt, bf, ctx):
         assert rc == 0
         want, size = dc.attention(q, v, dc.visible(None, nt, ctx, 0), None, sc, d)
         tt.check(dc.host(o) / top, want / top, size / top, bf)
+
+
+@pytest.mark.parametrize("fmt,bf", [(0, True), (1, True), (2, True), (2, False)])
+def test_the_mean_of_equal_rows_is_the_row(gpu, dsv4, fmt, bf):
+    """Rows that differ in their scores alone: whatever the weights and their
+    rounding, o is the row's values, which bf16 holds, as the weights are divided by
+    their own sum. The first tile's weights are 1; the later ones' would be 2^7 (1 +
+    0.0038), just under the middle of two bf16 numbers, over a maximum that has not
+    moved. f32 sums of 200 rows are off by 200 2^-24 at most, far under half a step
+    of bf16; with f32 q that is the bound."""
+    nt, h, dqk, dv, ctx = 64, 520, 64, 56, 136
+    n = ctx + nt
+    rng = np.random.default_rng(fmt)
+    rows = np.zeros((n, dqk))
+    rows[:, :dv] = 2.0 ** rng.integers(-1, 2, dv) * (1 + rng.integers(0, 8, dv) / 8)
+    rows[32:, dv], rows[32:, dv + 1] = 7.0, 0.75
+    q = np.zeros((nt, h, dqk), np.float32)
+    q[:, :, dv], q[:, :, dv + 1] = 1.0, dc.bf16(0.00555 / 0.75)
+    assert 0.0050 < 0.75 * q[0, 0, dv + 1] < np.log2(1 + 2.0 ** -8) - 1e-5
+    scales = np.exp2(rng.integers(-2, 3, n)) if fmt == 2 else None
+    cache, ks = dc.cache_of(rows, fmt, scales=scales)
+    words = dc.dev(np.full(nt, 2 ** 64 - 1, np.uint64))
+    rc, o = dc.tree(dsv4, dc.to_fmt(q, bf), bf, cache, ks, fmt, n, dqk, dv, ctx, words,
+                    scale=np.float32(np.log(2.0)))
+    assert rc == 0
+    want = np.broadcast_to(rows[0, :dv], (nt, h, dv))
+    if bf:
+        assert np.array_equal(dc.host(o), want)
+    else:
+        assert np.abs(dc.host(o) / want - 1).max() <= n * dc.U32
