@@ -18,13 +18,13 @@
  * hashes its tokens' rows into LDS and looks the entries up there, so that one
  * costs an LDS read however many tokens the workgroup has, and it takes more
  * of them, 256 at most, as the list grows: of rows of 512 f32 to FP8, 2000 take
- * 4.4 us compared and 4.8 looked up, 6000 9.1 and 8.2, 60000 270 and 46 (29 where
- * they follow row0); of rows of 32, 118000 take 824 and 70.
+ * 4.3 us compared and looked up, 6000 7.4 and 6.3, 60000 245 and 42 (27 where they
+ * follow row0); of rows of 32, 118000 take 817 and 70.
  *
  * READ. A thread makes 16 bytes of output at a time, so that stores, the
  * larger stream from an FP8 cache, are whole lines, and two of them: 131072
- * rows of 576 from FP8 to f32 take 70.4 us (5.4 TB/s), with four pieces a thread
- * 70.8 and with one 72.6; 2048 rows 3.1, 3.6 and 3.2.
+ * rows of 576 from FP8 to f32 take 69.2 us (5.5 TB/s), with four pieces a thread
+ * 69.7 and with one 71.7; 2048 rows 3.0, 3.4 and 2.7.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"

@@ -15,9 +15,9 @@
  * between rows. It leaves the best composite and the first allowed token of its
  * part of a row, and a second launch of one wave per row picks.
  *
- * 64 rows of 129280 with every rule and 16384 ids of history: 27.5 us from HBM,
+ * 64 rows of 129280 with every rule and 16384 ids of history: 24.6 us from HBM,
  * of which 14 are the 66 MB at a large copy's 4.6 TB/s, 3.5 the second launch
- * and some 4 the history. One row: 5.6 us, both launches' latency.
+ * and some 5 the history. One row: 5.7 us, both launches' latency.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -28,9 +28,9 @@ constexpr int LG_THREADS = 256;
 constexpr int LG_WAVES = LG_THREADS / 64;
 /* A longer history is counted by a launch of its own, with four times the
  * threads on a slice; a shorter one each workgroup counts for itself. For 1, 8
- * and 64 rows of 129280, without that launch and with it: 7.7, 10.7, 28.0 and 8.0, 11.5, 29.2
- * us at 16384 ids, 10.2 and 8.9 us for one row of 32768, and 27, 32, 57 and 14, 17,
- * 36 us at 131072. */
+ * and 64 rows of 129280, without that launch and with it: 7.6, 9.5, 26.0 and 7.9, 10.5, 26.0
+ * us at 16384 ids, 9.9 and 8.7 us for one row of 32768, and 24, 31, 54 and 13, 17,
+ * 32 us at 131072. */
 constexpr int LC_HIST = 24576;
 constexpr int LC_THREADS = 1024, LC_SLICE = 1024;
 constexpr int LG_ROWS = 8;                       /* most rows of a workgroup */
@@ -271,11 +271,11 @@ k_logits_pick(int *__restrict__ pick, const unsigned long long *__restrict__ bes
 }
 
 /* Pieces of a slice and rows of a workgroup. Few rows take short slices, so that
- * more workgroups share them (one row of 129280: 5.6 us, 6.2 with two pieces);
- * from four rows on a history counted for two pieces costs less than it gains
- * (4 rows 6.9 us both ways, 64 rows 28.4 and 27.7). Groups of rows are as small as
- * the card's 256 CUs hold at once, six workgroups each (64 rows: 1024 workgroups
- * 28.4 us, 1536 27.7, 2048 30.5, one row each 32.9). */
+ * more workgroups share them (one row of 129280: 5.7 us, 6.2 with two pieces);
+ * with more rows two pieces cost less than they gain (4 rows 6.4 us with one and 6.8
+ * with two, 8 8.3 and 7.4, 64 23.4 and 22.2). Groups of rows are as small as the
+ * card's 256 CUs hold at once, six workgroups each (64 rows and 16384 ids: 1024
+ * workgroups 25.8 us, 1536 25.9, 2048 27.7, one row each 30.7). */
 void plan(int nt, int vocab, int *np, int *rpg)
 {
     *np = nt >= 4 ? 2 : 1;

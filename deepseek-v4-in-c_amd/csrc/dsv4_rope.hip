@@ -12,10 +12,12 @@
  * owns one 16-byte piece (neighbours) or two pieces dim/2 apart (halves) of a
  * head, so a pair's elements meet in one thread and d_out may be d_x. Where a
  * head has elements outside the rotated part and d_out is not d_x, further
- * threads copy them. 4099 tokens of 64 heads of 128, bf16: 26.7 us (halves) and
- * 27.9 us (pairs) from HBM, 5.0 TB/s, a large copy's rate. Four heads a thread,
- * to read the tables' entries once for them, were slower nearly everywhere (31.1
- * us here, 4.2 against 2.7 us for one token).
+ * threads copy them. 4099 tokens of 64 heads of 128, bf16: 26.5 us (halves) and
+ * 27.6 us (pairs) from HBM, 5.1 TB/s, over a large copy's rate; a head or a part
+ * that is not whole pieces goes element by element (60 rotated elements of the
+ * 128: 100 us, 64 of them 29). Four heads a thread, to read the tables' entries
+ * once for them, were slower nearly everywhere (31.1 us against 26.7 for these
+ * tokens, 4.2 against 2.7 for one).
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"

@@ -43,6 +43,8 @@ int dsv4_tree_fp8_launch(const Dsv4TreeJob &a, int fmt, int kc, hipStream_t st);
 
 /* bf16 terms that carry an f32 value exactly. */
 constexpr int TR_TERMS = 3;
+/* bf16 q's weights in one, as a second would double the second product's matrix
+ * instructions for an error that is at most the output's own rounding. */
 constexpr int tree_terms(int fmt) { return fmt == DSV4_WF32 ? TR_TERMS : 1; }
 /* An F32 cache's elements in as many for f32 q, and in two, to 2^-18 of each, for
  * bf16 q, whose weights are rounded to 2^-9 (2048 rows of q over 16384 of 512: 195
@@ -152,9 +154,10 @@ __device__ __forceinline__ void tr_vm_wait()
 
 /* 16 bytes per lane from p to LDS byte dst + 16 lane (dst the same in every
  * lane). As the builtin the compiler would wait for it before each later
- * transposed read of LDS; this way nothing waits but tr_vm_wait. It writes no
- * register but M0, which the compiler sets anew before each use of its own, and
- * its addresses are read as it issues. */
+ * transposed read of LDS; this way nothing waits but tr_vm_wait. Its addresses
+ * are read as it issues, and it writes no register but M0. That cannot be named as
+ * clobbered; k_tree has no other use of it (no LDS-direct builtin, no indexed
+ * register, no message), as its assembly shows, and must not get one. */
 __device__ __forceinline__ void tr_to_lds(const void *p, uint32_t dst)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
@@ -215,11 +218,11 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * Bound: the matrix core where there are rows of q enough, and the start (q's
  * loads and terms, one tile's trip from HBM, about 4 us) where there are not.
  * 8192 rows of q in bf16 over 131072 cache rows in bf16 (d_qk 576, d_v 512): 2053
- * to 2230 us with the clock of the card, 1.05 to 1.14 PFLOP/s, where a library
+ * to 2290 us with the clock of the card, 1.02 to 1.14 PFLOP/s, where a library
  * product of 8192^3 reaches 1.20. Per tile and SIMD the products take 2176 cycles
  * of some 4000; the rest is the softmax's vector instructions (1000 cycles for two
  * waves) and the loads' issue, of which the other wave's products hide the most.
- * 1024 rows of f32 q over 32768 of FP8: 186 to 193 us, 1.07 to 1.11 PFLOP/s of bf16
+ * 1024 rows of f32 q over 32768 of FP8: 186 to 196 us, 1.05 to 1.11 PFLOP/s of bf16
  * terms. Waves half a tile apart, deeper reads ahead, wave priorities and loads issued between
  * products measured the same or slower; 32 rows of q a wave do not fit the
  * registers. */

@@ -180,6 +180,8 @@ struct TreePlan {
  * cache, at the best split for 16, 32 and 64 rows a workgroup: 16.0, 17.8 and 23.4 us
  * at 1500 rows of cache (and 14.1 with a tile a split where these had two), 21.4,
  * 23.2 and 28.7 at 8192, 41.9, 34.3 and 39.0 at 32768, 122, 77 and 74 at 131072.
+ * A tile has that price at every width and format, though those of narrower rows
+ * take less: such calls may take more splits than are best for them.
  * The narrowest rows with bf16 q share a CU by two workgroups, whose tiles then
  * take 1.6 times as long each (1920 rows over 65536 of 128 FP8: 139 us in 256
  * workgroups of 128 rows, 110 in 512). */
