@@ -46,8 +46,8 @@ constexpr int TR_TERMS = 3;
 /* bf16 q's weights in one, as a second would double the second product's matrix
  * instructions for an error that is at most the output's own rounding. */
 constexpr int tree_terms(int fmt) { return fmt == DSV4_WF32 ? TR_TERMS : 1; }
-/* An F32 cache's elements in as many for f32 q, and in two, to 2^-18 of each, for
- * bf16 q, whose weights are rounded to 2^-9 (2048 rows of q over 16384 of 512: 195
+/* An F32 cache's elements in as many for f32 q, and in two, to 2^-17 of each, for
+ * bf16 q, whose weights are rounded to 2^-8 (2048 rows of q over 16384 of 512: 195
  * us, 265 with three). */
 constexpr int tree_planes(int fmt, int kv_fmt)
 {

@@ -608,7 +608,7 @@ int dsv4_gpu_kv_read_d(void *d_out, int out_fmt, long long out_stride, const voi
  * row, taken in three terms as well, to 2^-23 of it: o is within 1e-5 relative.
  * With bf16 q the weights are rounded to bf16 before they meet the rows and
  * divided by the sum of the rounded ones, and an F32 cache's elements are taken
- * to 2^-18 of each. That holds for f32 elements that are 0 or at least 1e-30 in
+ * to 2^-17 of each. That holds for f32 elements that are 0 or at least 1e-30 in
  * magnitude (below, terms underflow), where the largest element a token sees
  * times the rows it sees is at most 1e36 (the sums are divided at the end, and a
  * row's weight in them reaches 2^8) and q . row stays below 3e38; F32 elements
