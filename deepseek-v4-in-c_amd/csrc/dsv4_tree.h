@@ -551,7 +551,9 @@ k_tree(Dsv4TreeJob a)
         if (a.window && a.window < a.nt)
             for (int j = 0; j < a.nt; j++) {
                 const unsigned long long oj = a.mask ? a.mask[j] : (2ull << j) - 1;
-                if (depth - __popcll(oj & all & ~(1ull << j)) >= a.window) see &= ~(1ull << j);
+                /* signed: a token may see one that is further on */
+                const int back = depth - (int)__popcll(oj & all & ~(1ull << j));
+                if (back >= a.window) see &= ~(1ull << j);
             }
         unsigned char *d = lds + L::ROWS + 16 * (16 * w + lane0);
         *(unsigned long long *)d = see;

@@ -79,3 +79,21 @@ def test_the_mean_of_equal_rows_is_the_row(gpu, dsv4, fmt, bf):
         assert np.array_equal(dc.host(o), want)
     else:
         assert np.abs(dc.host(o) / want - 1).max() <= n * dc.U32
+
+
+@pytest.mark.parametrize("fmt,bf", [(0, False), (1, True), (2, False)])
+@pytest.mark.parametrize("nt", [2, 7, 63, 64])
+def test_words_of_any_kind_under_a_window(gpu, dsv4, fmt, bf, nt):
+    """Tokens that see later ones, not themselves or bits past the last token: a
+    token further on than the one that sees it is not back behind its window."""
+    h, d, ctx = 3, 40, 50
+    rng, dq, q, v, cache, ks, rows, _ = tt.problem(nt, nt, h, d, ctx, fmt, bf)
+    w = [int(x) for x in rng.integers(0, 2 ** 64, nt, dtype=np.uint64)]
+    for window in (0, 1, 3, 20, 64):
+        rc, o = dc.tree(dsv4, dq, bf, cache, ks, fmt, rows, d, d, ctx,
+                        dc.dev(np.array(w, np.uint64)), window, scale=0.2)
+        assert rc == 0
+        see = dc.visible(w, nt, ctx, window)
+        want, size = dc.attention(q, v, see, None, 0.2, d)
+        tt.check(dc.host(o), want, size, bf)
+        assert (dc.host(o)[~see.any(1)] == 0).all()
