@@ -104,7 +104,9 @@ __device__ __forceinline__ void tr_terms(const float *v, tr_bf8 *t)
     }
 }
 
-/* The sum of eight f32, each rounded to bf16 (v_dot2_f32_bf16 with ones). */
+/* The sum of eight f32, each rounded to bf16 (v_dot2_f32_bf16 with ones, of the pairs
+ * as they are rounded: of the words of a vector of eight this compiler takes the
+ * first four times). */
 __device__ __forceinline__ float tr_sum8(const float *v)
 {
     const tr_bf2 one = __builtin_bit_cast(tr_bf2, 0x3F803F80u);

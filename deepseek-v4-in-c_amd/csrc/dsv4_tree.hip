@@ -227,7 +227,8 @@ TreePlan tree_plan(int fmt, int nt, int h, int d_qk, int d_v, int kv_fmt, int n_
      * rows of q grow, but the least that holds it and never falls with a size */
     const long long all = (long long)(up < TJ_SPLITS ? up : TJ_SPLITS) * nt * h;
     const long long most_rows = (long long)TJ_SPLITS * br;
-    p.bytes = up > 1 ? (size_t)(all < most_rows ? all : most_rows) * (p.dvp + 2) * sizeof(float) : 0;
+    p.bytes = up > 1 ? (size_t)(all < most_rows ? all : most_rows) * (p.dvp + 2) * sizeof(float)
+                     : 0;
     return p;
 }
 

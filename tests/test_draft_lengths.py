@@ -6,7 +6,11 @@ import hip_shim
 GRIDS = r"""
 static double most_threads;
 static long long groups;
-void shim_grids(double *t, long long *g) { *t = most_threads; *g = groups; most_threads = 0; groups = 0; }
+void shim_grids(double *t, long long *g)
+{
+    *t = most_threads; *g = groups;
+    most_threads = 0; groups = 0;
+}
 int __hipPushCallConfiguration(D3 g, D3 b, size_t l, void *s)
 {
     const double x = (double)g.x * b.x, y = (double)g.y * b.y;

@@ -12,8 +12,8 @@ size = L.dsv4_gpu_tree_attn_scratch_bytes
 def tree(shape, bytes):
     fmt, nt, h, dqk, dv, kf, ctx, window = shape
     shim.shim_reset(-1, 0)
-    return L.dsv4_gpu_tree_attn_d(p, p, fmt, nt, h, dqk, dv, p, p, kf, dqk, ctx + nt, None, 0, 0, ctx,
-                                  p, window, None, 1.0, p, bytes, None)
+    return L.dsv4_gpu_tree_attn_d(p, p, fmt, nt, h, dqk, dv, p, p, kf, dqk, ctx + nt, None, 0, 0,
+                                  ctx, p, window, None, 1.0, p, bytes, None)
 """
 
 
