@@ -98,6 +98,17 @@ class LogitRules(ctypes.Structure):
                 ("allow", _vp), ("allow_stride", _ci)]
 
 
+class Reqs(ctypes.Structure):
+    """dsv4_gpu_reqs (include/dsv4_gpu.h); device pointers."""
+    _fields_ = [(n, _vp) for n in ("len", "pages", "first")] + \
+               [(n, _ci) for n in ("n_req", "max_pages", "page_rows", "max_tok", "n_prefix")]
+
+
+class Sampling(ctypes.Structure):
+    """dsv4_gpu_sampling (include/dsv4_gpu.h); device pointers."""
+    _fields_ = [(n, _vp) for n in ("temperature", "top_k", "top_p", "min_p", "u")]
+
+
 def build():
     """Compile lib/libdsv4_gpu.so (hipcc, gfx950) and the CPU stub."""
     subprocess.run(["make", "-s", "-C", HERE, "all"], check=True)
@@ -110,6 +121,8 @@ _ACP = ctypes.POINTER(AttnCfg)
 _AWP = ctypes.POINTER(AttnW)
 _RP = ctypes.POINTER(Rope)
 _LRP = ctypes.POINTER(LogitRules)
+_RQP = ctypes.POINTER(Reqs)
+_SP = ctypes.POINTER(Sampling)
 _sz = ctypes.c_size_t
 _ll = ctypes.c_longlong
 
@@ -186,6 +199,9 @@ _SIGS = {
                                    _vp, _ci, _ci, _ci, _vp, _ci, _vp, _cf, _vp, _sz, _vp]),
     "dsv4_gpu_logits_scratch_bytes": (_sz, [_ci, _ci]),
     "dsv4_gpu_logits_adjust_d": (_ci, [_vp, _vp, _vp, _ci, _ci, _ll, _LRP, _vp, _sz, _vp]),
+    "dsv4_gpu_reqs_tables_d": (_ci, [_RQP, _vp, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dsv4_gpu_sample_scratch_bytes": (_sz, [_ci, _ci]),
+    "dsv4_gpu_sample_d": (_ci, [_vp, _vp, _vp, _vp, _ci, _ci, _ci, _ll, _SP, _vp, _sz, _vp]),
 }
 
 SYMBOLS = tuple(_SIGS)

@@ -229,3 +229,14 @@ int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, i
                              void *d_scratch, size_t scratch_bytes, void *stream)
 { (void)d_out; (void)d_pick; (void)d_logits; (void)nt; (void)vocab; (void)stride; (void)rules;
   (void)d_scratch; (void)scratch_bytes; (void)stream; return -1; }
+int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, const int *d_new, int *d_ring,
+                           int ring_cap, const int *d_free, int *d_free_out, int *d_rows,
+                           int *d_pos, int *d_req, void *stream)
+{ (void)r; (void)d_len; (void)d_new; (void)d_ring; (void)ring_cap; (void)d_free;
+  (void)d_free_out; (void)d_rows; (void)d_pos; (void)d_req; (void)stream; return -1; }
+size_t dsv4_gpu_sample_scratch_bytes(int n, int vocab) { (void)n; (void)vocab; return 0; }
+int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const void *d_logits, int fmt,
+                      int n, int vocab, long long stride, const dsv4_gpu_sampling *s,
+                      void *d_scratch, size_t scratch_bytes, void *stream)
+{ (void)d_pick; (void)d_prob; (void)d_kept; (void)d_logits; (void)fmt; (void)n; (void)vocab;
+  (void)stride; (void)s; (void)d_scratch; (void)scratch_bytes; (void)stream; return -1; }

@@ -344,3 +344,6 @@ int dsv4_comp_close_launch(float *out, float *kv_state, float *score_state, int 
 
 /* What is wrong with a rotation of heads of head_dim elements, or nullptr. */
 const char *dsv4_rope_bad(const dsv4_gpu_rope *r, int head_dim);
+
+/* What is wrong with a batch of requests' shape, or nullptr. */
+const char *dsv4_reqs_bad(const dsv4_gpu_reqs *r);

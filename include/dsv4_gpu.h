@@ -661,6 +661,86 @@ int dsv4_gpu_logits_adjust_d(float *d_out, int *d_pick, const float *d_logits, i
                              long long stride, const dsv4_gpu_logit_rules *rules,
                              void *d_scratch, size_t scratch_bytes, void *stream);
 
+/* ------------------------------------------------- batches of requests ----
+ * The device half of a step that serves many requests at once, each with its
+ * own pages of one latent cache: page tables and row maps made on the device
+ * from lengths, attention of every request's tokens with the prefix that they
+ * share read once for all, and sampling. Beside them a step uses the rotations,
+ * the cache rows and the logit rules above. The reference serves one sequence.
+ *
+ * As above: stream-ordered, on the current device, nothing allocated, kept
+ * between calls or taken from the library; calls that overlap need workspaces
+ * (and plans) of their own; capturable, and as the lengths lie on the device a
+ * captured step serves other lengths at its next replay. Results do not depend
+ * on what else runs. No counterpart in the reference's header. */
+
+/* A batch. Request i's position p is cache row pages[i * max_pages + p /
+ * page_rows] * page_rows + p % page_rows. Its tokens of this step are tokens
+ * first[i] .. first[i + 1] - 1 of the batch and its last positions, len[i] - (first[i
+ * + 1] - first[i]) .. len[i] - 1. n_req is at most 4096, max_tok 2^20 and max_pages *
+ * page_rows 2^30. */
+typedef struct {
+    int *len;              /* [n_req] positions in use, these tokens included  */
+    int *pages;            /* [n_req][max_pages]                              */
+    int *first;            /* [n_req + 1]                                     */
+    int n_req, max_pages, page_rows;
+    int max_tok;           /* tokens that a step's buffers have room for       */
+    int n_prefix;          /* the first positions hold the same rows in every
+                            * request that is as long, and whole pages of them
+                            * are all requests'                               */
+} dsv4_gpu_reqs;
+
+/* The tables of a step. d_len[i] positions of request i are in use; d_new[i] >
+ * 0 tokens are to be added, 0 none, and with d_new[i] < 0 the request ends.
+ * Free pages are a ring: d_free[0] is the place of the first and d_free[1]
+ * their number; ring_cap is at least the pages there are, at most 2^30.
+ *
+ * Request i is served if its tokens fit its table, if it needs no new page or
+ * the new pages of the requests up to i that fit their tables are no more than
+ * the free ones, and if its tokens and those of all before it that have their
+ * pages are at most max_tok. New pages are taken from the ring's first on, in
+ * the order of requests and positions, and entered in r->pages; an ended
+ * request's pages but for those all requests share are put behind the last, in
+ * the same order (a request that ended before has d_len 0). Written: r->first,
+ * r->len (0 for ended requests, which may be d_len), d_free_out[2] (which may be
+ * d_free), and for each token its cache row, position and request (any of the
+ * three may be NULL), -1 from the last token to max_tok and the row -1 where a
+ * page is negative or row 2^31 - 1 is passed: dsv4_gpu_kv_append_d writes
+ * nothing there. 0 / -1. */
+int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, const int *d_new, int *d_ring,
+                           int ring_cap, const int *d_free, int *d_free_out, int *d_rows,
+                           int *d_pos, int *d_req, void *stream);
+
+/* How a row of logits is sampled, one value a row (device arrays; NULL: no such
+ * rule). Of the tokens whose logit is over -infinity, ordered from the largest
+ * logit down, the lower id first among equals: the first top_k (0 or less: all);
+ * of them the fewest first ones whose probabilities, softmax(logit /
+ * temperature) among those top_k, sum to top_p (1 or more: all); and of them those
+ * with at least min_p (at most 1 counts) times the first's probability. The first
+ * always stays. The pick is the first in the order whose probability, summed with
+ * those before it, exceeds u times that of all that are left, u in [0, 1) (below:
+ * 0; above: the last one; NaN: 0). A temperature that is not over 0 picks the first. A logit of
+ * +infinity leaves the others no probability. */
+typedef struct {
+    const float *temperature;
+    const int *top_k;
+    const float *top_p, *min_p;
+    const float *u;        /* [n], not NULL                                   */
+} dsv4_gpu_sampling;
+
+/* Sample n <= 65536 rows of logits (fmt DSV4_WF32 or DSV4_WBF16, row t at t *
+ * stride, stride >= vocab, vocab <= 2^22): d_pick[t] the token, -1 where no
+ * logit is over -infinity; d_prob[t] (or NULL) its probability among the tokens
+ * left, d_kept[t] (or NULL) their number, 0 where there is none. Probabilities are
+ * summed as whole numbers, each within 2^-40 of the largest, so that a pick does
+ * not depend on the order of a sum. d_scratch: dsv4_gpu_sample_scratch_bytes of
+ * device memory, 16-byte aligned, not kept; the bytes do not fall as n or vocab
+ * grows. 0 / -1. */
+size_t dsv4_gpu_sample_scratch_bytes(int n, int vocab);
+int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const void *d_logits, int fmt,
+                      int n, int vocab, long long stride, const dsv4_gpu_sampling *s,
+                      void *d_scratch, size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
