@@ -200,6 +200,11 @@ _SIGS = {
     "dsv4_gpu_logits_scratch_bytes": (_sz, [_ci, _ci]),
     "dsv4_gpu_logits_adjust_d": (_ci, [_vp, _vp, _vp, _ci, _ci, _ll, _LRP, _vp, _sz, _vp]),
     "dsv4_gpu_reqs_tables_d": (_ci, [_RQP, _vp, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dsv4_gpu_reqs_plan_bytes": (_sz, [_ci, _ci, _ci]),
+    "dsv4_gpu_reqs_plan_d": (_ci, [_vp, _sz, _RQP, _ci, _ci, _ci, _ci, _ci, _ci, _vp]),
+    "dsv4_gpu_reqs_attn_scratch_bytes": (_sz, [_ci] * 7),
+    "dsv4_gpu_reqs_attn_d": (_ci, [_vp, _vp, _ci, _ci, _ci, _ci, _vp, _vp, _ci, _ci, _ci, _RQP,
+                                   _vp, _sz, _ci, _vp, _cf, _vp, _sz, _vp]),
     "dsv4_gpu_sample_scratch_bytes": (_sz, [_ci, _ci]),
     "dsv4_gpu_sample_d": (_ci, [_vp, _vp, _vp, _vp, _ci, _ci, _ci, _ll, _SP, _vp, _sz, _vp]),
 }

@@ -240,3 +240,22 @@ int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const void *d_log
                       void *d_scratch, size_t scratch_bytes, void *stream)
 { (void)d_pick; (void)d_prob; (void)d_kept; (void)d_logits; (void)fmt; (void)n; (void)vocab;
   (void)stride; (void)s; (void)d_scratch; (void)scratch_bytes; (void)stream; return -1; }
+size_t dsv4_gpu_reqs_plan_bytes(int n_req, int max_tok, int h)
+{ (void)n_req; (void)max_tok; (void)h; return 0; }
+int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_gpu_reqs *r, int fmt, int h,
+                         int d_qk, int d_v, int kv_fmt, int window, void *stream)
+{ (void)d_plan; (void)plan_bytes; (void)r; (void)fmt; (void)h; (void)d_qk; (void)d_v;
+  (void)kv_fmt; (void)window; (void)stream; return -1; }
+size_t dsv4_gpu_reqs_attn_scratch_bytes(int fmt, int h, int d_qk, int d_v, int kv_fmt, int n_req,
+                                        int max_tok)
+{ (void)fmt; (void)h; (void)d_qk; (void)d_v; (void)kv_fmt; (void)n_req; (void)max_tok;
+  return 0; }
+int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, int d_qk, int d_v,
+                         const void *d_kv, const float *d_kv_scales, int kv_fmt, int kv_stride,
+                         int kv_rows, const dsv4_gpu_reqs *r, const void *d_plan,
+                         size_t plan_bytes, int window, const float *d_sink, float scale,
+                         void *d_scratch, size_t scratch_bytes, void *stream)
+{ (void)d_o; (void)d_q; (void)fmt; (void)h; (void)d_qk; (void)d_v; (void)d_kv;
+  (void)d_kv_scales; (void)kv_fmt; (void)kv_stride; (void)kv_rows; (void)r; (void)d_plan;
+  (void)plan_bytes; (void)window; (void)d_sink; (void)scale; (void)d_scratch;
+  (void)scratch_bytes; (void)stream; return -1; }

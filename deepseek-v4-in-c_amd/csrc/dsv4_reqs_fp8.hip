@@ -1,0 +1,10 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/* dsv4_reqs_fp8.hip - the attention of a batch's requests (dsv4_tree.h) over
+ * FP8 caches. */
+#define DSV4_TREE_KERNEL
+#include "dsv4_tree.h"
+
+int dsv4_reqs_fp8_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st)
+{
+    return tree_format<DSV4_GPU_KV_FP8>(a, fmt, kc, groups, st);
+}

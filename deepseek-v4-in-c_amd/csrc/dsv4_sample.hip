@@ -42,7 +42,7 @@ struct SampleJob {
     uint32_t *count;
     double *top;                                  /* [n][ns]: the first bin's 32 z */
     float *cmax;                                  /* [n][nc]                 */
-    int *pick, *kept;
+    int *kept;
     float *prob;
 };
 
@@ -409,7 +409,7 @@ struct SmRow {
 };
 
 template <class T>
-__global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a)
+__global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_pick)
 {
     using Row = SmRow<T>;
     __shared__ typename Row::Lds s;
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a)
     Row r{a, s, (const T *)a.x + (size_t)row * a.stride, a.cmax + (size_t)row * a.nc,
           SmScale{0.0, false}, 0.0, 0.0};
     auto done = [&](int pick, float prob, int kept) {
-        a.pick[row] = pick;
+        d_pick[row] = pick;
         if (a.prob) a.prob[row] = prob;
         if (a.kept) a.kept[row] = kept;
     };
@@ -582,12 +582,13 @@ SamplePlan sample_plan(int n, int vocab)
 constexpr int SM_ROWS = 65536, SM_VOCAB = 1 << 22;
 
 template <class T>
-int sample_launch(const SampleJob &a, hipStream_t st)
+int sample_launch(const SampleJob &a, int *d_pick, hipStream_t st)
 {
     hipLaunchKernelGGL(k_sample_slices<T>, dim3((unsigned)a.n * (unsigned)a.ns), dim3(SM_THREADS),
                        0, st, a);
     HIP_OK(hipGetLastError(), "sample slices launch");
-    hipLaunchKernelGGL(k_sample_pick<T>, dim3((unsigned)a.n), dim3(SP_THREADS), 0, st, a);
+    hipLaunchKernelGGL(k_sample_pick<T>, dim3((unsigned)a.n), dim3(SP_THREADS), 0, st, a,
+                       d_pick);
     HIP_OK(hipGetLastError(), "sample pick launch");
     return 0;
 }
@@ -625,7 +626,8 @@ extern "C" int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const 
     char *base = (char *)d_scratch;
     SampleJob a{d_logits, stride, n, vocab, p.ns, p.nc, p.sh, *s, (u64 *)(base + p.mass),
                 (uint32_t *)(base + p.count), (double *)(base + p.top), (float *)(base + p.cmax),
-                d_pick, d_kept, d_prob};
+                d_kept, d_prob};
     hipStream_t st = (hipStream_t)stream;
-    return fmt == DSV4_WF32 ? sample_launch<float>(a, st) : sample_launch<uint16_t>(a, st);
+    return fmt == DSV4_WF32 ? sample_launch<float>(a, d_pick, st)
+                            : sample_launch<uint16_t>(a, d_pick, st);
 }

@@ -1,7 +1,8 @@
 /* SPDX-License-Identifier: Apache-2.0 */
-/* dsv4_tree.h - the attention of drafted tokens over a latent cache: the job
- * that dsv4_tree.hip plans, and the kernel, instantiated per cache format in
- * dsv4_tree_f32.hip, dsv4_tree_bf16.hip and dsv4_tree_fp8.hip. */
+/* dsv4_tree.h - the attention of drafted tokens, and of a batch's requests, over
+ * a latent cache: the jobs that dsv4_tree.hip and dsv4_reqs_attn.hip plan, and
+ * the kernel, instantiated per cache format in dsv4_{tree,reqs}_f32.hip,
+ * dsv4_{tree,reqs}_bf16.hip and dsv4_{tree,reqs}_fp8.hip. */
 #pragma once
 
 #include "dsv4_dev.h"
@@ -32,6 +33,43 @@ struct Dsv4TreeJob {
     int vec, qvec, ovec;                          /* the bf16 cache, q and o: whole
                                                    * and aligned pieces of 8, 8, 4 */
 };
+
+/* A workgroup's part of a batch's attention: rows [row0, row0 + rows) of q over
+ * positions of tiles [tile0, tile1) before `end`, by request req's pages. All its rows see
+ * positions [lo, hi). kind 0: every row sees all of it; 1: rows of one request, the
+ * token of row0 at pos0; 2: rows of any request. part: where its sums go, row by
+ * row, or -1 where they are the result. */
+struct Dsv4ReqsItem {
+    int row0, rows, req, tile0, tile1, end, lo, hi, kind, pos0, part, pad;
+};
+/* What a plan begins with: the number of items, those of the prefix first, of blocks
+ * of rows, and the signature of the arguments it was made for. */
+struct Dsv4ReqsHead {
+    uint32_t sig;
+    int items, prefix_items, blocks;
+    int prefix_splits, row0, rows, pad;           /* all requests' rows      */
+};
+/* A block of rows: its own splits' sums at part, `stride` rows apart. */
+struct Dsv4ReqsBlock {
+    int row0, rows, part, stride, splits, pad[3];
+};
+struct Dsv4ReqsJob : Dsv4TreeJob {
+    const Dsv4ReqsHead *head;
+    const Dsv4ReqsItem *items;
+    const int2 *req;                              /* first token, its position */
+    int n_req;
+    uint32_t sig;
+};
+int dsv4_reqs_f32_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st);
+int dsv4_reqs_bf16_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st);
+int dsv4_reqs_fp8_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st);
+
+/* The weight of a split's sums, its maximum ms and sum ls, in a row whose maximum
+ * is m. A split that saw nothing adds 0, whatever its maximum; NaN sums stay. */
+__device__ __forceinline__ float tree_join_weight(float ms, float ls, float m)
+{
+    return ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
+}
 
 /* The width class of a call (32-element chunks of d_qk that the kernel holds),
  * the rows of q that one workgroup takes and its launch; 0 / -1. */
@@ -228,10 +266,11 @@ constexpr int tr_fmt() { return sizeof(T) == 2 ? DSV4_WBF16 : DSV4_WF32; }
  * terms. Waves half a tile apart, deeper reads ahead, wave priorities and loads issued between
  * products measured the same or slower; 32 rows of q a wave do not fit the
  * registers. */
-template <class T, int KVF, int KC>
+template <class T, int KVF, int KC, class JOB>
 __global__ void __launch_bounds__(64 * TR_WAVES, TR_WAVES / 4 * tree_per_cu(tr_fmt<T>(), KC))
-k_tree(Dsv4TreeJob a)
+k_tree(JOB a)
 {
+    constexpr bool REQS = sizeof(JOB) != sizeof(Dsv4TreeJob);  /* a batch's items */
     constexpr int SPLIT = tree_split(tr_fmt<T>(), KVF, KC);
     using L = TreeLds<KVF, KC, SPLIT, tree_planes(tr_fmt<T>(), KVF)>;
     constexpr int NT = tree_terms(tr_fmt<T>()), KT = L::KT, NV = tree_vtiles(KC);
@@ -256,8 +295,26 @@ k_tree(Dsv4TreeJob a)
 
     /* Workgroup i runs on XCD i mod 8: each XCD takes a run of (split, block)
      * in split order, so blocks that read the same rows share its L2. */
-    int i0, i1, blk, split;
-    {
+    int i0, i1, blk = 0, split = 0;
+    Dsv4ReqsItem it{};
+    if constexpr (REQS) {
+        /* the prefix's items and then the others, each so */
+        const Dsv4ReqsHead hd = *a.head;
+        int id = blockIdx.x, base = 0, all = hd.prefix_items;
+        if (hd.sig != a.sig || id >= hd.items) return;
+        if (id >= all) {
+            base = all;
+            id -= all;
+            all = hd.items - all;
+        }
+        const int k = id & 7;
+        const Dsv4ReqsItem *p = a.items + base + k * (all >> 3) + min(k, all & 7) + (id >> 3);
+        auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        it = {uni(p->row0), uni(p->rows), uni(p->req),  uni(p->tile0), uni(p->tile1), uni(p->end),
+              uni(p->lo),   uni(p->hi),   uni(p->kind), uni(p->pos0),  uni(p->part),  0};
+        i0 = it.tile0;
+        i1 = it.tile1;
+    } else {
         const int all = gridDim.x, id = blockIdx.x, k = id & 7;
         const int at = k * (all >> 3) + min(k, all & 7) + (id >> 3);
         split = __builtin_amdgcn_readfirstlane(at / a.nb);
@@ -266,9 +323,12 @@ k_tree(Dsv4TreeJob a)
         i0 = a.tile0 + (int)((long long)tiles * split / a.ns);
         i1 = a.tile0 + (int)((long long)tiles * (split + 1) / a.ns);
     }
-    const int R = a.nt * a.h, end = a.ctx + a.nt;
-    const int row0 = blk * a.br + qb * 16;             /* this wave's rows of q  */
-    const bool live = 16 * qb < a.br && row0 < R;
+    const int R = REQS ? it.row0 + it.rows : a.nt * a.h, end = REQS ? it.end : a.ctx + a.nt;
+    /* this wave's rows of q */
+    const int row0 = (REQS ? it.row0 : blk * a.br) + qb * 16;
+    const bool live = (REQS || 16 * qb < a.br) && row0 < R;
+    const int *table = nullptr;
+    if constexpr (REQS) table = a.pages + (size_t)it.req * a.n_pages;
 
     /* ---- staging: a thread has place (lane % 8) of row sr of slabs ws, ws + WS,
      *      ... of a tile, which is piece (lane % 8) ^ (sr & 7) of 64 columns.
@@ -288,21 +348,21 @@ k_tree(Dsv4TreeJob a)
     /* the cache row of row r of tile i, -1 where there is none */
     auto find = [&](int i, int r) -> int {
         const int p = i * TR_TILE + r;
-        if (!a.pages) return p < min(end, a.rows) ? p : -1;
+        if (!REQS && !a.pages) return p < min(end, a.rows) ? p : -1;
         if (p >= end) return -1;
         const int k = (int)((__umulhi(a.page_m, (uint32_t)p) + (uint32_t)p) >> a.page_s);
         if (k >= a.n_pages) return -1;
-        const long long c = (long long)a.pages[k] * a.page + (p - k * a.page);
+        const long long c = (long long)(REQS ? table : a.pages)[k] * a.page + (p - k * a.page);
         return c >= 0 && c < a.rows ? (int)c : -1;
     };
     /* a page's entry is asked for a tile before it is needed: lane l has row l % 32
      * of the tile to be loaded next, and `there` says which of its rows exist */
     int ahead = -1;
     auto ask = [&](int i) {
-        if (a.pages && i < i1) ahead = find(i, tr_fresh(lane0) & 31);
+        if ((REQS || a.pages) && i < i1) ahead = find(i, tr_fresh(lane0) & 31);
     };
     auto there = [&](int i) -> uint32_t {
-        if (a.pages) return (uint32_t)__ballot(ahead >= 0);
+        if (REQS || a.pages) return (uint32_t)__ballot(ahead >= 0);
         const int n = min(end, a.rows) - i * TR_TILE;
         return n >= TR_TILE ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
     };
@@ -310,9 +370,10 @@ k_tree(Dsv4TreeJob a)
      * its reload would wait for all loads; the other formats measure better so) */
     auto my_row = [&](int i, const Place &h) {
         if constexpr (DMA)
-            return max(0, a.pages ? __builtin_amdgcn_ds_bpermute(4 * h.sr, ahead) : find(i, h.sr));
+            return max(0, REQS || a.pages ? __builtin_amdgcn_ds_bpermute(4 * h.sr, ahead)
+                                        : find(i, h.sr));
         else
-            return max(0, a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
+            return max(0, REQS || a.pages ? __shfl(ahead, h.sr, 64) : find(i, h.sr));
     };
     /* the eight elements from column c of a row: where they are all there, in one
      * or two loads that need no alignment (the target's own; the LDS-direct ones
@@ -545,7 +606,30 @@ k_tree(Dsv4TreeJob a)
     }
     /* ---- the drafts that the token of each row of q sees, and the first
      *      position ---- */
-    if (lane0 < 16) {
+    if constexpr (REQS) {
+        /* a batch's rows see positions [lo, hi) */
+        if (lane0 < 16) {
+            int lo = 0, hi = INT32_MAX;
+            if (it.kind != 0) {
+                const int t = min(row0 + lane0, R - 1) / a.h;
+                int pos = it.pos0 + t - it.row0 / a.h;
+                if (it.kind == 2) {                    /* whose token it is      */
+                    int r0 = 0, r1 = a.n_req;
+                    while (r1 - r0 > 1) {
+                        const int mid = (r0 + r1) >> 1;
+                        if (a.req[mid].x <= t) r0 = mid;
+                        else r1 = mid;
+                    }
+                    pos = a.req[r0].y + t - a.req[r0].x;
+                }
+                hi = pos + 1;
+                lo = a.window ? max(0, pos - a.window + 1) : 0;
+            }
+            unsigned char *d = lds + L::ROWS + 16 * (16 * w + lane0);
+            *(int *)d = hi;
+            *(int *)(d + 8) = lo;
+        }
+    } else if (lane0 < 16) {
         const int t = min(row0 + lane0, R - 1) / a.h;
         const unsigned long long all = a.nt >= 64 ? ~0ull : (1ull << a.nt) - 1;
         unsigned long long see = (a.mask ? a.mask[t] : (t >= 63 ? ~0ull : (2ull << t) - 1)) & all;
@@ -674,10 +758,14 @@ k_tree(Dsv4TreeJob a)
             const int lo = *(const int *)(rs + 8), p0 = i * TR_TILE;
             /* positions [lo, ctx) of the context, then the drafts' bits */
             uint32_t vis = 0u;
-            const int f = max(lo - p0, 0), e = min(a.ctx - p0, TR_TILE);
+            const int f = max(lo - p0, 0);
+            const int e = min((REQS ? (int)see : a.ctx) - p0, TR_TILE);
             if (f < e) vis = (e >= 32 ? ~0u : (1u << e) - 1u) & ~((1u << f) - 1u);
-            const int d = p0 - a.ctx;
-            if (d > -TR_TILE && d < 64) vis |= d >= 0 ? (uint32_t)(see >> d) : (uint32_t)(see << -d);
+            if constexpr (!REQS) {
+                const int d = p0 - a.ctx;
+                if (d > -TR_TILE && d < 64)
+                    vis |= d >= 0 ? (uint32_t)(see >> d) : (uint32_t)(see << -d);
+            }
             vis &= ok;
 #pragma unroll
             for (int k = 0; k < 2; k++)
@@ -749,8 +837,10 @@ k_tree(Dsv4TreeJob a)
     };
 
     /* every token sees every position of tiles [ic0, ic1) */
-    const int ic0 = a.window ? (max(0, a.ctx + a.nt - a.window) + TR_TILE - 1) / TR_TILE : 0;
-    const int ic1 = a.ctx / TR_TILE;
+    const int ic0 = REQS       ? (it.lo + TR_TILE - 1) / TR_TILE
+                    : a.window ? (max(0, a.ctx + a.nt - a.window) + TR_TILE - 1) / TR_TILE
+                               : 0;
+    const int ic1 = (REQS ? it.hi : a.ctx) / TR_TILE;
     if (!DMA && L::NBUF > 1 && i0 < i1) {
         store(0);
         if (i0 + 1 < i1) {
@@ -806,8 +896,8 @@ k_tree(Dsv4TreeJob a)
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (!live || rq >= R) return;
-    if (a.ns > 1) {
-        const size_t at = (size_t)split * R + rq;
+    if (REQS ? it.part >= 0 : a.ns > 1) {
+        const size_t at = REQS ? (size_t)it.part + (rq - it.row0) : (size_t)split * R + rq;
         if (g == 0 && half == 0) {
             a.pm[at] = m;
             a.pl[at] = l;
@@ -837,8 +927,8 @@ k_tree(Dsv4TreeJob a)
     }
 }
 
-template <class T, int KVF, int KC>
-int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
+template <class T, int KVF, int KC, class JOB>
+int tree_launch(const JOB &a, unsigned groups, hipStream_t st)
 {
     using L = TreeLds<KVF, KC, tree_split(tr_fmt<T>(), KVF, KC), tree_planes(tr_fmt<T>(), KVF)>;
     if (L::BYTES > 64 * 1024) {
@@ -847,32 +937,32 @@ int tree_launch(const Dsv4TreeJob &a, hipStream_t st)
         int dev = 0;
         HIP_OK(hipGetDevice(&dev), "hipGetDevice");
         if (dev < 0 || dev >= 64 || !asked[dev]) {
-            (void)dsv4_lds_optin((const void *)k_tree<T, KVF, KC>, L::BYTES, "tree attention");
+            (void)dsv4_lds_optin((const void *)k_tree<T, KVF, KC, JOB>, L::BYTES, "tree attention");
             if (dev >= 0 && dev < 64) asked[dev] = true;
         }
     }
-    hipLaunchKernelGGL((k_tree<T, KVF, KC>), dim3((unsigned)(a.ns * a.nb)),
-                       dim3(64 * TR_WAVES), L::BYTES, st, a);
+    hipLaunchKernelGGL((k_tree<T, KVF, KC, JOB>), dim3(groups), dim3(64 * TR_WAVES), L::BYTES, st,
+                       a);
     HIP_OK(hipGetLastError(), "tree attn launch");
     return 0;
 }
 
-template <class T, int KVF>
-int tree_width(const Dsv4TreeJob &a, int kc, hipStream_t st)
+template <class T, int KVF, class JOB>
+int tree_width(const JOB &a, int kc, unsigned groups, hipStream_t st)
 {
     switch (kc) {
-    case 4: return tree_launch<T, KVF, 4>(a, st);
-    case 8: return tree_launch<T, KVF, 8>(a, st);
-    case 16: return tree_launch<T, KVF, 16>(a, st);
-    default: return tree_launch<T, KVF, 18>(a, st);
+    case 4: return tree_launch<T, KVF, 4>(a, groups, st);
+    case 8: return tree_launch<T, KVF, 8>(a, groups, st);
+    case 16: return tree_launch<T, KVF, 16>(a, groups, st);
+    default: return tree_launch<T, KVF, 18>(a, groups, st);
     }
 }
 
-template <int KVF>
-int tree_format(const Dsv4TreeJob &a, int fmt, int kc, hipStream_t st)
+template <int KVF, class JOB>
+int tree_format(const JOB &a, int fmt, int kc, unsigned groups, hipStream_t st)
 {
-    return fmt == DSV4_WF32 ? tree_width<float, KVF>(a, kc, st)
-                            : tree_width<uint16_t, KVF>(a, kc, st);
+    return fmt == DSV4_WF32 ? tree_width<float, KVF>(a, kc, groups, st)
+                            : tree_width<uint16_t, KVF>(a, kc, groups, st);
 }
 
 } // namespace

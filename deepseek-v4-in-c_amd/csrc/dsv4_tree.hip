@@ -24,13 +24,6 @@ constexpr int TJ_COLS = 64;                       /* columns of a workgroup  */
 constexpr int TJ_GROUPS = TJ_THREADS / (TJ_COLS / 4);
 constexpr int TJ_SPLITS = 512;                    /* most splits of a call   */
 
-/* The weight of a split's sums, its maximum ms and sum ls, in a row whose maximum
- * is m. A split that saw nothing adds 0, whatever its maximum; NaN sums stay. */
-__device__ __forceinline__ float join_weight(float ms, float ls, float m)
-{
-    return ms == -INFINITY ? (ls == ls ? 0.0f : ls) : __builtin_amdgcn_exp2f(ms - m);
-}
-
 /* 1 / (a row's sum with its sink), 0 where the row saw nothing. */
 __device__ __forceinline__ float join_scale(const Dsv4TreeJob &a, int r, float m, float l)
 {
@@ -90,7 +83,7 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(Dsv4TreeJob a, T *o)
 #pragma unroll
     for (int k = 0; k < NK; k++) {
         if (64 * k >= a.ns) break;
-        ms[k] = join_weight(ms[k], ls[k], m);
+        ms[k] = tree_join_weight(ms[k], ls[k], m);
         l += ms[k] * ls[k];
     }
     l = wave_sum(l);
@@ -122,7 +115,7 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join_rows(Dsv4TreeJob a, T 
     if (r >= R) return;
     const float ms = lane < a.ns ? a.pm[(size_t)lane * R + r] : -INFINITY;
     const float ls = lane < a.ns ? a.pl[(size_t)lane * R + r] : 0.0f;
-    const float m = wave_max(ms), wt = join_weight(ms, ls, m);
+    const float m = wave_max(ms), wt = tree_join_weight(ms, ls, m);
     const float inv = join_scale(a, r, m, wave_sum(wt * ls));
     f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     const float *p = a.part + (size_t)r * a.dvp + 4 * lane;

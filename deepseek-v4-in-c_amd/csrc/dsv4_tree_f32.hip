@@ -6,5 +6,5 @@
 
 int dsv4_tree_f32_launch(const Dsv4TreeJob &a, int fmt, int kc, hipStream_t st)
 {
-    return tree_format<DSV4_GPU_KV_F32>(a, fmt, kc, st);
+    return tree_format<DSV4_GPU_KV_F32>(a, fmt, kc, (unsigned)(a.ns * a.nb), st);
 }

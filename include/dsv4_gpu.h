@@ -711,6 +711,40 @@ int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, const int *
                            int ring_cap, const int *d_free, int *d_free_out, int *d_rows,
                            int *d_pos, int *d_req, void *stream);
 
+/* The attention of a step's tokens, of all requests in one call: token t of the batch
+ * and each of its h heads, o[t][i] = softmax over the positions of its request up to
+ * its own (with window > 0 the last `window` of them) of q[t][i] . row[:d_qk] * scale,
+ * applied to row[:d_v]; sink[i] enters the denominator only, or is absent when
+ * NULL (q [max_tok][h][d_qk], o [max_tok][h][d_v], fmt DSV4_WF32 or DSV4_WBF16; d_v <=
+ * d_qk, d_qk <= 576, d_v <= 512; h * max_tok <= 2^28). The tokens' own rows are in the
+ * cache (dsv4_gpu_kv_append_d). Where several requests have tokens, the positions
+ * before r->n_prefix may be read by the pages of any one of those that are as long.
+ * Rows outside [0, kv_rows) and pages past the table are treated as masked and never
+ * read; a token that sees no row gets zeros; what a row holds does not reach tokens that
+ * do not see it. Rows of o behind the last token, and before token first[0], are left
+ * as they were. Scores, softmax and sums have dsv4_gpu_tree_attn_d's accuracy, under
+ * its conditions.
+ *
+ * dsv4_gpu_reqs_plan_d makes the step's plan from r->len and r->first on the device,
+ * once for all layers that have these sizes, formats and this window;
+ * dsv4_gpu_reqs_attn_d reads the plan and r->pages, and of r else only its sizes, which
+ * have to be the plan's. With a plan of other sizes, or where first does not ascend from 0
+ * or more to max_tok at most or a request with tokens has fewer positions than those or
+ * more than its table, all of o becomes NaN. d_plan: dsv4_gpu_reqs_plan_bytes of
+ * device memory, 16-byte aligned, kept from the plan to the last call that reads it;
+ * d_scratch: dsv4_gpu_reqs_attn_scratch_bytes, 16-byte aligned, not kept. Neither
+ * falls as n_req, max_tok or h grows. d_o must not overlap what the call reads. 0 / -1. */
+size_t dsv4_gpu_reqs_plan_bytes(int n_req, int max_tok, int h);
+int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_gpu_reqs *r, int fmt, int h,
+                         int d_qk, int d_v, int kv_fmt, int window, void *stream);
+size_t dsv4_gpu_reqs_attn_scratch_bytes(int fmt, int h, int d_qk, int d_v, int kv_fmt, int n_req,
+                                        int max_tok);
+int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, int d_qk, int d_v,
+                         const void *d_kv, const float *d_kv_scales, int kv_fmt, int kv_stride,
+                         int kv_rows, const dsv4_gpu_reqs *r, const void *d_plan,
+                         size_t plan_bytes, int window, const float *d_sink, float scale,
+                         void *d_scratch, size_t scratch_bytes, void *stream);
+
 /* How a row of logits is sampled, one value a row (device arrays; NULL: no such
  * rule). Of the tokens whose logit is over -infinity, ordered from the largest
  * logit down, the lower id first among equals: the first top_k (0 or less: all);

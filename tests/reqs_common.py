@@ -135,3 +135,116 @@ def run_sample(dsv4, x, bf=False, u=None, temperature=None, top_k=None, top_p=No
     got = [o.cpu().numpy() for o in out]
     assert all(g[n] == -7 for g in got)
     return [g[:n] for g in got]
+
+
+# --------------------------------------------------------------- attention
+class Batch:
+    """Requests of lens positions, of which their last news[i] are the step's tokens,
+    over a paged device cache; positions before `prefix` hold the same rows in all of
+    them (whole pages are shared, the rest copied)."""
+
+    def __init__(self, seed, lens, news, h, dqk, fmt, bf, page=16, prefix=0, scale=1.0, stride=None,
+                 spare=3, room=0):
+        rng = self.rng = np.random.default_rng(seed)
+        self.lens, self.news = [int(v) for v in lens], [int(v) for v in news]
+        self.h, self.dqk, self.fmt, self.bf, self.page, self.prefix = h, dqk, fmt, bf, page, prefix
+        width = max([-(-n // page) for n in self.lens] + [1]) + 1
+        own = prefix // page
+        need = own + sum(max(0, -(-n // page) - own) for n in self.lens) + spare
+        order = rng.permutation(need).astype(np.int32)
+        t = self.table = np.full((len(self.lens), width), -1, np.int32)
+        used = own
+        for i, n in enumerate(self.lens):
+            k = -(-n // page)
+            t[i, :min(own, width)] = order[:min(own, width)]
+            t[i, own:k] = order[used:used + max(0, k - own)]
+            used += max(0, k - own)
+        self.rows = need * page
+        x = rng.standard_normal((self.rows, dqk))
+        whole = [i for i, n in enumerate(self.lens) if n > prefix]
+        for i, n in enumerate(self.lens):
+            for p in range(own * page, min(n, prefix)):
+                x[self.row(i, p)] = x[self.row(whole[0], p)] if whole else 0.25
+        self.x, s = dc.stored(x, fmt)
+        self.stride = stride or dqk
+        self.cache, self.ks = dc.cache_of(self.x, fmt, self.stride, s)
+        self.first = np.concatenate([[0], np.cumsum(self.news)]).astype(np.int32)
+        self.tokens = int(self.first[-1])
+        self.max_tok = self.tokens + room
+        q = (rng.standard_normal((self.max_tok, h, dqk)) * scale).astype(np.float32)
+        self.q = dc.bf16(q) if bf else q
+        self.dq = dc.to_fmt(self.q, bf)
+        self.dev = {k: dc.dev(np.asarray(v, np.int32)) for k, v in
+                    dict(len=self.lens, pages=t, first=self.first).items()}
+
+    def row(self, i, p):
+        return int(self.table[i, p // self.page]) * self.page + p % self.page
+
+    def struct(self, dsv4, **kw):
+        d = self.dev
+        a = dict(length=d["len"], pages=d["pages"], first=d["first"], page=self.page,
+                 max_tok=self.max_tok, prefix=self.prefix)
+        a.update(kw)
+        return reqs(dsv4, **a)
+
+    def buffers(self, dsv4, dv):
+        import torch
+        L, h, n = dsv4.lib(), self.h, len(self.lens)
+        self.plan = torch.full((L.dsv4_gpu_reqs_plan_bytes(n, self.max_tok, h) + 16,), 255,
+                               device="cuda:0", dtype=torch.uint8)
+        self.space = torch.full((L.dsv4_gpu_reqs_attn_scratch_bytes(
+            int(self.bf), h, self.dqk, dv, self.fmt, n, self.max_tok) + 16,), 255, device="cuda:0",
+            dtype=torch.uint8)
+        self.o = torch.full((self.max_tok + 1, h, dv), 99.0, device="cuda:0", dtype=self.dq.dtype)
+        return self.o
+
+    def make_plan(self, dsv4, dv, window=0, st=None, **kw):
+        return dsv4.lib().dsv4_gpu_reqs_plan_d(
+            self.plan.data_ptr(), self.plan.numel() - 16, ctypes.byref(self.struct(dsv4, **kw)),
+            int(self.bf), self.h, self.dqk, dv, self.fmt, window, dc.stream() if st is None else st)
+
+    def attend(self, dsv4, dv, window=0, sink=None, scale=1.0, st=None, **kw):
+        return dsv4.lib().dsv4_gpu_reqs_attn_d(
+            self.o.data_ptr(), self.dq.data_ptr(), int(self.bf), self.h, self.dqk, dv,
+            self.cache.data_ptr(), dc.ptr(self.ks), self.fmt, self.stride, self.rows,
+            ctypes.byref(self.struct(dsv4, **kw)), self.plan.data_ptr(), self.plan.numel() - 16,
+            window, dc.ptr(sink), ctypes.c_float(scale), self.space.data_ptr(),
+            self.space.numel() - 16, dc.stream() if st is None else st)
+
+    def call(self, dsv4, dv, window=0, sink=None, scale=1.0):
+        """Plan and attention; what lies behind the buffers checked."""
+        import torch
+        self.buffers(dsv4, dv)
+        assert self.make_plan(dsv4, dv, window) == 0
+        assert self.attend(dsv4, dv, window, sink, scale) == 0
+        torch.cuda.synchronize()
+        assert (self.plan[-16:] == 255).all() and (self.space[-16:] == 255).all()
+        got = dc.host(self.o)
+        assert (got[self.tokens:] == 99).all()
+        return got[:self.tokens]
+
+    def sees(self, i, window):
+        """[tokens][positions] of request i."""
+        n, k = self.lens[i], self.news[i]
+        p, r = np.arange(n - k, n)[:, None], np.arange(n)[None, :]
+        return (r <= p) & ((p - r < window) if window else True)
+
+    def want(self, dv, window=0, sink=None, scale=1.0, x=None, gone=None):
+        """(o, sum of |weight value|) in 64 bits; gone: cache rows that are not there."""
+        x = self.x if x is None else x
+        o, size = np.zeros((self.tokens, self.h, dv)), np.zeros((self.tokens, self.h, dv))
+        for i, n in enumerate(self.lens):
+            f0, f1 = self.first[i], self.first[i + 1]
+            if f0 == f1:
+                continue
+            p = np.arange(n)
+            page = self.table[i, p // self.page].astype(np.int64)
+            at = page * self.page + p % self.page
+            see = self.sees(i, window)
+            there = (page >= 0) & (at < self.rows)
+            see &= there[None, :]
+            if gone is not None:
+                see &= ~gone[np.where(there, at, 0)][None, :]
+            o[f0:f1], size[f0:f1] = dc.attention(self.q[f0:f1], x[np.where(there, at, 0)], see, sink,
+                                                 np.float32(scale), dv)
+        return o, size
