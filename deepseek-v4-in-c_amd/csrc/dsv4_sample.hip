@@ -7,13 +7,13 @@
  * order passes u times the sum of what is left; so the rows need no sort but the
  * place of a few sums. The order is cut into bins by floor(32 z): a token's weight
  * is known to 2^(1/32) by its bin, and the sums over bins say which bin a limit or
- * the pick falls into. Only that bin's tokens are put in order.
+ * the pick falls into. Only those bins' tokens are put in order.
  *
- * Sums are of whole numbers, 2^(z - E) 2^sh with E an integer that no z of the
- * row passes, so that they do not depend on their order. A workgroup that has seen
- * a slice of a row takes its own E; the bins are at the same z for all, and
- * sums are shifted to the row's E when they are added. z and the weights are in
- * 64 bits: a pick that is wrong by a rounding is another token.
+ * Sums are of whole numbers, so that they do not depend on their order: of a bin the
+ * count and the sum of 2^(r/32) - 1, r the rest of 32 z, to 2^-42; over bins
+ * 2^(z - E) 2^sh, E an integer that no z of the row passes. The bins lie at the
+ * same z for all slices of a row. z and the weights are in 64 bits: a pick that is
+ * wrong by a rounding is another token.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -29,18 +29,31 @@ constexpr int SM_EACH = 32;                       /* tokens of a thread      */
 constexpr int SM_SLICE = SM_THREADS * SM_EACH;
 constexpr int SM_BINS = 1024;                     /* 32 octaves, the rest in the last */
 constexpr int SM_CHUNK = 64;                      /* tokens with one maximum */
+/* A bin of a slice in one word: the count from bit 50 on (8192 at most), and below
+ * it the sum of (2^(r/32) - 1) 2^42, which is under 8192 x 0.0219 x 2^42 < 2^50. */
+constexpr int SM_PART = 42, SM_COUNT = 50;
+static_assert(SM_SLICE <= 8192, "a bin's word");
 constexpr int SP_THREADS = 1024;                  /* of a row's pick         */
 constexpr int SP_WAVES = SP_THREADS / 64;
+constexpr int SP_LIST = SP_THREADS;               /* tokens put in order     */
+constexpr int SP_QUEUE = 2 * SP_LIST;              /* and looked through      */
+constexpr int SP_CHUNKS = 4096;                   /* chunks looked over at once */
+constexpr int SP_K = 512;                         /* a short top-k, for which no bins are made */
 static_assert(SP_THREADS == SM_BINS, "a bin a thread");
+
+struct SmTop {
+    double q;                                     /* 32 z of the first bin   */
+    u64 tail;                                     /* the last bin's sum      */
+    uint32_t tail_n, pad;
+};
 
 struct SampleJob {
     const void *x;
     long long stride;
     int n, vocab, ns, nc, sh;                     /* slices, chunks of a row */
     dsv4_gpu_sampling r;
-    u64 *mass;                                    /* [n][ns][bins]           */
-    uint32_t *count;
-    double *top;                                  /* [n][ns]: the first bin's 32 z */
+    u64 *bins;                                    /* [n][ns][bins]           */
+    SmTop *top;                                   /* [n][ns]                 */
     float *cmax;                                  /* [n][nc]                 */
     int *kept;
     float *prob;
@@ -106,13 +119,51 @@ __device__ __forceinline__ float sm_temperature(const SampleJob &a, int row)
     return a.r.temperature ? a.r.temperature[row] : 1.0f;
 }
 
-/* A slice of a row: the maxima of its chunks, and its bins' counts and sums. */
+/* 2^(r/32) - 1, 0 <= r < 1: the exponential's series to r^6, 5e-16 off at the most. */
+__device__ __forceinline__ double sm_bin_part(double r)
+{
+    double p = 1.4345655584131932e-13;
+    p = fma(p, r, 3.9737099845494154e-11);
+    p = fma(p, r, 9.172562701824643e-09);
+    p = fma(p, r, 1.6938509724371819e-06);
+    p = fma(p, r, 0.00023459619820224677);
+    p = fma(p, r, 0.02166084939249829);
+    return p * r;
+}
+
+/* (2^(r/32) - 1) 2^42 of a token, as a whole number. */
+__device__ __forceinline__ u64 sm_bin_word(double z, double q)
+{
+    const double v = fma(sm_bin_part(fma(z, 32.0, -q)), (double)(1ull << SM_PART), 4503599627370496.0);
+    return (u64)__double_as_longlong(v) & ((1ull << 52) - 1);
+}
+
+/* The sum of n tokens of a bin, `edge` the weight at its lower edge. Equal tokens sum
+ * to a multiple of a whole number, so that limits and picks that fall between two of
+ * them do so exactly. */
+__device__ __forceinline__ u64 sm_bin_sum(double edge, uint32_t n, u64 part)
+{
+    constexpr double ONE = 1.0 / (1ull << SM_PART);
+    const double each = __builtin_rint((double)part / (double)n);
+    if (n && (u64)each * n == part) return (u64)__builtin_rint(edge * (1.0 + each * ONE)) * n;
+    return (u64)__builtin_rint(edge * ((double)n + (double)part * ONE));
+}
+
+/* A top-k so short that the chunks with the k largest maxima, which have the k largest
+ * tokens, have hardly more that are as large (256 of 2020 chunks: 274 tokens). */
+__device__ __forceinline__ bool sm_short(const SampleJob &a, int top_k)
+{
+    return top_k > 0 && top_k <= SP_K && 2 * top_k <= a.nc && a.nc <= SP_CHUNKS;
+}
+
+/* A slice of a row: the maxima of its chunks, and its bins. */
 template <class T>
 __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
 {
-    __shared__ u64 mass[SM_BINS];
-    __shared__ uint32_t count[SM_BINS];
+    __shared__ __attribute__((aligned(16))) u64 bins[SM_BINS];
     __shared__ float wtop[SM_THREADS / 64];
+    __shared__ u64 tail;
+    __shared__ uint32_t tail_n;
     const int tid = threadIdx.x;
     const int row = blockIdx.x / a.ns, slice = blockIdx.x - row * a.ns;
     const int v0 = slice * SM_SLICE;
@@ -133,6 +184,11 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
         }
     }
     const float temp = sm_temperature(a, row);
+    for (int i = tid; i < SM_BINS; i += SM_THREADS) bins[i] = 0;
+    if (tid == 0) {
+        tail = 0;
+        tail_n = 0;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int p = 0; p < SM_EACH / 4; p++) {
@@ -147,39 +203,42 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
         if ((tid & 15) == 0 && chunk < a.nc) a.cmax[(size_t)row * a.nc + chunk] = m;
         top = fmaxf(top, m);
     }
-    if (!(temp > 0.0f)) return;                   /* the first is picked     */
+    /* the first is picked, or one of the first few */
+    if (!(temp > 0.0f) || (a.r.top_k && sm_short(a, a.r.top_k[row]))) return;
 
-    for (int i = tid; i < SM_BINS; i += SM_THREADS) {
-        mass[i] = 0;
-        count[i] = 0;
-    }
     top = wave_max(top);
     if ((tid & 63) == 0) wtop[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < SM_THREADS / 64; k++) top = fmaxf(top, wtop[k]);
     const size_t at = (size_t)row * a.ns + slice;
-    if (top == -INFINITY) {
-        if (tid == 0) a.top[at] = -INFINITY;
-        return;
-    }
     const SmScale sc{1.4426950408889634 / (double)temp, top == INFINITY};
     const double first = sm_q(sc.z(top)), e = sm_e(first);
+    u64 rest = 0;                                 /* of the last bin         */
+    uint32_t rest_n = 0;
+    if (top > -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < SM_EACH; k++) {
-        if (!(v[k] > -INFINITY)) continue;
-        const double z = sc.z(v[k]);
-        const int bin = sm_bin(first, sm_q(z));
-        const u64 w = sm_weight(z - e, a.sh);
-        atomicAdd(&count[bin], 1u);
-        if (w) atomicAdd(&mass[bin], w);
+        for (int k = 0; k < SM_EACH; k++) {
+            if (!(v[k] > -INFINITY)) continue;
+            const double z = sc.z(v[k]), q = sm_q(z);
+            const double d = first - q;
+            if (d < SM_BINS - 1) {
+                atomicAdd(&bins[(int)d], sm_bin_word(z, q) + (1ull << SM_COUNT));
+            } else {
+                rest += sm_weight(z - e, a.sh);
+                rest_n++;
+            }
+        }
+    }
+    if (__any(rest_n != 0)) {
+        atomicAdd(&tail, rest);
+        atomicAdd(&tail_n, rest_n);
     }
     __syncthreads();
-    for (int i = tid; i < SM_BINS; i += SM_THREADS) {
-        a.mass[at * SM_BINS + i] = mass[i];
-        a.count[at * SM_BINS + i] = count[i];
-    }
-    if (tid == 0) a.top[at] = sc.inf ? INFINITY : first;
+    for (int i = tid; i < SM_BINS / 2; i += SM_THREADS)
+        *(u32x4 *)(a.bins + at * SM_BINS + 2 * i) = *(const u32x4 *)(bins + 2 * i);
+    if (tid == 0)
+        a.top[at] = SmTop{top == -INFINITY ? -INFINITY : sc.inf ? INFINITY : first, tail, tail_n, 0};
 }
 
 /* u s for 0 <= u < 1 and s < 2^63, exactly, rounded down or up. */
@@ -218,22 +277,67 @@ struct SmPlace {
     int bin, n;
 };
 
-/* The workgroup of a row. */
+/* Inclusive sums over a wave, by moves within the vector unit. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sm_dpp(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 sm_dpp(u64 v)
+{
+    return (u64)sm_dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | sm_dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <class V>
+__device__ __forceinline__ V sm_wave_scan(V v)
+{
+    v += sm_dpp<0x111, 0xF>(v);                   /* row_shr:1, 2, 4, 8      */
+    v += sm_dpp<0x112, 0xF>(v);
+    v += sm_dpp<0x114, 0xF>(v);
+    v += sm_dpp<0x118, 0xF>(v);
+    v += sm_dpp<DPP_ROW_BCAST15, 0xA>(v);
+    v += sm_dpp<DPP_ROW_BCAST31, 0xC>(v);
+    return v;
+}
+
+/* The first of n <= 1024 places that pred holds for, n if none does; it holds for all
+ * behind the first. Each wave looks for itself: 64 places at once, then the 16 before
+ * the first of them that has it. */
+template <class F>
+__device__ __forceinline__ int sm_first(int n, F pred)
+{
+    const int lane = threadIdx.x & 63;
+    const int end = min(16 * lane + 15, n - 1);
+    const u64 far = __ballot(n > 0 && pred(max(end, 0)));
+    if (!far) return n;
+    const int at = min(16 * (int)__builtin_ctzll(far) + (lane & 15), n - 1);
+    const u64 near = __ballot(pred(at));
+    return __shfl(at, (int)__builtin_ctzll(near), 64);
+}
+
+/* The workgroup of a row. Its code is kept short, as all of it is fetched for a few
+ * microseconds' run: loops stay loops but where loads have to be out together. */
 template <class T>
 struct SmRow {
     struct Lds {
         u64 sum[SM_BINS];                         /* through a bin           */
         uint32_t n[SM_BINS];
-        u64 mass[SP_THREADS], best[SP_THREADS];   /* a split of a key range  */
-        uint32_t cnt[SP_THREADS];
-        u64 key[SP_THREADS], w[SP_THREADS];       /* a bin's tokens          */
+        int off[SM_BINS];                         /* a bin's place in the list, or -1 */
+        uint32_t cur[SM_BINS];                    /* a bin's tokens so far   */
+        union {
+            u64 queue[SP_QUEUE];                  /* tokens that may be listed */
+            struct {
+                u64 mass[SP_THREADS], best[SP_THREADS];   /* a split of a key range */
+            };
+        };
+        u64 key[SP_LIST], through[SP_LIST];       /* tokens in order, sums through them */
+        unsigned short chunk[SP_CHUNKS];          /* chunks to read          */
         u64 part[SP_WAVES];
         uint32_t npart[SP_WAVES];
         SmPlace hit;
-        u64 range[2];
-        int len, held;                            /* tokens listed, their bin */
-        double slices[2];
-        float top;
+        u64 tail;                                 /* the last bin's sum      */
+        uint32_t tail_n;
+        int len, chunks;                          /* tokens queued; to read  */
     };
     const SampleJob &a;
     Lds &s;
@@ -241,170 +345,187 @@ struct SmRow {
     const float *cmax;
     SmScale sc;
     double first, e;
+    float cm[SP_CHUNKS / SP_THREADS];             /* this thread's of the first chunks */
 
     /* Inclusive sums over the threads. */
-    __device__ void scan(u64 &m, uint32_t &n)
+    __device__ __forceinline__ void scan(u64 &m, uint32_t &n)
     {
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const u64 u = __shfl_up(m, o, 64);
-            const uint32_t v = __shfl_up(n, o, 64);
-            if (lane >= o) {
-                m += u;
-                n += v;
-            }
-        }
+        m = sm_wave_scan(m);
+        n = sm_wave_scan(n);
         __syncthreads();
         if (lane == 63) {
             s.part[w] = m;
             s.npart[w] = n;
         }
         __syncthreads();
-        for (int k = 0; k < w; k++) {
-            m += s.part[k];
-            n += s.npart[k];
+        /* lane k's sum of the waves 0 .. k, of which this wave takes those before it */
+        const u64 mw = sm_wave_scan(lane < SP_WAVES ? s.part[lane & (SP_WAVES - 1)] : 0);
+        const uint32_t nw = sm_wave_scan(lane < SP_WAVES ? s.npart[lane & (SP_WAVES - 1)] : 0u);
+        if (w) {
+            m += __shfl(mw, w - 1, 64);
+            n += __shfl(nw, w - 1, 64);
         }
     }
 
-    /* f(key, weight) for every token of a bin, from the row. A chunk whose largest
-     * is in a later bin has none. */
-    template <class F>
-    __device__ void each_of_row(int bin, F f)
+    __device__ __forceinline__ uint32_t n_before(int bin) const { return bin ? s.n[bin - 1] : 0; }
+    __device__ __forceinline__ u64 sum_before(int bin) const { return bin ? s.sum[bin - 1] : 0; }
+    __device__ __forceinline__ int bin_of(float v) const { return sm_bin(first, sm_q(sc.z(v))); }
+    /* The first bin through which the sum is; the last, where roundings pass it. */
+    __device__ __forceinline__ int sum_bin(u64 need) const
     {
-        constexpr int G = 8;                      /* chunks in flight        */
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-        for (int c0 = w * 64; c0 < a.nc; c0 += SP_THREADS) {
-            const int c = c0 + lane;
-            const float top = c < a.nc ? cmax[c] : -INFINITY;
-            u64 want = __ballot(top > -INFINITY && sm_bin(first, sm_q(sc.z(top))) <= bin);
-            while (want) {
-                float v[G];
+        return min(sm_first(SM_BINS, [&](int i) { return s.sum[i] >= need; }), SM_BINS - 1);
+    }
+
+    /* The weight at the lower edge of the bin of 32 z = q, and of a token in it. */
+    __device__ __forceinline__ double edge(double q) const
+    {
+        return sm_exp2(q * (1.0 / 32.0) - e) * __hiloint2double((1023 + a.sh) << 20, 0);
+    }
+    __device__ __forceinline__ u64 weight(double z) const
+    {
+        const double q = sm_q(z);
+        return first - q < SM_BINS - 1 ? sm_bin_sum(edge(q), 1, sm_bin_word(z, q))
+                                       : sm_weight(z - e, a.sh);
+    }
+
+    /* Logits between which all tokens of bins [b0, b1] lie. */
+    __device__ __forceinline__ void range_of(int b0, int b1, float *lo, float *hi) const
+    {
+        /* a margin for the roundings of z and of this */
+        const double l = (first - b1) / (32.0 * sc.c), h = (first - b0 + 1) / (32.0 * sc.c);
+        *lo = (float)(l - fabs(l) * 1e-6);
+        *hi = (float)(h + fabs(h) * 1e-6);
+        if (sc.inf || b1 == SM_BINS - 1 || !(*lo > -3.4028235e38f)) *lo = -3.4028235e38f;
+        if (sc.inf || b0 == 0 || !(*hi < INFINITY)) *hi = INFINITY;
+    }
+
+    /* f(x, token) for every token of the row from lo to hi, or from lo2 to hi2 (lo <= lo2):
+     * a chunk whose largest is less has none. The whole workgroup; 16 lanes a chunk, so that a load takes 1 KB of
+     * four chunks, and G loads in flight. */
+    template <int G, class F>
+    __device__ __forceinline__ void each_of_row(float lo, float hi, float lo2, float hi2, F f)
+    {
+        const int tid = threadIdx.x;
+#pragma unroll 1
+        for (int c0 = 0; c0 < a.nc; c0 += SP_CHUNKS) {
+            __syncthreads();
+            if (tid == 0) s.chunks = 0;
+            __syncthreads();
+#pragma unroll
+            for (int k = tid; k < SP_CHUNKS; k += SP_THREADS) {
+                const float top = c0 ? c0 + k < a.nc ? cmax[c0 + k] : -INFINITY : cm[k / SP_THREADS];
+                const bool want = top >= lo;
+                const u64 who = __ballot(want);
+                int at = 0;
+                if ((tid & 63) == 0 && who) at = atomicAdd(&s.chunks, (int)__popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at) +
+                     (int)__popcll(who & ((1ull << (tid & 63)) - 1));
+                if (want) s.chunk[at] = (unsigned short)k;
+            }
+            __syncthreads();
+            const int n = s.chunks;
+#pragma unroll 1
+            for (int i0 = tid / 16; i0 < n; i0 += G * (SP_THREADS / 16)) {
+                float v[G][4];
                 int t[G];
 #pragma unroll
                 for (int u = 0; u < G; u++) {
-                    t[u] = a.vocab;
-                    if (want) {
-                        t[u] = (c0 + __builtin_ctzll(want)) * SM_CHUNK + lane;
-                        want &= want - 1;
+                    const int i = min(i0 + u * (SP_THREADS / 16), n - 1);
+                    t[u] = (c0 + s.chunk[i]) * SM_CHUNK + 4 * (tid & 15);
+                    /* (past the vocabulary: its last four) */
+                    if (a.vocab >= 4) {
+                        io_load<T, 4>(x + min(t[u], a.vocab - 4), v[u]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) io_load<T, 1>(x + min(k, a.vocab - 1), v[u] + k);
                     }
-                    v[u] = -INFINITY;
-                    if (t[u] < a.vocab) io_load<T, 1>(x + t[u], v + u);
                 }
 #pragma unroll
                 for (int u = 0; u < G; u++) {
-                    if (!(v[u] > -INFINITY)) continue;
-                    const double z = sc.z(v[u]);
-                    if (sm_bin(first, sm_q(z)) == bin)
-                        f(am_key(v[u], t[u]), sm_weight(z - e, a.sh));
+                    const int t1 = i0 + u * (SP_THREADS / 16) < n ? a.vocab : 0;
+                    const int t0 = t[u];
+                    t[u] = min(t0, max(0, a.vocab - 4));
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (((v[u][k] >= lo && v[u][k] <= hi) || (v[u][k] >= lo2 && v[u][k] <= hi2)) &&
+                            t[u] + k >= t0 && t[u] + k < t1)
+                            f(v[u][k], t[u] + k);
                 }
             }
         }
+        __syncthreads();
     }
 
-    /* List a bin's tokens, if they fit. */
-    __device__ void hold(int bin)
+    /* Queue the tokens of two ranges of logits; how many, over SP_QUEUE: not all. */
+    __device__ __forceinline__ int queue(float lo, float hi, float lo2, float hi2)
     {
-        if (s.held == bin) return;                /* the same in every thread */
-        __syncthreads();
         if (threadIdx.x == 0) s.len = 0;
-        __syncthreads();
-        const uint32_t n = s.n[bin] - (bin ? s.n[bin - 1] : 0);
-        if (n <= SP_THREADS)
-            each_of_row(bin, [&](u64 key, u64 w) {
-                const int at = atomicAdd(&s.len, 1);
-                if (at < SP_THREADS) {
-                    s.key[at] = key;
-                    s.w[at] = w;
-                }
-            });
-        __syncthreads();
-        if (threadIdx.x == 0) s.held = n <= SP_THREADS ? bin : -1;
-        __syncthreads();
+        each_of_row<8>(lo, hi, lo2, hi2, [&](float v, int t) {
+            const int at = atomicAdd(&s.len, 1);
+            if (at < SP_QUEUE) s.queue[at] = am_key(v, t);
+        });
+        return s.len;
     }
 
-    template <class F>
-    __device__ void each(int bin, F f)
+    /* Put the tokens of the bins that have a place (s.off), of b0 to b1 or b2 to b3, into the
+     * list, in order, n in all; false where those between are too many. */
+    __device__ __forceinline__ bool list(int b0, int b1, int b2, int b3, int n)
     {
-        if (s.held != bin) each_of_row(bin, f);
-        else if ((int)threadIdx.x < s.len) f(s.key[threadIdx.x], s.w[threadIdx.x]);
-    }
-
-    /* Where the order passes `need` tokens (tokens true) or the sum `need`, in a bin
-     * which that is known to be: the first token through which there are as many,
-     * or, where roundings of the bins' sums leave them short, the bin's last. The
-     * bin's range of keys is split by 1024 until the token is alone. */
-    __device__ SmPlace cross(int bin, u64 need, bool tokens)
-    {
-        hold(bin);
         const int tid = threadIdx.x;
-        u64 lo = 0, hi = ~0ull, sum0 = bin ? s.sum[bin - 1] : 0;
-        uint32_t n0 = bin ? s.n[bin - 1] : 0;
-        if (s.held == bin) {
-            if (tid == 0) {
-                s.range[0] = ~0ull;
-                s.range[1] = 0;
-            }
-            __syncthreads();
-            if (tid < s.len) {
-                atomicMin(&s.range[0], s.key[tid]);
-                atomicMax(&s.range[1], s.key[tid]);
-            }
-            __syncthreads();
-            lo = s.range[0];
-            hi = s.range[1];
+        float lo, hi, lo2, hi2;
+        range_of(b0, b1, &lo, &hi);
+        range_of(b2, b3, &lo2, &hi2);
+        s.cur[tid] = 0;
+        if (lo2 < lo) {
+            float t = lo;
+            lo = lo2;
+            lo2 = t;
+            t = hi;
+            hi = hi2;
+            hi2 = t;
         }
-        for (;;) {
-            const int bits = 64 - __clzll((long long)((hi - lo) | 1));
-            const int sh = max(0, bits - 10);
-            s.mass[tid] = 0;
-            s.best[tid] = 0;
-            s.cnt[tid] = 0;
-            if (tid == 0) s.hit.bin = -1;
-            __syncthreads();
-            each(bin, [&](u64 key, u64 w) {
-                if (key < lo || key > hi) return;
-                const int d = (int)((hi - key) >> sh);
-                atomicAdd(&s.mass[d], w);
-                atomicAdd(&s.cnt[d], 1u);
-                atomicMax(&s.best[d], key);
-            });
-            __syncthreads();
-            const u64 m = s.mass[tid];
-            const uint32_t n = s.cnt[tid];
-            u64 mi = m;
-            uint32_t ni = n;
-            scan(mi, ni);
-            const u64 through = tokens ? n0 + ni : sum0 + mi;
-            const u64 before = tokens ? n0 + ni - n : sum0 + mi - m;
-            /* the split that passes it; the last one with tokens has no more behind */
-            if (n && before < need && through >= need) s.hit = {s.best[tid], sum0 + mi, tid, (int)(n0 + ni)};
-            __syncthreads();
-            if (s.hit.bin < 0) {
-                __syncthreads();
-                if (n) atomicMax(&s.hit.bin, tid);
-                __syncthreads();
-                const int last = s.hit.bin;
-                __syncthreads();
-                if (tid == last) s.hit = {s.best[tid], sum0 + mi, tid, (int)(n0 + ni)};
-                if (last < 0 && tid == 0) s.hit = {0, sum0, 0, (int)n0};
-                __syncthreads();
-            }
-            const int d = s.hit.bin;
-            SmPlace p = s.hit;
-            const uint32_t nd = s.cnt[d];
-            const u64 md = s.mass[d];
-            __syncthreads();
-            if (nd <= 1 || sh == 0) {
-                p.bin = bin;
-                return p;
-            }
-            n0 = p.n - nd;
-            sum0 = p.sum - md;
-            hi = p.key;
-            const u64 end = hi > ((1ull << sh) - 1) ? hi - ((1ull << sh) - 1) : 0;
-            lo = end > lo ? end : lo;
+        const int len = queue(lo, hi, lo2, hi2);
+        if (len > SP_QUEUE) return false;
+#pragma unroll 1
+        for (int i = tid; i < len; i += SP_THREADS) {
+            const u64 key = s.queue[i];
+            const int bin = bin_of(sm_value(key)), off = s.off[bin];
+            if (off < 0) continue;
+            const int at = off + (int)atomicAdd(&s.cur[bin], 1u);
+            if (at < n) s.key[at] = key;          /* (the counts say that it is) */
         }
+        __syncthreads();
+        u64 key = 0, w = 0;
+        int at = 0, bin = 0;
+        if (tid < n) {
+            key = s.key[tid];
+            const double z = sc.z(sm_value(key));
+            w = weight(z);
+            bin = sm_bin(first, sm_q(z));
+            const int i0 = s.off[bin], i1 = i0 + (int)(s.n[bin] - n_before(bin));
+            at = i0;
+#pragma unroll 8
+            for (int i = i0; i < i1; i++) at += s.key[i] > key;
+        }
+        __syncthreads();
+        if (tid < n) {
+            s.key[at] = key;
+            s.queue[at] = w;
+        }
+        __syncthreads();
+        u64 m = tid < n ? s.queue[tid] : 0;
+        w = m;
+        uint32_t k = 0;
+        scan(m, k);
+        s.queue[SP_LIST + tid] = m - w;           /* before it in the list   */
+        __syncthreads();
+        if (tid < n) {
+            bin = bin_of(sm_value(s.key[tid]));
+            s.through[tid] = sum_before(bin) + m - s.queue[SP_LIST + s.off[bin]];
+        }
+        __syncthreads();
+        return true;
     }
 };
 
@@ -413,34 +534,60 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
 {
     using Row = SmRow<T>;
     __shared__ typename Row::Lds s;
+    constexpr int LAST = SM_BINS - 1;
     const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
     const float temp = sm_temperature(a, row);
+    const int top_k = a.r.top_k ? a.r.top_k[row] : 0;
+    const float p = a.r.top_p ? a.r.top_p[row] : 1.0f;
+    const float floor_ = a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
+    const float u = a.r.u[row];
     Row r{a, s, (const T *)a.x + (size_t)row * a.stride, a.cmax + (size_t)row * a.nc,
-          SmScale{0.0, false}, 0.0, 0.0};
+          SmScale{0.0, false}, 0.0, 0.0, {}};
     auto done = [&](int pick, float prob, int kept) {
         d_pick[row] = pick;
         if (a.prob) a.prob[row] = prob;
         if (a.kept) a.kept[row] = kept;
     };
 
-    if (!(temp > 0.0f)) {
-        /* the first chunk with the largest, and the first in it */
-        u64 best = 0;
-        for (int c = tid; c < a.nc; c += SP_THREADS) {
-            const u64 k = r.cmax[c] > -INFINITY ? am_key(r.cmax[c], c) : 0;
-            best = k > best ? k : best;
-        }
-        best = wave_max_u64(best);
-        if (lane == 0) s.part[tid >> 6] = best;
-        __syncthreads();
+    /* the largest logit, and the first chunk that has it; the slices' first bins on
+     * their way meanwhile */
+    constexpr int G = 16;
+    const SmTop *tops = a.top + (size_t)row * a.ns;
+    const u64 *bins = a.bins + (size_t)row * a.ns * SM_BINS;
+    const bool sampled = temp > 0.0f;
+    SmTop mine{-INFINITY, 0, 0, 0};
+    if (sampled && !sm_short(a, top_k) && (lane & (G - 1)) < a.ns) mine = tops[lane & (G - 1)];
+    u64 most = 0;
+#pragma unroll
+    for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++) {
+        const int c = tid + k * SP_THREADS;
+        r.cm[k] = c < a.nc ? r.cmax[c] : -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++) {
+        const u64 key = r.cm[k] > -INFINITY ? am_key(r.cm[k], tid + k * SP_THREADS) : 0;
+        most = key > most ? key : most;
+    }
+#pragma unroll 1
+    for (int c = SP_CHUNKS + tid; c < a.nc; c += SP_THREADS) {
+        const u64 key = r.cmax[c] > -INFINITY ? am_key(r.cmax[c], c) : 0;
+        most = key > most ? key : most;
+    }
+    most = wave_max_u64(most);
+    if (lane == 0) s.part[tid >> 6] = most;
+    if (tid == 0) {
+        s.tail = 0;
+        s.tail_n = 0;
+    }
+    __syncthreads();
+    most = wave_max_u64(s.part[lane & (SP_WAVES - 1)]);
+    if (most == 0) {
+        if (tid == 0) done(-1, 0.0f, 0);
+        return;
+    }
+    if (!sampled) {
         if (tid >= 64) return;
-        best = 0;
-        for (int k = 0; k < SP_WAVES; k++) best = s.part[k] > best ? s.part[k] : best;
-        if (best == 0) {
-            if (tid == 0) done(-1, 0.0f, 0);
-            return;
-        }
-        const int t = sm_token(best) * SM_CHUNK + lane;
+        const int t = sm_token(most) * SM_CHUNK + lane;
         float v = -INFINITY;
         if (t < a.vocab) io_load<T, 1>(r.x + t, &v);
         const u64 k = wave_max_u64(v > -INFINITY ? am_key(v, t) : 0);
@@ -449,116 +596,379 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     }
 
     /* ---- the slices' bins as the row's ---- */
-    const double *tops = a.top + (size_t)row * a.ns;
-    double top = -INFINITY;
-    for (int k = 0; k < a.ns; k++) top = fmax(top, tops[k]);
-    if (top == -INFINITY) {
-        if (tid == 0) done(-1, 0.0f, 0);
-        return;
-    }
-    r.sc = SmScale{1.4426950408889634 / (double)temp, top == INFINITY};
-    r.first = r.sc.inf ? 0.0 : top;
+    const float largest = sm_value(most);
+    r.sc = SmScale{1.4426950408889634 / (double)temp, largest == INFINITY};
+    const double zmost = r.sc.z(largest);
+    r.first = sm_q(zmost);
     r.e = sm_e(r.first);
-    s.sum[tid] = 0;
-    s.n[tid] = 0;
-    if (tid == 0) s.held = -1;
-    __syncthreads();
-    for (int k = 0; k < a.ns; k++) {
-        const double t = tops[k];
-        if (t == -INFINITY) continue;
-        const size_t at = ((size_t)row * a.ns + k) * SM_BINS + tid;
-        const uint32_t n = a.count[at];
-        if (!n) continue;
-        u64 m = a.mass[at];
-        int d = 0, sh = 0;
-        if (t != top) {
-            const double de = r.e - sm_e(t);
-            d = r.sc.inf ? SM_BINS : sm_bin(top, t);
-            sh = r.sc.inf || de >= 63.0 ? 63 : (int)de;
-            if (sh) m = (m + (1ull << (sh - 1))) >> sh;
+    const double edge = r.edge(r.first - tid), unit = __hiloint2double((1023 + a.sh) << 20, 0);
+    auto part_of = [&](u64 total) {               /* top-p's sum             */
+        const u64 v = p > 0.0f ? sm_part(p, total, true) : 0;
+        return v > 1 ? v : 1;
+    };
+    auto place_of = [&](u64 total) {              /* the pick's              */
+        u64 t = total - 1;
+        if (!(u >= 1.0f)) t = min(t, u > 0.0f ? sm_part(u, total, false) : 0);
+        return t + 1;
+    };
+    auto under = [&](u64 key) {                   /* min_p                   */
+        return sm_exp2(r.sc.z(sm_value(key)) - zmost) < (double)floor_;
+    };
+    const bool by_p = p < 1.0f, by_floor = floor_ > 0.0f;
+
+    /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order ---- */
+    const bool brief = sm_short(a, top_k);
+    if (brief) {
+        /* that chunk's maximum, or a little less: the range of keys split by 1024 */
+        uint32_t key0 = (uint32_t)(am_key(-3.4028235e38f, 0) >> 32), key1 = (uint32_t)(most >> 32);
+        int n0 = 0;
+#pragma unroll 1
+        for (;;) {
+            const int sh = max(0, 22 - (int)__clz((int)((key1 - key0) | 1)));
+            __syncthreads();
+            s.cur[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++) {
+                const uint32_t key = (uint32_t)(am_key(r.cm[k], 0) >> 32);
+                if (r.cm[k] > -INFINITY && key >= key0 && key <= key1)
+                    atomicAdd(&s.cur[(key1 - key) >> sh], 1u);
+            }
+            __syncthreads();
+            u64 none = 0;
+            uint32_t c = s.cur[tid];
+            r.scan(none, c);
+            s.cur[tid] = n0 + c;
+            __syncthreads();
+            const int d = sm_first(SP_THREADS, [&](int i) { return s.cur[i] >= (uint32_t)top_k; });
+            if (d == SP_THREADS) break;           /* fewer chunks with tokens */
+            const uint32_t end = key1 - (((uint32_t)d << sh) | ((1u << sh) - 1));
+            n0 = d ? (int)s.cur[d - 1] : n0;
+            const int through = (int)s.cur[d];
+            key1 -= (uint32_t)d << sh;
+            key0 = end > key0 && end <= key1 ? end : key0;
+            if (sh == 0 || through <= top_k + top_k / 8 + 8) break;
         }
-        const int bin = tid == SM_BINS - 1 ? tid : min(tid + d, SM_BINS - 1);
-        atomicAdd(&s.n[bin], n);
-        atomicAdd(&s.sum[bin], m);
+        const int len = r.queue(sm_value((u64)key0 << 32), INFINITY, INFINITY, -INFINITY);
+        if (len <= SP_LIST) {
+            u64 key = 0;
+            int at = 0;
+            if (tid < len) {
+                key = s.queue[tid];
+#pragma unroll 8
+                for (int i = 0; i < len; i++) at += s.queue[i] > key;
+                s.key[at] = key;
+            }
+            __syncthreads();
+            const int end = min(top_k, len);
+            u64 m = tid < end ? sm_weight(r.sc.z(sm_value(s.key[tid])) - r.e, a.sh) : 0;
+            uint32_t none = 0;
+            r.scan(m, none);
+            s.through[tid] = m;
+            __syncthreads();
+            int kept = end;
+            if (by_p)
+                kept = min(kept, sm_first(end, [&, need = part_of(s.through[end - 1])](int i) {
+                                     return s.through[i] >= need;
+                                 }) + 1);
+            if (by_floor)
+                kept = min(kept, max(1, sm_first(end, [&](int i) { return under(s.key[i]); })));
+            const u64 total = s.through[kept - 1], need = place_of(total);
+            const int i = min(sm_first(kept, [&](int j) { return s.through[j] >= need; }), kept - 1);
+            if (tid == 0) {
+                const double v = sm_exp2(r.sc.z(sm_value(s.key[i])) - r.e) *
+                                 __hiloint2double((1023 + a.sh) << 20, 0);
+                done(sm_token(s.key[i]), (float)(v / (double)total), kept);
+            }
+            return;
+        }
+    }
+
+    /* a bin a thread. A slice's bins start d behind the row's: bin `tid` is its tid - d, and
+     * threads 0 .. d - 1 have its last d, which are behind the row's and join the last one */
+    const double edge_rest = r.edge(r.first - LAST - tid);
+    uint32_t n = 0, rest_n = 0;
+    u64 part = 0, rest = 0;
+#pragma unroll 1
+    for (int k0 = 0; !brief && k0 < a.ns; k0 += G) {
+        if (k0) {
+            mine = SmTop{-INFINITY, 0, 0, 0};
+            if (k0 + (lane & (G - 1)) < a.ns) mine = tops[k0 + (lane & (G - 1))];
+        }
+        const bool same = mine.q == (r.sc.inf ? INFINITY : r.first);
+        const int mine_d = same ? 0 : r.sc.inf ? LAST : sm_bin(r.first, mine.q);
+        /* how much less a slice's weights are where it starts more bins behind */
+        const double mine_far =
+            r.sc.inf ? 0.0 : sm_exp2(fmin((mine.q - r.first + mine_d) * (1.0 / 32.0), 0.0));
+        u64 word[G];
+#pragma unroll
+        for (int k = 0; k < G; k++) {
+            const int d = __builtin_amdgcn_readlane(mine_d, k);
+            const int j = tid < d ? LAST - d + tid : tid - d;
+            word[k] = k0 + k < a.ns && tid < LAST ? bins[(size_t)(k0 + k) * SM_BINS + j] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < G; k++) {
+            const int d = __builtin_amdgcn_readlane(mine_d, k);
+            const double far = __hiloint2double(
+                __builtin_amdgcn_readlane(__double2hiint(mine_far), k),
+                __builtin_amdgcn_readlane(__double2loint(mine_far), k));
+            const uint32_t wn = (uint32_t)(word[k] >> SM_COUNT);
+            const u64 wp = word[k] & ((1ull << SM_COUNT) - 1);
+            if (tid >= d) {
+                n += wn;
+                part += wp;
+            } else if (wn) {
+                rest_n += wn;
+                rest += (u64)__builtin_rint(edge_rest * far *
+                                            ((double)wn + (double)wp * (1.0 / (1ull << SM_PART))));
+            }
+        }
+        /* the slices' last bins, in units of 2^E of their own */
+        if (tid < G && mine.tail_n) {
+            u64 m = mine.tail;
+            if (r.sc.inf) {
+                m = 0;
+            } else if (!same) {
+                const double de = r.e - sm_e(mine.q);
+                const int sh = de >= 63.0 ? 63 : (int)de;
+                if (sh) m = (m + (1ull << (sh - 1))) >> sh;
+            }
+            rest_n += mine.tail_n;
+            rest += m;
+        }
+    }
+    if (brief) {
+        /* too many tokens as large: the bins from the row */
+        __syncthreads();
+        s.mass[tid] = 0;
+        s.cur[tid] = 0;
+        r.template each_of_row<2>(-3.4028235e38f, INFINITY, INFINITY, -INFINITY, [&](float v, int) {
+            const double z = r.sc.z(v), q = sm_q(z);
+            const int bin = sm_bin(r.first, q);
+            if (bin < LAST) {
+                atomicAdd(&s.cur[bin], 1u);
+                atomicAdd(&s.mass[bin], sm_bin_word(z, q));
+            } else {
+                rest_n++;
+                rest += sm_weight(z - r.e, a.sh);
+            }
+        });
+        n = s.cur[tid];
+        part = s.mass[tid];
+    }
+    if (rest_n) {
+        atomicAdd(&s.tail_n, rest_n);
+        atomicAdd(&s.tail, rest);
     }
     __syncthreads();
-    const u64 m = s.sum[tid];
-    const uint32_t n = s.n[tid];
+    if (tid == LAST) n = s.tail_n;
+    const u64 m = tid == LAST ? s.tail : sm_bin_sum(edge, n, part);
     u64 mi = m;
     uint32_t ni = n;
     r.scan(mi, ni);
     s.sum[tid] = mi;
     s.n[tid] = ni;
     __syncthreads();
+    const int all = (int)s.n[LAST];
 
-    /* ---- the last token left: key 0 is behind its whole bin ---- */
-    SmPlace cut{0, s.sum[SM_BINS - 1], SM_BINS - 1, (int)s.n[SM_BINS - 1]};
-    /* the first bin through which it is; the last, where roundings pass the sum */
-    auto bin_of = [&](u64 need, bool tokens) {
-        __syncthreads();
-        if (tid == 0) s.hit.bin = SM_BINS - 1;
-        __syncthreads();
-        const u64 through = tokens ? ni : mi, before = tokens ? ni - n : mi - m;
-        if (n && before < need && through >= need) s.hit.bin = tid;
-        __syncthreads();
-        return s.hit.bin;
-    };
-    const int k = a.r.top_k ? a.r.top_k[row] : 0;
-    if (k > 0 && k < cut.n) cut = r.cross(bin_of((u64)k, true), (u64)k, true);
-    const float p = a.r.top_p ? a.r.top_p[row] : 1.0f;
-    if (p < 1.0f) {
-        const u64 part = p > 0.0f ? sm_part(p, cut.sum, true) : 0;
-        const u64 need = part > 1 ? part : 1;
-        const int b = bin_of(need, false);
-        if (b < cut.bin || (b == cut.bin && need < cut.sum)) cut = r.cross(b, need, false);
+    /* ---- the bins where the limits and the pick may be: what comes before them and
+     *      what comes through them bounds every sum ---- */
+    const bool by_k = top_k > 0 && top_k < all;
+    int kb = LAST, pb0 = LAST, pb1 = LAST, mb = LAST;
+    if (by_k) kb = sm_first(SM_BINS, [&](int i) { return s.n[i] >= (uint32_t)top_k; });
+    u64 lo = by_k ? r.sum_before(kb) : s.sum[LAST], hi = s.sum[kb];
+    if (by_p) {
+        pb0 = min(kb, r.sum_bin(part_of(lo ? lo : 1)));
+        pb1 = min(kb, r.sum_bin(part_of(hi)));
     }
-    const float floor_ = a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
-    if (floor_ > 0.0f) {
-        /* tokens from z of the largest + log2(min_p) on */
-        float best = -INFINITY;
-        for (int c = tid; c < a.nc; c += SP_THREADS) best = fmaxf(best, r.cmax[c]);
-        best = wave_max(best);
-        __syncthreads();
-        if (lane == 0) s.part[tid >> 6] = __float_as_uint(best);
-        __syncthreads();
-        for (int w = 0; w < SP_WAVES; w++) best = fmaxf(best, __uint_as_float((uint32_t)s.part[w]));
-        const double zmin = r.sc.z(best) + log2((double)floor_);
-        const int b = sm_bin(r.first, sm_q(zmin));
-        if (b <= cut.bin) {
-            r.hold(b);
-            __syncthreads();
-            if (tid == 0) s.hit = {~0ull, b ? s.sum[b - 1] : 0, b, (int)(b ? s.n[b - 1] : 0)};
-            __syncthreads();
-            const u64 last = cut.bin == b ? cut.key : 0;
-            r.each(b, [&](u64 key, u64 w) {
-                if (key < last || r.sc.z(sm_value(key)) < zmin) return;
-                atomicMin(&s.hit.key, key);
-                atomicAdd(&s.hit.sum, w);
-                atomicAdd(&s.hit.n, 1);
-            });
-            __syncthreads();
-            if (s.hit.n < cut.n) cut = s.hit;
-            __syncthreads();
+    /* the first bin whose lower edge is under the floor has the last that stays */
+    if (by_floor)
+        mb = min(sm_first(SM_BINS, [&](int i) {
+                     return sm_exp2(fmin((r.first - i) * (1.0 / 32.0) - zmost, 0.0)) < (double)floor_;
+                 }), LAST);
+    const int c0 = min(min(kb, pb0), mb), c1 = min(min(kb, pb1), mb);
+    if (by_k || by_p || by_floor) {
+        lo = max(r.sum_before(c0), 1ull);
+        hi = s.sum[c1];
+    }
+    const int ub0 = min(r.sum_bin(place_of(lo)), c1), ub1 = min(r.sum_bin(place_of(hi)), c1);
+    /* listed are all bins up to the last cut, if they fit, else the ones that may be
+     * needed; top-k's is if it is the cut or top-p takes a part of its sum */
+    const bool need_k = by_k && (by_p || kb <= c1);
+    const int kn = need_k && kb > c1 ? (int)(s.n[kb] - r.n_before(kb)) : 0;
+    const bool whole = (int)s.n[c1] + kn <= SP_LIST;
+    const bool in = (need_k && tid == kb) ||
+                    (whole ? tid <= c1
+                           : (by_p && tid >= pb0 && tid <= pb1) || (by_floor && tid == mb) ||
+                                 (tid >= ub0 && tid <= ub1));
+    /* which lie in two ranges */
+    int b0 = 0, b1 = c1, b2 = need_k ? kb : 0, b3 = need_k ? kb : c1;
+    if (!whole) {
+        b0 = min(min(need_k ? kb : LAST, by_p ? pb0 : LAST), by_floor ? mb : LAST);
+        b1 = max(max(need_k ? kb : 0, by_p ? pb1 : 0), by_floor ? mb : 0);
+        if (b0 > b1) b0 = b1 = ub0;
+        b2 = ub0;
+        b3 = ub1;
+    }
+    u64 none = 0;
+    uint32_t len = in ? n : 0;
+    r.scan(none, len);
+    s.off[tid] = in && n ? (int)(len - n) : -1;
+    if (tid == LAST) s.len = (int)len;
+    __syncthreads();
+    const int listed = s.len;
+    __syncthreads();
+    /* key 0 is behind the whole bin */
+    SmPlace cut{0, s.sum[LAST], LAST, all};
+    if (listed <= SP_LIST && r.list(b0, b1, b2, b3, listed)) {
+        auto place = [&](int b, int i) {
+            return SmPlace{s.key[i], s.through[i], b, (int)r.n_before(b) + i - s.off[b] + 1};
+        };
+        /* the token of bin b that passes the sum, or the bin's last */
+        auto at = [&](int b, u64 need) {
+            const int off = s.off[b], end = off + (int)(s.n[b] - r.n_before(b)) - 1;
+            const int i = sm_first(listed, [&](int j) { return s.through[j] >= need; });
+            return place(b, min(max(i, off), end));
+        };
+        if (need_k) cut = place(kb, s.off[kb] + top_k - 1 - (int)r.n_before(kb));
+        if (by_p) {
+            const u64 need = part_of(cut.sum);
+            const int b = min(max(r.sum_bin(need), pb0), pb1);
+            if (s.off[b] >= 0) {                  /* else min_p cuts before it */
+                const SmPlace c = at(b, need);
+                if (c.n < cut.n) cut = c;
+            }
         }
+        if (by_floor && mb <= cut.bin) {
+            /* up to the first of the bin that is under it */
+            SmPlace c{~0ull, r.sum_before(mb), mb, (int)r.n_before(mb)};
+            const int off = s.off[mb];
+            if (off >= 0) {
+                const int i = sm_first((int)(s.n[mb] - r.n_before(mb)),
+                                       [&](int j) { return under(s.key[off + j]); });
+                if (i > 0) c = place(mb, off + i - 1);
+            }
+            if (c.n < cut.n) cut = c;
+        }
+        const u64 need = place_of(cut.sum);
+        const SmPlace got = at(min(min(max(r.sum_bin(need), ub0), ub1), cut.bin), need);
+        if (tid == 0) {
+            /* behind the cut only by the roundings of the bins' sums */
+            const u64 best = got.n > cut.n ? cut.key : got.key;
+            const double v = sm_exp2(r.sc.z(sm_value(best)) - r.e) * unit;
+            done(sm_token(best), (float)(v / (double)cut.sum), cut.n);
+        }
+        return;
     }
 
-    /* ---- the pick ---- */
-    float u = a.r.u[row];
-    u64 t = cut.sum - 1;
-    if (!(u >= 1.0f)) t = min(t, u > 0.0f ? sm_part(u, cut.sum, false) : 0);
-    const int b = min(bin_of(t + 1, false), cut.bin);
-    const SmPlace at = r.cross(b, t + 1, false);
-    if (tid == 0) {
-        /* behind the cut only by the roundings of the bins' sums */
-        const u64 key = b == cut.bin && at.key < cut.key ? cut.key : at.key;
-        const double w = sm_exp2(r.sc.z(sm_value(key)) - r.e) * __hiloint2double((1023 + a.sh) << 20, 0);
-        done(sm_token(key), (float)(w / (double)cut.sum), cut.n);
+    /* ---- more tokens than the list takes: each limit and then the pick by passes over the
+     *      row. Where the order passes `need` tokens or the sum `need`, in a bin that is
+     *      known: the bin's range of keys is split by 1024 until the token that does is alone,
+     *      or, where roundings of the bins' sums leave the tokens short, the bin's last. ---- */
+#pragma unroll 1
+    for (int phase = 0; phase < 4; phase++) {     /* top-k, top-p, min-p, the pick */
+        u64 need = 0;
+        int b = 0;
+        if (phase == 0) {
+            if (!by_k) continue;
+            need = (u64)top_k;
+            b = kb;
+        } else if (phase == 1) {
+            if (!by_p) continue;
+            need = part_of(cut.sum);
+            b = r.sum_bin(need);
+            if (b > cut.bin || need >= cut.sum) continue;
+        } else if (phase == 2) {
+            if (!by_floor || mb > cut.bin) continue;
+            b = mb;
+        } else {
+            need = place_of(cut.sum);
+            b = min(r.sum_bin(need), cut.bin);
+        }
+        float xlo, xhi;
+        r.range_of(b, b, &xlo, &xhi);
+        u64 key0 = am_key(xlo, INT32_MAX), key1 = am_key(xhi, 0), sum0 = r.sum_before(b);
+        uint32_t n0 = r.n_before(b);
+        const u64 stay = cut.bin == b ? cut.key : 0;
+        SmPlace got;
+#pragma unroll 1
+        for (;;) {
+            const int bits = 64 - __clzll((long long)((key1 - key0) | 1));
+            const int sh = max(0, bits - 10);
+            __syncthreads();
+            s.mass[tid] = 0;
+            s.best[tid] = 0;
+            s.cur[tid] = 0;
+            if (tid == 0) s.hit = {~0ull, sum0, phase == 2 ? b : -1, (int)n0};
+            r.template each_of_row<2>(xlo, xhi, xlo, xhi, [&](float v, int t) {
+                const double z = r.sc.z(v);
+                if (sm_bin(r.first, sm_q(z)) != b) return;
+                const u64 key = am_key(v, t), w = r.weight(z);
+                if (phase == 2) {
+                    if (key < stay || under(key)) return;
+                    atomicMin(&s.hit.key, key);
+                    atomicAdd(&s.hit.sum, w);
+                    atomicAdd(&s.hit.n, 1);
+                    return;
+                }
+                if (key < key0 || key > key1) return;
+                const int d = (int)((key1 - key) >> sh);
+                atomicAdd(&s.mass[d], w);
+                atomicAdd(&s.cur[d], 1u);
+                atomicMax(&s.best[d], key);
+            });
+            if (phase == 2) {
+                got = s.hit;
+                break;
+            }
+            const u64 dm = s.mass[tid];
+            const uint32_t dn = s.cur[tid];
+            u64 dmi = dm;
+            uint32_t dni = dn;
+            r.scan(dmi, dni);
+            const u64 through = phase == 0 ? n0 + dni : sum0 + dmi;
+            const u64 before = phase == 0 ? n0 + dni - dn : sum0 + dmi - dm;
+            if (dn && before < need && through >= need)
+                s.hit = {s.best[tid], sum0 + dmi, tid, (int)(n0 + dni)};
+            __syncthreads();
+            int d = s.hit.bin;
+            __syncthreads();
+            if (d < 0) {
+                if (dn) atomicMax(&s.hit.bin, tid);
+                __syncthreads();
+                d = max(0, s.hit.bin);
+                __syncthreads();
+                if (tid == d) s.hit = {s.best[tid], sum0 + dmi, tid, (int)(n0 + dni)};
+                __syncthreads();
+            }
+            got = s.hit;
+            got.bin = b;
+            const uint32_t nd = s.cur[d];
+            const u64 md = s.mass[d];
+            if (nd <= 1 || sh == 0) break;
+            n0 = got.n - nd;
+            sum0 = got.sum - md;
+            key1 = got.key;
+            const u64 end = key1 > ((1ull << sh) - 1) ? key1 - ((1ull << sh) - 1) : 0;
+            key0 = end > key0 ? end : key0;
+        }
+        __syncthreads();
+        if (phase == 3) {
+            if (tid == 0) {
+                const u64 key = b == cut.bin && got.key < cut.key ? cut.key : got.key;
+                const double v = sm_exp2(r.sc.z(sm_value(key)) - r.e) * unit;
+                done(sm_token(key), (float)(v / (double)cut.sum), cut.n);
+            }
+        } else if (got.n < cut.n) {
+            cut = got;
+        }
     }
 }
 
 struct SamplePlan {
     int ns, nc, sh;
-    size_t mass, count, top, cmax, bytes;         /* offsets                 */
+    size_t top, cmax, bytes;                      /* offsets; the bins are first */
 };
 
 SamplePlan sample_plan(int n, int vocab)
@@ -571,10 +981,8 @@ SamplePlan sample_plan(int n, int vocab)
     while ((1ll << bits) < vocab) bits++;
     p.sh = 62 - bits < 50 ? 62 - bits : 50;
     const size_t slices = (size_t)n * p.ns;
-    p.mass = 0;
-    p.top = p.mass + slices * SM_BINS * sizeof(u64);
-    p.count = p.top + slices * sizeof(double);
-    p.cmax = p.count + slices * SM_BINS * sizeof(uint32_t);
+    p.top = slices * SM_BINS * sizeof(u64);
+    p.cmax = p.top + slices * sizeof(SmTop);
     p.bytes = (p.cmax + (size_t)n * p.nc * sizeof(float) + 15) / 16 * 16;
     return p;
 }
@@ -624,9 +1032,8 @@ extern "C" int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const 
         return -1;
     }
     char *base = (char *)d_scratch;
-    SampleJob a{d_logits, stride, n, vocab, p.ns, p.nc, p.sh, *s, (u64 *)(base + p.mass),
-                (uint32_t *)(base + p.count), (double *)(base + p.top), (float *)(base + p.cmax),
-                d_kept, d_prob};
+    SampleJob a{d_logits, stride, n, vocab, p.ns, p.nc, p.sh, *s, (u64 *)base,
+                (SmTop *)(base + p.top), (float *)(base + p.cmax), d_kept, d_prob};
     hipStream_t st = (hipStream_t)stream;
     return fmt == DSV4_WF32 ? sample_launch<float>(a, d_pick, st)
                             : sample_launch<uint16_t>(a, d_pick, st);

@@ -99,6 +99,35 @@ def test_equal_logits(gpu, dsv4, vocab):
         check(dsv4, x, u=us, min_p=np.array([1, 0.5, 1e-6, 2, 0]))
 
 
+@pytest.mark.parametrize("vocab", [20000, 129280, 262145, 300000])
+def test_likely_tokens_that_stand_together(gpu, dsv4, vocab):
+    """Sorted logits, and a block of equal ones: many tokens of few chunks as large as
+    the k-th largest chunk."""
+    rng = np.random.default_rng(vocab)
+    n = 9
+    x = -np.sort(-logits(rng, n, vocab, "flat"), axis=1)
+    x[3:6] = x[3:6, ::-1]
+    x[6:, 1000:4000] = 20.0
+    k = np.array([1, 40, 512, 2, 200, 513, 50, 3, 400])
+    r = rules(rng, n)
+    for keys in (("u",), ("u", "top_p"), ("u", "min_p", "temperature"), tuple(r)):
+        kw = {name: r[name] for name in keys}
+        kw["top_k"] = k
+        check(dsv4, x, **kw)
+    check(dsv4, x, True, u=r["u"], top_k=k)
+
+
+def test_far_ahead(gpu, dsv4):
+    """One token far ahead of the rest, the k-th among the tokens of no weight."""
+    rng = np.random.default_rng(31)
+    n, vocab = 8, 129280
+    x = logits(rng, n, vocab, "flat")
+    x[:, 77] = 60
+    check(dsv4, x, u=rng.random(n), temperature=np.full(n, 0.5), top_k=np.full(n, 50),
+          top_p=np.array([0.5, 0.9, 1, 1, 0.99, 0.999, 1, 0.3]))
+    check(dsv4, x, u=rng.random(n), top_k=np.full(n, 5000), top_p=np.full(n, 0.9))
+
+
 def test_two_values(gpu, dsv4):
     """Long runs of equal logits on both sides of a border."""
     rng = np.random.default_rng(8)
