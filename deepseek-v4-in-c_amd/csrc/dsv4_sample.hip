@@ -24,8 +24,8 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SM_THREADS = 256;
-constexpr int SM_EACH = 32;                       /* tokens of a thread      */
+constexpr int SM_THREADS = 512;
+constexpr int SM_EACH = 16;                       /* tokens of a thread      */
 constexpr int SM_SLICE = SM_THREADS * SM_EACH;
 constexpr int SM_BINS = 1024;                     /* 32 octaves, the rest in the last */
 constexpr int SM_CHUNK = 64;                      /* tokens with one maximum */
@@ -119,23 +119,23 @@ __device__ __forceinline__ float sm_temperature(const SampleJob &a, int row)
     return a.r.temperature ? a.r.temperature[row] : 1.0f;
 }
 
-/* 2^(r/32) - 1, 0 <= r < 1: the exponential's series to r^6, 5e-16 off at the most. */
-__device__ __forceinline__ double sm_bin_part(double r)
+/* (2^(r/32) - 1) 2^42 of a token, r in [0, 1), as a whole number: the polynomial of
+ * degree 5 through its values at Chebyshev's points, 2^-53 off at the most (its
+ * constant term is 3e-4 of a unit), added to 2^52, which rounds it. sm_bin_bits: still
+ * with 2^52's exponent above bit 51. */
+__device__ __forceinline__ u64 sm_bin_bits(double r)
 {
-    double p = 1.4345655584131932e-13;
-    p = fma(p, r, 3.9737099845494154e-11);
-    p = fma(p, r, 9.172562701824643e-09);
-    p = fma(p, r, 1.6938509724371819e-06);
-    p = fma(p, r, 0.00023459619820224677);
-    p = fma(p, r, 0.02166084939249829);
-    return p * r;
+    static_assert(SM_PART == 42, "the coefficients' unit");
+    double p = 176.66942619745828;
+    p = fma(p, r, 40339.21157864393);
+    p = fma(p, r, 7449636.473277472);
+    p = fma(p, r, 1031764990.7605293);
+    p = fma(p, r, 95265423098.24869);
+    return (u64)__double_as_longlong(fma(p, r, 4503599627370496.0));
 }
-
-/* (2^(r/32) - 1) 2^42 of a token, as a whole number. */
 __device__ __forceinline__ u64 sm_bin_word(double z, double q)
 {
-    const double v = fma(sm_bin_part(fma(z, 32.0, -q)), (double)(1ull << SM_PART), 4503599627370496.0);
-    return (u64)__double_as_longlong(v) & ((1ull << 52) - 1);
+    return sm_bin_bits(fma(z, 32.0, -q)) & ((1ull << 52) - 1);
 }
 
 /* The sum of n tokens of a bin, `edge` the weight at its lower edge. Equal tokens sum
@@ -144,7 +144,9 @@ __device__ __forceinline__ u64 sm_bin_word(double z, double q)
 __device__ __forceinline__ u64 sm_bin_sum(double edge, uint32_t n, u64 part)
 {
     constexpr double ONE = 1.0 / (1ull << SM_PART);
-    const double each = __builtin_rint((double)part / (double)n);
+    /* the quotient, which is below 2^37, to 2^-10 */
+    const double r = __builtin_amdgcn_rcp((double)n);
+    const double each = __builtin_rint((double)part * fma(fma(-(double)n, r, 1.0), r, r));
     if (n && (u64)each * n == part) return (u64)__builtin_rint(edge * (1.0 + each * ONE)) * n;
     return (u64)__builtin_rint(edge * ((double)n + (double)part * ONE));
 }
@@ -214,24 +216,33 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
     const size_t at = (size_t)row * a.ns + slice;
     const SmScale sc{1.4426950408889634 / (double)temp, top == INFINITY};
     const double first = sm_q(sc.z(top)), e = sm_e(first);
-    u64 rest = 0;                                 /* of the last bin         */
-    uint32_t rest_n = 0;
-    if (top > -INFINITY) {
+    /* of the last bin, whose weights of at most 2^-32 need 2^-14 of their own */
+    uint32_t rest = 0, rest_n = 0;
+    const float unit = __uint_as_float((uint32_t)(127 + a.sh) << 23);
+    if (sc.inf) {
 #pragma unroll
         for (int k = 0; k < SM_EACH; k++) {
-            if (!(v[k] > -INFINITY)) continue;
-            const double z = sc.z(v[k]), q = sm_q(z);
-            const double d = first - q;
+            if (v[k] == INFINITY) atomicAdd(&bins[0], 1ull << SM_COUNT);
+            else rest_n += v[k] > -INFINITY;
+        }
+    } else if (top > -INFINITY) {
+        const double c32 = sc.c * 32.0;           /* exact, and so is y - q   */
+#pragma unroll
+        for (int k = 0; k < SM_EACH; k++) {
+            const double y = (double)v[k] * c32, q = floor(y), d = first - q;
             if (d < SM_BINS - 1) {
-                atomicAdd(&bins[(int)d], sm_bin_word(z, q) + (1ull << SM_COUNT));
-            } else {
-                rest += sm_weight(z - e, a.sh);
+                /* 2^52's exponent becomes the count */
+                constexpr uint32_t ONE = (1u << (SM_COUNT - 32)) - (0x433u << 20);
+                const u64 bits = sm_bin_bits(y - q);
+                atomicAdd(&bins[(int)d], (u64)((uint32_t)(bits >> 32) + ONE) << 32 | (uint32_t)bits);
+            } else if (v[k] > -INFINITY) {
+                rest += (uint32_t)(__builtin_amdgcn_exp2f((float)(y * (1.0 / 32.0) - e)) * unit);
                 rest_n++;
             }
         }
     }
-    if (__any(rest_n != 0)) {
-        atomicAdd(&tail, rest);
+    if (rest_n) {
+        atomicAdd(&tail, (u64)rest);
         atomicAdd(&tail_n, rest_n);
     }
     __syncthreads();
@@ -300,6 +311,11 @@ __device__ __forceinline__ V sm_wave_scan(V v)
     return v;
 }
 
+/* The bins of top-k, top-p (between two), min-p, the last cut (at most) and the pick. */
+struct SmWhere {
+    int kb, pb0, pb1, mb, c1, ub0, ub1, need_k, whole;
+};
+
 /* The first of n <= 1024 places that pred holds for, n if none does; it holds for all
  * behind the first. Each wave looks for itself: 64 places at once, then the 16 before
  * the first of them that has it. */
@@ -320,21 +336,23 @@ __device__ __forceinline__ int sm_first(int n, F pred)
 template <class T>
 struct SmRow {
     struct Lds {
-        u64 sum[SM_BINS];                         /* through a bin           */
-        uint32_t n[SM_BINS];
-        int off[SM_BINS];                         /* a bin's place in the list, or -1 */
-        uint32_t cur[SM_BINS];                    /* a bin's tokens so far   */
         union {
-            u64 queue[SP_QUEUE];                  /* tokens that may be listed */
+            __attribute__((aligned(16))) u64 queue[SP_QUEUE];  /* tokens that may be listed */
             struct {
                 u64 mass[SP_THREADS], best[SP_THREADS];   /* a split of a key range */
             };
         };
-        u64 key[SP_LIST], through[SP_LIST];       /* tokens in order, sums through them */
+        __attribute__((aligned(16))) u64 key[SP_LIST];    /* tokens in order */
+        u64 through[SP_LIST];                     /* and the sums through them */
+        u64 sum[SM_BINS];                         /* through a bin           */
+        uint32_t n[SM_BINS];
+        int off[SM_BINS];                         /* a bin's place in the list, or -1 */
+        uint32_t cur[SM_BINS];                    /* a bin's tokens so far   */
         unsigned short chunk[SP_CHUNKS];          /* chunks to read          */
         u64 part[SP_WAVES];
         uint32_t npart[SP_WAVES];
         SmPlace hit;
+        SmWhere where;
         u64 tail;                                 /* the last bin's sum      */
         uint32_t tail_n;
         int len, chunks;                          /* tokens queued; to read  */
@@ -345,6 +363,7 @@ struct SmRow {
     const float *cmax;
     SmScale sc;
     double first, e;
+    float width;                                  /* of a bin, in logits     */
     float cm[SP_CHUNKS / SP_THREADS];             /* this thread's of the first chunks */
 
     /* Inclusive sums over the threads. */
@@ -389,13 +408,13 @@ struct SmRow {
                                        : sm_weight(z - e, a.sh);
     }
 
-    /* Logits between which all tokens of bins [b0, b1] lie. */
+    /* Logits between which all tokens of bins [b0, b1] lie, with a margin for the roundings
+     * of z and of this. */
     __device__ __forceinline__ void range_of(int b0, int b1, float *lo, float *hi) const
     {
-        /* a margin for the roundings of z and of this */
-        const double l = (first - b1) / (32.0 * sc.c), h = (first - b0 + 1) / (32.0 * sc.c);
-        *lo = (float)(l - fabs(l) * 1e-6);
-        *hi = (float)(h + fabs(h) * 1e-6);
+        const float l = (float)(first - b1) * width, h = (float)(first - b0 + 1.0) * width;
+        *lo = l - fabsf(l) * 4e-6f;
+        *hi = h + fabsf(h) * 4e-6f;
         if (sc.inf || b1 == SM_BINS - 1 || !(*lo > -3.4028235e38f)) *lo = -3.4028235e38f;
         if (sc.inf || b0 == 0 || !(*hi < INFINITY)) *hi = INFINITY;
     }
@@ -425,36 +444,44 @@ struct SmRow {
             }
             __syncthreads();
             const int n = s.chunks;
-#pragma unroll 1
-            for (int i0 = tid / 16; i0 < n; i0 += G * (SP_THREADS / 16)) {
-                float v[G][4];
-                int t[G];
-#pragma unroll
-                for (int u = 0; u < G; u++) {
-                    const int i = min(i0 + u * (SP_THREADS / 16), n - 1);
-                    t[u] = (c0 + s.chunk[i]) * SM_CHUNK + 4 * (tid & 15);
-                    /* (past the vocabulary: its last four) */
-                    if (a.vocab >= 4) {
-                        io_load<T, 4>(x + min(t[u], a.vocab - 4), v[u]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) io_load<T, 1>(x + min(k, a.vocab - 1), v[u] + k);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < G; u++) {
-                    const int t1 = i0 + u * (SP_THREADS / 16) < n ? a.vocab : 0;
-                    const int t0 = t[u];
-                    t[u] = min(t0, max(0, a.vocab - 4));
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (((v[u][k] >= lo && v[u][k] <= hi) || (v[u][k] >= lo2 && v[u][k] <= hi2)) &&
-                            t[u] + k >= t0 && t[u] + k < t1)
-                            f(v[u][k], t[u] + k);
-                }
-            }
+            if (n <= SP_THREADS / 16) chunks<1>(c0, n, lo, hi, lo2, hi2, f);
+            else chunks<G>(c0, n, lo, hi, lo2, hi2, f);
         }
         __syncthreads();
+    }
+
+    /* The listed chunks, 16 lanes each, G of them in flight. */
+    template <int G, class F>
+    __device__ __forceinline__ void chunks(int c0, int n, float lo, float hi, float lo2, float hi2, F f)
+    {
+        constexpr int EACH = SP_THREADS / 16;
+        const int tid = threadIdx.x, whole = a.vocab / SM_CHUNK;
+#pragma unroll 1
+        for (int i0 = tid / 16; i0 < n; i0 += G * EACH) {
+            float v[G][4];
+            int t[G];
+#pragma unroll
+            for (int u = 0; u < G; u++) {
+                const int c = i0 + u * EACH < n ? c0 + s.chunk[i0 + u * EACH] : INT32_MAX;
+                t[u] = c * SM_CHUNK + 4 * (tid & 15);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[u][k] = -INFINITY;
+                if (c < whole) {
+                    io_load<T, 4>(x + t[u], v[u]);
+                } else if (c == whole) {          /* the row's last, not whole */
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (t[u] + k < a.vocab) io_load<T, 1>(x + t[u] + k, v[u] + k);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < G; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (__builtin_amdgcn_fmed3f(v[u][k], lo, hi) == v[u][k] ||
+                        __builtin_amdgcn_fmed3f(v[u][k], lo2, hi2) == v[u][k])
+                        f(v[u][k], t[u] + k);
+        }
     }
 
     /* Queue the tokens of two ranges of logits; how many, over SP_QUEUE: not all. */
@@ -466,6 +493,20 @@ struct SmRow {
             if (at < SP_QUEUE) s.queue[at] = am_key(v, t);
         });
         return s.len;
+    }
+
+    /* How many of keys i0 .. i1 - 1 are over one. */
+    __device__ __forceinline__ int rank(const u64 *keys, int i0, int i1, u64 key) const
+    {
+        int n = 0, i = i0;
+        if (i & 1) n += keys[i++] > key;
+#pragma unroll 4
+        for (; i + 2 <= i1; i += 2) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(keys + i);
+            n += (k.x > key) + (k.y > key);
+        }
+        if (i < i1) n += keys[i] > key;
+        return n;
     }
 
     /* Put the tokens of the bins that have a place (s.off), of b0 to b1 or b2 to b3, into the
@@ -505,8 +546,7 @@ struct SmRow {
             bin = sm_bin(first, sm_q(z));
             const int i0 = s.off[bin], i1 = i0 + (int)(s.n[bin] - n_before(bin));
             at = i0;
-#pragma unroll 8
-            for (int i = i0; i < i1; i++) at += s.key[i] > key;
+            at += rank(s.key, i0, i1, key);
         }
         __syncthreads();
         if (tid < n) {
@@ -542,7 +582,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const float floor_ = a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
     const float u = a.r.u[row];
     Row r{a, s, (const T *)a.x + (size_t)row * a.stride, a.cmax + (size_t)row * a.nc,
-          SmScale{0.0, false}, 0.0, 0.0, {}};
+          SmScale{0.0, false}, 0.0, 0.0, temp * 0.021660849f, {}};
     auto done = [&](int pick, float prob, int kept) {
         d_pick[row] = pick;
         if (a.prob) a.prob[row] = prob;
@@ -573,8 +613,18 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         const u64 key = r.cmax[c] > -INFINITY ? am_key(r.cmax[c], c) : 0;
         most = key > most ? key : most;
     }
+    /* and the least of the chunks with tokens */
+    uint32_t least = ~0u;
+#pragma unroll
+    for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++)
+        if (r.cm[k] > -INFINITY) least = min(least, (uint32_t)(am_key(r.cm[k], 0) >> 32));
     most = wave_max_u64(most);
-    if (lane == 0) s.part[tid >> 6] = most;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+    if (lane == 0) {
+        s.part[tid >> 6] = most;
+        s.npart[tid >> 6] = least;
+    }
     if (tid == 0) {
         s.tail = 0;
         s.tail_n = 0;
@@ -620,7 +670,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const bool brief = sm_short(a, top_k);
     if (brief) {
         /* that chunk's maximum, or a little less: the range of keys split by 1024 */
-        uint32_t key0 = (uint32_t)(am_key(-3.4028235e38f, 0) >> 32), key1 = (uint32_t)(most >> 32);
+        uint32_t key0 = s.npart[lane & (SP_WAVES - 1)], key1 = (uint32_t)(most >> 32);
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) key0 = min(key0, (uint32_t)__shfl_xor((int)key0, o, 64));
         int n0 = 0;
 #pragma unroll 1
         for (;;) {
@@ -649,14 +701,13 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             key0 = end > key0 && end <= key1 ? end : key0;
             if (sh == 0 || through <= top_k + top_k / 8 + 8) break;
         }
-        const int len = r.queue(sm_value((u64)key0 << 32), INFINITY, INFINITY, -INFINITY);
+        const int len = r.queue(sm_value((u64)key0 << 32), INFINITY, INFINITY, INFINITY);
         if (len <= SP_LIST) {
             u64 key = 0;
             int at = 0;
             if (tid < len) {
                 key = s.queue[tid];
-#pragma unroll 8
-                for (int i = 0; i < len; i++) at += s.queue[i] > key;
+                at = r.rank(s.queue, 0, len, key);
                 s.key[at] = key;
             }
             __syncthreads();
@@ -666,6 +717,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             r.scan(m, none);
             s.through[tid] = m;
             __syncthreads();
+            if (tid >= 64) return;
             int kept = end;
             if (by_p)
                 kept = min(kept, sm_first(end, [&, need = part_of(s.through[end - 1])](int i) {
@@ -743,7 +795,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         __syncthreads();
         s.mass[tid] = 0;
         s.cur[tid] = 0;
-        r.template each_of_row<2>(-3.4028235e38f, INFINITY, INFINITY, -INFINITY, [&](float v, int) {
+        r.template each_of_row<2>(-3.4028235e38f, INFINITY, INFINITY, INFINITY, [&](float v, int) {
             const double z = r.sc.z(v), q = sm_q(z);
             const int bin = sm_bin(r.first, q);
             if (bin < LAST) {
@@ -757,9 +809,13 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         n = s.cur[tid];
         part = s.mass[tid];
     }
-    if (rest_n) {
-        atomicAdd(&s.tail_n, rest_n);
-        atomicAdd(&s.tail, rest);
+    if (__any(rest_n != 0)) {
+        rest_n = sm_wave_scan(rest_n);
+        rest = sm_wave_scan(rest);
+        if (lane == 63) {
+            atomicAdd(&s.tail_n, rest_n);
+            atomicAdd(&s.tail, rest);
+        }
     }
     __syncthreads();
     if (tid == LAST) n = s.tail_n;
@@ -775,35 +831,47 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     /* ---- the bins where the limits and the pick may be: what comes before them and
      *      what comes through them bounds every sum ---- */
     const bool by_k = top_k > 0 && top_k < all;
-    int kb = LAST, pb0 = LAST, pb1 = LAST, mb = LAST;
-    if (by_k) kb = sm_first(SM_BINS, [&](int i) { return s.n[i] >= (uint32_t)top_k; });
-    u64 lo = by_k ? r.sum_before(kb) : s.sum[LAST], hi = s.sum[kb];
-    if (by_p) {
-        pb0 = min(kb, r.sum_bin(part_of(lo ? lo : 1)));
-        pb1 = min(kb, r.sum_bin(part_of(hi)));
+    if (tid < 64) {
+        int kb = LAST, pb0 = LAST, pb1 = LAST, mb = LAST;
+        if (by_k) kb = sm_first(SM_BINS, [&](int i) { return s.n[i] >= (uint32_t)top_k; });
+        u64 lo = by_k ? r.sum_before(kb) : s.sum[LAST], hi = s.sum[kb];
+        if (by_p) {
+            pb1 = min(kb, r.sum_bin(part_of(hi)));
+            pb0 = by_k ? min(kb, r.sum_bin(part_of(lo ? lo : 1))) : pb1;
+        }
+        /* the first bin whose lower edge is under the floor has the last that stays */
+        if (by_floor)
+            mb = min(sm_first(SM_BINS, [&](int i) {
+                         return sm_exp2(fmin((r.first - i) * (1.0 / 32.0) - zmost, 0.0)) <
+                                (double)floor_;
+                     }), LAST);
+        const int c0 = min(min(kb, pb0), mb), c1 = min(min(kb, pb1), mb);
+        /* listed are all bins up to the last cut, if they fit, else the ones that may be
+         * needed; top-k's is if it is the cut or top-p takes a part of its sum */
+        const bool need_k = by_k && (by_p || kb <= c1);
+        const int kn = need_k && kb > c1 ? (int)(s.n[kb] - r.n_before(kb)) : 0;
+        const bool whole = (int)s.n[c1] + kn <= SP_LIST;
+        int ub0 = 0, ub1 = c1;
+        if (!whole) {
+            if (by_k || by_p || by_floor) {
+                lo = max(r.sum_before(c0), 1ull);
+                hi = s.sum[c1];
+            }
+            ub0 = min(r.sum_bin(place_of(lo)), c1);
+            ub1 = min(r.sum_bin(place_of(hi)), c1);
+        }
+        if (tid == 0) s.where = SmWhere{kb, pb0, pb1, mb, c1, ub0, ub1, need_k, whole};
     }
-    /* the first bin whose lower edge is under the floor has the last that stays */
-    if (by_floor)
-        mb = min(sm_first(SM_BINS, [&](int i) {
-                     return sm_exp2(fmin((r.first - i) * (1.0 / 32.0) - zmost, 0.0)) < (double)floor_;
-                 }), LAST);
-    const int c0 = min(min(kb, pb0), mb), c1 = min(min(kb, pb1), mb);
-    if (by_k || by_p || by_floor) {
-        lo = max(r.sum_before(c0), 1ull);
-        hi = s.sum[c1];
-    }
-    const int ub0 = min(r.sum_bin(place_of(lo)), c1), ub1 = min(r.sum_bin(place_of(hi)), c1);
-    /* listed are all bins up to the last cut, if they fit, else the ones that may be
-     * needed; top-k's is if it is the cut or top-p takes a part of its sum */
-    const bool need_k = by_k && (by_p || kb <= c1);
-    const int kn = need_k && kb > c1 ? (int)(s.n[kb] - r.n_before(kb)) : 0;
-    const bool whole = (int)s.n[c1] + kn <= SP_LIST;
+    __syncthreads();
+    const SmWhere at = s.where;
+    const int kb = at.kb, pb0 = at.pb0, pb1 = at.pb1, mb = at.mb, ub0 = at.ub0, ub1 = at.ub1;
+    const bool need_k = at.need_k, whole = at.whole;
     const bool in = (need_k && tid == kb) ||
-                    (whole ? tid <= c1
+                    (whole ? tid <= at.c1
                            : (by_p && tid >= pb0 && tid <= pb1) || (by_floor && tid == mb) ||
                                  (tid >= ub0 && tid <= ub1));
     /* which lie in two ranges */
-    int b0 = 0, b1 = c1, b2 = need_k ? kb : 0, b3 = need_k ? kb : c1;
+    int b0 = 0, b1 = at.c1, b2 = need_k ? kb : 0, b3 = need_k ? kb : at.c1;
     if (!whole) {
         b0 = min(min(need_k ? kb : LAST, by_p ? pb0 : LAST), by_floor ? mb : LAST);
         b1 = max(max(need_k ? kb : 0, by_p ? pb1 : 0), by_floor ? mb : 0);
@@ -822,11 +890,12 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     /* key 0 is behind the whole bin */
     SmPlace cut{0, s.sum[LAST], LAST, all};
     if (listed <= SP_LIST && r.list(b0, b1, b2, b3, listed)) {
+        if (tid >= 64) return;
         auto place = [&](int b, int i) {
             return SmPlace{s.key[i], s.through[i], b, (int)r.n_before(b) + i - s.off[b] + 1};
         };
         /* the token of bin b that passes the sum, or the bin's last */
-        auto at = [&](int b, u64 need) {
+        auto token = [&](int b, u64 need) {
             const int off = s.off[b], end = off + (int)(s.n[b] - r.n_before(b)) - 1;
             const int i = sm_first(listed, [&](int j) { return s.through[j] >= need; });
             return place(b, min(max(i, off), end));
@@ -836,7 +905,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             const u64 need = part_of(cut.sum);
             const int b = min(max(r.sum_bin(need), pb0), pb1);
             if (s.off[b] >= 0) {                  /* else min_p cuts before it */
-                const SmPlace c = at(b, need);
+                const SmPlace c = token(b, need);
                 if (c.n < cut.n) cut = c;
             }
         }
@@ -852,7 +921,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             if (c.n < cut.n) cut = c;
         }
         const u64 need = place_of(cut.sum);
-        const SmPlace got = at(min(min(max(r.sum_bin(need), ub0), ub1), cut.bin), need);
+        const SmPlace got = token(min(min(max(r.sum_bin(need), ub0), ub1), cut.bin), need);
         if (tid == 0) {
             /* behind the cut only by the roundings of the bins' sums */
             const u64 best = got.n > cut.n ? cut.key : got.key;
