@@ -29,15 +29,14 @@ constexpr int RP_ROWS = 65536, RP_PREFIX_ROWS = 262144;  /* rows of sums      */
 
 /* What a batch's plan and workspace have room for. */
 struct ReqsRoom {
-    long long rows, items, blocks, parts;
+    long long rows, items, parts;
 };
 ReqsRoom reqs_room(int n_req, int max_tok, int h)
 {
     ReqsRoom m;
     m.rows = (long long)max_tok * h;
-    /* blocks of 64 rows, the fewest that a workgroup takes at most, or of 16 */
-    const long long few = m.rows / 16 + n_req, many = m.rows / 64 + n_req + RP_EXTRA;
-    m.blocks = few < many ? few : many;
+    /* blocks of 64 rows, the fewest that a workgroup takes at most, of the requests and
+     * of the prefix */
     m.items = 2 * (m.rows / 64) + n_req + 1 + RP_EXTRA;
     m.parts = RP_ROWS + (2 * m.rows < RP_PREFIX_ROWS ? 2 * m.rows : RP_PREFIX_ROWS);
     return m;
@@ -45,13 +44,13 @@ ReqsRoom reqs_room(int n_req, int max_tok, int h)
 
 struct PlanJob {
     Dsv4ReqsHead *head;
-    Dsv4ReqsBlock *blocks;
     Dsv4ReqsItem *items;
-    int2 *req;
+    Dsv4ReqsReq *req;
     const int *len, *first;
     int n_req, max_tok, h, window, prefix, room;  /* room: positions of a table */
+    IoDiv by_h;
     int br, br_split, per_cu, dvp;                /* most rows, waves a block of 16 */
-    int max_items, max_blocks, max_parts;
+    int max_items, max_parts;
     uint32_t sig;
 };
 
@@ -59,21 +58,6 @@ struct PlanJob {
 struct PlanReq {
     int n, pos, tile0, tile1;
 };
-__device__ __forceinline__ PlanReq plan_req(const PlanJob &a, int b, int prefix_tiles)
-{
-    PlanReq r;
-    r.n = a.first[b + 1] - a.first[b];
-    const int len = a.len[b];
-    r.pos = len - r.n;
-    const int lo = a.window ? max(0, r.pos - a.window + 1) : 0;
-    r.tile0 = max(prefix_tiles, lo / TR_TILE);
-    r.tile1 = max(r.tile0, (len + TR_TILE - 1) / TR_TILE);
-    return r;
-}
-__device__ __forceinline__ int plan_splits(int tiles, int each)
-{
-    return min((tiles + each - 1) / each, RP_SPLITS);
-}
 
 template <class V, class F>
 __device__ __forceinline__ V wave_all(V v, F f)
@@ -82,6 +66,17 @@ __device__ __forceinline__ V wave_all(V v, F f)
     for (int o = 32; o >= 1; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
     return v;
 }
+
+/* Tiles cut into items of about `each`: how many, to RP_SPLITS. A quotient of floats
+ * may be one off, which makes an item a little longer or shorter. */
+struct PlanCut {
+    float by;
+    __device__ __forceinline__ explicit PlanCut(int each) : by(1.0f / (float)each) {}
+    __device__ __forceinline__ int splits(int tiles) const
+    {
+        return tiles ? max(1, min((int)ceilf((float)tiles * by - 1e-3f), RP_SPLITS)) : 0;
+    }
+};
 
 /* One workgroup. A plan is: with the prefix apart or not, the rows of a block and
  * the tiles of an item. 64 of them are priced as dsv4_tree.hip prices its own (in
@@ -92,9 +87,10 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     extern __shared__ int lds[];
     __shared__ unsigned long long best, owner, work[8];
     __shared__ int bad, active, hi_min, lo_max, lo_min, longest[8];
-    __shared__ int part_w[RP_THREADS / 64][3];
+    __shared__ int part_w[RP_THREADS / 64][2];
     __shared__ int rows_each, tiles_each, tiles_from;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, nr = a.n_req;
+    int *s_first = lds, *s_len = lds + nr + 1, *s_item = s_len + nr, *s_part = s_item + nr + 1;
     if (tid == 0) {
         best = ~0ull;
         owner = 0;
@@ -105,48 +101,63 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         work[tid] = 0;
         longest[tid] = 0;
     }
+    for (int b = tid; b <= nr; b += RP_THREADS) {
+        s_first[b] = nr ? a.first[b] : 0;
+        if (b < nr) s_len[b] = a.len[b];
+    }
     __syncthreads();
-    const int tok0 = a.n_req ? a.first[0] : 0, tok1 = a.n_req ? a.first[a.n_req] : 0;
+    const int tok0 = s_first[0], tok1 = s_first[nr];
+    auto lo_of = [&](int pos) { return a.window ? max(0, pos - a.window + 1) : 0; };
+    auto request = [&](int b, int prefix_tiles) {
+        PlanReq r;
+        r.n = s_first[b + 1] - s_first[b];
+        r.pos = s_len[b] - r.n;
+        r.tile0 = max(prefix_tiles, lo_of(r.pos) / TR_TILE);
+        r.tile1 = max(r.tile0, (s_len[b] + TR_TILE - 1) / TR_TILE);
+        return r;
+    };
+    auto hi = [](auto x, auto y) { return x > y ? x : y; };
+    auto lo = [](auto x, auto y) { return x < y ? x : y; };
+    auto plus = [](auto x, auto y) { return x + y; };
     {
-        int b_bad = tok0 < 0 || tok1 > a.max_tok, n_act = 0, hmin = INT32_MAX, lmax = 0, lmin = INT32_MAX;
+        int b_bad = tok0 < 0 || tok1 > a.max_tok, n_act = 0, hmin = INT32_MAX, lmax = 0,
+            lmin = INT32_MAX;
         unsigned long long own = 0;
-        for (int b = tid; b < a.n_req; b += RP_THREADS) {
-            const int f0 = a.first[b], f1 = a.first[b + 1], len = a.len[b], n = f1 - f0;
+        for (int b = tid; b < nr; b += RP_THREADS) {
+            const int f0 = s_first[b], f1 = s_first[b + 1], len = s_len[b], n = f1 - f0;
             if (f0 < 0 || f1 < f0 || f1 > a.max_tok || (n && (len < n || len > a.room))) {
                 b_bad = 1;
                 continue;
             }
-            a.req[b] = int2{f0, len - n};
             if (!n) continue;
             n_act++;
             hmin = min(hmin, len - n + 1);
-            lmax = max(lmax, a.window ? max(0, len - a.window) : 0);
-            lmin = min(lmin, a.window ? max(0, len - n - a.window + 1) : 0);
+            lmax = max(lmax, lo_of(len - 1));
+            lmin = min(lmin, lo_of(len - n));
             const unsigned long long o = (unsigned long long)len << 32 | (uint32_t)b;
             own = o > own ? o : own;
         }
-        auto hi = [](auto x, auto y) { return x > y ? x : y; };
-        auto lo = [](auto x, auto y) { return x < y ? x : y; };
-        auto plus = [](int x, int y) { return x + y; };
-        b_bad = wave_all(b_bad, hi);
-        n_act = wave_all(n_act, plus);
-        hmin = wave_all(hmin, lo);
-        lmax = wave_all(lmax, hi);
-        lmin = wave_all(lmin, lo);
-        own = wave_all(own, hi);
-        if (lane == 0) {
-            if (b_bad) bad = 1;
-            atomicAdd(&active, n_act);
-            atomicMin(&hi_min, hmin);
-            atomicMax(&lo_max, lmax);
-            atomicMin(&lo_min, lmin);
-            atomicMax(&owner, own);
+        if ((tid & ~63) < nr) {                   /* a wave, whole or not at all */
+            b_bad = wave_all(b_bad, hi);
+            n_act = wave_all(n_act, plus);
+            hmin = wave_all(hmin, lo);
+            lmax = wave_all(lmax, hi);
+            lmin = wave_all(lmin, lo);
+            own = wave_all(own, hi);
+            if (lane == 0) {
+                if (b_bad) bad = 1;
+                atomicAdd(&active, n_act);
+                atomicMin(&hi_min, hmin);
+                atomicMax(&lo_max, lmax);
+                atomicMin(&lo_min, lmin);
+                atomicMax(&owner, own);
+            }
         }
     }
     __syncthreads();
     const int R0 = tok0 * a.h, R = (tok1 - tok0) * a.h;
     if (bad || active == 0) {
-        if (tid == 0) *a.head = Dsv4ReqsHead{bad ? ~a.sig : a.sig, 0, 0, 0, 0, 0, 0, 0};
+        if (tid == 0) *a.head = Dsv4ReqsHead{bad ? ~a.sig : a.sig, 0, 0, 0, 0, 0, {0, 0}};
         return;
     }
     /* whole tiles of the prefix, as far as the longest request has it */
@@ -154,22 +165,22 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     const int pt1 = min(a.prefix, max_len) / TR_TILE, pt0 = min(pt1, lo_min / TR_TILE);
     const bool may = active > 1 && pt1 > pt0;
 
-    /* group g (two waves): the prefix apart (g & 1), blocks of 16 << (g >> 1) rows */
-    const int g = tid >> 7, gt = tid & 127, r = 16 << (g >> 1);
+    /* group g (two waves): the prefix apart (g & 1), blocks of 1 << rs rows */
+    const int g = tid >> 7, gt = tid & 127, rs = 4 + (g >> 1), r = 1 << rs;
     const bool apart = g & 1, on = r <= a.br && (!apart || may);
     const int from = apart ? pt1 : 0, ptiles = apart ? pt1 - pt0 : 0;
-    const int pblocks = apart ? (R + r - 1) / r : 0;
+    const int pblocks = apart ? (R + r - 1) >> rs : 0;
     if (on) {
         unsigned long long w = 0;
         int l = ptiles;
-        for (int b = gt; b < a.n_req; b += 128) {
-            const PlanReq q = plan_req(a, b, from);
+        for (int b = gt; b < nr; b += 128) {
+            const PlanReq q = request(b, from);
             if (!q.n) continue;
-            w += (unsigned long long)((q.n * a.h + r - 1) / r) * (q.tile1 - q.tile0);
+            w += (unsigned long long)((q.n * a.h + r - 1) >> rs) * (q.tile1 - q.tile0);
             l = max(l, q.tile1 - q.tile0);
         }
-        w = wave_all(w, [](auto x, auto y) { return x + y; });
-        l = wave_all(l, [](int x, int y) { return max(x, y); });
+        w = wave_all(w, plus);
+        l = wave_all(l, hi);
         if (lane == 0) {
             atomicAdd(&work[g], w);
             atomicMax(&longest[g], l);
@@ -180,35 +191,33 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         /* tiles of an item, so that they are about so many workgroups' worth of the card */
         const int c = gt >> 4, cl = gt & 15;
         const unsigned long long w = work[g] + (unsigned long long)pblocks * ptiles;
-        constexpr int SHARE[7] = {128, 256, 384, 512, 768, 1024, 1536};
-        unsigned long long l = 1ull << 30;
-        if (c < 7) l = (w + SHARE[c] - 1) / SHARE[c];
-        const int each = (int)max(1ull, min(l, 1ull << 30));
-        unsigned long long items = 0, blocks = 0, parts = 0;
+        constexpr float SHARE[7] = {1.f / 128, 1.f / 256, 1.f / 384, 1.f / 512, 1.f / 768, 1.f / 1024,
+                                    1.f / 1536};
+        const int each = c < 7 ? max(1, (int)ceilf(fminf((float)w * SHARE[c], 1e9f))) : 1 << 30;
+        const PlanCut cut(each);
+        unsigned long long items = 0, parts = 0;
         if (on) {
-            for (int b = cl; b < a.n_req; b += 16) {
-                const PlanReq q = plan_req(a, b, from);
+            for (int b = cl; b < nr; b += 16) {
+                const PlanReq q = request(b, from);
                 if (!q.n) continue;
-                const int rows = q.n * a.h, nb = (rows + r - 1) / r;
-                int ns = plan_splits(q.tile1 - q.tile0, each);
+                const int rows = q.n * a.h;
+                int ns = cut.splits(q.tile1 - q.tile0);
                 if (!apart && ns < 1) ns = 1;
-                items += (unsigned long long)nb * ns;
-                blocks += nb;
+                items += (unsigned long long)((rows + r - 1) >> rs) * ns;
                 if (apart || ns > 1) parts += (unsigned long long)ns * rows;
             }
         }
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) {
             items += __shfl_xor(items, o, 64);
-            blocks += __shfl_xor(blocks, o, 64);
             parts += __shfl_xor(parts, o, 64);
         }
-        const int ps = plan_splits(ptiles, each);
+        const int ps = cut.splits(ptiles);
         items += (unsigned long long)pblocks * ps;
-        parts += (unsigned long long)ps * R * apart;
+        parts += (unsigned long long)ps * R;
         if (on && cl == 0 && items <= (unsigned long long)a.max_items &&
-            blocks <= (unsigned long long)a.max_blocks && parts <= (unsigned long long)a.max_parts) {
-            const int waves = r / 16 * a.br_split;
+            parts <= (unsigned long long)a.max_parts) {
+            const int waves = (r >> 4) * a.br_split;
             const float tile = waves > 4 ? 3.0f : 2.0f, start = 8.0f + 2.0f * waves;
             const float slots = 256.0f * a.per_cu, n = (float)items;
             const float one = (float)min(each, longest[g]) * tile + start;
@@ -221,96 +230,72 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         }
         __syncthreads();
         if ((int)(best & 63) == (g << 3 | c) && cl == 0) {
-            rows_each = r;
+            rows_each = rs;
             tiles_each = each;
             tiles_from = from;
         }
         __syncthreads();
     }
-    const int br = rows_each, each = tiles_each, start = tiles_from;
-    const int ps = start ? plan_splits(pt1 - pt0, each) : 0;
-    const int pb = start ? (R + br - 1) / br : 0, pitems = ps * pb;
+    const int bs = rows_each, br = 1 << bs, start = tiles_from;
+    const PlanCut cut(tiles_each);
+    const int ps = start ? cut.splits(pt1 - pt0) : 0;
+    const int pb = start ? (R + br - 1) >> bs : 0, pitems = ps * pb;
 
-    /* where each request's items, blocks and sums begin */
-    int *s_item = lds, *s_block = lds + a.n_req + 1, *s_part = s_block + a.n_req + 1;
-    const int per = (a.n_req + RP_THREADS - 1) / RP_THREADS;
-    const int b0 = min(a.n_req, tid * per), b1 = min(a.n_req, b0 + per);
-    auto cut = [&](int b, int *n) {               /* items, blocks, rows of sums */
-        const PlanReq q = plan_req(a, b, start);
-        n[0] = n[1] = n[2] = 0;
-        if (!q.n) return;
-        const int rows = q.n * a.h;
-        int ns = plan_splits(q.tile1 - q.tile0, each);
-        if (!start && ns < 1) ns = 1;
-        n[1] = (rows + br - 1) / br;
-        n[0] = n[1] * ns;
-        n[2] = start || ns > 1 ? ns * rows : 0;
+    /* where each request's items and sums begin */
+    const int per = (nr + RP_THREADS - 1) / RP_THREADS;
+    const int b0 = min(nr, tid * per), b1 = min(nr, b0 + per);
+    auto splits = [&](const PlanReq &q) {
+        const int ns = cut.splits(q.tile1 - q.tile0);
+        return start ? ns : max(ns, 1);
     };
-    int sum[3] = {0, 0, 0};
+    int sum[2] = {0, 0};
     for (int b = b0; b < b1; b++) {
-        int n[3];
-        cut(b, n);
-        for (int k = 0; k < 3; k++) sum[k] += n[k];
+        const PlanReq q = request(b, start);
+        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0;
+        sum[0] += ((rows + br - 1) >> bs) * ns;
+        sum[1] += start || ns > 1 ? ns * rows : 0;
     }
-    int x[3] = {sum[0], sum[1], sum[2]};
+    int x[2] = {sum[0], sum[1]};
 #pragma unroll
     for (int o = 1; o < 64; o *= 2)
 #pragma unroll
-        for (int k = 0; k < 3; k++) {
+        for (int k = 0; k < 2; k++) {
             const int v = __shfl_up(x[k], o, 64);
             if (lane >= o) x[k] += v;
         }
     if (lane == 63)
-        for (int k = 0; k < 3; k++) part_w[tid >> 6][k] = x[k];
+        for (int k = 0; k < 2; k++) part_w[tid >> 6][k] = x[k];
     __syncthreads();
-    for (int k = 0; k < 3; k++) {
-        x[k] -= sum[k];
-        for (int w = 0; w < tid >> 6; w++) x[k] += part_w[w][k];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        /* the waves before this one */
+        int v = lane < tid >> 6 ? part_w[lane & (RP_THREADS / 64 - 1)][k] : 0;
+#pragma unroll
+        for (int o = RP_THREADS / 128; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+        x[k] += __builtin_amdgcn_readfirstlane(v) - sum[k];
     }
-    x[2] += ps * R;
+    x[1] += ps * R;
     for (int b = b0; b < b1; b++) {
-        int n[3];
-        cut(b, n);
+        const PlanReq q = request(b, start);
+        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0;
+        const bool direct = !start && ns <= 1;
         s_item[b] = x[0];
-        s_block[b] = x[1];
-        s_part[b] = x[2];
-        for (int k = 0; k < 3; k++) x[k] += n[k];
+        s_part[b] = direct ? -1 : x[1];
+        a.req[b] = Dsv4ReqsReq{s_first[b], q.pos, s_part[b], q.n << 8 | ns};
+        x[0] += ((rows + br - 1) >> bs) * ns;
+        x[1] += direct ? 0 : ns * rows;
     }
-    if (b0 < b1 && b1 == a.n_req) {
-        s_item[b1] = x[0];
-        s_block[b1] = x[1];
-    }
+    if (b0 < b1 && b1 == nr) s_item[b1] = x[0];
     __syncthreads();
-    const int items = s_item[a.n_req], blocks = s_block[a.n_req];
+    const int items = s_item[nr];
     if (tid == 0)
-        *a.head = Dsv4ReqsHead{a.sig, pitems + items, pitems, blocks, ps, R0, R, 0};
-    auto owner_of = [&](const int *base, int i) { /* the request with number i */
-        int lo = 0, hi = a.n_req;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (base[mid] <= i) lo = mid;
-            else hi = mid;
-        }
-        return lo;
-    };
-    /* (a request without items or blocks has the next one's numbers: the search ends
-     * at the last of them, which has some) */
-    for (int i = tid; i < blocks; i += RP_THREADS) {
-        const int b = owner_of(s_block, i), blk = i - s_block[b];
-        const PlanReq q = plan_req(a, b, start);
-        const int rows = q.n * a.h;
-        int ns = plan_splits(q.tile1 - q.tile0, each);
-        if (!start && ns < 1) ns = 1;
-        const bool direct = !start && ns == 1;
-        a.blocks[i] = Dsv4ReqsBlock{a.first[b] * a.h + blk * br, min(br, rows - blk * br),
-                                    direct ? -1 : s_part[b] + blk * br, rows, ns, {0, 0, 0}};
-    }
+        *a.head = Dsv4ReqsHead{a.sig, pitems + items, pitems, ps, R0, R, {0, 0}};
     const bool all_see = hi_min >= pt1 * TR_TILE && lo_max == 0;
     for (int i = tid; i < pitems; i += RP_THREADS) {
         const int s = i / pb, blk = i - s * pb;
         Dsv4ReqsItem it{};
-        it.row0 = R0 + blk * br;
-        it.rows = min(br, R - blk * br);
+        it.row0 = R0 + (blk << bs);
+        it.rows = min(br, R - (blk << bs));
         it.req = (int)(uint32_t)owner;
         it.tile0 = pt0 + (int)((long long)(pt1 - pt0) * s / ps);
         it.tile1 = pt0 + (int)((long long)(pt1 - pt0) * (s + 1) / ps);
@@ -318,128 +303,180 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         it.lo = all_see ? 0 : lo_max;
         it.hi = all_see ? INT32_MAX : hi_min;
         it.kind = all_see ? 0 : 2;
-        it.part = s * R + blk * br;
+        it.part = s * R + (blk << bs);
         a.items[i] = it;
     }
     for (int i = tid; i < items; i += RP_THREADS) {
-        const int b = owner_of(s_item, i), k = i - s_item[b];
-        const PlanReq q = plan_req(a, b, start);
-        const int rows = q.n * a.h, nb = (rows + br - 1) / br, s = k / nb, blk = k - s * nb;
-        const int ns = (s_item[b + 1] - s_item[b]) / nb;
+        int b = 0, end = nr;                      /* the last request that starts here or
+                                                   * before (one without items has the
+                                                   * next one's number) */
+        while (end - b > 1) {
+            const int mid = (b + end) >> 1;
+            if (s_item[mid] <= i) b = mid;
+            else end = mid;
+        }
+        const PlanReq q = request(b, start);
+        const int rows = q.n * a.h, nb = (rows + br - 1) >> bs, ns = splits(q);
+        const int k = i - s_item[b], s = nb == 1 ? k : k / nb, r0 = (k - s * nb) << bs;
         Dsv4ReqsItem it{};
-        it.rows = min(br, rows - blk * br);
-        it.row0 = a.first[b] * a.h + blk * br;
+        it.rows = min(br, rows - r0);
+        it.row0 = s_first[b] * a.h + r0;
         it.req = b;
         /* a block's first and last tokens bound what its rows see */
-        const int p0 = q.pos + blk * br / a.h, p1 = q.pos + (blk * br + it.rows - 1) / a.h;
-        const int t0 = max(q.tile0, a.window ? max(0, p0 - a.window + 1) / TR_TILE : 0);
-        const int t1 = max(t0, p1 / TR_TILE + 1);
+        const int p0 = q.pos + (int)a.by_h.div((uint32_t)r0);
+        const int p1 = q.pos + (int)a.by_h.div((uint32_t)(r0 + it.rows - 1));
+        const int t0 = max(q.tile0, lo_of(p0) / TR_TILE), t1 = max(t0, p1 / TR_TILE + 1);
         it.tile0 = t0 + (int)((long long)(t1 - t0) * s / ns);
         it.tile1 = t0 + (int)((long long)(t1 - t0) * (s + 1) / ns);
         it.end = p1 + 1;
-        it.lo = a.window ? max(0, p1 - a.window + 1) : 0;
+        it.lo = lo_of(p1);
         it.hi = p0 + 1;
         it.kind = 1;
         it.pos0 = p0;
-        it.part = !start && ns == 1 ? -1 : s_part[b] + s * rows + blk * br;
+        it.part = s_part[b] < 0 ? -1 : s_part[b] + s * rows + r0;
         a.items[pitems + i] = it;
     }
 }
 
 constexpr int RJ_THREADS = 256, RJ_WAVES = RJ_THREADS / 64;
+constexpr int RJ_ROWS = 2048;
 
 struct JoinJob {
     const Dsv4ReqsHead *head;
-    const Dsv4ReqsBlock *blocks;
+    const Dsv4ReqsReq *req;
     const float *part, *pm, *pl, *sink;
-    int h, dv, dvp, ovec;
+    int n_req, h, dv, dvp, ovec;
     long long rows;                               /* of the whole buffer     */
+    IoDiv by_h;
     uint32_t sig;
 };
 
-/* Rows of a block whose sums lie in several places: the prefix's splits and then
- * the request's. Every wave has the weights, and adds every fourth place. */
-template <class T>
+/* Rows whose sums lie in several places: the prefix's splits and then the request's.
+ * WAVES waves a row: each has the weights, and adds every WAVES-th place. */
+template <class T, int WAVES>
 __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
 {
-    __shared__ f32x4 sum[RJ_WAVES][TR_DV / 4];
+    __shared__ f32x4 sum[WAVES][TR_DV / 4];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = WAVES > 1 ? wave : 0;
     const Dsv4ReqsHead hd = *a.head;
     if (hd.sig != a.sig) {                        /* not this call's plan    */
         const float nan = __uint_as_float(0x7FC00000u);
-        const long long n = a.rows * a.dv, step = (long long)gridDim.x * gridDim.y * RJ_THREADS;
-        for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RJ_THREADS + tid;
-             i < n; i += step)
+        const long long n = a.rows * a.dv, step = (long long)gridDim.x * RJ_THREADS;
+        for (long long i = (long long)blockIdx.x * RJ_THREADS + tid; i < n; i += step)
             io_store<T, 1>(o + i, &nan);
         return;
     }
-    if ((int)blockIdx.x >= hd.blocks) return;
-    const Dsv4ReqsBlock b = a.blocks[blockIdx.x];
-    if (b.part < 0) return;
-    const int ps = hd.prefix_splits, n = ps + b.splits;
-    for (int i = blockIdx.y; i < b.rows; i += gridDim.y) {
-        const int r = b.row0 + i;
-        auto place = [&](int s) {
-            return s < ps ? (size_t)s * hd.rows + (r - hd.row0)
-                          : (size_t)b.part + (size_t)(s - ps) * b.stride + i;
-        };
-        constexpr int NK = (2 * RP_SPLITS + 63) / 64;
-        float ms[NK], ls[NK], m = -INFINITY, l = 0.0f;
+    const int i = WAVES > 1 ? (int)blockIdx.x : (int)blockIdx.x * RJ_WAVES + wave;
+    if (i >= hd.rows) return;
+    const int r = hd.row0 + i, t = (int)a.by_h.div((uint32_t)r);
+    /* the last request whose first token is t or before it: of every step-th one, then
+     * of those behind it */
+    const int step = (a.n_req + 63) / 64;
+    int b = 0;
+    for (int s = step; s >= 1; s = s > 1 ? 1 : 0) {
+        const int k = b + lane * s;
+        const unsigned long long before =
+            __ballot(lane < (s > 1 ? 64 : step > 1 ? step : 64) && k < a.n_req &&
+                     a.req[min(k, a.n_req - 1)].first <= t);
+        b += (63 - (int)__builtin_clzll(before | 1)) * s;
+    }
+    const Dsv4ReqsReq q = a.req[b];
+    if (q.part < 0) return;
+    const int ps = hd.prefix_splits, n = ps + (q.cut & 255), rows = (q.cut >> 8) * a.h;
+    const size_t own = (size_t)q.part + (r - q.first * a.h);
+    auto place = [&](int s) {
+        return s < ps ? (size_t)s * hd.rows + i : own + (size_t)(s - ps) * rows;
+    };
+    constexpr int NK = (2 * RP_SPLITS + 63) / 64;
+    float ms[NK], ls[NK], m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            const int s = 64 * k + lane;
-            ms[k] = -INFINITY;
-            ls[k] = 0.0f;
-            if (64 * k < n && s < n) {
-                ms[k] = a.pm[place(s)];
-                ls[k] = a.pl[place(s)];
-            }
-            m = fmaxf(m, ms[k]);
+    for (int k = 0; k < NK; k++) {
+        const int s = 64 * k + lane;
+        ms[k] = -INFINITY;
+        ls[k] = 0.0f;
+        if (64 * k < n && s < n) {
+            ms[k] = a.pm[place(s)];
+            ls[k] = a.pl[place(s)];
         }
-        m = wave_max(m);
+        m = fmaxf(m, ms[k]);
+    }
+    m = wave_max(m);
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            if (64 * k >= n) break;
-            ms[k] = tree_join_weight(ms[k], ls[k], m);
-            l += ms[k] * ls[k];
-        }
-        l = wave_sum(l);
-        if (a.sink && l != 0.0f)
-            l += __builtin_amdgcn_exp2f(a.sink[r % a.h] * 1.44269504088896340736f - m);
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    for (int k = 0; k < NK; k++) {
+        if (64 * k >= n) break;
+        ms[k] = tree_join_weight(ms[k], ls[k], m);
+        l += ms[k] * ls[k];
+    }
+    l = wave_sum(l);
+    if (a.sink && l != 0.0f)
+        l += __builtin_amdgcn_exp2f(a.sink[r - t * a.h] * 1.44269504088896340736f - m);
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    constexpr int G = 4;                          /* places in flight        */
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            if (64 * k >= n) break;
-            for (int s = 64 * k + w; s < min(n, 64 * k + 64); s += RJ_WAVES) {
-                const float e = __shfl(ms[k], s & 63, 64);
-                const float *p = a.part + place(s) * a.dvp + 4 * lane;
+    for (int k = 0; k < NK; k++) {
+        if (64 * k >= n) break;
+        const int end = min(n, 64 * k + 64);
+        for (int s0 = 64 * k + w; s0 < end; s0 += G * WAVES) {
+            f32x4 x[G][2];
+#pragma unroll
+            for (int u = 0; u < G; u++) {
+                const float *p = a.part + place(min(s0 + u * WAVES, n - 1)) * a.dvp + 4 * lane;
 #pragma unroll
                 for (int c = 0; c < 2; c++)
-                    if (256 * c + 4 * lane < a.dvp) v[c] += e * ldf4(p + 256 * c);
+                    x[u][c] = 256 * c + 4 * lane < a.dvp ? ldf4(p + 256 * c)
+                                                         : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < G; u++) {
+                const int s = s0 + u * WAVES;
+                const float e = __shfl(ms[k], s & 63, 64);
+                if (s < end)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) v[c] += e * x[u][c];
             }
         }
+    }
+    auto store = [&](int c, f32x4 y4) {
+        if (c >= a.dv) return;
+        y4 = y4 * inv;
+        const float y[4] = {y4.x, y4.y, y4.z, y4.w};
+        T *d = o + (size_t)r * a.dv + c;
+        if (a.ovec) {
+            io_store<T, 4>(d, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
+        }
+    };
+    if constexpr (WAVES == 1) {
+        store(4 * lane, v[0]);
+        store(256 + 4 * lane, v[1]);
+    } else {
         sum[w][lane] = v[0];
         sum[w][64 + lane] = v[1];
         __syncthreads();
-        if (tid < TR_DV / 4 && 4 * tid < a.dv) {
-            f32x4 t = sum[0][tid];
+        if (tid < TR_DV / 4) {
+            f32x4 y = sum[0][tid];
 #pragma unroll
-            for (int k = 1; k < RJ_WAVES; k++) t += sum[k][tid];
-            t = t * inv;
-            const float y[4] = {t.x, t.y, t.z, t.w};
-            T *d = o + (size_t)r * a.dv + 4 * tid;
-            if (a.ovec) {
-                io_store<T, 4>(d, y);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (4 * tid + e < a.dv) io_store<T, 1>(d + e, y + e);
-            }
+            for (int k = 1; k < WAVES; k++) y += sum[k][tid];
+            store(4 * tid, y);
         }
-        __syncthreads();
     }
+}
+
+/* A wave a row where the rows fill the card. */
+template <class T>
+void join_launch(const JoinJob &a, T *o, hipStream_t st)
+{
+    if (a.rows >= RJ_ROWS)
+        hipLaunchKernelGGL((k_reqs_join<T, 1>), dim3((unsigned)((a.rows + RJ_WAVES - 1) / RJ_WAVES)),
+                           dim3(RJ_THREADS), 0, st, a, o);
+    else
+        hipLaunchKernelGGL((k_reqs_join<T, RJ_WAVES>), dim3((unsigned)a.rows), dim3(RJ_THREADS), 0, st,
+                           a, o);
 }
 
 /* What is wrong with a call's shape, or nullptr. */
@@ -474,16 +511,15 @@ uint32_t reqs_sig(const dsv4_gpu_reqs *r, int fmt, int h, int d_qk, int d_v, int
 }
 
 struct PlanParts {
-    size_t blocks, items, req, bytes;
+    size_t items, req, bytes;
 };
 PlanParts plan_parts(int n_req, int max_tok, int h)
 {
     const ReqsRoom m = reqs_room(n_req, max_tok, h);
     PlanParts p;
-    p.blocks = 64;
-    p.items = p.blocks + (size_t)m.blocks * sizeof(Dsv4ReqsBlock);
+    p.items = 64;
     p.req = p.items + (size_t)m.items * sizeof(Dsv4ReqsItem);
-    p.bytes = (p.req + (size_t)n_req * sizeof(int2) + 15) / 16 * 16;
+    p.bytes = p.req + (size_t)n_req * sizeof(Dsv4ReqsReq);
     return p;
 }
 static_assert(sizeof(Dsv4ReqsHead) <= 64, "the plan's head");
@@ -529,11 +565,10 @@ extern "C" int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_
     const ReqsRoom m = reqs_room(r->n_req, r->max_tok, h);
     const int kc = dsv4_tree_chunks(d_qk, d_v);
     char *p = (char *)d_plan;
-    PlanJob a{};
+    PlanJob a{.by_h = IoDiv((uint32_t)h)};
     a.head = (Dsv4ReqsHead *)p;
-    a.blocks = (Dsv4ReqsBlock *)(p + pp.blocks);
     a.items = (Dsv4ReqsItem *)(p + pp.items);
-    a.req = (int2 *)(p + pp.req);
+    a.req = (Dsv4ReqsReq *)(p + pp.req);
     a.len = r->len;
     a.first = r->first;
     a.n_req = r->n_req;
@@ -547,11 +582,19 @@ extern "C" int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_
     a.per_cu = tree_per_cu(fmt, kc);
     a.dvp = (d_v + 15) / 16 * 16;
     a.max_items = (int)m.items;
-    a.max_blocks = (int)m.blocks;
     a.max_parts = (int)m.parts;
     a.sig = reqs_sig(r, fmt, h, d_qk, d_v, kv_fmt, window);
-    hipLaunchKernelGGL(k_reqs_plan, dim3(1), dim3(RP_THREADS),
-                       3 * ((size_t)r->n_req + 1) * sizeof(int), (hipStream_t)stream, a);
+    const size_t lds = 4 * ((size_t)r->n_req + 1) * sizeof(int);
+    if (lds > 64 * 1024 - 1024) {
+        static bool asked[64];
+        int dev = 0;
+        HIP_OK(hipGetDevice(&dev), "hipGetDevice");
+        if (dev < 0 || dev >= 64 || !asked[dev]) {
+            (void)dsv4_lds_optin((const void *)k_reqs_plan, 4 * 4097 * sizeof(int), "reqs plan");
+            if (dev >= 0 && dev < 64) asked[dev] = true;
+        }
+    }
+    hipLaunchKernelGGL(k_reqs_plan, dim3(1), dim3(RP_THREADS), lds, (hipStream_t)stream, a);
     HIP_OK(hipGetLastError(), "reqs plan launch");
     return 0;
 }
@@ -614,7 +657,7 @@ extern "C" int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, 
     a.ovec = d_v % 4 == 0 && (uintptr_t)d_o % (4 * es) == 0;
     a.head = (const Dsv4ReqsHead *)p;
     a.items = (const Dsv4ReqsItem *)(p + pp.items);
-    a.req = (const int2 *)(p + pp.req);
+    a.req = (const Dsv4ReqsReq *)(p + pp.req);
     a.n_req = r->n_req;
     a.sig = reqs_sig(r, fmt, h, d_qk, d_v, kv_fmt, window);
     hipStream_t st = (hipStream_t)stream;
@@ -627,15 +670,10 @@ extern "C" int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, 
                      ? dsv4_reqs_bf16_launch(a, fmt, kc, (unsigned)groups, st)
                      : dsv4_reqs_fp8_launch(a, fmt, kc, (unsigned)groups, st);
     if (rc != 0) return rc;
-    const JoinJob j{a.head, (const Dsv4ReqsBlock *)(p + pp.blocks), a.part, a.pm, a.pl, d_sink, h,
-                    d_v, a.dvp, a.ovec, m.rows, a.sig};
-    const long long y = 4096 / m.blocks;
-    const dim3 grid((unsigned)m.blocks, (unsigned)(y < 8 ? 8 : y > 64 ? 64 : y));
-    if (fmt == DSV4_WF32)
-        hipLaunchKernelGGL(k_reqs_join<float>, grid, dim3(RJ_THREADS), 0, st, j, (float *)d_o);
-    else
-        hipLaunchKernelGGL(k_reqs_join<uint16_t>, grid, dim3(RJ_THREADS), 0, st, j,
-                           (uint16_t *)d_o);
+    const JoinJob j{a.head, a.req, a.part, a.pm, a.pl, d_sink, r->n_req, h, d_v, a.dvp, a.ovec, m.rows,
+                    IoDiv((uint32_t)h), a.sig};
+    if (fmt == DSV4_WF32) join_launch(j, (float *)d_o, st);
+    else join_launch(j, (uint16_t *)d_o, st);
     HIP_OK(hipGetLastError(), "reqs join launch");
     return 0;
 }

@@ -42,21 +42,22 @@ struct Dsv4TreeJob {
 struct Dsv4ReqsItem {
     int row0, rows, req, tile0, tile1, end, lo, hi, kind, pos0, part, pad;
 };
-/* What a plan begins with: the number of items, those of the prefix first, of blocks
- * of rows, and the signature of the arguments it was made for. */
+/* What a plan begins with: the number of items, those of the prefix first, the rows of
+ * all requests, and the signature of the arguments it was made for. */
 struct Dsv4ReqsHead {
     uint32_t sig;
-    int items, prefix_items, blocks;
-    int prefix_splits, row0, rows, pad;           /* all requests' rows      */
+    int items, prefix_items, prefix_splits;
+    int row0, rows, pad[2];
 };
-/* A block of rows: its own splits' sums at part, `stride` rows apart. */
-struct Dsv4ReqsBlock {
-    int row0, rows, part, stride, splits, pad[3];
+/* A request: its first token and that one's position, where the sums of its own splits
+ * are (-1: its items wrote the result), and its tokens << 8 | splits. */
+struct Dsv4ReqsReq {
+    int first, pos, part, cut;
 };
 struct Dsv4ReqsJob : Dsv4TreeJob {
     const Dsv4ReqsHead *head;
     const Dsv4ReqsItem *items;
-    const int2 *req;                              /* first token, its position */
+    const Dsv4ReqsReq *req;
     int n_req;
     uint32_t sig;
 };
@@ -617,10 +618,10 @@ k_tree(JOB a)
                     int r0 = 0, r1 = a.n_req;
                     while (r1 - r0 > 1) {
                         const int mid = (r0 + r1) >> 1;
-                        if (a.req[mid].x <= t) r0 = mid;
+                        if (a.req[mid].first <= t) r0 = mid;
                         else r1 = mid;
                     }
-                    pos = a.req[r0].y + t - a.req[r0].x;
+                    pos = a.req[r0].pos + t - a.req[r0].first;
                 }
                 hi = pos + 1;
                 lo = a.window ? max(0, pos - a.window + 1) : 0;
