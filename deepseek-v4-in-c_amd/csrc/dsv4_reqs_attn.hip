@@ -24,6 +24,7 @@ namespace {
 
 constexpr int RP_THREADS = 1024;
 constexpr int RP_SPLITS = 255;                    /* most of a request's, or of the prefix */
+constexpr int RP_KINDS = DSV4_REQS_KINDS - 1;      /* of the requests' items, by length */
 constexpr int RP_EXTRA = 1024;                    /* items for splits        */
 constexpr int RP_ROWS = 65536, RP_PREFIX_ROWS = 262144;  /* rows of sums      */
 
@@ -50,6 +51,7 @@ struct PlanJob {
     int n_req, max_tok, h, window, prefix, room;  /* room: positions of a table */
     IoDiv by_h;
     int br, br_split, per_cu, dvp;                /* most rows, waves a block of 16 */
+    float inv_h, tile_us, wave_more;                     /* a tile's time, and how a wave of rows adds */
     int max_items, max_parts;
     uint32_t sig;
 };
@@ -78,29 +80,31 @@ struct PlanCut {
     }
 };
 
-/* One workgroup. A plan is: with the prefix apart or not, the rows of a block and
- * the tiles of an item. 64 of them are priced as dsv4_tree.hip prices its own (in
- * halves of the time of a tile on a lone wave), the workgroups as rounds of the card
- * or as a stream of items that ends with the longest, whichever is less. */
+/* One workgroup. A plan is: with the prefix apart or not, the rows of a block and the
+ * tiles of an item. 128 of them are priced in microseconds: a tile takes what its loads and
+ * the waits between them take, whatever rows of q it serves (1.65 us for 16, 32 and 64 rows
+ * of bf16, 576 columns), 2.2 and half a microsecond a wave of 16 rows are an item's start,
+ * and then come the sums that are joined. Workgroups begin in their order, and those of
+ * one XCD go to its four engines in turn, so the longest items come first and the short ones
+ * fill what the last round of these leaves free, if every engine has a free CU. */
 __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 {
     extern __shared__ int lds[];
-    __shared__ unsigned long long best, owner, work[8];
+    __shared__ unsigned long long best, owner;
+    __shared__ float work[2 * 8];
     __shared__ int bad, active, hi_min, lo_max, lo_min, longest[8];
-    __shared__ int part_w[RP_THREADS / 64][2];
-    __shared__ int rows_each, tiles_each, tiles_from;
+    __shared__ int part_w[RP_THREADS / 64][2 + RP_KINDS];
+    __shared__ int rows_each, tiles_each, tiles_from, longest_own;
     const int tid = threadIdx.x, lane = tid & 63, nr = a.n_req;
-    int *s_first = lds, *s_len = lds + nr + 1, *s_item = s_len + nr, *s_part = s_item + nr + 1;
+    int *s_first = lds, *s_len = lds + nr + 1, *s_item = s_len + nr, *s_part = s_item + nr + 1,
+        *s_to = s_part + nr;                      /* four a request */
     if (tid == 0) {
         best = ~0ull;
         owner = 0;
         bad = active = lo_max = 0;
         hi_min = lo_min = INT32_MAX;
     }
-    if (tid < 8) {
-        work[tid] = 0;
-        longest[tid] = 0;
-    }
+    if (tid < 8) longest[tid] = 0;
     for (int b = tid; b <= nr; b += RP_THREADS) {
         s_first[b] = nr ? a.first[b] : 0;
         if (b < nr) s_len[b] = a.len[b];
@@ -115,6 +119,13 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         r.tile0 = max(prefix_tiles, lo_of(r.pos) / TR_TILE);
         r.tile1 = max(r.tile0, (s_len[b] + TR_TILE - 1) / TR_TILE);
         return r;
+    };
+    /* tiles of a request's block on average: an earlier one ends earlier, and with a window
+     * one of more rows begins earlier */
+    auto mean_tiles = [&](const PlanReq &q, int rows) {
+        const int t = q.tile1 - q.tile0;
+        const float less = fmaxf((float)q.n - (float)rows * a.inv_h, 0.0f);
+        return t ? fmaxf((float)t - less * (a.window ? 1.0f / TR_TILE : 0.5f / TR_TILE), 1.0f) : 0.0f;
     };
     auto hi = [](auto x, auto y) { return x > y ? x : y; };
     auto lo = [](auto x, auto y) { return x < y ? x : y; };
@@ -157,7 +168,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     __syncthreads();
     const int R0 = tok0 * a.h, R = (tok1 - tok0) * a.h;
     if (bad || active == 0) {
-        if (tid == 0) *a.head = Dsv4ReqsHead{bad ? ~a.sig : a.sig, 0, 0, 0, 0, 0, {0, 0}};
+        if (tid == 0) *a.head = Dsv4ReqsHead{bad ? ~a.sig : a.sig, {}, 0, 0, 0};
         return;
     }
     /* whole tiles of the prefix, as far as the longest request has it */
@@ -171,68 +182,79 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     const int from = apart ? pt1 : 0, ptiles = apart ? pt1 - pt0 : 0;
     const int pblocks = apart ? (R + r - 1) >> rs : 0;
     if (on) {
-        unsigned long long w = 0;
+        float w = 0.0f;
         int l = ptiles;
         for (int b = gt; b < nr; b += 128) {
             const PlanReq q = request(b, from);
             if (!q.n) continue;
-            w += (unsigned long long)((q.n * a.h + r - 1) >> rs) * (q.tile1 - q.tile0);
+            w += (float)((q.n * a.h + r - 1) >> rs) * mean_tiles(q, r);
             l = max(l, q.tile1 - q.tile0);
         }
         w = wave_all(w, plus);
         l = wave_all(l, hi);
         if (lane == 0) {
-            atomicAdd(&work[g], w);
+            work[tid >> 6] = w;
             atomicMax(&longest[g], l);
         }
     }
     __syncthreads();
     {
         /* tiles of an item, so that they are about so many workgroups' worth of the card */
-        const int c = gt >> 4, cl = gt & 15;
-        const unsigned long long w = work[g] + (unsigned long long)pblocks * ptiles;
-        constexpr float SHARE[7] = {1.f / 128, 1.f / 256, 1.f / 384, 1.f / 512, 1.f / 768, 1.f / 1024,
-                                    1.f / 1536};
-        const int each = c < 7 ? max(1, (int)ceilf(fminf((float)w * SHARE[c], 1e9f))) : 1 << 30;
+        const int c = gt >> 3, cl = gt & 7;
+        constexpr float SHARE[16] = {96,  128, 192, 208, 224, 256, 320, 416, 448, 480, 512, 640, 704,
+                                     960, 1472, 0};
+        const float w = work[2 * g] + work[2 * g + 1] + (float)pblocks * (float)ptiles;
+        const int each = c < 15 ? max(1, (int)ceilf(fminf(w / SHARE[c], 1e9f))) : 1 << 30;
+        const int most = min(each, longest[g]), ps = PlanCut(each).splits(ptiles);
         const PlanCut cut(each);
+        const float half = 0.5f * (float)most;
         unsigned long long items = 0, parts = 0;
+        float big = 0.0f;                         /* items of half the longest or more */
         if (on) {
-            for (int b = cl; b < nr; b += 16) {
+            for (int b = cl; b < nr; b += 8) {
                 const PlanReq q = request(b, from);
                 if (!q.n) continue;
-                const int rows = q.n * a.h;
-                int ns = cut.splits(q.tile1 - q.tile0);
+                const int rows = q.n * a.h, t = q.tile1 - q.tile0;
+                int ns = cut.splits(t);
                 if (!apart && ns < 1) ns = 1;
-                items += (unsigned long long)((rows + r - 1) >> rs) * ns;
+                const int n = ((rows + r - 1) >> rs) * ns;
+                items += (unsigned)n;
                 if (apart || ns > 1) parts += (unsigned long long)ns * rows;
+                const float spread = fmaxf(2.0f * ((float)t - mean_tiles(q, r)), 1e-3f);
+                big += (float)n * fminf(fmaxf(((float)t - half * ns) / spread, 0.0f), 1.0f);
             }
         }
 #pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) {
+        for (int o = 4; o >= 1; o >>= 1) {
             items += __shfl_xor(items, o, 64);
             parts += __shfl_xor(parts, o, 64);
+            big += __shfl_xor(big, o, 64);
         }
-        const int ps = cut.splits(ptiles);
         items += (unsigned long long)pblocks * ps;
         parts += (unsigned long long)ps * R;
         if (on && cl == 0 && items <= (unsigned long long)a.max_items &&
             parts <= (unsigned long long)a.max_parts) {
             const int waves = (r >> 4) * a.br_split;
-            const float tile = waves > 4 ? 3.0f : 2.0f, start = 8.0f + 2.0f * waves;
             const float slots = 256.0f * a.per_cu, n = (float)items;
-            const float one = (float)min(each, longest[g]) * tile + start;
-            const float rounds = ceilf(n / slots) * one;
-            const float flow = ((float)w * tile + n * start) / slots + one;
-            const float cost = fminf(rounds, flow) + (parts ? 5.0f : 0.0f) +
-                               (float)parts * (float)a.dvp * (1.0f / (1 << 20));
+            const float tile = a.tile_us * (1.0f + a.wave_more * waves);
+            const float start = 2.2f + 0.55f * waves;
+            if (ps && (float)ptiles >= half * ps) big += (float)pblocks * ps;
+            const float one = (float)most * tile + start, all = w * tile + n * start;
+            const float rounds = fmaxf(ceilf(big / slots), 1.0f);
+            const float flow = all / slots + 0.6f * one;
+            const bool fits = big >= n || (rounds * slots - big >= 0.125f * slots &&
+                                           all <= 0.97f * rounds * slots * one);
+            float cost = fmaxf(fits ? big >= n ? fminf(rounds * one, flow) : rounds * one : flow, one);
+            cost += (parts ? 1.4f : 0.0f) + (float)parts * (float)a.dvp * 0.92e-6f;
             /* a price over 0 orders as its bits do */
-            atomicMin(&best, (unsigned long long)__float_as_uint(cost) << 32 | (uint32_t)(g << 3 | c));
+            atomicMin(&best, (unsigned long long)__float_as_uint(cost) << 32 | (uint32_t)(g << 4 | c));
         }
         __syncthreads();
-        if ((int)(best & 63) == (g << 3 | c) && cl == 0) {
+        if ((int)(best & 127) == (g << 4 | c) && cl == 0) {
             rows_each = rs;
             tiles_each = each;
             tiles_from = from;
+            longest_own = max(1, longest[g]);
         }
         __syncthreads();
     }
@@ -248,48 +270,86 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         const int ns = cut.splits(q.tile1 - q.tile0);
         return start ? ns : max(ns, 1);
     };
-    int sum[2] = {0, 0};
+    /* Items by their length, in quarters of the longest: the first block with three of
+     * them or more, with two and with one. Without a window a block's last row decides. */
+    const int most = min(tiles_each, longest_own);
+    auto quarters = [&](const PlanReq &q, int nb, int ns, int *from) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const long long need = (long long)((most * (3 - k) + 3) / 4) * ns;
+            const long long row = ((need + q.tile0 - 1) * TR_TILE - q.pos) * a.h;
+            from[k] = a.window ? q.tile1 - q.tile0 >= need ? 0 : nb
+                               : (int)min(max(row, 0ll) >> bs, (long long)nb);
+            if (!a.window && row >= (long long)q.n * a.h) from[k] = nb;
+        }
+    };
+    constexpr int NX = 2 + RP_KINDS;              /* items, rows of sums, items by length */
+    int sum[NX] = {};
     for (int b = b0; b < b1; b++) {
         const PlanReq q = request(b, start);
-        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0;
-        sum[0] += ((rows + br - 1) >> bs) * ns;
+        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0, nb = (rows + br - 1) >> bs;
+        int f[3];
+        quarters(q, nb, ns, f);
+        sum[0] += nb * ns;
         sum[1] += start || ns > 1 ? ns * rows : 0;
+        sum[2] += (nb - f[0]) * ns;
+        sum[3] += (f[0] - f[1]) * ns;
+        sum[4] += (f[1] - f[2]) * ns;
+        sum[5] += f[2] * ns;
     }
-    int x[2] = {sum[0], sum[1]};
+    int x[NX];
+#pragma unroll
+    for (int k = 0; k < NX; k++) x[k] = sum[k];
 #pragma unroll
     for (int o = 1; o < 64; o *= 2)
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < NX; k++) {
             const int v = __shfl_up(x[k], o, 64);
             if (lane >= o) x[k] += v;
         }
     if (lane == 63)
-        for (int k = 0; k < 2; k++) part_w[tid >> 6][k] = x[k];
+#pragma unroll
+        for (int k = 0; k < NX; k++) part_w[tid >> 6][k] = x[k];
     __syncthreads();
+    Dsv4ReqsHead head{a.sig, {pitems}, ps, R0, R};
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        /* the waves before this one */
-        int v = lane < tid >> 6 ? part_w[lane & (RP_THREADS / 64 - 1)][k] : 0;
+    for (int k = 0; k < NX; k++) {
+        /* the waves before this one, and all */
+        int all = part_w[lane & (RP_THREADS / 64 - 1)][k];
+        int v = (lane & (RP_THREADS / 64 - 1)) < tid >> 6 ? all : 0;
 #pragma unroll
-        for (int o = RP_THREADS / 128; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-        x[k] += __builtin_amdgcn_readfirstlane(v) - sum[k];
+        for (int o = RP_THREADS / 128; o >= 1; o >>= 1) {
+            v += __shfl_xor(v, o, 64);
+            all += __shfl_xor(all, o, 64);
+        }
+        x[k] += v - sum[k];
+        if (k >= 2) {
+            x[k] += head.end[k - 2];
+            head.end[k - 1] = head.end[k - 2] + all;
+        }
     }
     x[1] += ps * R;
     for (int b = b0; b < b1; b++) {
         const PlanReq q = request(b, start);
-        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0;
+        const int rows = q.n * a.h, ns = q.n ? splits(q) : 0, nb = (rows + br - 1) >> bs;
         const bool direct = !start && ns <= 1;
+        int f[3];
+        quarters(q, nb, ns, f);
         s_item[b] = x[0];
+        for (int k = 0; k < RP_KINDS; k++) s_to[RP_KINDS * b + k] = x[2 + k];
         s_part[b] = direct ? -1 : x[1];
         a.req[b] = Dsv4ReqsReq{s_first[b], q.pos, s_part[b], q.n << 8 | ns};
-        x[0] += ((rows + br - 1) >> bs) * ns;
+        x[0] += nb * ns;
         x[1] += direct ? 0 : ns * rows;
+        x[2] += (nb - f[0]) * ns;
+        x[3] += (f[0] - f[1]) * ns;
+        x[4] += (f[1] - f[2]) * ns;
+        x[5] += f[2] * ns;
     }
     if (b0 < b1 && b1 == nr) s_item[b1] = x[0];
     __syncthreads();
     const int items = s_item[nr];
-    if (tid == 0)
-        *a.head = Dsv4ReqsHead{a.sig, pitems + items, pitems, ps, R0, R, {0, 0}};
+    if (tid == 0) *a.head = head;
     const bool all_see = hi_min >= pt1 * TR_TILE && lo_max == 0;
     for (int i = tid; i < pitems; i += RP_THREADS) {
         const int s = i / pb, blk = i - s * pb;
@@ -317,7 +377,14 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         }
         const PlanReq q = request(b, start);
         const int rows = q.n * a.h, nb = (rows + br - 1) >> bs, ns = splits(q);
-        const int k = i - s_item[b], s = nb == 1 ? k : k / nb, r0 = (k - s * nb) << bs;
+        const int k = i - s_item[b], s = nb == 1 ? k : k / nb, blk = k - s * nb, r0 = blk << bs;
+        int f[3];
+        quarters(q, nb, ns, f);
+        /* of its quarter, the last block first */
+        const int c = blk >= f[0] ? 0 : blk >= f[1] ? 1 : blk >= f[2] ? 2 : 3;
+        const int c1 = c == 0 ? nb : c == 1 ? f[0] : c == 2 ? f[1] : f[2];
+        const int c0 = c == 0 ? f[0] : c == 1 ? f[1] : c == 2 ? f[2] : 0;
+        const int to = s_to[RP_KINDS * b + c] + s * (c1 - c0) + c1 - 1 - blk;
         Dsv4ReqsItem it{};
         it.rows = min(br, rows - r0);
         it.row0 = s_first[b] * a.h + r0;
@@ -334,7 +401,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         it.kind = 1;
         it.pos0 = p0;
         it.part = s_part[b] < 0 ? -1 : s_part[b] + s * rows + r0;
-        a.items[pitems + i] = it;
+        a.items[to] = it;
     }
 }
 
@@ -581,16 +648,24 @@ extern "C" int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_
     a.br_split = tree_split(fmt, kv_fmt, kc);
     a.per_cu = tree_per_cu(fmt, kc);
     a.dvp = (d_v + 15) / 16 * 16;
+    /* A lone workgroup's tile: bf16 1.66 us (576 columns) and 0.78 (128), f32 q over bf16
+     * 1.94, f32 over f32 4.8, bf16 q over f32 2.8; over FP8 1.8 and, with the card full, 3.3.
+     * From 16 rows to 64 it grows by 2 percent (bf16) to 25 (several products). */
+    const int planes = tree_planes(fmt, kv_fmt), products = fmt == DSV4_WF32 ? planes == 1 ? 3 : 6 : planes;
+    a.tile_us = 0.5f + 32.0f * kc * (0.002f * planes + 0.00025f * products +
+                                     (kv_fmt == DSV4_WFP8 ? 0.001f : 0.0f));
+    a.inv_h = 1.0f / (float)h;
+    a.wave_more = products > 1 ? 0.05f : 0.02f;
     a.max_items = (int)m.items;
     a.max_parts = (int)m.parts;
     a.sig = reqs_sig(r, fmt, h, d_qk, d_v, kv_fmt, window);
-    const size_t lds = 4 * ((size_t)r->n_req + 1) * sizeof(int);
+    const size_t lds = 8 * ((size_t)r->n_req + 1) * sizeof(int);
     if (lds > 64 * 1024 - 1024) {
         static bool asked[64];
         int dev = 0;
         HIP_OK(hipGetDevice(&dev), "hipGetDevice");
         if (dev < 0 || dev >= 64 || !asked[dev]) {
-            (void)dsv4_lds_optin((const void *)k_reqs_plan, 4 * 4097 * sizeof(int), "reqs plan");
+            (void)dsv4_lds_optin((const void *)k_reqs_plan, 8 * 4097 * sizeof(int), "reqs plan");
             if (dev >= 0 && dev < 64) asked[dev] = true;
         }
     }

@@ -42,12 +42,14 @@ struct Dsv4TreeJob {
 struct Dsv4ReqsItem {
     int row0, rows, req, tile0, tile1, end, lo, hi, kind, pos0, part, pad;
 };
-/* What a plan begins with: the number of items, those of the prefix first, the rows of
- * all requests, and the signature of the arguments it was made for. */
+/* What a plan begins with: the signature of the arguments it was made for, where its
+ * items of a kind end (those of the prefix, then the requests' from the longest to the
+ * shortest), the prefix's splits and the rows of all requests. */
+constexpr int DSV4_REQS_KINDS = 5;
 struct Dsv4ReqsHead {
     uint32_t sig;
-    int items, prefix_items, prefix_splits;
-    int row0, rows, pad[2];
+    int end[DSV4_REQS_KINDS];
+    int prefix_splits, row0, rows;
 };
 /* A request: its first token and that one's position, where the sums of its own splits
  * are (-1: its items wrote the result), and its tokens << 8 | splits. */
@@ -299,17 +301,20 @@ k_tree(JOB a)
     int i0, i1, blk = 0, split = 0;
     Dsv4ReqsItem it{};
     if constexpr (REQS) {
-        /* the prefix's items and then the others, each so */
+        /* each kind so */
         const Dsv4ReqsHead hd = *a.head;
-        int id = blockIdx.x, base = 0, all = hd.prefix_items;
-        if (hd.sig != a.sig || id >= hd.items) return;
-        if (id >= all) {
-            base = all;
-            id -= all;
-            all = hd.items - all;
-        }
-        const int k = id & 7;
-        const Dsv4ReqsItem *p = a.items + base + k * (all >> 3) + min(k, all & 7) + (id >> 3);
+        const int id = blockIdx.x;
+        if (hd.sig != a.sig || id >= hd.end[DSV4_REQS_KINDS - 1]) return;
+        int base = 0, all = hd.end[0];
+#pragma unroll
+        for (int e = 0; e + 1 < DSV4_REQS_KINDS; e++)
+            if (id >= hd.end[e]) {
+                base = hd.end[e];
+                all = hd.end[e + 1] - base;
+            }
+        const int k = (id - base) & 7;
+        const Dsv4ReqsItem *p =
+            a.items + base + k * (all >> 3) + min(k, all & 7) + ((id - base) >> 3);
         auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
         it = {uni(p->row0), uni(p->rows), uni(p->req),  uni(p->tile0), uni(p->tile1), uni(p->end),
               uni(p->lo),   uni(p->hi),   uni(p->kind), uni(p->pos0),  uni(p->part),  0};
