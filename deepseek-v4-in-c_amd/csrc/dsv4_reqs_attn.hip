@@ -51,7 +51,7 @@ struct PlanJob {
     int n_req, max_tok, h, window, prefix, room;  /* room: positions of a table */
     IoDiv by_h;
     int br, br_split, per_cu, dvp;                /* most rows, waves a block of 16 */
-    float inv_h, tile_us, wave_more;                     /* a tile's time, and how a wave of rows adds */
+    float by_slots, inv_h, tile_us, wave_more;    /* a tile's time, and how a wave of rows adds */
     int max_items, max_parts;
     uint32_t sig;
 };
@@ -61,19 +61,11 @@ struct PlanReq {
     int n, pos, tile0, tile1;
 };
 
-template <class V, class F>
-__device__ __forceinline__ V wave_all(V v, F f)
-{
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
-    return v;
-}
-
 /* Tiles cut into items of about `each`: how many, to RP_SPLITS. A quotient of floats
  * may be one off, which makes an item a little longer or shorter. */
 struct PlanCut {
     float by;
-    __device__ __forceinline__ explicit PlanCut(int each) : by(1.0f / (float)each) {}
+    __device__ __forceinline__ explicit PlanCut(int each) : by(__builtin_amdgcn_rcpf((float)each)) {}
     __device__ __forceinline__ int splits(int tiles) const
     {
         return tiles ? max(1, min((int)ceilf((float)tiles * by - 1e-3f), RP_SPLITS)) : 0;
@@ -81,7 +73,7 @@ struct PlanCut {
 };
 
 /* One workgroup. A plan is: with the prefix apart or not, the rows of a block and the
- * tiles of an item. 128 of them are priced in microseconds: a tile takes what its loads and
+ * tiles of an item. 64 of them are priced in microseconds: a tile takes what its loads and
  * the waits between them take, whatever rows of q it serves (1.65 us for 16, 32 and 64 rows
  * of bf16, 576 columns), 2.2 and half a microsecond a wave of 16 rows are an item's start,
  * and then come the sums that are joined. Workgroups begin in their order, and those of
@@ -89,15 +81,16 @@ struct PlanCut {
  * fill what the last round of these leaves free, if every engine has a free CU. */
 __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 {
-    extern __shared__ int lds[];
+    extern __shared__ __align__(16) int lds[];
     __shared__ unsigned long long best, owner;
     __shared__ float work[2 * 8];
     __shared__ int bad, active, hi_min, lo_max, lo_min, longest[8];
     __shared__ int part_w[RP_THREADS / 64][2 + RP_KINDS];
     __shared__ int rows_each, tiles_each, tiles_from, longest_own;
     const int tid = threadIdx.x, lane = tid & 63, nr = a.n_req;
-    int *s_first = lds, *s_len = lds + nr + 1, *s_item = s_len + nr, *s_part = s_item + nr + 1,
-        *s_to = s_part + nr;                      /* four a request */
+    int *s_first = lds, *s_len = lds + nr + 1, *s_item = s_len + nr,
+        *s_to = lds + ((3 * nr + 2 + 3) & ~3),    /* four a request */
+        *s_part = s_to + RP_KINDS * nr;
     if (tid == 0) {
         best = ~0ull;
         owner = 0;
@@ -122,14 +115,10 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     };
     /* tiles of a request's block on average: an earlier one ends earlier, and with a window
      * one of more rows begins earlier */
-    auto mean_tiles = [&](const PlanReq &q, int rows) {
-        const int t = q.tile1 - q.tile0;
-        const float less = fmaxf((float)q.n - (float)rows * a.inv_h, 0.0f);
-        return t ? fmaxf((float)t - less * (a.window ? 1.0f / TR_TILE : 0.5f / TR_TILE), 1.0f) : 0.0f;
+    const float tiles_less = a.window ? 1.0f / TR_TILE : 0.5f / TR_TILE;
+    auto mean_tiles = [&](int n, int t, float toks) {
+        return t ? fmaxf((float)t - fmaxf((float)n - toks, 0.0f) * tiles_less, 1.0f) : 0.0f;
     };
-    auto hi = [](auto x, auto y) { return x > y ? x : y; };
-    auto lo = [](auto x, auto y) { return x < y ? x : y; };
-    auto plus = [](auto x, auto y) { return x + y; };
     {
         int b_bad = tok0 < 0 || tok1 > a.max_tok, n_act = 0, hmin = INT32_MAX, lmax = 0,
             lmin = INT32_MAX;
@@ -149,12 +138,16 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
             own = o > own ? o : own;
         }
         if ((tid & ~63) < nr) {                   /* a wave, whole or not at all */
-            b_bad = wave_all(b_bad, hi);
-            n_act = wave_all(n_act, plus);
-            hmin = wave_all(hmin, lo);
-            lmax = wave_all(lmax, hi);
-            lmin = wave_all(lmin, lo);
-            own = wave_all(own, hi);
+#pragma unroll 1                                  /* run once: short code is fast code */
+            for (int o = 32; o >= 1; o >>= 1) {
+                b_bad |= __shfl_xor(b_bad, o, 64);
+                n_act += __shfl_xor(n_act, o, 64);
+                hmin = min(hmin, __shfl_xor(hmin, o, 64));
+                lmax = max(lmax, __shfl_xor(lmax, o, 64));
+                lmin = min(lmin, __shfl_xor(lmin, o, 64));
+                const unsigned long long v = __shfl_xor(own, o, 64);
+                own = v > own ? v : own;
+            }
             if (lane == 0) {
                 if (b_bad) bad = 1;
                 atomicAdd(&active, n_act);
@@ -175,23 +168,35 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     const int max_len = (int)(owner >> 32);
     const int pt1 = min(a.prefix, max_len) / TR_TILE, pt0 = min(pt1, lo_min / TR_TILE);
     const bool may = active > 1 && pt1 > pt0;
+    /* a request's tokens, rows, tiles and tiles behind the prefix, where s_to will be */
+    for (int b = tid; b < nr; b += RP_THREADS) {
+        const PlanReq q = request(b, 0), p = request(b, pt1);
+        s_to[4 * b] = q.n;
+        s_to[4 * b + 1] = q.n * a.h;
+        s_to[4 * b + 2] = q.tile1 - q.tile0;
+        s_to[4 * b + 3] = p.tile1 - p.tile0;
+    }
+    __syncthreads();
 
     /* group g (two waves): the prefix apart (g & 1), blocks of 1 << rs rows */
     const int g = tid >> 7, gt = tid & 127, rs = 4 + (g >> 1), r = 1 << rs;
     const bool apart = g & 1, on = r <= a.br && (!apart || may);
     const int from = apart ? pt1 : 0, ptiles = apart ? pt1 - pt0 : 0;
     const int pblocks = apart ? (R + r - 1) >> rs : 0;
+    const float toks = (float)r * a.inv_h;
     if (on) {
         float w = 0.0f;
         int l = ptiles;
         for (int b = gt; b < nr; b += 128) {
-            const PlanReq q = request(b, from);
-            if (!q.n) continue;
-            w += (float)((q.n * a.h + r - 1) >> rs) * mean_tiles(q, r);
-            l = max(l, q.tile1 - q.tile0);
+            const int n = s_to[4 * b], rows = s_to[4 * b + 1], t = s_to[4 * b + 2 + apart];
+            w += (float)((rows + r - 1) >> rs) * mean_tiles(n, t, toks);
+            l = max(l, t);
         }
-        w = wave_all(w, plus);
-        l = wave_all(l, hi);
+#pragma unroll 1
+        for (int o = 32; o >= 1; o >>= 1) {
+            w += __shfl_xor(w, o, 64);
+            l = max(l, __shfl_xor(l, o, 64));
+        }
         if (lane == 0) {
             work[tid >> 6] = w;
             atomicMax(&longest[g], l);
@@ -200,57 +205,63 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     __syncthreads();
     {
         /* tiles of an item, so that they are about so many workgroups' worth of the card */
-        const int c = gt >> 3, cl = gt & 7;
-        constexpr float SHARE[16] = {96,  128, 192, 208, 224, 256, 320, 416, 448, 480, 512, 640, 704,
-                                     960, 1472, 0};
+        const int c = gt >> 4, cl = gt & 15;
+        constexpr float SHARE[8] = {1.0f / 112, 1.0f / 208, 1.0f / 224, 1.0f / 256,
+                                    1.0f / 448, 1.0f / 480, 1.0f / 704, 0.0f};
         const float w = work[2 * g] + work[2 * g + 1] + (float)pblocks * (float)ptiles;
-        const int each = c < 15 ? max(1, (int)ceilf(fminf(w / SHARE[c], 1e9f))) : 1 << 30;
+        const int each = c < 7 ? max(1, (int)ceilf(fminf(w * SHARE[c], 1e9f))) : 1 << 30;
         const int most = min(each, longest[g]), ps = PlanCut(each).splits(ptiles);
         const PlanCut cut(each);
         const float half = 0.5f * (float)most;
-        unsigned long long items = 0, parts = 0;
-        float big = 0.0f;                         /* items of half the longest or more */
+        float items = 0.0f, parts = 0.0f, big = 0.0f;  /* big: of half the longest or more */
         if (on) {
-            for (int b = cl; b < nr; b += 8) {
-                const PlanReq q = request(b, from);
-                if (!q.n) continue;
-                const int rows = q.n * a.h, t = q.tile1 - q.tile0;
-                int ns = cut.splits(t);
-                if (!apart && ns < 1) ns = 1;
-                const int n = ((rows + r - 1) >> rs) * ns;
-                items += (unsigned)n;
-                if (apart || ns > 1) parts += (unsigned long long)ns * rows;
-                const float spread = fmaxf(2.0f * ((float)t - mean_tiles(q, r)), 1e-3f);
-                big += (float)n * fminf(fmaxf(((float)t - half * ns) / spread, 0.0f), 1.0f);
+            for (int b = cl; b < nr; b += 16) {
+                const int toks_b = s_to[4 * b], rows = s_to[4 * b + 1], t = s_to[4 * b + 2 + apart];
+                const int ns = max(cut.splits(t), apart || !toks_b ? 0 : 1);
+                const float n = (float)((rows + r - 1) >> rs) * (float)ns;
+                items += n;
+                parts += apart || ns > 1 ? (float)ns * (float)rows : 0.0f;
+                const float spread = fmaxf(2.0f * ((float)t - mean_tiles(toks_b, t, toks)), 1e-3f);
+                big += n * fminf(fmaxf(((float)t - half * (float)ns) * __builtin_amdgcn_rcpf(spread), 0.0f), 1.0f);
             }
         }
-#pragma unroll
-        for (int o = 4; o >= 1; o >>= 1) {
+#pragma unroll 1
+        for (int o = 8; o >= 1; o >>= 1) {
             items += __shfl_xor(items, o, 64);
             parts += __shfl_xor(parts, o, 64);
             big += __shfl_xor(big, o, 64);
         }
-        items += (unsigned long long)pblocks * ps;
-        parts += (unsigned long long)ps * R;
-        if (on && cl == 0 && items <= (unsigned long long)a.max_items &&
-            parts <= (unsigned long long)a.max_parts) {
+        items += (float)pblocks * (float)ps;
+        parts += (float)ps * (float)R;
+        /* Sums of at most 4096 floats: 2^-12 off at most. The largest blocks, whole, are
+         * what the plan's and the sums' rooms are made for. */
+        const bool whole = c == 7 && !apart && r == a.br;
+        unsigned long long price = ~0ull;
+        if (on && (whole || (items * 1.001f <= (float)a.max_items &&
+                             parts * 1.001f <= (float)a.max_parts))) {
             const int waves = (r >> 4) * a.br_split;
-            const float slots = 256.0f * a.per_cu, n = (float)items;
+            const float slots = 256.0f * a.per_cu, by = a.by_slots, n = items;
             const float tile = a.tile_us * (1.0f + a.wave_more * waves);
             const float start = 2.2f + 0.55f * waves;
             if (ps && (float)ptiles >= half * ps) big += (float)pblocks * ps;
             const float one = (float)most * tile + start, all = w * tile + n * start;
-            const float rounds = fmaxf(ceilf(big / slots), 1.0f);
-            const float flow = all / slots + 0.6f * one;
+            const float rounds = fmaxf(ceilf(big * by), 1.0f);
+            const float flow = all * by + 0.6f * one;
             const bool fits = big >= n || (rounds * slots - big >= 0.125f * slots &&
                                            all <= 0.97f * rounds * slots * one);
             float cost = fmaxf(fits ? big >= n ? fminf(rounds * one, flow) : rounds * one : flow, one);
-            cost += (parts ? 1.4f : 0.0f) + (float)parts * (float)a.dvp * 0.92e-6f;
+            cost += (parts > 0.0f ? 1.4f : 0.0f) + parts * (float)a.dvp * 0.92e-6f;
             /* a price over 0 orders as its bits do */
-            atomicMin(&best, (unsigned long long)__float_as_uint(cost) << 32 | (uint32_t)(g << 4 | c));
+            price = (unsigned long long)__float_as_uint(cost) << 32 | (uint32_t)(g << 3 | c);
         }
+#pragma unroll
+        for (int o = 32; o >= 16; o >>= 1) {
+            const unsigned long long v = __shfl_xor(price, o, 64);
+            price = v < price ? v : price;
+        }
+        if (lane == 0 && price != ~0ull) atomicMin(&best, price);
         __syncthreads();
-        if ((int)(best & 127) == (g << 4 | c) && cl == 0) {
+        if ((int)(best & 63) == (g << 3 | c) && cl == 0) {
             rows_each = rs;
             tiles_each = each;
             tiles_from = from;
@@ -276,11 +287,10 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     auto quarters = [&](const PlanReq &q, int nb, int ns, int *from) {
 #pragma unroll
         for (int k = 0; k < 3; k++) {
-            const long long need = (long long)((most * (3 - k) + 3) / 4) * ns;
-            const long long row = ((need + q.tile0 - 1) * TR_TILE - q.pos) * a.h;
-            from[k] = a.window ? q.tile1 - q.tile0 >= need ? 0 : nb
-                               : (int)min(max(row, 0ll) >> bs, (long long)nb);
-            if (!a.window && row >= (long long)q.n * a.h) from[k] = nb;
+            const int need = min(((most * (3 - k) + 3) / 4) * ns, q.tile1 - q.tile0 + 1);
+            const int tok = (int)((uint32_t)(need + q.tile0 - 1) * TR_TILE - (uint32_t)q.pos);
+            from[k] = a.window ? need <= q.tile1 - q.tile0 ? 0 : nb
+                               : tok >= q.n ? nb : (max(tok, 0) * a.h) >> bs;
         }
     };
     constexpr int NX = 2 + RP_KINDS;              /* items, rows of sums, items by length */
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     int x[NX];
 #pragma unroll
     for (int k = 0; k < NX; k++) x[k] = sum[k];
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 64; o *= 2)
 #pragma unroll
         for (int k = 0; k < NX; k++) {
@@ -312,20 +322,22 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         for (int k = 0; k < NX; k++) part_w[tid >> 6][k] = x[k];
     __syncthreads();
     Dsv4ReqsHead head{a.sig, {pitems}, ps, R0, R};
+    int all[NX] = {};
+    const int waves = ((nr + per - 1) / per + 63) / 64;
+#pragma unroll 1
+    for (int w = 0; w < waves; w++)
+#pragma unroll
+        for (int k = 0; k < NX; k++) {
+            const int v = part_w[w][k];
+            x[k] += w < tid >> 6 ? v : 0;
+            all[k] += v;
+        }
 #pragma unroll
     for (int k = 0; k < NX; k++) {
-        /* the waves before this one, and all */
-        int all = part_w[lane & (RP_THREADS / 64 - 1)][k];
-        int v = (lane & (RP_THREADS / 64 - 1)) < tid >> 6 ? all : 0;
-#pragma unroll
-        for (int o = RP_THREADS / 128; o >= 1; o >>= 1) {
-            v += __shfl_xor(v, o, 64);
-            all += __shfl_xor(all, o, 64);
-        }
-        x[k] += v - sum[k];
+        x[k] -= sum[k];
         if (k >= 2) {
             x[k] += head.end[k - 2];
-            head.end[k - 1] = head.end[k - 2] + all;
+            head.end[k - 1] = head.end[k - 2] + all[k];
         }
     }
     x[1] += ps * R;
@@ -655,6 +667,7 @@ extern "C" int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_
     a.tile_us = 0.5f + 32.0f * kc * (0.002f * planes + 0.00025f * products +
                                      (kv_fmt == DSV4_WFP8 ? 0.001f : 0.0f));
     a.inv_h = 1.0f / (float)h;
+    a.by_slots = 1.0f / (256.0f * (float)a.per_cu);
     a.wave_more = products > 1 ? 0.05f : 0.02f;
     a.max_items = (int)m.items;
     a.max_parts = (int)m.parts;
