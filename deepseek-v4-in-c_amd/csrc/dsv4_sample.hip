@@ -39,6 +39,8 @@ constexpr int SP_LIST = SP_THREADS;               /* tokens put in order     */
 constexpr int SP_QUEUE = 2 * SP_LIST;              /* and looked through      */
 constexpr int SP_CHUNKS = 4096;                   /* chunks looked over at once */
 constexpr int SP_K = 512;                         /* a short top-k, for which no bins are made */
+constexpr int SP_DIRECT = 96;
+constexpr float SP_FLOOR = 0.0078125f;             /* a min_p for which none are made */
 static_assert(SP_THREADS == SM_BINS, "a bin a thread");
 
 struct SmTop {
@@ -158,6 +160,21 @@ __device__ __forceinline__ bool sm_short(const SampleJob &a, int top_k)
     return top_k > 0 && top_k <= SP_K && 2 * top_k <= a.nc && a.nc <= SP_CHUNKS;
 }
 
+/* A row whose only other limit is min_p: what is under it has no part in any sum, so
+ * that its tokens are all that is looked at, if they fit the list. */
+__device__ __forceinline__ float sm_floor(const SampleJob &a, int row)
+{
+    return a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
+}
+__device__ __forceinline__ bool sm_above(const SampleJob &a, int row, float floor_)
+{
+    return floor_ >= SP_FLOOR && a.nc <= SP_CHUNKS && !(a.r.top_p && a.r.top_p[row] < 1.0f);
+}
+__device__ __forceinline__ bool sm_brief(const SampleJob &a, int row)
+{
+    return (a.r.top_k && sm_short(a, a.r.top_k[row])) || sm_above(a, row, sm_floor(a, row));
+}
+
 /* A slice of a row: the maxima of its chunks, and its bins. */
 template <class T>
 __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
@@ -171,43 +188,47 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
     const int v0 = slice * SM_SLICE;
     const T *x = (const T *)a.x + (size_t)row * a.stride + v0;
     const int lim = min(SM_SLICE, a.vocab - v0);
+    constexpr int W = 4;                          /* tokens of a load: 8 of bf16 took 28 us for 23 */
     float v[SM_EACH];
 #pragma unroll
-    for (int p = 0; p < SM_EACH / 4; p++) {
-        const int c = (p * SM_THREADS + tid) * 4;
+    for (int p = 0; p < SM_EACH / W; p++) {
+        const int c = (p * SM_THREADS + tid) * W;
         if (lim == SM_SLICE) {
-            io_load<T, 4>(x + c, v + 4 * p);
+            io_load<T, W>(x + c, v + W * p);
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v[4 * p + k] = -INFINITY;
-                if (c + k < lim) io_load<T, 1>(x + c + k, v + 4 * p + k);
+            for (int k = 0; k < W; k++) {
+                v[W * p + k] = -INFINITY;
+                if (c + k < lim) io_load<T, 1>(x + c + k, v + W * p + k);
             }
         }
     }
     const float temp = sm_temperature(a, row);
+    const bool brief = sm_brief(a, row);
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < SM_EACH / W; p++) {
+        /* (NaN: fmaxf takes the other) */
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < W; k++) m = fmaxf(m, v[W * p + k]);
+        m = fmaxf(m, dpp_f<DPP_QUAD_XOR1, 0xF>(m));
+        m = fmaxf(m, dpp_f<DPP_QUAD_XOR2, 0xF>(m));
+        m = fmaxf(m, dpp_f<DPP_ROW_HMIRROR, 0xF>(m));
+        if (W == 4) m = fmaxf(m, dpp_f<DPP_ROW_MIRROR, 0xF>(m));
+        constexpr int LANES = SM_CHUNK / W;
+        const int chunk = (v0 + p * SM_THREADS * W) / SM_CHUNK + tid / LANES;
+        if ((tid & (LANES - 1)) == 0 && chunk < a.nc) a.cmax[(size_t)row * a.nc + chunk] = m;
+        top = fmaxf(top, m);
+    }
+    /* the first is picked, or one of the first few */
+    if (!(temp > 0.0f) || brief) return;
+
     for (int i = tid; i < SM_BINS; i += SM_THREADS) bins[i] = 0;
     if (tid == 0) {
         tail = 0;
         tail_n = 0;
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < SM_EACH / 4; p++) {
-        /* (NaN: fmaxf takes the other) */
-        float m = fmaxf(fmaxf(v[4 * p], v[4 * p + 1]), fmaxf(v[4 * p + 2], v[4 * p + 3]));
-        m = fmaxf(m, -INFINITY);
-        m = fmaxf(m, dpp_f<DPP_QUAD_XOR1, 0xF>(m));
-        m = fmaxf(m, dpp_f<DPP_QUAD_XOR2, 0xF>(m));
-        m = fmaxf(m, dpp_f<DPP_ROW_HMIRROR, 0xF>(m));
-        m = fmaxf(m, dpp_f<DPP_ROW_MIRROR, 0xF>(m));
-        const int chunk = (v0 + p * SM_THREADS * 4) / SM_CHUNK + tid / 16;
-        if ((tid & 15) == 0 && chunk < a.nc) a.cmax[(size_t)row * a.nc + chunk] = m;
-        top = fmaxf(top, m);
-    }
-    /* the first is picked, or one of the first few */
-    if (!(temp > 0.0f) || (a.r.top_k && sm_short(a, a.r.top_k[row]))) return;
-
     top = wave_max(top);
     if ((tid & 63) == 0) wtop[tid >> 6] = top;
     __syncthreads();
@@ -343,7 +364,7 @@ struct SmRow {
             };
         };
         __attribute__((aligned(16))) u64 key[SP_LIST];    /* tokens in order */
-        u64 through[SP_LIST];                     /* and the sums through them */
+        __attribute__((aligned(16))) u64 through[SP_LIST];  /* and the sums through them */
         u64 sum[SM_BINS];                         /* through a bin           */
         uint32_t n[SM_BINS];
         int off[SM_BINS];                         /* a bin's place in the list, or -1 */
@@ -495,18 +516,62 @@ struct SmRow {
         return s.len;
     }
 
-    /* How many of keys i0 .. i1 - 1 are over one. */
-    __device__ __forceinline__ int rank(const u64 *keys, int i0, int i1, u64 key) const
+    /* The place of thread tid's key among those of threads 0 .. n - 1, the largest first.
+     * All keys read by all threads are n^2 reads of LDS, 7 us for 444; over SP_DIRECT of
+     * them the range of their logits is cut into SP_THREADS parts first, 3 us. */
+    __device__ __forceinline__ int order(int n, u64 key)
     {
-        int n = 0, i = i0;
-        if (i & 1) n += keys[i++] > key;
-#pragma unroll 4
-        for (; i + 2 <= i1; i += 2) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(keys + i);
-            n += (k.x > key) + (k.y > key);
+        const int tid = threadIdx.x, lane = tid & 63;
+        int i0 = 0, i1 = n, at = tid, d = 0;
+        if (n > SP_DIRECT) {
+            uint32_t k0 = tid < n ? (uint32_t)(key >> 32) : ~0u, k1 = tid < n ? k0 : 0;
+#pragma unroll 1
+            for (int o = 32; o >= 1; o >>= 1) {
+                k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
+                k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
+            }
+            __syncthreads();
+            if (lane == 0) s.part[tid >> 6] = (u64)k0 << 32 | k1;
+            s.cur[tid] = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (int w = 0; w < SP_WAVES; w++) {
+                const u64 v = s.part[w];
+                k0 = min(k0, (uint32_t)(v >> 32));
+                k1 = max(k1, (uint32_t)v);
+            }
+            /* (a range that is not finite, or 0: all in one, as NaN becomes 0) */
+            const float top = sm_value((u64)k1 << 32), by = (SP_THREADS - 1) / (top - sm_value((u64)k0 << 32));
+            d = (int)fminf(fmaxf((top - sm_value(key)) * by, 0.0f), SP_THREADS - 1.0f);
+            if (tid < n) at = (int)atomicAdd(&s.cur[d], 1u);
+            __syncthreads();
+            u64 none = 0;
+            const uint32_t c = s.cur[tid];
+            uint32_t e = c;
+            scan(none, e);
+            s.cur[tid] = e;
+            __syncthreads();
+            if (tid < n) {
+                i0 = d ? (int)s.cur[d - 1] : 0;
+                i1 = (int)s.cur[d];
+                at += i0;
+            }
         }
-        if (i < i1) n += keys[i] > key;
-        return n;
+        if (tid < n) s.through[at] = key;
+        __syncthreads();
+        int place = i0;
+        if (tid < n) {
+            int i = i0;
+            if (i & 1) place += s.through[i++] > key;
+#pragma unroll 4
+            for (; i + 2 <= i1; i += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(s.through + i);
+                place += (k.x > key) + (k.y > key);
+            }
+            if (i < i1) place += s.through[i] > key;
+        }
+        __syncthreads();
+        return place;
     }
 
     /* Put the tokens of the bins that have a place (s.off), of b0 to b1 or b2 to b3, into the
@@ -537,31 +602,21 @@ struct SmRow {
             if (at < n) s.key[at] = key;          /* (the counts say that it is) */
         }
         __syncthreads();
-        u64 key = 0, w = 0;
-        int at = 0, bin = 0;
-        if (tid < n) {
-            key = s.key[tid];
-            const double z = sc.z(sm_value(key));
-            w = weight(z);
-            bin = sm_bin(first, sm_q(z));
-            const int i0 = s.off[bin], i1 = i0 + (int)(s.n[bin] - n_before(bin));
-            at = i0;
-            at += rank(s.key, i0, i1, key);
-        }
-        __syncthreads();
+        const u64 key = tid < n ? s.key[tid] : 0;
+        const int at = order(n, key);
         if (tid < n) {
             s.key[at] = key;
-            s.queue[at] = w;
+            s.queue[at] = weight(sc.z(sm_value(key)));
         }
         __syncthreads();
         u64 m = tid < n ? s.queue[tid] : 0;
-        w = m;
+        const u64 w = m;
         uint32_t k = 0;
         scan(m, k);
         s.queue[SP_LIST + tid] = m - w;           /* before it in the list   */
         __syncthreads();
         if (tid < n) {
-            bin = bin_of(sm_value(s.key[tid]));
+            const int bin = bin_of(sm_value(s.key[tid]));
             s.through[tid] = sum_before(bin) + m - s.queue[SP_LIST + s.off[bin]];
         }
         __syncthreads();
@@ -579,7 +634,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const float temp = sm_temperature(a, row);
     const int top_k = a.r.top_k ? a.r.top_k[row] : 0;
     const float p = a.r.top_p ? a.r.top_p[row] : 1.0f;
-    const float floor_ = a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
+    const float floor_ = sm_floor(a, row);
+    const bool few = sm_short(a, top_k), brief = few || sm_above(a, row, floor_);
     const float u = a.r.u[row];
     Row r{a, s, (const T *)a.x + (size_t)row * a.stride, a.cmax + (size_t)row * a.nc,
           SmScale{0.0, false}, 0.0, 0.0, temp * 0.021660849f, {}};
@@ -596,7 +652,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const u64 *bins = a.bins + (size_t)row * a.ns * SM_BINS;
     const bool sampled = temp > 0.0f;
     SmTop mine{-INFINITY, 0, 0, 0};
-    if (sampled && !sm_short(a, top_k) && (lane & (G - 1)) < a.ns) mine = tops[lane & (G - 1)];
+    if (sampled && !brief && (lane & (G - 1)) < a.ns) mine = tops[lane & (G - 1)];
     u64 most = 0;
 #pragma unroll
     for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++) {
@@ -666,9 +722,11 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     };
     const bool by_p = p < 1.0f, by_floor = floor_ > 0.0f;
 
-    /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order ---- */
-    const bool brief = sm_short(a, top_k);
-    if (brief) {
+    /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order; or a
+     *      min_p alone: those that it may leave ---- */
+    bool fits = brief;
+    float low = INFINITY;
+    if (few) {
         /* that chunk's maximum, or a little less: the range of keys split by 1024 */
         uint32_t key0 = s.npart[lane & (SP_WAVES - 1)], key1 = (uint32_t)(most >> 32);
 #pragma unroll
@@ -701,17 +759,30 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             key0 = end > key0 && end <= key1 ? end : key0;
             if (sh == 0 || through <= top_k + top_k / 8 + 8) break;
         }
-        const int len = r.queue(sm_value((u64)key0 << 32), INFINITY, INFINITY, INFINITY);
+        low = sm_value((u64)key0 << 32);
+    } else if (brief) {
+        /* with a margin for the logarithm and the quotient; every chunk above has a token */
+        if (!r.sc.inf) {
+            low = (float)((zmost + (double)__builtin_amdgcn_logf(floor_) - 1e-5) / r.sc.c);
+            low = fmaxf(low - fabsf(low) * 1e-6f, -3.4028235e38f);
+        }
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++) n += (int)__popcll(__ballot(r.cm[k] >= low));
+        __syncthreads();
+        if (lane == 0) s.npart[tid >> 6] = (uint32_t)n;
+        __syncthreads();
+        fits = sm_wave_scan(lane < SP_WAVES ? s.npart[lane & (SP_WAVES - 1)] : 0u) <= SP_LIST;
+        fits = __all(fits);
+    }
+    if (fits) {
+        const int len = r.queue(low, INFINITY, INFINITY, INFINITY);
         if (len <= SP_LIST) {
-            u64 key = 0;
-            int at = 0;
-            if (tid < len) {
-                key = s.queue[tid];
-                at = r.rank(s.queue, 0, len, key);
-                s.key[at] = key;
-            }
+            const u64 key = tid < len ? s.queue[tid] : 0;
+            const int at = r.order(len, key);
+            if (tid < len) s.key[at] = key;
             __syncthreads();
-            const int end = min(top_k, len);
+            const int end = top_k > 0 ? min(top_k, len) : len;
             u64 m = tid < end ? sm_weight(r.sc.z(sm_value(s.key[tid])) - r.e, a.sh) : 0;
             uint32_t none = 0;
             r.scan(m, none);
@@ -791,7 +862,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         }
     }
     if (brief) {
-        /* too many tokens as large: the bins from the row */
+        /* too many tokens: the bins from the row */
         __syncthreads();
         s.mass[tid] = 0;
         s.cur[tid] = 0;

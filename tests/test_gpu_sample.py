@@ -99,6 +99,30 @@ def test_equal_logits(gpu, dsv4, vocab):
         check(dsv4, x, u=us, min_p=np.array([1, 0.5, 1e-6, 2, 0]))
 
 
+@pytest.mark.parametrize("vocab", [700, 40000, 129280, 262145])
+@pytest.mark.parametrize("few", [1, 2, 1023, 1024, 1025, 2048, 2049, 30000])
+def test_min_p_alone(gpu, dsv4, vocab, few):
+    """Of a row, `few` tokens at or above min_p and the others a step below it, in a
+    heap, spread and one in each chunk; top-k long, off and at the number."""
+    few = min(few, vocab)
+    rng = np.random.default_rng(vocab + few)
+    low = np.float32(-4.5)                       # e^-4.5 = 0.0111, under 0.012 and over 0.011
+    x = np.full((6, vocab), low, np.float32)
+    for r in range(6):
+        at = (rng.permutation(vocab)[:few], np.arange(vocab - few, vocab),
+              (np.arange(few) * 64 + np.arange(few) * 64 // vocab) % vocab)[r % 3]
+        x[r, at] = rng.uniform(-4.42, -1, len(at)).astype(np.float32)
+        x[r, at[0]] = 0
+    x[5, rng.integers(0, vocab)] = INF
+    k = np.array([0, vocab, few, max(1, few - 1), 600, 0])
+    for min_p in (0.012, 0.011, 1.0):
+        check(dsv4, x, min_p=np.full(6, min_p), top_k=k, u=rng.random(6).astype(np.float32))
+        check(dsv4, x * 1e30, temperature=np.full(6, 1e30), min_p=np.full(6, min_p), top_k=k,
+              u=rng.random(6).astype(np.float32))
+    check(dsv4, x, True, min_p=np.full(6, 0.0078125), top_p=np.where(k == 600, 0.5, 1.0),
+          u=rng.random(6).astype(np.float32))
+
+
 @pytest.mark.parametrize("vocab", [20000, 129280, 262145, 300000])
 def test_likely_tokens_that_stand_together(gpu, dsv4, vocab):
     """Sorted logits, and a block of equal ones: many tokens of few chunks as large as
