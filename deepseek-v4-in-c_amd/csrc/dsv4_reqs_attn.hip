@@ -25,7 +25,7 @@ namespace {
 constexpr int RP_THREADS = 1024;
 constexpr int RP_SPLITS = 255;                    /* most of a request's, or of the prefix */
 constexpr int RP_KINDS = DSV4_REQS_KINDS - 1;      /* of the requests' items, by length */
-constexpr int RP_EXTRA = 1024;                    /* items for splits        */
+constexpr int RP_EXTRA = 1024, RP_PREFIX = 4096;  /* items for splits; blocks of the prefix */
 constexpr int RP_ROWS = 65536, RP_PREFIX_ROWS = 262144;  /* rows of sums      */
 
 /* What a batch's plan and workspace have room for. */
@@ -41,6 +41,15 @@ ReqsRoom reqs_room(int n_req, int max_tok, int h)
     m.items = 2 * (m.rows / 64) + n_req + 1 + RP_EXTRA;
     m.parts = RP_ROWS + (2 * m.rows < RP_PREFIX_ROWS ? 2 * m.rows : RP_PREFIX_ROWS);
     return m;
+}
+
+/* The items of a plan whose blocks have up to br rows, as many as are launched: all
+ * requests' whole blocks, the prefix's, which few rows of each request make worth it, and
+ * some for splits. A workgroup without one ends at once, 256 of them in a microsecond. */
+int reqs_items(const ReqsRoom &m, int n_req, int br)
+{
+    const long long blocks = m.rows / br;
+    return (int)(blocks + (blocks < RP_PREFIX ? blocks : RP_PREFIX) + n_req + 1 + RP_EXTRA);
 }
 
 struct PlanJob {
@@ -173,8 +182,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         const PlanReq q = request(b, 0), p = request(b, pt1);
         s_to[4 * b] = q.n;
         s_to[4 * b + 1] = q.n * a.h;
-        s_to[4 * b + 2] = q.tile1 - q.tile0;
-        s_to[4 * b + 3] = p.tile1 - p.tile0;
+        s_to[4 * b + 2] = q.n ? q.tile1 - q.tile0 : 0;
+        s_to[4 * b + 3] = q.n ? p.tile1 - p.tile0 : 0;
     }
     __syncthreads();
 
@@ -418,7 +427,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 }
 
 constexpr int RJ_THREADS = 256, RJ_WAVES = RJ_THREADS / 64;
-constexpr int RJ_ROWS = 2048;
+constexpr int RJ_ROWS = 2048, RJ_GROUPS = 4096;
 
 struct JoinJob {
     const Dsv4ReqsHead *head;
@@ -446,103 +455,109 @@ __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
             io_store<T, 1>(o + i, &nan);
         return;
     }
-    const int i = WAVES > 1 ? (int)blockIdx.x : (int)blockIdx.x * RJ_WAVES + wave;
-    if (i >= hd.rows) return;
-    const int r = hd.row0 + i, t = (int)a.by_h.div((uint32_t)r);
-    /* the last request whose first token is t or before it: of every step-th one, then
-     * of those behind it */
-    const int step = (a.n_req + 63) / 64;
-    int b = 0;
-    for (int s = step; s >= 1; s = s > 1 ? 1 : 0) {
-        const int k = b + lane * s;
-        const unsigned long long before =
-            __ballot(lane < (s > 1 ? 64 : step > 1 ? step : 64) && k < a.n_req &&
-                     a.req[min(k, a.n_req - 1)].first <= t);
-        b += (63 - (int)__builtin_clzll(before | 1)) * s;
-    }
-    const Dsv4ReqsReq q = a.req[b];
-    if (q.part < 0) return;
-    const int ps = hd.prefix_splits, n = ps + (q.cut & 255), rows = (q.cut >> 8) * a.h;
-    const size_t own = (size_t)q.part + (r - q.first * a.h);
-    auto place = [&](int s) {
-        return s < ps ? (size_t)s * hd.rows + i : own + (size_t)(s - ps) * rows;
-    };
-    constexpr int NK = (2 * RP_SPLITS + 63) / 64;
-    float ms[NK], ls[NK], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NK; k++) {
-        const int s = 64 * k + lane;
-        ms[k] = -INFINITY;
-        ls[k] = 0.0f;
-        if (64 * k < n && s < n) {
-            ms[k] = a.pm[place(s)];
-            ls[k] = a.pl[place(s)];
+    auto row = [&](int i) {
+        const int r = hd.row0 + i, t = (int)a.by_h.div((uint32_t)r);
+        /* the last request whose first token is t or before it: of every step-th one, then
+         * of those behind it */
+        const int step = (a.n_req + 63) / 64;
+        int b = 0;
+        for (int s = step; s >= 1; s = s > 1 ? 1 : 0) {
+            const int k = b + lane * s;
+            const unsigned long long before =
+                __ballot(lane < (s > 1 ? 64 : step > 1 ? step : 64) && k < a.n_req &&
+                         a.req[min(k, a.n_req - 1)].first <= t);
+            b += (63 - (int)__builtin_clzll(before | 1)) * s;
         }
-        m = fmaxf(m, ms[k]);
-    }
-    m = wave_max(m);
+        const Dsv4ReqsReq q = a.req[b];
+        if (q.part < 0) return;
+        const int ps = hd.prefix_splits, n = ps + (q.cut & 255), rows = (q.cut >> 8) * a.h;
+        const size_t own = (size_t)q.part + (r - q.first * a.h);
+        auto place = [&](int s) {
+            return s < ps ? (size_t)s * hd.rows + i : own + (size_t)(s - ps) * rows;
+        };
+        constexpr int NK = (2 * RP_SPLITS + 63) / 64;
+        float ms[NK], ls[NK], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NK; k++) {
-        if (64 * k >= n) break;
-        ms[k] = tree_join_weight(ms[k], ls[k], m);
-        l += ms[k] * ls[k];
-    }
-    l = wave_sum(l);
-    if (a.sink && l != 0.0f)
-        l += __builtin_amdgcn_exp2f(a.sink[r - t * a.h] * 1.44269504088896340736f - m);
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    constexpr int G = 4;                          /* places in flight        */
-#pragma unroll
-    for (int k = 0; k < NK; k++) {
-        if (64 * k >= n) break;
-        const int end = min(n, 64 * k + 64);
-        for (int s0 = 64 * k + w; s0 < end; s0 += G * WAVES) {
-            f32x4 x[G][2];
-#pragma unroll
-            for (int u = 0; u < G; u++) {
-                const float *p = a.part + place(min(s0 + u * WAVES, n - 1)) * a.dvp + 4 * lane;
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-                    x[u][c] = 256 * c + 4 * lane < a.dvp ? ldf4(p + 256 * c)
-                                                         : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < NK; k++) {
+            const int s = 64 * k + lane;
+            ms[k] = -INFINITY;
+            ls[k] = 0.0f;
+            if (64 * k < n && s < n) {
+                ms[k] = a.pm[place(s)];
+                ls[k] = a.pl[place(s)];
             }
+            m = fmaxf(m, ms[k]);
+        }
+        m = wave_max(m);
 #pragma unroll
-            for (int u = 0; u < G; u++) {
-                const int s = s0 + u * WAVES;
-                const float e = __shfl(ms[k], s & 63, 64);
-                if (s < end)
+        for (int k = 0; k < NK; k++) {
+            if (64 * k >= n) break;
+            ms[k] = tree_join_weight(ms[k], ls[k], m);
+            l += ms[k] * ls[k];
+        }
+        l = wave_sum(l);
+        if (a.sink && l != 0.0f)
+            l += __builtin_amdgcn_exp2f(a.sink[r - t * a.h] * 1.44269504088896340736f - m);
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        constexpr int G = 4;                          /* places in flight        */
 #pragma unroll
-                    for (int c = 0; c < 2; c++) v[c] += e * x[u][c];
+        for (int k = 0; k < NK; k++) {
+            if (64 * k >= n) break;
+            const int end = min(n, 64 * k + 64);
+            for (int s0 = 64 * k + w; s0 < end; s0 += G * WAVES) {
+                f32x4 x[G][2];
+#pragma unroll
+                for (int u = 0; u < G; u++) {
+                    const float *p = a.part + place(min(s0 + u * WAVES, n - 1)) * a.dvp + 4 * lane;
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        x[u][c] = 256 * c + 4 * lane < a.dvp ? ldf4(p + 256 * c)
+                                                             : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int u = 0; u < G; u++) {
+                    const int s = s0 + u * WAVES;
+                    const float e = __shfl(ms[k], s & 63, 64);
+                    if (s < end)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) v[c] += e * x[u][c];
+                }
             }
         }
-    }
-    auto store = [&](int c, f32x4 y4) {
-        if (c >= a.dv) return;
-        y4 = y4 * inv;
-        const float y[4] = {y4.x, y4.y, y4.z, y4.w};
-        T *d = o + (size_t)r * a.dv + c;
-        if (a.ovec) {
-            io_store<T, 4>(d, y);
+        auto store = [&](int c, f32x4 y4) {
+            if (c >= a.dv) return;
+            y4 = y4 * inv;
+            const float y[4] = {y4.x, y4.y, y4.z, y4.w};
+            T *d = o + (size_t)r * a.dv + c;
+            if (a.ovec) {
+                io_store<T, 4>(d, y);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
+            }
+        };
+        if constexpr (WAVES == 1) {
+            store(4 * lane, v[0]);
+            store(256 + 4 * lane, v[1]);
         } else {
+            sum[w][lane] = v[0];
+            sum[w][64 + lane] = v[1];
+            __syncthreads();
+            if (tid < TR_DV / 4) {
+                f32x4 y = sum[0][tid];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (c + e < a.dv) io_store<T, 1>(d + e, y + e);
+                for (int k = 1; k < WAVES; k++) y += sum[k][tid];
+                store(4 * tid, y);
+            }
         }
     };
-    if constexpr (WAVES == 1) {
-        store(4 * lane, v[0]);
-        store(256 + 4 * lane, v[1]);
+    if constexpr (WAVES > 1) {
+        if ((int)blockIdx.x < hd.rows) row(blockIdx.x);
     } else {
-        sum[w][lane] = v[0];
-        sum[w][64 + lane] = v[1];
-        __syncthreads();
-        if (tid < TR_DV / 4) {
-            f32x4 y = sum[0][tid];
-#pragma unroll
-            for (int k = 1; k < WAVES; k++) y += sum[k][tid];
-            store(4 * tid, y);
-        }
+        for (int i = (int)blockIdx.x * RJ_WAVES + wave; i < hd.rows; i += (int)gridDim.x * RJ_WAVES)
+            row(i);
     }
 }
 
@@ -550,8 +565,9 @@ __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
 template <class T>
 void join_launch(const JoinJob &a, T *o, hipStream_t st)
 {
+    const long long groups = (a.rows + RJ_WAVES - 1) / RJ_WAVES;
     if (a.rows >= RJ_ROWS)
-        hipLaunchKernelGGL((k_reqs_join<T, 1>), dim3((unsigned)((a.rows + RJ_WAVES - 1) / RJ_WAVES)),
+        hipLaunchKernelGGL((k_reqs_join<T, 1>), dim3((unsigned)(groups < RJ_GROUPS ? groups : RJ_GROUPS)),
                            dim3(RJ_THREADS), 0, st, a, o);
     else
         hipLaunchKernelGGL((k_reqs_join<T, RJ_WAVES>), dim3((unsigned)a.rows), dim3(RJ_THREADS), 0, st,
@@ -669,7 +685,7 @@ extern "C" int dsv4_gpu_reqs_plan_d(void *d_plan, size_t plan_bytes, const dsv4_
     a.inv_h = 1.0f / (float)h;
     a.by_slots = 1.0f / (256.0f * (float)a.per_cu);
     a.wave_more = products > 1 ? 0.05f : 0.02f;
-    a.max_items = (int)m.items;
+    a.max_items = reqs_items(m, r->n_req, a.br);
     a.max_parts = (int)m.parts;
     a.sig = reqs_sig(r, fmt, h, d_qk, d_v, kv_fmt, window);
     const size_t lds = 8 * ((size_t)r->n_req + 1) * sizeof(int);
@@ -752,7 +768,8 @@ extern "C" int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, 
     /* a workgroup for every item that there may be: blocks of 16 rows by tiles */
     const long long tiles = (long long)r->max_pages * r->page_rows / TR_TILE + 2;
     long long groups = (2 * (m.rows / 16) + r->n_req + 1) * tiles;
-    if (groups > m.items) groups = m.items;
+    const int items = reqs_items(m, r->n_req, dsv4_tree_block_rows(fmt, kv_fmt, kc));
+    if (groups > items) groups = items;
     const int rc = kv_fmt == DSV4_GPU_KV_F32 ? dsv4_reqs_f32_launch(a, fmt, kc, (unsigned)groups, st)
                  : kv_fmt == DSV4_GPU_KV_BF16
                      ? dsv4_reqs_bf16_launch(a, fmt, kc, (unsigned)groups, st)

@@ -81,6 +81,21 @@ def test_batches(gpu, dsv4, fmt, bf, dqk, dv, n_req, h, prefix, longest):
     check(got, *b.want(dv, 0, sink, 0.06), bf)
 
 
+@pytest.mark.parametrize("fmt,bf", [(1, True), (0, False)])
+@pytest.mark.parametrize("n_req,h,prefix,length,room", [
+    (3, 64, 0, 300, 9000), (300, 64, 96, 110, 0), (300, 64, 96, 110, 3000), (2, 1, 0, 2000, 100000)])
+def test_room_for_many_more_tokens(gpu, dsv4, fmt, bf, n_req, h, prefix, length, room):
+    """Few tokens where the step's buffers hold many, and many rows that are joined."""
+    b = rc.Batch(room + n_req, [length] * n_req, [1] * n_req, h, 40, fmt, bf, prefix=prefix, room=room)
+    check(b.call(dsv4, 24), *b.want(24), bf)
+
+
+def test_idle_requests_that_are_long(gpu, dsv4):
+    """Requests without tokens in this step have no part in it, whatever their length."""
+    b = rc.Batch(3, [70, 9000, 40, 130, 20000], [1, 0, 3, 1, 0], 16, 128, 1, True, prefix=64)
+    check(b.call(dsv4, 128), *b.want(128), True)
+
+
 def test_the_most_requests(gpu, dsv4):
     rng = np.random.default_rng(2)
     lens = rng.integers(0, 50, 4096)
