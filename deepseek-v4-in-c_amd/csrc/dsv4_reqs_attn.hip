@@ -17,6 +17,7 @@
 #include "dsv4_tree.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -440,13 +441,17 @@ struct JoinJob {
 };
 
 /* Rows whose sums lie in several places: the prefix's splits and then the request's.
- * WAVES waves a row: each has the weights, and adds every WAVES-th place. */
-template <class T, int WAVES>
+ * WAVES waves a row: each has the weights, and adds every WAVES-th place. Few rows have
+ * their workgroups' four (16 rows of 125 places 10 us, a wave a row 30; 512 of 4 6 and 7;
+ * 2048 the same), many a wave each (4096 of 4 places 9 us, with four waves 11; of 128
+ * columns 5 and 10). Bound: the places' bytes, 6 TB/s from L2 for many rows, and for few
+ * a chain of the head, the request, the maxima and the sums. */
+template <class T>
 __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
 {
-    __shared__ f32x4 sum[WAVES][TR_DV / 4];
+    __shared__ f32x4 sum[RJ_WAVES][TR_DV / 4];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = WAVES > 1 ? wave : 0;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Dsv4ReqsHead hd = *a.head;
     if (hd.sig != a.sig) {                        /* not this call's plan    */
         const float nan = __uint_as_float(0x7FC00000u);
@@ -455,7 +460,9 @@ __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
             io_store<T, 1>(o + i, &nan);
         return;
     }
-    auto row = [&](int i) {
+    auto row = [&](int i, auto waves) {
+        constexpr int WAVES = decltype(waves)::value;
+        const int w = WAVES > 1 ? wave : 0;
         const int r = hd.row0 + i, t = (int)a.by_h.div((uint32_t)r);
         /* the last request whose first token is t or before it: of every step-th one, then
          * of those behind it */
@@ -553,25 +560,20 @@ __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
             }
         }
     };
-    if constexpr (WAVES > 1) {
-        if ((int)blockIdx.x < hd.rows) row(blockIdx.x);
+    if (hd.rows < RJ_ROWS) {                      /* a workgroup for each at least */
+        if ((int)blockIdx.x < hd.rows) row(blockIdx.x, std::integral_constant<int, RJ_WAVES>());
     } else {
         for (int i = (int)blockIdx.x * RJ_WAVES + wave; i < hd.rows; i += (int)gridDim.x * RJ_WAVES)
-            row(i);
+            row(i, std::integral_constant<int, 1>());
     }
 }
 
-/* A wave a row where the rows fill the card. */
 template <class T>
 void join_launch(const JoinJob &a, T *o, hipStream_t st)
 {
-    const long long groups = (a.rows + RJ_WAVES - 1) / RJ_WAVES;
-    if (a.rows >= RJ_ROWS)
-        hipLaunchKernelGGL((k_reqs_join<T, 1>), dim3((unsigned)(groups < RJ_GROUPS ? groups : RJ_GROUPS)),
-                           dim3(RJ_THREADS), 0, st, a, o);
-    else
-        hipLaunchKernelGGL((k_reqs_join<T, RJ_WAVES>), dim3((unsigned)a.rows), dim3(RJ_THREADS), 0, st,
-                           a, o);
+    const long long waves = (a.rows + RJ_WAVES - 1) / RJ_WAVES, some = a.rows < RJ_ROWS ? a.rows : RJ_ROWS;
+    const long long groups = waves < some ? some : waves < RJ_GROUPS ? waves : RJ_GROUPS;
+    hipLaunchKernelGGL(k_reqs_join<T>, dim3((unsigned)groups), dim3(RJ_THREADS), 0, st, a, o);
 }
 
 /* What is wrong with a call's shape, or nullptr. */
