@@ -88,7 +88,13 @@ struct PlanCut {
  * of bf16, 576 columns), 2.2 and half a microsecond a wave of 16 rows are an item's start,
  * and then come the sums that are joined. Workgroups begin in their order, and those of
  * one XCD go to its four engines in turn, so the longest items come first and the short ones
- * fill what the last round of these leaves free, if every engine has a free CU. */
+ * fill what the last round of these leaves free, if every engine has a free CU: items by
+ * request took 420 us for 64 requests behind 32768 positions and these 364, 128 ragged
+ * ones 240 and 207, 570 tokens of prompts 125 and 89.
+ *
+ * Bound: the chain of a load, five reductions and two scans, and the fetch of code that
+ * runs once: 10 us for 8 requests, 13 for 128. Sums that are only compared are floats, and
+ * loops that could be unrolled are not (20 us unrolled, in whole numbers). */
 __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 {
     extern __shared__ __align__(16) int lds[];
@@ -428,7 +434,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 }
 
 constexpr int RJ_THREADS = 256, RJ_WAVES = RJ_THREADS / 64;
-constexpr int RJ_ROWS = 2048, RJ_GROUPS = 4096;
+constexpr int RJ_ROWS = 2048;                     /* from here on a wave a row */
+constexpr int RJ_GROUPS = 4096;
 
 struct JoinJob {
     const Dsv4ReqsHead *head;

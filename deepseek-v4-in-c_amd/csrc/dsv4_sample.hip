@@ -14,6 +14,11 @@
  * 2^(z - E) 2^sh, E an integer that no z of the row passes. The bins lie at the
  * same z for all slices of a row. z and the weights are in 64 bits: a pick that is
  * wrong by a rounding is another token.
+ *
+ * Two launches: slices of 8192 tokens, and a workgroup for each row. Bound: the
+ * vector unit and one LDS add a token where bins are made (256 rows of 129280 50 us),
+ * HBM where they are not (23 us, 2.9 TB/s), and for few rows the pick's chain of scans
+ * (16 us for 64 rows of top-k 200, 25 with bins) and its code's first fetch.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -39,7 +44,7 @@ constexpr int SP_LIST = SP_THREADS;               /* tokens put in order     */
 constexpr int SP_QUEUE = 2 * SP_LIST;              /* and looked through      */
 constexpr int SP_CHUNKS = 4096;                   /* chunks looked over at once */
 constexpr int SP_K = 512;                         /* a short top-k, for which no bins are made */
-constexpr int SP_DIRECT = 96;
+constexpr int SP_DIRECT = 128;                    /* tokens compared with all others */
 constexpr float SP_FLOOR = 0.0078125f;             /* a min_p for which none are made */
 static_assert(SP_THREADS == SM_BINS, "a bin a thread");
 
@@ -154,14 +159,19 @@ __device__ __forceinline__ u64 sm_bin_sum(double edge, uint32_t n, u64 part)
 }
 
 /* A top-k so short that the chunks with the k largest maxima, which have the k largest
- * tokens, have hardly more that are as large (256 of 2020 chunks: 274 tokens). */
+ * tokens, have hardly more that are as large (256 of 2020 chunks: 274 tokens). One row of
+ * 129280 and 64 take 12 and 18 us so for top-k 8 and 21 and 27 for 512, with bins 23 and
+ * 32, 31 and 40; for 800 there may be more than the list takes, 75 and 102 us for 35 and
+ * 46. */
 __device__ __forceinline__ bool sm_short(const SampleJob &a, int top_k)
 {
     return top_k > 0 && top_k <= SP_K && 2 * top_k <= a.nc && a.nc <= SP_CHUNKS;
 }
 
 /* A row whose only other limit is min_p: what is under it has no part in any sum, so
- * that its tokens are all that is looked at, if they fit the list. */
+ * that its tokens are all that is looked at, if they fit the list. 1 to 256 rows of 129280
+ * take 11 to 36 us so and 23 to 56 with bins; with 11000 tokens over it, which make the
+ * row's workgroup count the bins after all, 71 to 198 and 47 to 169. */
 __device__ __forceinline__ float sm_floor(const SampleJob &a, int row)
 {
     return a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
@@ -517,8 +527,9 @@ struct SmRow {
     }
 
     /* The place of thread tid's key among those of threads 0 .. n - 1, the largest first.
-     * All keys read by all threads are n^2 reads of LDS, 7 us for 444; over SP_DIRECT of
-     * them the range of their logits is cut into SP_THREADS parts first, 3 us. */
+     * All keys read by all threads are n^2 reads of LDS; over SP_DIRECT of them the range
+     * of their logits is cut into SP_THREADS parts first. One row's call takes 15.7 us for
+     * 100 so and 16.7 by parts, for 200 18.7 and 17.8, for 512 29 and 21. */
     __device__ __forceinline__ int order(int n, u64 key)
     {
         const int tid = threadIdx.x, lane = tid & 63;

@@ -301,7 +301,8 @@ k_tree(JOB a)
     int i0, i1, blk = 0, split = 0;
     Dsv4ReqsItem it{};
     if constexpr (REQS) {
-        /* each kind so */
+        /* Each kind of a plan's items so. An item a workgroup: a loop over items keeps
+         * too much alive across it and spills. */
         const Dsv4ReqsHead hd = *a.head;
         const int id = blockIdx.x;
         if (hd.sig != a.sig || id >= hd.end[DSV4_REQS_KINDS - 1]) return;
