@@ -287,7 +287,9 @@ k_tree(JOB a)
     /* where the next tile and all of q are in registers, few are left: with operands
      * six ahead spills took 1052 us where two ahead take 734 (8192 rows of bf16 q over
      * 32768 of FP8); with the widest rows the scales are read twice as well (687 us,
-     * and 639 so; narrower rows lose 2 % by it) */
+     * and 639 so; narrower rows lose 2 % by it). A batch's items, which keep less
+     * alive, have room for more ahead in the scores: 128 requests of 512 columns 213 us
+     * with two, 199 with three, 204 with six; of 576 241, 241 and 218 */
     constexpr bool SHALLOW = NT == 1 && KVF == DSV4_GPU_KV_FP8 && KC >= 16;
     constexpr bool AGAIN = SHALLOW && KC > 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -679,7 +681,10 @@ k_tree(JOB a)
         const int kb = ka ^ (KC1 & 1 & half) * 64;
         const int up = (KC1 & 1 & half) * L::SLAB;
         /* reads of 16 keys' piece of a chunk, KD of them ahead of the products */
-        constexpr int KU = 2 * KC1, KD = KT > 1 || SHALLOW ? 2 : KU < 6 ? KU : 6;
+        constexpr int KU = 2 * KC1, KD = SHALLOW && REQS ? (KC > 16 ? 6 : 3)
+                                         : KT > 1 || SHALLOW ? 2
+                                         : KU < 6            ? KU
+                                                             : 6;
         tr_bf8 row[KD][KT];
         auto rows_of = [&](int u) {
             const int kc = u >> 1;
