@@ -526,39 +526,49 @@ struct SmRow {
         return s.len;
     }
 
-    /* The place of thread tid's key among those of threads 0 .. n - 1, the largest first.
-     * All keys read by all threads are n^2 reads of LDS; over SP_DIRECT of them the range
-     * of their logits is cut into SP_THREADS parts first. One row's call takes 15.7 us for
-     * 100 so and 16.7 by parts, for 200 18.7 and 17.8, for 512 29 and 21. */
-    __device__ __forceinline__ int order(int n, u64 key)
+    /* Of SP_THREADS parts of the range of the keys of threads 0 .. n - 1, which has thread
+     * tid's, the largest first. */
+    __device__ __forceinline__ int part_of_range(int n, u64 key)
     {
-        const int tid = threadIdx.x, lane = tid & 63;
-        int i0 = 0, i1 = n, at = tid, d = 0;
-        if (n > SP_DIRECT) {
-            uint32_t k0 = tid < n ? (uint32_t)(key >> 32) : ~0u, k1 = tid < n ? k0 : 0;
+        const int tid = threadIdx.x;
+        uint32_t k0 = tid < n ? (uint32_t)(key >> 32) : ~0u, k1 = tid < n ? k0 : 0;
 #pragma unroll 1
-            for (int o = 32; o >= 1; o >>= 1) {
-                k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
-                k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
-            }
-            __syncthreads();
-            if (lane == 0) s.part[tid >> 6] = (u64)k0 << 32 | k1;
+        for (int o = 32; o >= 1; o >>= 1) {
+            k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
+            k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
+        }
+        __syncthreads();
+        if ((tid & 63) == 0) s.part[tid >> 6] = (u64)k0 << 32 | k1;
+        __syncthreads();
+        const u64 v = s.part[tid & (SP_WAVES - 1)];
+        k0 = (uint32_t)(v >> 32);
+        k1 = (uint32_t)v;
+#pragma unroll 1
+        for (int o = SP_WAVES / 2; o >= 1; o >>= 1) {
+            k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
+            k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
+        }
+        /* (a range that is not finite, or 0: all in one, as NaN becomes 0) */
+        const float top = sm_value((u64)k1 << 32), by = (SP_THREADS - 1) / (top - sm_value((u64)k0 << 32));
+        return (int)fminf(fmaxf((top - sm_value(key)) * by, 0.0f), SP_THREADS - 1.0f);
+    }
+
+    /* The place of thread tid's key among those of threads 0 .. n - 1, the largest first.
+     * All keys read by all threads are n^2 reads of LDS; over SP_DIRECT of them each is
+     * compared with those of its part d only, of SP_THREADS in the same order. One row's
+     * call takes 15.7 us for 100 so and 16.7 by parts, for 200 18.7 and 17.8, for 512 29 and
+     * 21. */
+    __device__ __forceinline__ int order(int n, u64 key, int d)
+    {
+        const int tid = threadIdx.x;
+        int i0 = 0, i1 = n, at = tid;
+        if (n > SP_DIRECT) {
             s.cur[tid] = 0;
             __syncthreads();
-#pragma unroll 1
-            for (int w = 0; w < SP_WAVES; w++) {
-                const u64 v = s.part[w];
-                k0 = min(k0, (uint32_t)(v >> 32));
-                k1 = max(k1, (uint32_t)v);
-            }
-            /* (a range that is not finite, or 0: all in one, as NaN becomes 0) */
-            const float top = sm_value((u64)k1 << 32), by = (SP_THREADS - 1) / (top - sm_value((u64)k0 << 32));
-            d = (int)fminf(fmaxf((top - sm_value(key)) * by, 0.0f), SP_THREADS - 1.0f);
             if (tid < n) at = (int)atomicAdd(&s.cur[d], 1u);
             __syncthreads();
             u64 none = 0;
-            const uint32_t c = s.cur[tid];
-            uint32_t e = c;
+            uint32_t e = s.cur[tid];
             scan(none, e);
             s.cur[tid] = e;
             __syncthreads();
@@ -614,7 +624,15 @@ struct SmRow {
         }
         __syncthreads();
         const u64 key = tid < n ? s.key[tid] : 0;
-        const int at = order(n, key);
+        int d = 0;
+        if (tid < n) {                            /* a part for each of a bin's tokens */
+            const double z = sc.z(sm_value(key)), q = sm_q(z);
+            const int bin = sm_bin(first, q), many = (int)(s.n[bin] - n_before(bin));
+            const float r = bin == SM_BINS - 1 ? 0.0f : 1.0f - (float)fma(z, 32.0, -q);
+            d = s.off[bin] + max(0, min((int)(r * (float)many), many - 1));
+        }
+        __syncthreads();
+        const int at = order(n, key, d);
         if (tid < n) {
             s.key[at] = key;
             s.queue[at] = weight(sc.z(sm_value(key)));
@@ -790,7 +808,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         const int len = r.queue(low, INFINITY, INFINITY, INFINITY);
         if (len <= SP_LIST) {
             const u64 key = tid < len ? s.queue[tid] : 0;
-            const int at = r.order(len, key);
+            const int at = r.order(len, key, len > SP_DIRECT ? r.part_of_range(len, key) : 0);
             if (tid < len) s.key[at] = key;
             __syncthreads();
             const int end = top_k > 0 ? min(top_k, len) : len;
@@ -948,31 +966,44 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const SmWhere at = s.where;
     const int kb = at.kb, pb0 = at.pb0, pb1 = at.pb1, mb = at.mb, ub0 = at.ub0, ub1 = at.ub1;
     const bool need_k = at.need_k, whole = at.whole;
-    const bool in = (need_k && tid == kb) ||
-                    (whole ? tid <= at.c1
-                           : (by_p && tid >= pb0 && tid <= pb1) || (by_floor && tid == mb) ||
-                                 (tid >= ub0 && tid <= ub1));
-    /* which lie in two ranges */
-    int b0 = 0, b1 = at.c1, b2 = need_k ? kb : 0, b3 = need_k ? kb : at.c1;
-    if (!whole) {
-        b0 = min(min(need_k ? kb : LAST, by_p ? pb0 : LAST), by_floor ? mb : LAST);
-        b1 = max(max(need_k ? kb : 0, by_p ? pb1 : 0), by_floor ? mb : 0);
-        if (b0 > b1) b0 = b1 = ub0;
-        b2 = ub0;
-        b3 = ub1;
-    }
-    u64 none = 0;
-    uint32_t len = in ? n : 0;
-    r.scan(none, len);
-    s.off[tid] = in && n ? (int)(len - n) : -1;
-    if (tid == LAST) s.len = (int)len;
-    __syncthreads();
-    const int listed = s.len;
-    __syncthreads();
-    /* key 0 is behind the whole bin */
-    SmPlace cut{0, s.sum[LAST], LAST, all};
-    if (listed <= SP_LIST && r.list(b0, b1, b2, b3, listed)) {
-        if (tid >= 64) return;
+    /* The list has the bins of the limits and of the pick; where they are too many
+     * together, of the limits first and then, as the cut is known, of the pick. */
+    SmPlace cut{0, s.sum[LAST], LAST, all};       /* key 0 is behind the whole bin */
+    bool limits = true, pick = true;
+    int u0 = ub0, u1 = ub1;
+#pragma unroll 1
+    for (;;) {
+        const bool in = whole ? (need_k && tid == kb) || tid <= at.c1
+                              : (limits && ((need_k && tid == kb) ||
+                                            (by_p && tid >= pb0 && tid <= pb1) ||
+                                            (by_floor && tid == mb))) ||
+                                    (pick && tid >= u0 && tid <= u1);
+        /* which lie in two ranges */
+        int b0 = 0, b1 = at.c1, b2 = need_k ? kb : 0, b3 = need_k ? kb : at.c1;
+        if (!whole) {
+            b0 = min(min(limits && need_k ? kb : LAST, limits && by_p ? pb0 : LAST),
+                     limits && by_floor ? mb : LAST);
+            b1 = max(max(limits && need_k ? kb : 0, limits && by_p ? pb1 : 0),
+                     limits && by_floor ? mb : 0);
+            if (b0 > b1) b0 = b1 = u0;
+            b2 = pick ? u0 : b0;
+            b3 = pick ? u1 : b1;
+        }
+        u64 none = 0;
+        uint32_t len = in ? n : 0;
+        r.scan(none, len);
+        s.off[tid] = in && n ? (int)(len - n) : -1;
+        if (tid == LAST) s.len = (int)len;
+        __syncthreads();
+        const int listed = s.len;
+        __syncthreads();
+        if (listed > SP_LIST) {
+            if (!(limits && pick) || whole || !(by_k || by_p || by_floor)) break;
+            pick = false;
+            continue;
+        }
+        if (!r.list(b0, b1, b2, b3, listed)) break;
+        if (pick && tid >= 64) return;
         auto place = [&](int b, int i) {
             return SmPlace{s.key[i], s.through[i], b, (int)r.n_before(b) + i - s.off[b] + 1};
         };
@@ -982,28 +1013,37 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             const int i = sm_first(listed, [&](int j) { return s.through[j] >= need; });
             return place(b, min(max(i, off), end));
         };
-        if (need_k) cut = place(kb, s.off[kb] + top_k - 1 - (int)r.n_before(kb));
-        if (by_p) {
-            const u64 need = part_of(cut.sum);
-            const int b = min(max(r.sum_bin(need), pb0), pb1);
-            if (s.off[b] >= 0) {                  /* else min_p cuts before it */
-                const SmPlace c = token(b, need);
+        if (limits) {
+            if (need_k) cut = place(kb, s.off[kb] + top_k - 1 - (int)r.n_before(kb));
+            if (by_p) {
+                const u64 need = part_of(cut.sum);
+                const int b = min(max(r.sum_bin(need), pb0), pb1);
+                if (s.off[b] >= 0) {              /* else min_p cuts before it */
+                    const SmPlace c = token(b, need);
+                    if (c.n < cut.n) cut = c;
+                }
+            }
+            if (by_floor && mb <= cut.bin) {
+                /* up to the first of the bin that is under it */
+                SmPlace c{~0ull, r.sum_before(mb), mb, (int)r.n_before(mb)};
+                const int off = s.off[mb];
+                if (off >= 0) {
+                    const int i = sm_first((int)(s.n[mb] - r.n_before(mb)),
+                                           [&](int j) { return under(s.key[off + j]); });
+                    if (i > 0) c = place(mb, off + i - 1);
+                }
                 if (c.n < cut.n) cut = c;
             }
         }
-        if (by_floor && mb <= cut.bin) {
-            /* up to the first of the bin that is under it */
-            SmPlace c{~0ull, r.sum_before(mb), mb, (int)r.n_before(mb)};
-            const int off = s.off[mb];
-            if (off >= 0) {
-                const int i = sm_first((int)(s.n[mb] - r.n_before(mb)),
-                                       [&](int j) { return under(s.key[off + j]); });
-                if (i > 0) c = place(mb, off + i - 1);
-            }
-            if (c.n < cut.n) cut = c;
-        }
         const u64 need = place_of(cut.sum);
-        const SmPlace got = token(min(min(max(r.sum_bin(need), ub0), ub1), cut.bin), need);
+        if (!pick) {
+            u0 = u1 = min(min(max(r.sum_bin(need), ub0), ub1), cut.bin);
+            limits = false;
+            pick = true;
+            __syncthreads();
+            continue;
+        }
+        const SmPlace got = token(min(min(max(r.sum_bin(need), u0), u1), cut.bin), need);
         if (tid == 0) {
             /* behind the cut only by the roundings of the bins' sums */
             const u64 best = got.n > cut.n ? cut.key : got.key;
@@ -1012,6 +1052,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         }
         return;
     }
+    cut = SmPlace{0, s.sum[LAST], LAST, all};
 
     /* ---- more tokens than the list takes: each limit and then the pick by passes over the
      *      row. Where the order passes `need` tokens or the sum `need`, in a bin that is
