@@ -23,6 +23,8 @@
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
 
+#include <type_traits>
+
 namespace {
 
 #include "dsv4_rows_io.h"
@@ -450,11 +452,11 @@ struct SmRow {
         if (sc.inf || b0 == 0 || !(*hi < INFINITY)) *hi = INFINITY;
     }
 
-    /* f(x, token) for every token of the row from lo to hi, or from lo2 to hi2 (lo <= lo2):
-     * a chunk whose largest is less has none. The whole workgroup; 16 lanes a chunk, so that a load takes 1 KB of
-     * four chunks, and G loads in flight. */
+    /* f(G, x [G][4], token [G]) for the row's chunks whose largest is lo or more, G times four
+     * tokens of a lane at once (-infinity where there are none). The whole workgroup; 16
+     * lanes a chunk, so that a load takes 1 KB of four chunks. */
     template <int G, class F>
-    __device__ __forceinline__ void each_of_row(float lo, float hi, float lo2, float hi2, F f)
+    __device__ __forceinline__ void each_of_row(float lo, F f)
     {
         const int tid = threadIdx.x;
 #pragma unroll 1
@@ -475,15 +477,15 @@ struct SmRow {
             }
             __syncthreads();
             const int n = s.chunks;
-            if (n <= SP_THREADS / 16) chunks<1>(c0, n, lo, hi, lo2, hi2, f);
-            else chunks<G>(c0, n, lo, hi, lo2, hi2, f);
+            if (n <= SP_THREADS / 16) chunks<1>(c0, n, f);
+            else chunks<G>(c0, n, f);
         }
         __syncthreads();
     }
 
     /* The listed chunks, 16 lanes each, G of them in flight. */
     template <int G, class F>
-    __device__ __forceinline__ void chunks(int c0, int n, float lo, float hi, float lo2, float hi2, F f)
+    __device__ __forceinline__ void chunks(int c0, int n, F f)
     {
         constexpr int EACH = SP_THREADS / 16;
         const int tid = threadIdx.x, whole = a.vocab / SM_CHUNK;
@@ -505,23 +507,54 @@ struct SmRow {
                         if (t[u] + k < a.vocab) io_load<T, 1>(x + t[u] + k, v[u] + k);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < G; u++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (__builtin_amdgcn_fmed3f(v[u][k], lo, hi) == v[u][k] ||
-                        __builtin_amdgcn_fmed3f(v[u][k], lo2, hi2) == v[u][k])
-                        f(v[u][k], t[u] + k);
+            f(std::integral_constant<int, G>(), v, t);
         }
     }
 
-    /* Queue the tokens of two ranges of logits; how many, over SP_QUEUE: not all. */
+    /* Queue the tokens that in(x) holds for, of chunks whose largest is lo or more. One
+     * add for all of a wave's. */
+    template <class F>
+    __device__ __forceinline__ void queue_where(float lo, F in)
+    {
+        const int lane = threadIdx.x & 63;
+        each_of_row<2>(lo, [&](auto groups, float (*v)[4], const int *t) {
+            constexpr int G = decltype(groups)::value;
+            u64 hit[G][4];
+            int many = 0;
+#pragma unroll
+            for (int u = 0; u < G; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    hit[u][k] = __ballot(in(v[u][k]));
+                    many += (int)__popcll(hit[u][k]);
+                }
+            if (!many) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&s.len, many);
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int u = 0; u < G; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (!hit[u][k]) continue;
+                    const int i = at + (int)__popcll(hit[u][k] & ((1ull << lane) - 1));
+                    if (hit[u][k] >> lane & 1 && i < SP_QUEUE) s.queue[i] = am_key(v[u][k], t[u] + k);
+                    at += (int)__popcll(hit[u][k]);
+                }
+        });
+    }
+    /* Of one range of logits, or of two (lo <= lo2); how many, over SP_QUEUE: not all. */
+    __device__ __forceinline__ int queue(float lo, float hi)
+    {
+        if (threadIdx.x == 0) s.len = 0;
+        queue_where(lo, [&](float x) { return __builtin_amdgcn_fmed3f(x, lo, hi) == x; });
+        return s.len;
+    }
     __device__ __forceinline__ int queue(float lo, float hi, float lo2, float hi2)
     {
         if (threadIdx.x == 0) s.len = 0;
-        each_of_row<8>(lo, hi, lo2, hi2, [&](float v, int t) {
-            const int at = atomicAdd(&s.len, 1);
-            if (at < SP_QUEUE) s.queue[at] = am_key(v, t);
+        queue_where(lo, [&](float x) {
+            return __builtin_amdgcn_fmed3f(x, lo, hi) == x || __builtin_amdgcn_fmed3f(x, lo2, hi2) == x;
         });
         return s.len;
     }
@@ -612,7 +645,7 @@ struct SmRow {
             hi = hi2;
             hi2 = t;
         }
-        const int len = queue(lo, hi, lo2, hi2);
+        const int len = hi2 <= hi ? queue(lo, hi) : queue(lo, hi, lo2, hi2);
         if (len > SP_QUEUE) return false;
 #pragma unroll 1
         for (int i = tid; i < len; i += SP_THREADS) {
@@ -750,6 +783,14 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         return sm_exp2(r.sc.z(sm_value(key)) - zmost) < (double)floor_;
     };
     const bool by_p = p < 1.0f, by_floor = floor_ > 0.0f;
+    auto each = [](auto f) {                      /* f(x, token) for a batch of them */
+        return [f](auto groups, float (*v)[4], const int *t) {
+#pragma unroll
+            for (int u = 0; u < decltype(groups)::value; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) f(v[u][k], t[u] + k);
+        };
+    };
 
     /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order; or a
      *      min_p alone: those that it may leave ---- */
@@ -805,7 +846,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         fits = __all(fits);
     }
     if (fits) {
-        const int len = r.queue(low, INFINITY, INFINITY, INFINITY);
+        const int len = r.queue(low, INFINITY);
         if (len <= SP_LIST) {
             const u64 key = tid < len ? s.queue[tid] : 0;
             const int at = r.order(len, key, len > SP_DIRECT ? r.part_of_range(len, key) : 0);
@@ -895,7 +936,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         __syncthreads();
         s.mass[tid] = 0;
         s.cur[tid] = 0;
-        r.template each_of_row<2>(-3.4028235e38f, INFINITY, INFINITY, INFINITY, [&](float v, int) {
+        r.template each_of_row<2>(-3.4028235e38f, each([&](float v, int) {
+            if (!(v > -INFINITY)) return;
             const double z = r.sc.z(v), q = sm_q(z);
             const int bin = sm_bin(r.first, q);
             if (bin < LAST) {
@@ -905,7 +947,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
                 rest_n++;
                 rest += sm_weight(z - r.e, a.sh);
             }
-        });
+        }));
         n = s.cur[tid];
         part = s.mass[tid];
     }
@@ -1093,7 +1135,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             s.best[tid] = 0;
             s.cur[tid] = 0;
             if (tid == 0) s.hit = {~0ull, sum0, phase == 2 ? b : -1, (int)n0};
-            r.template each_of_row<2>(xlo, xhi, xlo, xhi, [&](float v, int t) {
+            r.template each_of_row<2>(xlo, each([&](float v, int t) {
+                if (__builtin_amdgcn_fmed3f(v, xlo, xhi) != v) return;
                 const double z = r.sc.z(v);
                 if (sm_bin(r.first, sm_q(z)) != b) return;
                 const u64 key = am_key(v, t), w = r.weight(z);
@@ -1109,7 +1152,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
                 atomicAdd(&s.mass[d], w);
                 atomicAdd(&s.cur[d], 1u);
                 atomicMax(&s.best[d], key);
-            });
+            }));
             if (phase == 2) {
                 got = s.hit;
                 break;
