@@ -123,6 +123,20 @@ def test_min_p_alone(gpu, dsv4, vocab, few):
           u=rng.random(6).astype(np.float32))
 
 
+@pytest.mark.parametrize("vocab", [60000, 129280])
+@pytest.mark.parametrize("bf", [False, True])
+def test_flat_rows(gpu, dsv4, vocab, bf):
+    """Rows whose limits' and pick's tokens stand among hundreds to thousands that weigh
+    about the same, which are too many together or alone."""
+    rng = np.random.default_rng(vocab + bf)
+    x = rng.standard_normal((32, vocab)).astype(np.float32) * np.float32(2)
+    t = np.exp(rng.uniform(np.log(0.5), np.log(6), 32))
+    k = np.where(np.arange(32) % 4 == 3, rng.integers(2000, vocab, 32), 0)
+    p = np.where(np.arange(32) % 4 == 2, 1.0, rng.uniform(0.5, 0.99, 32))
+    m = np.where(np.arange(32) % 8 == 1, 10.0 ** rng.uniform(-4, -1, 32), 0.0)
+    check(dsv4, x, bf, temperature=t, top_k=k, top_p=p, min_p=m, u=rng.random(32).astype(np.float32))
+
+
 @pytest.mark.parametrize("vocab", [20000, 129280, 262145, 300000])
 def test_likely_tokens_that_stand_together(gpu, dsv4, vocab):
     """Sorted logits, and a block of equal ones: many tokens of few chunks as large as
