@@ -90,7 +90,7 @@ struct PlanCut {
  * one XCD go to its four engines in turn, so the longest items come first and the short ones
  * fill what the last round of these leaves free, if every engine has a free CU: items by
  * request took 420 us for 64 requests behind 32768 positions and these 364, 128 ragged
- * ones 240 and 207, 570 tokens of prompts 125 and 89.
+ * ones 240 and 201, 570 tokens of prompts 125 and 73.
  *
  * Bound: the chain of a load, five reductions and two scans, and the fetch of code that
  * runs once: 10 us for 8 requests, 13 for 128. Sums that are only compared are floats, and
@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
         const int most = min(each, longest[g]), ps = PlanCut(each).splits(ptiles);
         const PlanCut cut(each);
         const float half = 0.5f * (float)most;
-        float items = 0.0f, parts = 0.0f, big = 0.0f;  /* big: of half the longest or more */
+        float items = 0.0f, parts = 0.0f;
+        float big = 0.0f, big_tiles = 0.0f;       /* of half the longest or more */
         if (on) {
             for (int b = cl; b < nr; b += 16) {
                 const int toks_b = s_to[4 * b], rows = s_to[4 * b + 1], t = s_to[4 * b + 2 + apart];
@@ -237,8 +238,14 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
                 const float n = (float)((rows + r - 1) >> rs) * (float)ns;
                 items += n;
                 parts += apart || ns > 1 ? (float)ns * (float)rows : 0.0f;
-                const float spread = fmaxf(2.0f * ((float)t - mean_tiles(toks_b, t, toks)), 1e-3f);
-                big += n * fminf(fmaxf(((float)t - half * (float)ns) * __builtin_amdgcn_rcpf(spread), 0.0f), 1.0f);
+                /* blocks' tiles lie about evenly from 2 mean - t to t */
+                const float least = fmaxf(2.0f * mean_tiles(toks_b, t, toks) - (float)t, 0.0f);
+                const float of_item = half * (float)ns, spread = fmaxf((float)t - least, 1e-3f);
+                const float longer = n * fminf(fmaxf(((float)t - of_item) * __builtin_amdgcn_rcpf(spread),
+                                                     0.0f), 1.0f);
+                big += longer;
+                big_tiles += longer * 0.5f * ((float)t + fmaxf(of_item, least)) *
+                             __builtin_amdgcn_rcpf((float)max(ns, 1));
             }
         }
 #pragma unroll 1
@@ -246,6 +253,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
             items += __shfl_xor(items, o, 64);
             parts += __shfl_xor(parts, o, 64);
             big += __shfl_xor(big, o, 64);
+            big_tiles += __shfl_xor(big_tiles, o, 64);
         }
         items += (float)pblocks * (float)ps;
         parts += (float)ps * (float)R;
@@ -259,12 +267,16 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
             const float slots = 256.0f * a.per_cu, by = a.by_slots, n = items;
             const float tile = a.tile_us * (1.0f + a.wave_more * waves);
             const float start = 2.2f + 0.55f * waves;
-            if (ps && (float)ptiles >= half * ps) big += (float)pblocks * ps;
+            if (ps && (float)ptiles >= half * ps) {
+                big += (float)pblocks * ps;
+                big_tiles += (float)pblocks * (float)ptiles;
+            }
             const float one = (float)most * tile + start, all = w * tile + n * start;
             const float rounds = fmaxf(ceilf(big * by), 1.0f);
             const float flow = all * by + 0.6f * one;
-            const bool fits = big >= n || (rounds * slots - big >= 0.125f * slots &&
-                                           all <= 0.97f * rounds * slots * one);
+            const float rest = (w - big_tiles) * tile + (n - big) * start;
+            const float spare = rounds * slots - big;
+            const bool fits = big >= n || (spare >= 0.125f * slots && rest <= 0.9f * spare * one);
             float cost = fmaxf(fits ? big >= n ? fminf(rounds * one, flow) : rounds * one : flow, one);
             cost += (parts > 0.0f ? 1.4f : 0.0f) + parts * (float)a.dvp * 0.92e-6f;
             /* a price over 0 orders as its bits do */
