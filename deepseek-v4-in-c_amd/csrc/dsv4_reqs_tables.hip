@@ -13,7 +13,7 @@
  * Bound: latency, a chain of one load, two scans of the workgroup and the search
  * (12 n_tok bytes are written). Each workgroup makes the sums of all requests for
  * itself in LDS rather than wait for a launch that does. 64 requests of a token 8.6
- * us; 1000 requests with about 40000 tokens 13 and 6.6 for the state's launch.
+ * us; 1000 requests with about 40000 tokens 13, and 6.6 for a launch of the state's own.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -96,8 +96,8 @@ __device__ __forceinline__ void rt_top(int &a, int &b, int (*part)[2])
 }
 
 /* tokens: this launch writes the maps, the new entries and the ended requests'
- * pages; state: the lengths, first tokens and the ring's place (by one
- * workgroup, after every read of the old ones). */
+ * pages; state: the first workgroup writes the lengths, first tokens and the ring's
+ * place (after every read of the old ones, where it may write over them). */
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) k_reqs_tables(TablesJob a, bool tokens, bool state)
 {
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(THREADS) k_reqs_tables(TablesJob a, bool token
             }
         }
     }
-    if (state) {
+    if (state && blockIdx.x == 0) {
         for (int i = tid; i <= n; i += THREADS) a.first[i] = first[i];
         for (int i = tid; i < n; i += THREADS)
             a.len[i] = a.add[i] < 0 ? 0 : have[i] + first[i + 1] - first[i];
@@ -275,12 +275,26 @@ extern "C" int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, 
                                state);
         return hipGetLastError();
     };
-    /* one workgroup's tokens and state in one launch; else the state, which may lie
-     * where the old one does, after the workgroups that read that */
+    /* One launch, where it is one workgroup's or the state is not written over the old one
+     * that others read; else the state after them (1000 requests with about 40000 tokens
+     * 20 us, in one launch 14). */
     const int threads = r->n_req <= 256 ? 256 : 1024, each = threads * RT_TOKENS;
     const int groups = (r->max_tok + each - 1) / each;
-    if (groups <= 1) {
-        HIP_OK(launch(1, true, true), "reqs tables launch");
+    auto meet = [](const int *w, size_t nw, const int *v, size_t nv) {
+        const uintptr_t a0 = (uintptr_t)w, b0 = (uintptr_t)v;
+        return a0 < b0 + nv * sizeof(int) && b0 < a0 + nw * sizeof(int);
+    };
+    const size_t n = (size_t)r->n_req;
+    const struct {
+        const int *p;
+        size_t n;
+    } writes[3] = {{r->len, n}, {r->first, n + 1}, {d_free_out, 2}},
+      reads[3] = {{d_len, n}, {d_new, n}, {d_free, 2}};
+    bool over = false;
+    for (const auto &w : writes)
+        for (const auto &v : reads) over |= meet(w.p, w.n, v.p, v.n);
+    if (groups <= 1 || !over) {
+        HIP_OK(launch(groups < 1 ? 1 : groups < 256 ? groups : 256, true, true), "reqs tables launch");
         return 0;
     }
     HIP_OK(launch(groups < 256 ? groups : 256, true, false), "reqs tables launch");

@@ -666,7 +666,7 @@ struct SmRow {
             const double z = sc.z(sm_value(key)), q = sm_q(z);
             const int bin = sm_bin(first, q), many = (int)(s.n[bin] - n_before(bin));
             const float r = bin == SM_BINS - 1 ? 0.0f : 1.0f - (float)fma(z, 32.0, -q);
-            d = s.off[bin] + max(0, min((int)(r * (float)many), many - 1));
+            d = max(0, s.off[bin] + max(0, min((int)(r * (float)many), many - 1)));
         }
         __syncthreads();
         const int at = order(n, key, d);
