@@ -71,6 +71,43 @@ struct PlanReq {
     int n, pos, tile0, tile1;
 };
 
+/* The sum of lanes 0 to this one's, by moves within the vector unit. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v)
+{
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += moved<0x111, 0xF>(v);                    /* row_shr:1, 2, 4, 8      */
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<DPP_ROW_BCAST15, 0xA>(v);
+    v += moved<DPP_ROW_BCAST31, 0xC>(v);
+    return v;
+}
+
+/* The largest of all lanes' v, none of them negative. */
+__device__ __forceinline__ int wave_top(int v)
+{
+    v = max(v, moved<DPP_QUAD_XOR1, 0xF>(v));
+    v = max(v, moved<DPP_QUAD_XOR2, 0xF>(v));
+    v = max(v, moved<DPP_ROW_HMIRROR, 0xF>(v));
+    v = max(v, moved<DPP_ROW_MIRROR, 0xF>(v));
+    v = max(v, moved<DPP_ROW_BCAST15, 0xA>(v));
+    v = max(v, moved<DPP_ROW_BCAST31, 0xC>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+/* The sum over 16 lanes. */
+__device__ __forceinline__ float row_sum(float v)
+{
+    v += dpp_f<DPP_QUAD_XOR1, 0xF>(v);
+    v += dpp_f<DPP_QUAD_XOR2, 0xF>(v);
+    v += dpp_f<DPP_ROW_HMIRROR, 0xF>(v);
+    return v + dpp_f<DPP_ROW_MIRROR, 0xF>(v);
+}
+
 /* Tiles cut into items of about `each`: how many, to RP_SPLITS. A quotient of floats
  * may be one off, which makes an item a little longer or shorter. */
 struct PlanCut {
@@ -93,8 +130,9 @@ struct PlanCut {
  * ones 240 and 201, 570 tokens of prompts 125 and 73.
  *
  * Bound: the chain of a load, five reductions and two scans, and the fetch of code that
- * runs once: 10 us for 8 requests, 13 for 128. Sums that are only compared are floats, and
- * loops that could be unrolled are not (20 us unrolled, in whole numbers). */
+ * runs once: 8 us for 8 requests, 12 for 128. Sums that are only compared are floats,
+ * lanes add up within the vector unit (through LDS 10 and 13), loops that could be unrolled
+ * are not (20 us unrolled, in whole numbers). */
 __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
 {
     extern __shared__ __align__(16) int lds[];
@@ -154,16 +192,14 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
             own = o > own ? o : own;
         }
         if ((tid & ~63) < nr) {                   /* a wave, whole or not at all */
-#pragma unroll 1                                  /* run once: short code is fast code */
-            for (int o = 32; o >= 1; o >>= 1) {
-                b_bad |= __shfl_xor(b_bad, o, 64);
-                n_act += __shfl_xor(n_act, o, 64);
-                hmin = min(hmin, __shfl_xor(hmin, o, 64));
-                lmax = max(lmax, __shfl_xor(lmax, o, 64));
-                lmin = min(lmin, __shfl_xor(lmin, o, 64));
-                const unsigned long long v = __shfl_xor(own, o, 64);
-                own = v > own ? v : own;
-            }
+            b_bad = wave_top(b_bad);
+            n_act = __builtin_amdgcn_readlane(wave_scan(n_act), 63);
+            hmin = INT32_MAX - wave_top(INT32_MAX - hmin);
+            lmax = wave_top(lmax);
+            lmin = INT32_MAX - wave_top(INT32_MAX - lmin);
+            const int len = wave_top((int)(own >> 32));
+            own = (unsigned long long)len << 32 |
+                  (uint32_t)wave_top((int)(own >> 32) == len ? (int)own : 0);
             if (lane == 0) {
                 if (b_bad) bad = 1;
                 atomicAdd(&active, n_act);
@@ -208,11 +244,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
             w += (float)((rows + r - 1) >> rs) * mean_tiles(n, t, toks);
             l = max(l, t);
         }
-#pragma unroll 1
-        for (int o = 32; o >= 1; o >>= 1) {
-            w += __shfl_xor(w, o, 64);
-            l = max(l, __shfl_xor(l, o, 64));
-        }
+        w = wave_sum(w);
+        l = wave_top(l);
         if (lane == 0) {
             work[tid >> 6] = w;
             atomicMax(&longest[g], l);
@@ -248,13 +281,10 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
                              __builtin_amdgcn_rcpf((float)max(ns, 1));
             }
         }
-#pragma unroll 1
-        for (int o = 8; o >= 1; o >>= 1) {
-            items += __shfl_xor(items, o, 64);
-            parts += __shfl_xor(parts, o, 64);
-            big += __shfl_xor(big, o, 64);
-            big_tiles += __shfl_xor(big_tiles, o, 64);
-        }
+        items = row_sum(items);
+        parts = row_sum(parts);
+        big = row_sum(big);
+        big_tiles = row_sum(big_tiles);
         items += (float)pblocks * (float)ps;
         parts += (float)ps * (float)R;
         /* Sums of at most 4096 floats: 2^-12 off at most. The largest blocks, whole, are
@@ -337,14 +367,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_reqs_plan(PlanJob a)
     }
     int x[NX];
 #pragma unroll
-    for (int k = 0; k < NX; k++) x[k] = sum[k];
-#pragma unroll 1
-    for (int o = 1; o < 64; o *= 2)
-#pragma unroll
-        for (int k = 0; k < NX; k++) {
-            const int v = __shfl_up(x[k], o, 64);
-            if (lane >= o) x[k] += v;
-        }
+    for (int k = 0; k < NX; k++) x[k] = wave_scan(sum[k]);
     if (lane == 63)
 #pragma unroll
         for (int k = 0; k < NX; k++) part_w[tid >> 6][k] = x[k];
