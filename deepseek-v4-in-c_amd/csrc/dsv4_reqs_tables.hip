@@ -12,8 +12,8 @@
  *
  * Bound: latency, a chain of one load, two scans of the workgroup and the search
  * (12 n_tok bytes are written). Each workgroup makes the sums of all requests for
- * itself in LDS rather than wait for a launch that does. 64 requests of a token 8.6
- * us; 1000 requests with about 40000 tokens 13, and 6.6 for a launch of the state's own.
+ * itself in LDS rather than wait for a launch that does. 64 requests of a token 7.8
+ * us; 1000 requests with about 40000 tokens 11.7, and 6 for a launch of the state's own.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
@@ -45,20 +45,38 @@ __device__ __forceinline__ int rt_add(int a, int b)
     return s > (uint32_t)RT_MAX ? RT_MAX : (int)s;
 }
 
+/* The sum of lanes 0 to this one's, by moves within the vector unit. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int rt_moved(int v)
+{
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int rt_wave_scan(int v)
+{
+    v = rt_add(v, rt_moved<0x111, 0xF>(v));       /* row_shr:1, 2, 4, 8      */
+    v = rt_add(v, rt_moved<0x112, 0xF>(v));
+    v = rt_add(v, rt_moved<0x114, 0xF>(v));
+    v = rt_add(v, rt_moved<0x118, 0xF>(v));
+    v = rt_add(v, rt_moved<DPP_ROW_BCAST15, 0xA>(v));
+    return rt_add(v, rt_moved<DPP_ROW_BCAST31, 0xC>(v));
+}
+/* The largest of all lanes' v, none of them negative, in lane 63. */
+__device__ __forceinline__ int rt_wave_top(int v)
+{
+    v = max(v, rt_moved<DPP_QUAD_XOR1, 0xF>(v));
+    v = max(v, rt_moved<DPP_QUAD_XOR2, 0xF>(v));
+    v = max(v, rt_moved<DPP_ROW_HMIRROR, 0xF>(v));
+    v = max(v, rt_moved<DPP_ROW_MIRROR, 0xF>(v));
+    v = max(v, rt_moved<DPP_ROW_BCAST15, 0xA>(v));
+    return max(v, rt_moved<DPP_ROW_BCAST31, 0xC>(v));
+}
+
 /* Exclusive sums of a and b over the workgroup's threads. */
 template <int W>
 __device__ __forceinline__ void rt_scan(int &a, int &b, int (*part)[2])
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int x = a, y = b;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int u = __shfl_up(x, o, 64), v = __shfl_up(y, o, 64);
-        if (lane >= o) {
-            x = rt_add(x, u);
-            y = rt_add(y, v);
-        }
-    }
+    const int x = rt_wave_scan(a), y = rt_wave_scan(b);
     __syncthreads();                              /* part was read           */
     if (lane == 63) {
         part[w][0] = x;
@@ -78,13 +96,10 @@ __device__ __forceinline__ void rt_scan(int &a, int &b, int (*part)[2])
 template <int W>
 __device__ __forceinline__ void rt_top(int &a, int &b, int (*part)[2])
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        a = max(a, __shfl_xor(a, o, 64));
-        b = max(b, __shfl_xor(b, o, 64));
-    }
+    a = rt_wave_top(a);
+    b = rt_wave_top(b);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
+    if ((threadIdx.x & 63) == 63) {
         part[threadIdx.x >> 6][0] = a;
         part[threadIdx.x >> 6][1] = b;
     }
@@ -277,7 +292,7 @@ extern "C" int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, 
     };
     /* One launch, where it is one workgroup's or the state is not written over the old one
      * that others read; else the state after them (1000 requests with about 40000 tokens
-     * 20 us, in one launch 14). */
+     * 17 us, in one launch 11). */
     const int threads = r->n_req <= 256 ? 256 : 1024, each = threads * RT_TOKENS;
     const int groups = (r->max_tok + each - 1) / each;
     auto meet = [](const int *w, size_t nw, const int *v, size_t nv) {
