@@ -344,6 +344,23 @@ __device__ __forceinline__ V sm_wave_scan(V v)
     return v;
 }
 
+/* The largest of all lanes' v; of their pairs. */
+__device__ __forceinline__ uint32_t sm_wave_top(uint32_t v)
+{
+    v = max(v, sm_dpp<DPP_QUAD_XOR1, 0xF>(v));
+    v = max(v, sm_dpp<DPP_QUAD_XOR2, 0xF>(v));
+    v = max(v, sm_dpp<DPP_ROW_HMIRROR, 0xF>(v));
+    v = max(v, sm_dpp<DPP_ROW_MIRROR, 0xF>(v));
+    v = max(v, sm_dpp<DPP_ROW_BCAST15, 0xA>(v));
+    v = max(v, sm_dpp<DPP_ROW_BCAST31, 0xC>(v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ u64 sm_wave_top(u64 v)
+{
+    const uint32_t h = sm_wave_top((uint32_t)(v >> 32));
+    return (u64)h << 32 | sm_wave_top((uint32_t)(v >> 32) == h ? (uint32_t)v : 0u);
+}
+
 /* The bins of top-k, top-p (between two), min-p, the last cut (at most) and the pick. */
 struct SmWhere {
     int kb, pb0, pb1, mb, c1, ub0, ub1, need_k, whole;
@@ -569,22 +586,14 @@ struct SmRow {
     {
         const int tid = threadIdx.x;
         uint32_t k0 = tid < n ? (uint32_t)(key >> 32) : ~0u, k1 = tid < n ? k0 : 0;
-#pragma unroll 1
-        for (int o = 32; o >= 1; o >>= 1) {
-            k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
-            k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
-        }
+        k0 = ~sm_wave_top(~k0);
+        k1 = sm_wave_top(k1);
         __syncthreads();
         if ((tid & 63) == 0) s.part[tid >> 6] = (u64)k0 << 32 | k1;
         __syncthreads();
         const u64 v = s.part[tid & (SP_WAVES - 1)];
-        k0 = (uint32_t)(v >> 32);
-        k1 = (uint32_t)v;
-#pragma unroll 1
-        for (int o = SP_WAVES / 2; o >= 1; o >>= 1) {
-            k0 = min(k0, (uint32_t)__shfl_xor((int)k0, o, 64));
-            k1 = max(k1, (uint32_t)__shfl_xor((int)k1, o, 64));
-        }
+        k0 = ~sm_wave_top(~(uint32_t)(v >> 32));
+        k1 = sm_wave_top((uint32_t)v);
         /* (a range that is not finite, or 0: all in one, as NaN becomes 0) */
         const float top = sm_value((u64)k1 << 32), by = (SP_THREADS - 1) / (top - sm_value((u64)k0 << 32));
         return (int)fminf(fmaxf((top - sm_value(key)) * by, 0.0f), SP_THREADS - 1.0f);
@@ -740,9 +749,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
 #pragma unroll
     for (int k = 0; k < SP_CHUNKS / SP_THREADS; k++)
         if (r.cm[k] > -INFINITY) least = min(least, (uint32_t)(am_key(r.cm[k], 0) >> 32));
-    most = wave_max_u64(most);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+    most = sm_wave_top(most);
+    least = ~sm_wave_top(~least);
     if (lane == 0) {
         s.part[tid >> 6] = most;
         s.npart[tid >> 6] = least;
@@ -752,7 +760,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         s.tail_n = 0;
     }
     __syncthreads();
-    most = wave_max_u64(s.part[lane & (SP_WAVES - 1)]);
+    most = sm_wave_top(s.part[lane & (SP_WAVES - 1)]);
     if (most == 0) {
         if (tid == 0) done(-1, 0.0f, 0);
         return;
@@ -762,7 +770,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         const int t = sm_token(most) * SM_CHUNK + lane;
         float v = -INFINITY;
         if (t < a.vocab) io_load<T, 1>(r.x + t, &v);
-        const u64 k = wave_max_u64(v > -INFINITY ? am_key(v, t) : 0);
+        const u64 k = sm_wave_top(v > -INFINITY ? am_key(v, t) : 0);
         if (tid == 0) done(sm_token(k), 1.0f, 1);
         return;
     }
@@ -802,9 +810,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     float low = INFINITY;
     if (few) {
         /* that chunk's maximum, or a little less: the range of keys split by 1024 */
-        uint32_t key0 = s.npart[lane & (SP_WAVES - 1)], key1 = (uint32_t)(most >> 32);
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) key0 = min(key0, (uint32_t)__shfl_xor((int)key0, o, 64));
+        uint32_t key0 = ~sm_wave_top(~s.npart[lane & (SP_WAVES - 1)]), key1 = (uint32_t)(most >> 32);
         int n0 = 0;
 #pragma unroll 1
         for (;;) {
