@@ -18,7 +18,7 @@
  * Two launches: slices of 8192 tokens, and a workgroup for each row. Bound: the
  * vector unit and one LDS add a token where bins are made (256 rows of 129280 50 us),
  * HBM where they are not (23 us, 2.9 TB/s), and for few rows the pick's chain of scans
- * (16 us for 64 rows of top-k 200, 25 with bins) and its code's first fetch.
+ * (13 us for 64 rows of top-k 200, 21 with bins) and its code's first fetch.
  */
 #include "dsv4_dev.h"
 #include "dsv4_internal.h"
