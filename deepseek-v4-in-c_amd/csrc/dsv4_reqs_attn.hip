@@ -88,7 +88,7 @@ __device__ __forceinline__ int wave_scan(int v)
     return v;
 }
 
-/* The largest of all lanes' v, none of them negative. */
+/* The largest of all lanes' v, a whole number not negative. */
 __device__ __forceinline__ int wave_top(int v)
 {
     v = max(v, moved<DPP_QUAD_XOR1, 0xF>(v));
@@ -98,6 +98,22 @@ __device__ __forceinline__ int wave_top(int v)
     v = max(v, moved<DPP_ROW_BCAST15, 0xA>(v));
     v = max(v, moved<DPP_ROW_BCAST31, 0xC>(v));
     return __builtin_amdgcn_readlane(v, 63);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float top_with(float v)
+{
+    const int i = __float_as_int(v);              /* itself where no lane is moved */
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ float wave_top(float v)
+{
+    v = top_with<DPP_QUAD_XOR1, 0xF>(v);
+    v = top_with<DPP_QUAD_XOR2, 0xF>(v);
+    v = top_with<DPP_ROW_HMIRROR, 0xF>(v);
+    v = top_with<DPP_ROW_MIRROR, 0xF>(v);
+    v = top_with<DPP_ROW_BCAST15, 0xA>(v);
+    v = top_with<DPP_ROW_BCAST31, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 /* The sum over 16 lanes. */
 __device__ __forceinline__ float row_sum(float v)
@@ -537,7 +553,7 @@ __global__ void __launch_bounds__(RJ_THREADS) k_reqs_join(JoinJob a, T *o)
             }
             m = fmaxf(m, ms[k]);
         }
-        m = wave_max(m);
+        m = wave_top(m);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             if (64 * k >= n) break;
