@@ -164,7 +164,8 @@ __device__ __forceinline__ u64 sm_bin_sum(double edge, uint32_t n, u64 part)
  * tokens, have hardly more that are as large (256 of 2020 chunks: 274 tokens). One row of
  * 129280 and 64 take 12 and 18 us so for top-k 8 and 21 and 27 for 512, with bins 23 and
  * 32, 31 and 40; for 800 there may be more than the list takes, 75 and 102 us for 35 and
- * 46. */
+ * 46. Where fewer than k chunks have a token, as under a mask, there is no k-th maximum
+ * and all tokens are looked at. */
 __device__ __forceinline__ bool sm_short(const SampleJob &a, int top_k)
 {
     return top_k > 0 && top_k <= SP_K && 2 * top_k <= a.nc && a.nc <= SP_CHUNKS;
@@ -804,8 +805,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
         };
     };
 
-    /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order; or a
-     *      min_p alone: those that it may leave ---- */
+    /* ---- a short top-k: the tokens as large as the k-th largest chunk, in order, or all
+     *      where fewer chunks have any; or a min_p alone: those that it may leave ---- */
     bool fits = brief;
     float low = INFINITY;
     if (few) {
@@ -831,7 +832,10 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
             s.cur[tid] = n0 + c;
             __syncthreads();
             const int d = sm_first(SP_THREADS, [&](int i) { return s.cur[i] >= (uint32_t)top_k; });
-            if (d == SP_THREADS) break;           /* fewer chunks with tokens */
+            if (d == SP_THREADS) {                /* fewer chunks with tokens: all of those */
+                key0 = (uint32_t)(am_key(-3.4028235e38f, 0) >> 32);
+                break;
+            }
             const uint32_t end = key1 - (((uint32_t)d << sh) | ((1u << sh) - 1));
             n0 = d ? (int)s.cur[d - 1] : n0;
             const int through = (int)s.cur[d];
