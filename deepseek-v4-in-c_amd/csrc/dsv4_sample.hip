@@ -414,7 +414,7 @@ struct SmRow {
     const float *cmax;
     SmScale sc;
     double first, e;
-    float width;                                  /* of a bin, in logits     */
+    double width;                                 /* of a bin, in logits     */
     float cm[SP_CHUNKS / SP_THREADS];             /* this thread's of the first chunks */
 
     /* Inclusive sums over the threads. */
@@ -460,12 +460,13 @@ struct SmRow {
     }
 
     /* Logits between which all tokens of bins [b0, b1] lie, with a margin for the roundings
-     * of z and of this. */
+     * of z and of this, in 64 bits: a width that f32 holds with few bits, as of a
+     * temperature under 2^-120, would put the bins beside their tokens. */
     __device__ __forceinline__ void range_of(int b0, int b1, float *lo, float *hi) const
     {
-        const float l = (float)(first - b1) * width, h = (float)(first - b0 + 1.0) * width;
-        *lo = l - fabsf(l) * 4e-6f;
-        *hi = h + fabsf(h) * 4e-6f;
+        const double l = (first - b1) * width, h = (first - b0 + 1.0) * width;
+        *lo = (float)(l - fabs(l) * 4e-6);
+        *hi = (float)(h + fabs(h) * 4e-6);
         if (sc.inf || b1 == SM_BINS - 1 || !(*lo > -3.4028235e38f)) *lo = -3.4028235e38f;
         if (sc.inf || b0 == 0 || !(*hi < INFINITY)) *hi = INFINITY;
     }
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     const bool few = sm_short(a, top_k), brief = few || sm_above(a, row, floor_);
     const float u = a.r.u[row];
     Row r{a, s, (const T *)a.x + (size_t)row * a.stride, a.cmax + (size_t)row * a.nc,
-          SmScale{0.0, false}, 0.0, 0.0, temp * 0.021660849f, {}};
+          SmScale{0.0, false}, 0.0, 0.0, (double)temp * 0.02166084939249829, {}};
     auto done = [&](int pick, float prob, int kept) {
         d_pick[row] = pick;
         if (a.prob) a.prob[row] = prob;
