@@ -85,10 +85,10 @@ __device__ __forceinline__ double sm_exp2_part(double f)
     return fma(p, f, 1.0);
 }
 
-/* 2^t, t <= 0; 0 below 2^-64. */
+/* 2^t, t <= 0; 0 below 2^-1000, which is under every min_p over 0. */
 __device__ __forceinline__ double sm_exp2(double t)
 {
-    if (!(t > -64.0)) return 0.0;
+    if (!(t > -1000.0)) return 0.0;
     const double n = __builtin_rint(t);
     return sm_exp2_part(t - n) * __hiloint2double((1023 + (int)n) << 20, 0);
 }
