@@ -177,7 +177,8 @@ __device__ __forceinline__ bool sm_short(const SampleJob &a, int top_k)
  * row's workgroup count the bins after all, 71 to 198 and 47 to 169. */
 __device__ __forceinline__ float sm_floor(const SampleJob &a, int row)
 {
-    return a.r.min_p ? fminf(a.r.min_p[row], 1.0f) : 0.0f;
+    const float v = a.r.min_p ? a.r.min_p[row] : 0.0f;
+    return v > 0.0f ? fminf(v, 1.0f) : 0.0f;      /* NaN: no such rule       */
 }
 __device__ __forceinline__ bool sm_above(const SampleJob &a, int row, float floor_)
 {

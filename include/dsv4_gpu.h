@@ -751,10 +751,10 @@ int dsv4_gpu_reqs_attn_d(void *d_o, const void *d_q, int fmt, int h, int d_qk, i
  * of them the fewest first ones whose probabilities, softmax(logit /
  * temperature) among those top_k, sum to top_p (1 or more: all); and of them those
  * with at least min_p (at most 1 counts) times the first's probability. The first
- * always stays. The pick is the first in the order whose probability, summed with
- * those before it, exceeds u times that of all that are left, u in [0, 1) (below:
- * 0; above: the last one; NaN: 0). A temperature that is not over 0 picks the first. A logit of
- * +infinity leaves the others no probability. */
+ * always stays; a top_p or min_p that is NaN is no rule. The pick is the first in the
+ * order whose probability, summed with those before it, exceeds u times that of all
+ * that are left, u in [0, 1) (below: 0; above: the last one; NaN: 0). A temperature that
+ * is not over 0 picks the first. A logit of +infinity leaves the others no probability. */
 typedef struct {
     const float *temperature;
     const int *top_k;

@@ -1,9 +1,10 @@
-"""min_p of dsv4_gpu_sample_d so low that it reaches tokens whose weight is no part of any
-sum."""
+"""min_p of dsv4_gpu_sample_d at its ends: so low that it reaches tokens whose weight is
+no part of any sum, and not a number."""
 import numpy as np
 import pytest
 
-from test_gpu_sample import check
+import reqs_common as rc
+from test_gpu_sample import NAN, check
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +24,17 @@ def test_floors_under_the_sums(gpu, dsv4, vocab, bf):
     for kw in (dict(), dict(top_k=few), dict(top_k=np.full(n, 600)), dict(top_p=np.full(n, 0.999)),
                dict(temperature=np.linspace(0.7, 1.4, n))):
         check(dsv4, x, bf, u=u, min_p=floor, **kw)
+
+
+@pytest.mark.parametrize("vocab", [700, 40000])
+def test_a_floor_that_is_not_a_number(gpu, dsv4, vocab):
+    """No such rule, as with top_p."""
+    rng = np.random.default_rng(vocab)
+    n = 6
+    x = rng.standard_normal((n, vocab)).astype(np.float32) * np.float32(2)
+    u = rng.random(n).astype(np.float32)
+    for kw in (dict(), dict(top_k=np.full(n, 9)), dict(top_k=np.full(n, 600)),
+               dict(top_p=np.full(n, 0.7)), dict(temperature=np.full(n, 0.8))):
+        got = check(dsv4, x, u=u, min_p=np.full(n, NAN), **kw)
+        want = rc.run_sample(dsv4, x, u=u, **kw)
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
