@@ -59,7 +59,7 @@ struct SmTop {
 struct SampleJob {
     const void *x;
     long long stride;
-    int n, vocab, ns, nc, sh;                     /* slices, chunks of a row */
+    int row0, vocab, ns, nc, sh;                  /* first row; slices, chunks of one */
     dsv4_gpu_sampling r;
     u64 *bins;                                    /* [n][ns][bins]           */
     SmTop *top;                                   /* [n][ns]                 */
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_slices(SampleJob a)
     __shared__ u64 tail;
     __shared__ uint32_t tail_n;
     const int tid = threadIdx.x;
-    const int row = blockIdx.x / a.ns, slice = blockIdx.x - row * a.ns;
+    const int of = blockIdx.x / a.ns, slice = blockIdx.x - of * a.ns, row = a.row0 + of;
     const int v0 = slice * SM_SLICE;
     const T *x = (const T *)a.x + (size_t)row * a.stride + v0;
     const int lim = min(SM_SLICE, a.vocab - v0);
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_pick(SampleJob a, int *d_
     using Row = SmRow<T>;
     __shared__ typename Row::Lds s;
     constexpr int LAST = SM_BINS - 1;
-    const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, row = a.row0 + blockIdx.x;
     const float temp = sm_temperature(a, row);
     const int top_k = a.r.top_k ? a.r.top_k[row] : 0;
     const float p = a.r.top_p ? a.r.top_p[row] : 1.0f;
@@ -1240,15 +1240,19 @@ SamplePlan sample_plan(int n, int vocab)
 
 constexpr int SM_ROWS = 65536, SM_VOCAB = 1 << 22;
 
+/* As many rows a launch as keep its threads under 2^32; one launch up to 2^23 slices. */
 template <class T>
-int sample_launch(const SampleJob &a, int *d_pick, hipStream_t st)
+int sample_launch(SampleJob a, int n, int *d_pick, hipStream_t st)
 {
-    hipLaunchKernelGGL(k_sample_slices<T>, dim3((unsigned)a.n * (unsigned)a.ns), dim3(SM_THREADS),
-                       0, st, a);
-    HIP_OK(hipGetLastError(), "sample slices launch");
-    hipLaunchKernelGGL(k_sample_pick<T>, dim3((unsigned)a.n), dim3(SP_THREADS), 0, st, a,
-                       d_pick);
-    HIP_OK(hipGetLastError(), "sample pick launch");
+    const int most = (int)(((1ll << 32) / SM_THREADS - 1) / a.ns);
+    for (a.row0 = 0; a.row0 < n; a.row0 += most) {
+        const unsigned rows = (unsigned)(n - a.row0 < most ? n - a.row0 : most);
+        hipLaunchKernelGGL(k_sample_slices<T>, dim3(rows * (unsigned)a.ns), dim3(SM_THREADS), 0, st,
+                           a);
+        HIP_OK(hipGetLastError(), "sample slices launch");
+        hipLaunchKernelGGL(k_sample_pick<T>, dim3(rows), dim3(SP_THREADS), 0, st, a, d_pick);
+        HIP_OK(hipGetLastError(), "sample pick launch");
+    }
     return 0;
 }
 
@@ -1283,9 +1287,9 @@ extern "C" int dsv4_gpu_sample_d(int *d_pick, float *d_prob, int *d_kept, const 
         return -1;
     }
     char *base = (char *)d_scratch;
-    SampleJob a{d_logits, stride, n, vocab, p.ns, p.nc, p.sh, *s, (u64 *)base,
+    SampleJob a{d_logits, stride, 0, vocab, p.ns, p.nc, p.sh, *s, (u64 *)base,
                 (SmTop *)(base + p.top), (float *)(base + p.cmax), d_kept, d_prob};
     hipStream_t st = (hipStream_t)stream;
-    return fmt == DSV4_WF32 ? sample_launch<float>(a, d_pick, st)
-                            : sample_launch<uint16_t>(a, d_pick, st);
+    return fmt == DSV4_WF32 ? sample_launch<float>(a, n, d_pick, st)
+                            : sample_launch<uint16_t>(a, n, d_pick, st);
 }
