@@ -47,7 +47,7 @@ struct Dsv4ReqsItem {
  * shortest), the prefix's splits and the rows of all requests. */
 constexpr int DSV4_REQS_KINDS = 5;
 struct Dsv4ReqsHead {
-    uint32_t sig;
+    uint64_t sig;
     int end[DSV4_REQS_KINDS];
     int prefix_splits, row0, rows;
 };
@@ -61,7 +61,7 @@ struct Dsv4ReqsJob : Dsv4TreeJob {
     const Dsv4ReqsItem *items;
     const Dsv4ReqsReq *req;
     int n_req;
-    uint32_t sig;
+    uint64_t sig;
 };
 int dsv4_reqs_f32_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st);
 int dsv4_reqs_bf16_launch(const Dsv4ReqsJob &a, int fmt, int kc, unsigned groups, hipStream_t st);

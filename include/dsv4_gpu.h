@@ -728,9 +728,9 @@ int dsv4_gpu_reqs_tables_d(const dsv4_gpu_reqs *r, const int *d_len, const int *
  * dsv4_gpu_reqs_plan_d makes the step's plan from r->len and r->first on the device,
  * once for all layers that have these sizes, formats and this window;
  * dsv4_gpu_reqs_attn_d reads the plan and r->pages, and of r else only its sizes, which
- * have to be the plan's. With a plan of other sizes, or where first does not ascend from 0
- * or more to max_tok at most or a request with tokens has fewer positions than those or
- * more than its table, all of o becomes NaN. d_plan: dsv4_gpu_reqs_plan_bytes of
+ * have to be the plan's. With a plan of other sizes, formats or window, or where first does
+ * not ascend from 0 or more to max_tok at most or a request with tokens has fewer positions
+ * than those or more than its table, all of o becomes NaN. d_plan: dsv4_gpu_reqs_plan_bytes of
  * device memory, 16-byte aligned, kept from the plan to the last call that reads it;
  * d_scratch: dsv4_gpu_reqs_attn_scratch_bytes, 16-byte aligned, not kept. Neither
  * falls as n_req, max_tok or h grows. d_o must not overlap what the call reads. 0 / -1. */
