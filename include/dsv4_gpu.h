@@ -685,9 +685,9 @@ typedef struct {
     int *first;            /* [n_req + 1]                                     */
     int n_req, max_pages, page_rows;
     int max_tok;           /* tokens that a step's buffers have room for       */
-    int n_prefix;          /* the first positions hold the same rows in every
-                            * request that is as long, and whole pages of them
-                            * are all requests'                               */
+    int n_prefix;          /* a position before it holds the same row in every
+                            * request that has that position, and whole pages
+                            * of these are all requests'; 0: none             */
 } dsv4_gpu_reqs;
 
 /* The tables of a step. d_len[i] positions of request i are in use; d_new[i] >
@@ -701,7 +701,10 @@ typedef struct {
  * pages are at most max_tok. New pages are taken from the ring's first on, in
  * the order of requests and positions, and entered in r->pages; an ended
  * request's pages but for those all requests share are put behind the last, in
- * the same order (a request that ended before has d_len 0). Written: r->first,
+ * the same order (a request that ended before has d_len 0). The shared ones are the
+ * caller's: a request begins with them in its table and d_len behind them. One that grows
+ * through them, to fill them for the others, takes pages that no request's end puts
+ * back; their numbers are then in its table. Written: r->first,
  * r->len (0 for ended requests, which may be d_len), d_free_out[2] (which may be
  * d_free), and for each token its cache row, position and request (any of the
  * three may be NULL), -1 from the last token to max_tok and the row -1 where a
