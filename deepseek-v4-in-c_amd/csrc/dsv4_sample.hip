@@ -16,8 +16,9 @@
  * wrong by a rounding is another token.
  *
  * Two launches: slices of 8192 tokens, and a workgroup for each row. Bound: the
- * vector unit and one LDS add a token where bins are made (256 rows of 129280 50 us),
- * HBM where they are not (23 us, 2.9 TB/s), and for few rows the pick's chain of scans
+ * vector unit, busy 92 %, and one LDS add a token where bins are made (256 rows of 129280
+ * 50 us); where they are not a slice's loads, as none are in flight while it is reduced
+ * (23 us, 2.9 TB/s, the waves wait 72 % of it); and for few rows the pick's chain of scans
  * (13 us for 64 rows of top-k 200, 21 with bins) and its code's first fetch.
  */
 #include "dsv4_dev.h"
